@@ -430,7 +430,7 @@ REFERENCE_QUIRKS, KV_FP32, ALL_LOGITS_FP32 = 1, 2, 4
 
 
 # ---- layered models (include/cml_lm.h and the kernels behind it) ---------------------------------
-DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+DT_F32, DT_BF16, DT_F16, DT_I8, DT_E4M3 = 0, 1, 2, 3, 4
 ACT_SILU, ACT_GELU_TANH, ACT_CLAMPED, ACT_GELU_ERF = 0, 1, 2, 3
 DTYPE_FLOAT32, DTYPE_BFLOAT16 = 0, 6
 
@@ -447,7 +447,7 @@ class Attn(C.Structure):
                 ("temp_every", C.c_float), ("gate_col", ci), ("cache_dtype", ci), ("k_pool", vp), ("v_pool", vp), ("block_size", ci),
                 ("block_table", vp), ("table_ld", ci), ("gate_wide", ci), ("keep", ci), ("chunk", ci), ("sinks", vp), ("head_norm", ci), ("keys_as_values", ci),
                 ("out_scale", C.c_float), ("freq", vp), ("rot_dims", ci), ("taps", ci), ("conv", vp), ("ring", vp), ("cap", C.c_float), ("talk", vp),
-                ("scores", vp), ("scores_ld", ci)]
+                ("scores", vp), ("scores_ld", ci), ("k_scale", vp), ("v_scale", vp)]
 
 
 class Latent(C.Structure):
@@ -491,6 +491,11 @@ class GatedJoin(C.Structure):
                 ("table", vp), ("table_dtype", ci), ("vocab", ci), ("tokens", vp)]
 
 
+class Pages(C.Structure):
+    """cmlb200_pages; its pools are device arrays of cmlb200_page_pool (three 64-bit numbers each)."""
+    _fields_ = [("pools", ci), ("pool", vp), ("most", C.c_size_t), ("pages", ci), ("table", vp), ("slots", ci), ("table_ld", ci)]
+
+
 class LMOptions(C.Structure):
     _fields_ = [("dtype", ci), ("max_tokens", ci), ("max_sequences", ci), ("max_step_rows", ci)]
 
@@ -500,6 +505,9 @@ class LMEntry(C.Structure):
 
 
 _sig("cmlb200_embed_rows", ci, vp, ci, vp, vp, vp, ci, ci, ci, vp, vp)
+_sig("cmlb200_token_scores", ci, vp, ci, C.c_long, ci, ci, vp, ci, vp, vp, vp, vp, vp)
+_sig("cmlb200_pages_copy", ci, C.POINTER(Pages), vp, ci, vp)
+_sig("cmlb200_pages_fork", ci, C.POINTER(Pages), vp, ci, vp)
 _sig("cmlb200_residual_norm", ci, vp, vp, ci, vp, vp, C.c_float, ci, ci, vp, vp, ci, ci, vp)
 _sig("cmlb200_qk_norm_append", ci, C.POINTER(Attn), vp, ci, vp, vp, ci, vp)
 _sig("cmlb200_attention_tiles", ci, C.POINTER(Attn), vp, ci, vp, ci, vp, ci, vp)

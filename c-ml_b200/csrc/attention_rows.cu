@@ -17,7 +17,7 @@
 //
 // Scores are kept in units of log2 in the first two kernels (the scale carries log2 e). A sink starts
 // the running maximum at its score, so its weight joins the denominator exactly once.
-#include "lm_util.cuh"
+#include "cache8.cuh"
 
 namespace {
 
@@ -574,7 +574,9 @@ extern "C" int cmlb200_attn_check_(const cmlb200_attn* a, const char* who) {
     CMLB_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, "%s: heads %d, kv_heads %d", who, a->heads, a->kv_heads);
     CMLB_REQUIRE(a->dim > 0 && a->vdim > 0 && a->dim_ld >= a->dim && a->vdim_ld >= a->vdim && a->dim_ld % 16 == 0 && a->vdim_ld % 16 == 0,
                  "%s: head sizes %d (stride %d) / %d (stride %d)", who, a->dim, a->dim_ld, a->vdim, a->vdim_ld);
-    CMLB_REQUIRE(a->cache_dtype == CMLB200_DT_F32 || a->cache_dtype == CMLB200_DT_F16, "%s: cache dtype %d", who, a->cache_dtype);
+    CMLB_REQUIRE(a->cache_dtype == CMLB200_DT_F32 || a->cache_dtype == CMLB200_DT_F16 || is_cache8(a->cache_dtype), "%s: cache dtype %d", who, a->cache_dtype);
+    CMLB_REQUIRE(!is_cache8(a->cache_dtype) || (a->k_scale && a->v_scale && !a->scores && !a->talk && a->taps == 0 && a->cap == 0.f && a->dim_ld <= 256 && a->vdim_ld <= 256),
+                 "%s: an 8-bit cache needs scales and heads up to 256 (here %d / %d), and goes with neither convolution nor capped, mixed or given scores", who, a->dim, a->vdim);
     CMLB_REQUIRE(!a->gate_wide || a->gate_col >= 0, "%s: gate_wide without a gate column", who);
     CMLB_REQUIRE(a->keep >= 0 && a->chunk >= 0 && (!a->keys_as_values || a->dim == a->vdim), "%s: kept tokens %d, chunk %d, values as keys of %d / %d", who, a->keep,
                  a->chunk, a->dim, a->vdim);
@@ -591,8 +593,9 @@ extern "C" int cmlb200_attention_tiles(const cmlb200_attn* a, const float* d_qkv
     CMLB_REQUIRE(a && d_qkv && d_tiles && tiles > 0 && d_out_bf16, "cmlb200_attention_tiles: bad argument");
     const int rc = cmlb200_attn_check_(a, "cmlb200_attention_tiles");
     if (rc) return rc;
-    CMLB_REQUIRE(a->cache_dtype == CMLB200_DT_F16 && a->vdim_ld <= 256 && a->heads <= 65535, "cmlb200_attention_tiles: fp16 cache and value heads up to 256");
+    CMLB_REQUIRE(a->cache_dtype != CMLB200_DT_F32 && a->vdim_ld <= 256 && a->heads <= 65535, "cmlb200_attention_tiles: fp16 or 8-bit cache and value heads up to 256");
     CMLB_REQUIRE(((uintptr_t)d_tiles & 15) == 0, "cmlb200_attention_tiles: the tile list must be 16-byte aligned");
+    if (is_cache8(a->cache_dtype)) return cmlb_attention8_tiles(a, d_qkv, ld, d_tiles, tiles, (__nv_bfloat16*)d_out_bf16, out_ld, as_stream(stream));
     const bool scored = a->scores != nullptr;
     CMLB_REQUIRE(!scored || (a->scores_ld % 64 == 0 && ((uintptr_t)a->scores & 15) == 0), "cmlb200_attention_tiles: score stride %d", a->scores_ld);
     const size_t smem = 2 * ((scored ? 0 : (size_t)(QT + 2 * KT) * (a->dim_ld + 8)) + (size_t)2 * KT * (a->vdim_ld + 8));
@@ -626,8 +629,9 @@ extern "C" int cmlb200_attention_one(const cmlb200_attn* a, const float* d_qkv, 
     CMLB_REQUIRE(a && d_qkv && d_row_pos && d_row_slot && rows > 0 && max_keys >= 0 && d_out_bf16, "cmlb200_attention_one: bad argument");
     const int rc = cmlb200_attn_check_(a, "cmlb200_attention_one");
     if (rc) return rc;
-    CMLB_REQUIRE(a->cache_dtype == CMLB200_DT_F16 && a->vdim_ld <= 256 && rows <= 65535, "cmlb200_attention_one: fp16 cache and value heads up to 256");
+    CMLB_REQUIRE(a->cache_dtype != CMLB200_DT_F32 && a->vdim_ld <= 256 && rows <= 65535, "cmlb200_attention_one: fp16 or 8-bit cache and value heads up to 256");
     CMLB_REQUIRE(!a->gate_wide, "cmlb200_attention_one: one gate per head");
+    if (is_cache8(a->cache_dtype)) return cmlb_attention8_one(a, d_qkv, ld, d_row_pos, d_row_slot, rows, max_keys, (__nv_bfloat16*)d_out_bf16, out_ld, as_stream(stream));
     // Few rows: fewer heads per CTA, so that more CTAs share the work (the keys are read again from L2). One head where that makes no
     // more CTAs than SMs: 8 rows of 16 on 4 heads take 232 instead of 278 us a decode step of four layers behind 40 tokens, 290
     // and 287 behind 1,000; 12 rows (192 CTAs) would take 384 instead of 323.

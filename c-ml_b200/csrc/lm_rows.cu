@@ -4,7 +4,7 @@
 // query/key norm with query temperature and paged cache append, and the gated activation of the
 // 32-bit path. The residual and every norm are fp32; the operand handed to the next matrix product
 // is bf16 or fp32.
-#include "lm_util.cuh"
+#include "cache8.cuh"
 
 namespace {
 
@@ -841,6 +841,7 @@ extern "C" int cmlb200_qk_norm_append(const cmlb200_attn* a, float* d_qkv, int l
     const int rc = cmlb200_attn_check_(a, "cmlb200_qk_norm_append");
     if (rc) return rc;
     CMLB_REQUIRE(ld >= a->heads * a->dim + a->kv_heads * (a->dim + (a->keys_as_values ? 0 : a->vdim)), "cmlb200_qk_norm_append: row stride %d", ld);
+    if (is_cache8(a->cache_dtype)) return cmlb_cache8_append(a, d_qkv, ld, d_row_pos, d_row_slot, 0, rows, false, true, as_stream(stream));
     const size_t smem = a->head_norm ? (size_t)(a->heads + a->kv_heads) * 4 : 0;
     CMLB_REQUIRE(smem <= 40 * 1024, "cmlb200_qk_norm_append: %d heads", a->heads);
     cudaStream_t st = as_stream(stream);

@@ -10,7 +10,7 @@
 // A ring holds `taps` entries, position p in entry p mod taps. A decoded token reads the entries before its own and
 // writes its own, which no other row of the launch looks at; the rows of a portion would overwrite what its first rows still
 // read, so theirs are written by a launch of their own.
-#include "lm_util.cuh"
+#include "cache8.cuh"
 
 namespace {
 
@@ -171,6 +171,10 @@ extern "C" int cmlb200_rotate_append(const cmlb200_attn* a, float* d_qkv, int ld
     const int rc = check_rotated(a, ld, who);
     if (rc) return rc;
     CMLB_REQUIRE(a->taps == 0 || d_q_out, "%s: convolved queries go to rows of their own", who);
+    if (is_cache8(a->cache_dtype)) {
+        CMLB_REQUIRE(!d_q_out, "%s: queries stay in place over an 8-bit cache", who);
+        return cmlb_cache8_append(a, d_qkv, ld, d_row_pos, d_row_slot, first, rows, true, true, as_stream(stream));
+    }
     const bool vec = a->dim % 4 == 0 && a->vdim % 4 == 0 && ld % 4 == 0 && (((uintptr_t)d_qkv | (uintptr_t)a->conv | (uintptr_t)a->ring | (uintptr_t)d_q_out) & 15) == 0;
     const int units = (a->heads + a->kv_heads) * (a->dim_ld / (vec ? 4 : 2)) + a->kv_heads * (a->vdim_ld / (vec ? 4 : 2)), most = (units + 255) / 256;
     const int group = rows >= 64 ? 8 : 1, groups = (rows + group - 1) / group;

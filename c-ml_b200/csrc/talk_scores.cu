@@ -291,6 +291,7 @@ int check_talk(const cmlb200_attn* a, const void* q, const float* scores, int ld
     if (rc) return rc;
     CMLB_REQUIRE(q && scores && ld > 0 && ld % 4 == 0 && (((uintptr_t)q | (uintptr_t)scores) & 15) == 0, "%s: queries, scores or their stride %d", who, ld);
     CMLB_REQUIRE(!a->slopes && a->chunk == 0 && a->keep == 0, "%s: windows alone", who);
+    CMLB_REQUIRE(a->cache_dtype == CMLB200_DT_F32 || a->cache_dtype == CMLB200_DT_F16, "%s: fp32 or fp16 cache", who);
     return CMLB200_OK;
 }
 

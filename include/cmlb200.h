@@ -410,6 +410,10 @@ int cmlb200_ipc_close(void* d_ptr);
 #define CMLB200_DT_F32 0
 #define CMLB200_DT_BF16 1
 #define CMLB200_DT_F16 2
+/* Caches alone: 8-bit codes with a scale for every group of 16 tokens of a page and key/value head, int8 and e4m3 */
+#define CMLB200_DT_I8 3
+#define CMLB200_DT_E4M3 4
+#define CMLB200_SCALE_TOKENS 16
 #define CMLB200_ACT_SILU 0
 #define CMLB200_ACT_GELU_TANH 1
 #define CMLB200_ACT_CLAMPED 2     /* g = min(gate, limit), u = clamp(up, -limit, limit): g sigmoid(1.702 g) (u + 1) */
@@ -440,7 +444,7 @@ typedef struct cmlb200_attn {
     float eps;
     float temp_coef, temp_every;  /* q *= 1 + coef ln(floor((i + 1) / every) + 1); every <= 0: none */
     int gate_col;               /* column of the first of `heads` gate logits in a projection row; -1: none */
-    int cache_dtype;            /* CMLB200_DT_F32 or CMLB200_DT_F16 */
+    int cache_dtype;            /* CMLB200_DT_F32 or CMLB200_DT_F16; _I8 or _E4M3 where neither conv nor scores are given */
     void *k_pool, *v_pool;      /* [blocks][block_size][kv_heads][dim_ld] and [..][vdim_ld] */
     int block_size;             /* a power of two >= 16 */
     const int* block_table;     /* device, [slots][table_ld] block ids */
@@ -461,6 +465,7 @@ typedef struct cmlb200_attn {
     const float* talk;          /* device, [heads][heads]: a head's score is that combination of all heads' scores (the same); NULL: its own */
     const float* scores;        /* device: scores made by cmlb200_talk_scores_*, which q . k is then not computed for; NULL: none */
     int scores_ld;
+    float *k_scale, *v_scale;   /* device, [blocks][block_size / 16][kv_heads]: a cached number of CMLB200_DT_I8 or _E4M3 is its code times that */
 } cmlb200_attn;
 
 /* Latent attention over a paged cache of one vector per token: a normed latent of `rank` values and a rotated key
@@ -577,6 +582,14 @@ int cmlb200_embed_rows(const void* d_table, int dtype, const int* d_tokens, cons
  * w_next is given. Without y, d_row_idx (optional) picks the rows of x. out: fp32 or bf16, stride ldo. */
 int cmlb200_residual_norm(float* d_x, const float* d_y, int ldy, const float* d_w_post, const float* d_w_next, float eps, int rows, int dim,
                           const int* d_row_idx, void* d_out, int out_dtype, int ldo, void* stream);
+/* 8-bit caches (CMLB200_DT_I8, CMLB200_DT_E4M3). Whatever appends to one sets a group's scale to the smallest power of two, at least
+ * 2^-126, that holds the largest of the group's new numbers in 127 (int8) or 448 (e4m3) steps, or leaves it as it is where the sequence's
+ * earlier tokens in the group have a larger one; codes are numbers over the scale, rounded to even, and earlier codes are rounded to a scale that
+ * has grown. Numbers beyond 65504 are held there, NaN is cached as 0. Attention is over what the cache then holds, the row's own key and value
+ * included. The rows of one sequence follow one another in a call, in order of position, and nothing else of the device writes or reads their
+ * groups meanwhile. Entry points: cmlb200_qk_norm_append, cmlb200_rotate_append (no conv), cmlb200_attention_tiles, cmlb200_attention_one;
+ * value heads up to 256, key heads up to 256. */
+
 /* Norms q (in place) and k of projection rows, applies the query temperature, appends k and v to the cache. */
 int cmlb200_qk_norm_append(const cmlb200_attn* a, float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, void* stream);
 /* Attention of prompt portions whose q is normed and whose k, v are appended already: tiles of up to 64
@@ -714,6 +727,37 @@ int cmlb200_moe_gemv_act(const cmlb200_moe* m, const cmlb200_dense* W, const uin
 int cmlb200_moe_gemm_act(const cmlb200_moe* m, const cmlb200_dense* W, const uint16_t* d_x, int ldx, int rows, int ff, int act, uint16_t* d_f, int ldf, void* stream);
 int cmlb200_act_rows_f32(const float* d_z, int ld, int rows, int ff, int act, float* d_f, int ldf, void* stream);
 int cmlb200_moe_glu_rows_f32(const float* d_gu, int ld, int rows, int ff, int act, float limit, float* d_f, int ldf, void* stream);
+/* What rows of logits (fp32, bf16 or fp16, row stride ld) say about tokens, in one pass over them: logprob[r] = ln softmax(row)[tokens[r]],
+ * entropy[r] of that distribution in nats, and the `top` (0 .. 32) likeliest tokens of the row, best first, the lower id first among equals, with their
+ * log probabilities: top_ids, top_logprob [rows][top]. tokens and logprob, entropy, and either of the last two may be NULL. Logits of -inf are
+ * tokens that cannot come: log probability -inf, no part of the entropy, no alternative (places without one hold id -1 and -inf). A row of
+ * nothing but such has log probabilities of -inf, entropy 0 and no alternatives; a token outside the vocabulary has -inf. A row that holds NaN or +inf has NaN
+ * for log probabilities and entropy, and its alternatives are those of its other numbers and +inf. Sums are fp32. Stands for the
+ * softmax loops on the host of src/nn/llama.c:662-737. */
+int cmlb200_token_scores(const void* d_logits, int dtype, long ld, int rows, int vocab, const int* d_tokens, int top, float* d_logprob, float* d_entropy, int* d_top_ids,
+                         float* d_top_logprob, void* stream);
+
+/* Pools whose slots are named by the same page ids: page i of a pool is `bytes` bytes at base + i * stride. */
+typedef struct cmlb200_page_pool {
+    void* base;
+    size_t stride, bytes;
+} cmlb200_page_pool;
+typedef struct cmlb200_pages {
+    int pools;
+    const cmlb200_page_pool* pool;  /* device, [pools] */
+    size_t most;                /* no pool's `bytes` is larger */
+    int pages;                  /* ids are 0 .. pages - 1; a move or fork that names another is not made */
+    int* table;                 /* device, block table [slots][table_ld]; NULL: none (_copy only) */
+    int slots, table_ld;
+} cmlb200_pages;
+/* Copies pages in all pools: moves[i] = {from, to}, device. A page is the target of one move at most, and no target is a source. With a table, its
+ * entries that name a source name its target afterwards; the moves are then in ascending order of their sources, each of them once. */
+int cmlb200_pages_copy(const cmlb200_pages* p, const int* d_moves, int moves, void* stream);
+/* Sequences that go on from others: forks[i] = {parent slot, child slot, shared pages, own page}, device, 16-byte aligned. The child's table row begins with the parent's
+ * first `shared` entries; own page >= 0: the page behind those is copied into it in all pools, and it is the child's next entry. The rest of the row
+ * stays. No child is a parent of the same call, no own page another's page. */
+int cmlb200_pages_fork(const cmlb200_pages* p, const int* d_forks, int forks, void* stream);
+
 /* tokens[i] = picked[i], pos[i] += 1, hist[step * rows + i] = picked[i], step += 1 */
 int cmlb200_advance_tokens(const int* d_picked, int rows, int* d_tokens, int* d_pos, int* d_hist, int* d_step, void* stream);
 
