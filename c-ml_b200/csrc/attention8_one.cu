@@ -1,0 +1,518 @@
+// Decoded tokens over 8-bit caches (cache8.cuh), one row per sequence: norm, rotation, append, attention and gate in one launch.
+//
+// A step reads every cached byte of its sequences once, so HBM bounds it; codes have to become MMA operands in few instructions. A warp
+// takes 16 keys (a scale group) at a time and all query heads of a key/value head, on mma.sync m16n8k16 with fp16 operands, into which codes
+// convert exactly:
+//   S^T [16 keys x 8 heads] = K q        A: a lane holds 16-byte pieces of the keys g and g + 8. Which dimension an MMA's column k stands for is free, so
+//                                        a lane's four consecutive codes are its four columns, and no shuffle or shared memory is needed
+//   O^T [16 dims x 8 heads] += V^T P^T   A: a lane holds the same 8, 16 or 32 dimensions of the keys 2t, 2t + 1, 2t + 8, 2t + 9; bytes of two keys are
+//                                        interleaved, which makes the operand's pairs. P^T comes from S^T by movmatrix
+// so the codes go from global memory to registers to the tensor cores. A lane requests the next group's codes before it uses this one's.
+// A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
+// where m, the warp's reference for the exponentials, moves only when a score has passed it by 7 (powers of two; sums are fp32). Queries are fp16 over
+// a power of two of their own per head, so their size is no matter.
+// 4 warps a CTA take groups in turn; a cluster of up to 8 CTAs splits a row's keys and merges through distributed shared memory, each CTA a
+// share of the outputs. The group that the row's own token joins belongs to rank 0 alone, which settles its scales, rewrites it where they have grown and
+// attends to it from shared memory; nobody else looks at it.
+#include "cache8.cuh"
+
+namespace {
+
+constexpr int A1_THREADS = 128, A1_WARPS = A1_THREADS / 32, A1_SPLITS = 8;
+constexpr float kWeightUnit = 256.f;
+
+__device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
+    if (a.chunk > 0) return p / a.chunk * a.chunk;
+    return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
+}
+__device__ __forceinline__ uint4 ld_codes(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ld_codes8(const uint8_t* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float cluster_load(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// KC: 16-code pieces of a key per lane (64 dimensions each). VW: words of a value per lane (32 dimensions each).
+template <int KC, int VW>
+struct Codes {
+    uint32_t k[2][KC][4];                              // keys g, g + 8
+    uint32_t v[4][VW];                                 // keys 2t, 2t + 1, 2t + 8, 2t + 9
+    float ks, vs;
+};
+// from: a group's first token's codes for this key/value head; `last`: its last token that may be read. GLOBAL: the cache, else shared memory.
+template <bool GLOBAL, int KC, int VW>
+__device__ __forceinline__ void load_group(Codes<KC, VW>& x, const uint8_t* k, const uint8_t* v, int kstride, int vstride, int dk, int dv, int last, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    auto wide = [](const uint8_t* p) { return GLOBAL ? ld_codes(p) : *reinterpret_cast<const uint4*>(p); };
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint8_t* r = k + (size_t)min(g + 8 * i, last) * kstride + 16 * t;
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (64 * c + 16 * t < dk) u = wide(r + 64 * c);
+            x.k[i][c][0] = u.x; x.k[i][c][1] = u.y; x.k[i][c][2] = u.z; x.k[i][c][3] = u.w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint8_t* r = v + (size_t)min(2 * t + (i & 1) + 8 * (i >> 1), last) * vstride;
+        if constexpr (VW == 2) {
+            uint2 u = make_uint2(0u, 0u);
+            if (8 * g < dv) u = GLOBAL ? ld_codes8(r + 8 * g) : *reinterpret_cast<const uint2*>(r + 8 * g);
+            x.v[i][0] = u.x; x.v[i][1] = u.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < VW / 4; c++) {
+                uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                if (128 * c + 16 * g < dv) u = wide(r + 128 * c + 16 * g);
+                x.v[i][4 * c] = u.x; x.v[i][4 * c + 1] = u.y; x.v[i][4 * c + 2] = u.z; x.v[i][4 * c + 3] = u.w;
+            }
+        }
+    }
+}
+
+// What a warp carries: per head 8 n + 2 t + e the reference m and the sum l (this lane's keys), and O^T.
+template <int VW, int NT>
+struct State {
+    float m[NT][2], l[NT][2], o[NT][2 * VW][4];
+    float vref, vinv;                                  // largest value scale so far, one over it
+};
+
+// S, the weights and O of a group whose first key is `key0` for the row at position p. qs: per head its queries' power of two.
+template <bool I8, int KC, int VW, int NT>
+__device__ __forceinline__ void take_group(State<VW, NT>& st, const Codes<KC, VW>& x, const uint32_t (&q)[NT][KC][4][2], const float (&qs)[NT][2], const float (&slope)[NT][2], int key0, int p,
+                                           int k_lo, int keep, int lane) {
+    const int g = lane >> 2;
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) { s[n][0] = 0.f; s[n][1] = 0.f; s[n][2] = 0.f; s[n][3] = 0.f; }
+#pragma unroll
+    for (int c = 0; c < KC; c++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t a[4];
+            unpack8<I8>(x.k[0][c][j], a[0], a[2]);
+            unpack8<I8>(x.k[1][c][j], a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma_f16(s[n], a, q[n][c][j][0], q[n][c][j][1]);
+        }
+    const float back = (float)(p - key0 - g);
+    const bool edge = key0 + kScaleTokens - 1 > p || (key0 < k_lo && key0 + kScaleTokens > keep);
+    bool over = x.vs > st.vref;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float f = qs[n][e] * x.ks;
+            s[n][e] = fmaf(s[n][e], f, -slope[n][e] * back);
+            s[n][2 + e] = fmaf(s[n][2 + e], f, -slope[n][e] * (back - 8.f));
+        }
+    if (edge) {
+        const int k0 = key0 + g, k1 = k0 + 8;
+        const bool out0 = k0 > p || (k0 < k_lo && k0 >= keep), out1 = k1 > p || (k1 < k_lo && k1 >= keep);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                if (out0) s[n][e] = -INFINITY;
+                if (out1) s[n][2 + e] = -INFINITY;
+            }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) over |= fmaxf(s[n][e], s[n][2 + e]) > st.m[n][e] + 7.f;
+    if (__any_sync(0xffffffffu, over)) {
+        const float vnew = fmaxf(st.vref, x.vs), cv = st.vref > 0.f ? st.vref / vnew : 0.f;
+        st.vref = vnew;
+        st.vinv = vnew > 0.f ? 1.0f / vnew : 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float mx = fmaxf(s[n][e], s[n][2 + e]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                mx = fmaxf(st.m[n][e], mx);
+                const float c = mx == -INFINITY ? 1.f : ex2(st.m[n][e] - mx);
+                st.m[n][e] = mx;
+                st.l[n][e] *= c;
+#pragma unroll
+                for (int i = 0; i < 2 * VW; i++) { st.o[n][i][e] *= c * cv; st.o[n][i][2 + e] *= c * cv; }
+            }
+    }
+    const float f = x.vs * st.vinv * kWeightUnit;
+    uint32_t b[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w[e] = ex2(s[n][e] - st.m[n][e & 1]);
+            st.l[n][e & 1] += w[e];
+        }
+        const __half2 h0 = __floats2half2_rn(w[0] * f, w[1] * f), h1 = __floats2half2_rn(w[2] * f, w[3] * f);
+        b[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
+        b[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
+    }
+#pragma unroll
+    for (int i = 0; i < VW; i++) {
+        uint32_t a[4], c[4];                           // dimensions 4 i, 4 i + 1 of the lane's piece, then 4 i + 2, 4 i + 3
+        unpack8<I8>(__byte_perm(x.v[0][i], x.v[1][i], 0x5140), a[0], a[1]);
+        unpack8<I8>(__byte_perm(x.v[2][i], x.v[3][i], 0x5140), a[2], a[3]);
+        unpack8<I8>(__byte_perm(x.v[0][i], x.v[1][i], 0x7362), c[0], c[1]);
+        unpack8<I8>(__byte_perm(x.v[2][i], x.v[3][i], 0x7362), c[2], c[3]);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            mma_f16(st.o[n][2 * i], a, b[n][0], b[n][1]);
+            mma_f16(st.o[n][2 * i + 1], c, b[n][0], b[n][1]);
+        }
+    }
+}
+
+// grid = (splits, kv_heads * passes, rows), clusters of `splits`. A pass is 8 NT query heads. append: the row's key and value enter the cache here
+// (one pass then), otherwise they are in it.
+template <bool I8, int KC, int VW, int NT>
+__global__ void __launch_bounds__(A1_THREADS)
+attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int ld, const int* __restrict__ row_pos, const int* __restrict__ row_slot, int append,
+                      __nv_bfloat16* __restrict__ out, int out_ld) {
+    constexpr int HN = 8 * NT, DK = 64 * KC, DV = 32 * VW, PER = DK > DV ? DK / 32 : DV / 32;
+    extern __shared__ __align__(16) uint8_t sm[];
+    const int dk = a.dim_ld, dv = a.vdim_ld;
+    __half* q_s = reinterpret_cast<__half*>(sm);                             // [HN][DK]
+    uint8_t* tail_k = sm + HN * DK * 2;                                      // [16][DK], [16][DV]: the row's own group
+    uint8_t* tail_v = tail_k + kScaleTokens * DK;
+    float* fresh = reinterpret_cast<float*>(tail_v + kScaleTokens * DV);     // [DK], [DV]: the row's own key and value
+    float* w_acc = reinterpret_cast<float*>(sm);                             // [A1_WARPS][HN][DV] at the end, over all of the above
+    __shared__ float w_m[A1_WARPS][HN], w_l[A1_WARPS][HN], c_m[HN], c_l[HN], q_unit[HN], tail_scale[2];
+    __shared__ float2 red[A1_WARPS];
+    dep_trigger();
+    dep_wait();
+    const int splits = gridDim.x, rank = blockIdx.x, group = a.heads / a.kv_heads, passes = gridDim.y / a.kv_heads, kh = blockIdx.y / passes, pass = blockIdx.y % passes, r = blockIdx.z;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int h0 = kh * group + pass * HN, nh = min(HN, group - pass * HN);
+    const float* row = qkv + (size_t)r * ld;
+    const int p = row_pos[r], qw = a.heads * a.dim, kw = a.kv_heads * a.dim, shift = __ffs(a.block_size) - 1;
+    const int* table = a.block_table + (size_t)row_slot[r] * a.table_ld;
+    const int kstride = a.kv_heads * dk, vstride = a.kv_heads * dv;
+    // the groups in sight, numbered from 0: those of the kept tokens, then those from k_lo on (one run where they meet)
+    const int k_lo = first_key8(a, p), keep = a.keep, tail = p / kScaleTokens;
+    int near = k_lo / kScaleTokens, kept = (min(keep, k_lo) + kScaleTokens - 1) / kScaleTokens;
+    if (kept >= near) { near = 0; kept = 0; }
+    const int groups = kept + tail - near + (append ? 0 : 1), step = splits * A1_WARPS;
+    auto first_of = [&](int i) { return kScaleTokens * (i < kept ? i : near + i - kept); };
+    auto page_of = [&](int i) { return i < groups ? table[first_of(i) >> shift] : 0; };
+    Codes<KC, VW> x[2];
+    auto fetch = [&](Codes<KC, VW>& c, int i, int page) {
+        const int key0 = first_of(i);
+        const size_t token = ((size_t)page << shift) + (key0 & (a.block_size - 1)), sc = token / kScaleTokens * a.kv_heads + kh;
+        load_group<true>(c, static_cast<const uint8_t*>(a.k_pool) + (token * a.kv_heads + kh) * dk, static_cast<const uint8_t*>(a.v_pool) + (token * a.kv_heads + kh) * dv, kstride, vstride, dk, dv,
+                         p - key0, lane);
+        c.ks = a.k_scale[sc];
+        c.vs = a.v_scale[sc];
+    };
+    int i = rank * A1_WARPS + warp, page = page_of(i);
+    if (i < groups) fetch(x[0], i, page);              // under way while the queries are made
+    page = page_of(i + step);
+
+    // ---- the row's queries, and on rank 0 its key and value
+    const size_t own = ((size_t)table[p >> shift] << shift) + (p & (a.block_size - 1)), own_group = own / kScaleTokens * a.kv_heads + kh;
+    const int off = p & (kScaleTokens - 1);
+    const bool joins = append && rank == 0;
+    uint8_t* kd = static_cast<uint8_t*>(a.k_pool) + ((own - off) * a.kv_heads + kh) * dk;
+    uint8_t* vd = static_cast<uint8_t*>(a.v_pool) + ((own - off) * a.kv_heads + kh) * dv;
+    constexpr int OLD = (kScaleTokens * (DK + DV) / 16 + A1_THREADS - 1) / A1_THREADS;
+    uint4 old[OLD];                                    // piece threadIdx.x + A1_THREADS j of the group: token i / pieces, piece i % pieces
+    const int kc = dk >> 4, pieces = kc + (dv >> 4);
+    float was_k = 0.f, was_v = 0.f;
+    if (joins && off) {
+        was_k = a.k_scale[own_group];
+        was_v = a.v_scale[own_group];
+#pragma unroll
+        for (int j = 0; j < OLD; j++) {
+            const int e = threadIdx.x + A1_THREADS * j, tok = e / pieces, c = e - tok * pieces;
+            if (tok < off) old[j] = *reinterpret_cast<const uint4*>(c < kc ? kd + (size_t)tok * kstride + 16 * c : vd + (size_t)tok * vstride + 16 * (c - kc));
+        }
+    }
+    float iq = 1.0f, ik = 1.0f;
+    if (!a.head_norm && (a.q_norm || a.k_norm)) {
+        const float2 ss = block_sum2(a.q_norm ? square_share(row, qw) : 0.f, a.k_norm && joins ? square_share(row + qw, kw) : 0.f, red);
+        if (a.q_norm) iq = 1.0f / sqrtf(ss.x / (float)qw + a.eps);
+        if (a.k_norm) ik = 1.0f / sqrtf(ss.y / (float)kw + a.eps);
+    }
+    const float temp = a.temp_every > 0.f ? 1.0f + a.temp_coef * logf(floorf((float)(p + 1) / a.temp_every) + 1.0f) : 1.0f;
+    // what a warp does with one head: entries lane + 32 j of v, normed and turned
+    auto prepare = [&](float (&y)[PER], const float* v, int n, const float* norm, float inv, bool head_norm, bool turns) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) { const int d = lane + 32 * j; y[j] = d < n ? v[d] : 0.f; }
+        if (head_norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < PER; j++) ss = fmaf(y[j], y[j], ss);
+            inv = 1.0f / sqrtf(lane_sum(ss) / (float)n + a.eps);
+        }
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int d = lane + 32 * j;
+            y[j] *= inv * (norm && d < n ? norm[d] : 1.0f);
+            if (turns) {
+                const float z = __shfl_xor_sync(0xffffffffu, y[j], 1);
+                if (d < a.rot_dims) {
+                    float c, s;
+                    sincosf((float)p * a.freq[d >> 1], &s, &c);
+                    y[j] = (d & 1) ? y[j] * c + z * s : y[j] * c - z * s;
+                }
+            }
+        }
+    };
+    for (int j = warp; j < HN + (joins ? 2 : 0); j += A1_WARPS) {
+        float y[PER], most = 0.f;
+        if (j < HN) {
+            if (j < nh) {
+                prepare(y, row + (h0 + j) * a.dim, a.dim, a.q_norm ? a.q_norm + (a.head_norm ? 0 : (h0 + j) * a.dim) : nullptr, iq, a.q_norm && a.head_norm, a.freq != nullptr);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; e++) y[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < PER; e++) { y[e] *= temp * a.scale * kLog2e; most = fmaxf(most, fabsf(y[e])); }
+            most = lane_max(most);
+            // a power of two that leaves 1 <= largest < 2 (2^-126 at least, so that its inverse is finite)
+            const float unit = most > 0.f ? __uint_as_float(max(min(__float_as_uint(most) & 0x7F800000u, 0x7E000000u), 0x00800000u)) : 1.0f, inv = 1.0f / unit;
+            if (lane == 0) q_unit[j] = unit;
+#pragma unroll
+            for (int e = 0; e < PER; e++) if (lane + 32 * e < DK) q_s[j * DK + lane + 32 * e] = __float2half_rn(y[e] * inv);
+        } else {
+            const bool key = j == HN;
+            if (key) prepare(y, row + qw + kh * a.dim, a.dim, a.k_norm ? a.k_norm + (a.head_norm ? 0 : kh * a.dim) : nullptr, ik, a.k_norm && a.head_norm, a.freq != nullptr);
+            else prepare(y, row + qw + (a.keys_as_values ? 0 : kw) + kh * a.vdim, a.vdim, nullptr, 1.0f, false, false);
+#pragma unroll
+            for (int e = 0; e < PER; e++) { y[e] = cached8(y[e]); most = fmaxf(most, fabsf(y[e])); }
+            most = lane_max(most);
+            if (lane == 0) tail_scale[key ? 0 : 1] = scale8_for<I8>(most);
+#pragma unroll
+            for (int e = 0; e < PER; e++) if (lane + 32 * e < (key ? DK : DV)) fresh[(key ? 0 : DK) + lane + 32 * e] = y[e];
+        }
+    }
+    __syncthreads();
+    if (joins) {
+        const float sk = fmaxf(tail_scale[0], was_k), sv = fmaxf(tail_scale[1], was_v), rk = off ? was_k / sk : 1.f, rv = off ? was_v / sv : 1.f, ik8 = 1.0f / sk, iv8 = 1.0f / sv;
+#pragma unroll
+        for (int j = 0; j < OLD; j++) {
+            const int e = threadIdx.x + A1_THREADS * j, tok = e / pieces, c = e - tok * pieces;
+            if (tok >= kScaleTokens) break;
+            const bool key = c < kc;
+            const float ratio = key ? rk : rv;
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (tok < off) {
+                u = old[j];
+                if (ratio != 1.f) { u.x = rescale8<I8>(u.x, ratio); u.y = rescale8<I8>(u.y, ratio); u.z = rescale8<I8>(u.z, ratio); u.w = rescale8<I8>(u.w, ratio); }
+            } else if (tok == off) {
+                const float* f = key ? fresh + 16 * c : fresh + DK + 16 * (c - kc);
+                const float inv = key ? ik8 : iv8;
+                u.x = pack8<I8>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+                u.y = pack8<I8>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+                u.z = pack8<I8>(f[8] * inv, f[9] * inv, f[10] * inv, f[11] * inv);
+                u.w = pack8<I8>(f[12] * inv, f[13] * inv, f[14] * inv, f[15] * inv);
+            }
+            *reinterpret_cast<uint4*>(key ? tail_k + tok * DK + 16 * c : tail_v + tok * DV + 16 * (c - kc)) = u;
+            if (tok == off || (tok < off && ratio != 1.f)) *reinterpret_cast<uint4*>(key ? kd + (size_t)tok * kstride + 16 * c : vd + (size_t)tok * vstride + 16 * (c - kc)) = u;
+        }
+        __syncthreads();                               // (all have read tail_scale)
+        if (threadIdx.x == 0) { a.k_scale[own_group] = sk; a.v_scale[own_group] = sv; tail_scale[0] = sk; tail_scale[1] = sv; }
+        __syncthreads();
+    }
+    uint32_t q[NT][KC][4][2];
+    float qs[NT][2], slope[NT][2];
+    State<VW, NT> st;
+    st.vref = 0.f;
+    st.vinv = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint2 u = *reinterpret_cast<const uint2*>(q_s + (8 * n + g) * DK + 64 * c + 16 * t + 4 * j);
+                q[n][c][j][0] = u.x;
+                q[n][c][j][1] = u.y;
+            }
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int j = 8 * n + 2 * t + e;
+            qs[n][e] = q_unit[j];
+            slope[n][e] = a.slopes && j < nh ? a.slopes[h0 + j] * kLog2e : 0.f;
+            st.m[n][e] = -INFINITY;
+            st.l[n][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 2 * VW; k++) { st.o[n][k][e] = 0.f; st.o[n][k][2 + e] = 0.f; }
+        }
+    }
+    // ---- the cached groups
+    while (i < groups) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            if (i >= groups) break;
+            const int next = i + step;
+            if (next < groups) {
+                fetch(x[b ^ 1], next, page);
+                page = page_of(next + step);
+            }
+            take_group<I8, KC, VW, NT>(st, x[b], q, qs, slope, first_of(i), p, k_lo, keep, lane);
+            i = next;
+        }
+    }
+    if (joins && warp == 0) {
+        load_group<false>(x[0], tail_k, tail_v, DK, DV, dk, dv, off, lane);
+        x[0].ks = tail_scale[0];
+        x[0].vs = tail_scale[1];
+        take_group<I8, KC, VW, NT>(st, x[0], q, qs, slope, tail * kScaleTokens, p, k_lo, keep, lane);
+    }
+    // ---- merge the warps, then the CTAs of the cluster
+    __syncthreads();                                   // queries and tail are done with
+    const float unit = st.vref / kWeightUnit;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float l = st.l[n][e];
+            l += __shfl_xor_sync(0xffffffffu, l, 4);
+            l += __shfl_xor_sync(0xffffffffu, l, 8);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const int j = 8 * n + 2 * t + e;
+            if (g == 0) { w_m[warp][j] = st.m[n][e]; w_l[warp][j] = l; }
+            float* d = w_acc + (warp * HN + j) * DV;
+#pragma unroll
+            for (int w = 0; w < VW; w++) {
+                const int at = VW == 2 ? 8 * g + 4 * w : 128 * (w / 4) + 16 * g + 4 * (w % 4);
+                *reinterpret_cast<float4*>(d + at) = make_float4(st.o[n][2 * w][e] * unit, st.o[n][2 * w][2 + e] * unit, st.o[n][2 * w + 1][e] * unit, st.o[n][2 * w + 1][2 + e] * unit);
+            }
+        }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nh * DV; e += A1_THREADS) {
+        const int j = e / DV;
+        float mx = w_m[0][j];
+#pragma unroll
+        for (int w = 1; w < A1_WARPS; w++) mx = fmaxf(mx, w_m[w][j]);
+        float v = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < A1_WARPS; w++) {
+            const float mw = w_m[w][j], c = mw == -INFINITY ? 0.f : exp2f(mw - mx);
+            v = fmaf(w_acc[w * HN * DV + e], c, v);
+            sum = fmaf(w_l[w][j], c, sum);
+        }
+        w_acc[e] = v;                                  // element e of warp 0's part is read and written by this thread alone
+        if (e - j * DV == 0) { c_m[j] = mx; c_l[j] = sum; }
+    }
+    if (splits > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
+    for (int e = rank * A1_THREADS + threadIdx.x; e < nh * DV; e += splits * A1_THREADS) {
+        const int j = e / DV, d = e - j * DV;
+        float v, sum, mx;
+        if (splits > 1) {
+            float ms[A1_SPLITS], ls[A1_SPLITS], vs[A1_SPLITS];
+#pragma unroll
+            for (int s = 0; s < A1_SPLITS; s++) {
+                ms[s] = -INFINITY; ls[s] = 0.f; vs[s] = 0.f;
+                if (s < splits) {
+                    ms[s] = cluster_load(cluster_addr(c_m + j, s));
+                    ls[s] = cluster_load(cluster_addr(c_l + j, s));
+                    vs[s] = cluster_load(cluster_addr(w_acc + e, s));
+                }
+            }
+            mx = ms[0];
+#pragma unroll
+            for (int s = 1; s < A1_SPLITS; s++) mx = fmaxf(mx, ms[s]);
+            v = 0.f; sum = 0.f;
+#pragma unroll
+            for (int s = 0; s < A1_SPLITS; s++) {
+                const float c = ms[s] == -INFINITY ? 0.f : exp2f(ms[s] - mx);
+                v = fmaf(vs[s], c, v);
+                sum = fmaf(ls[s], c, sum);
+            }
+        } else {
+            v = w_acc[e]; sum = c_l[j]; mx = c_m[j];
+        }
+        if (a.sink) {                                  // it carries no value
+            const float sk = (a.sinks ? a.sinks[h0 + j] : 0.f) * kLog2e, mt = fmaxf(mx, sk), c = exp2f(mx - mt);
+            v *= c;
+            sum = sum * c + exp2f(sk - mt);
+        }
+        v = v / sum * (a.out_scale == 0.f ? 1.f : a.out_scale);
+        if (a.gate_col >= 0) v *= sigmoidf(row[a.gate_col + h0 + j]);
+        if (d < a.vdim) out[(size_t)r * out_ld + (h0 + j) * a.vdim + d] = __float2bfloat16_rn(v);
+    }
+    if (splits > 1) {                                  // nobody leaves while others read its shared memory
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+
+template <bool I8, int KC, int VW, int NT>
+int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int splits, int passes, int append, __nv_bfloat16* d_out, int out_ld,
+               cudaStream_t st) {
+    constexpr size_t HN = 8 * NT, DK = 64 * KC, DV = 32 * VW;
+    constexpr size_t before = HN * DK * 2 + kScaleTokens * (DK + DV) + 4 * (DK + DV), after = 4 * A1_WARPS * HN * DV, smem = before > after ? before : after;
+    static size_t attr[kMaxDevices] = {};
+    auto kern = attention8_one_kernel<I8, KC, VW, NT>;
+    CMLB_CUDA(cmlb_ensure_smem(kern, smem, attr));
+    CMLB_CUDA(launch_chain(kern, dim3(splits, a->kv_heads * passes, rows), dim3(A1_THREADS), smem, splits, st, *a, d_qkv, ld, d_row_pos, d_row_slot, append, d_out, out_ld));
+    return CMLB200_OK;
+}
+
+}  // namespace
+
+int cmlb_attention8_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int max_keys, __nv_bfloat16* d_out, int out_ld,
+                        cudaStream_t st) {
+    const int widest = a->dim_ld > a->vdim_ld ? a->dim_ld : a->vdim_ld;
+    // (heads of 256 with 16 of them in a pass would not fit registers: their keys are read twice)
+    const int group = a->heads / a->kv_heads, nt = group <= 8 || widest > 128 ? 1 : 2, passes = (group + 8 * nt - 1) / (8 * nt), append = passes == 1;
+    CMLB_REQUIRE((long long)a->kv_heads * passes <= 65535, "cmlb200_attention_one: too many heads");
+    if (!append) {                                     // several passes read the row's own group: it is written by a launch of its own
+        const int rc = cmlb_cache8_append(a, const_cast<float*>(d_qkv), ld, d_row_pos, d_row_slot, 0, rows, true, false, st);
+        if (rc) return rc;
+    }
+    const int reach = a->chunk > 0 ? a->chunk : a->window;
+    const int keys = (reach > 0 && reach < max_keys - a->keep) ? reach + a->keep : max_keys;
+    const long long base = (long long)rows * a->kv_heads * passes;
+    int splits = 1;
+    while (splits < A1_SPLITS && base * splits < 3 * cmlb_num_sms() && keys > splits * A1_WARPS * kScaleTokens) splits *= 2;
+#define A1_ARGS a, d_qkv, ld, d_row_pos, d_row_slot, rows, splits, passes, append, d_out, out_ld, st
+#define A1_HEADS(I8, KC, VW) return nt == 1 ? launch_one<I8, KC, VW, 1>(A1_ARGS) : launch_one<I8, KC, VW, 2>(A1_ARGS)
+#define A1_SIZES(I8)                            \
+    do {                                         \
+        if (widest <= 64) A1_HEADS(I8, 1, 2);    \
+        if (widest <= 128) A1_HEADS(I8, 2, 4);   \
+        return launch_one<I8, 4, 8, 1>(A1_ARGS); \
+    } while (0)
+    if (a->cache_dtype == CMLB200_DT_I8) A1_SIZES(true);
+    A1_SIZES(false);
+#undef A1_SIZES
+#undef A1_HEADS
+#undef A1_ARGS
+}

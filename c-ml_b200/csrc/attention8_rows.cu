@@ -119,13 +119,6 @@ int launch(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_p
 
 }  // namespace
 
-int cmlb_attention8_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int max_keys, __nv_bfloat16* d_out, int out_ld,
-                        cudaStream_t st) {
-    (void)max_keys;
-    const int rc = cmlb_cache8_append(a, const_cast<float*>(d_qkv), ld, d_row_pos, d_row_slot, 0, rows, true, false, st);
-    return rc ? rc : launch(a, d_qkv, ld, d_row_pos, d_row_slot, rows, nullptr, 1, d_out, out_ld, st);
-}
-
 int cmlb_attention8_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_tiles, int tiles, __nv_bfloat16* d_out, int out_ld, cudaStream_t st) {
     return launch(a, d_qkv, ld, nullptr, nullptr, tiles * 64, d_tiles, 0, d_out, out_ld, st);
 }
