@@ -546,6 +546,7 @@ for _n in ("cmlb200_latent_query", "cmlb200_latent_query_f32"):
 _sig("cmlb200_attention_latent", ci, _LAT, vp, ci, vp, vp, ci, ci, vp, ci, vp, vp)
 _sig("cmlb200_set_attention_latent_form", ci, ci)
 _sig("cmlb200_attention_latent_tc_fits", ci, _LAT)
+_sig("cmlb200_attention8_status", ci, C.POINTER(ci), ci)
 _sig("cmlb200_attention_latent_status", ci, C.POINTER(ci), ci)
 for _n in ("cmlb200_latent_output", "cmlb200_latent_output_f32"):
     _sig(_n, ci, _LAT, vp, vp, vp, ci, ci, vp, ci, vp)

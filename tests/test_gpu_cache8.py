@@ -340,3 +340,19 @@ def test_streams_and_graphs(pkg, torch_dev):
             assert (np.abs(got[s] - o.reshape(-1)) <= co.bound(o, w, reach, np.abs(hv).max()).reshape(-1)).all()
         pos += 1
     L.check_cache()
+
+
+@pytest.mark.parametrize("form,dim,what", [("i8", 128, {}), ("e4m3", 64, dict(slopes=True, sink="own", window=300)), ("i8", 64, dict(window=200, keep=150)), ("e4m3", 128, dict(chunk=256, gate="head"))])
+def test_portions_of_many_tiles(pkg, torch_dev, form, dim, what):
+    """Enough tiles for two blocks of rows a CTA."""
+    L = Layer(pkg, torch_dev, form, 32, 8, dim, dim, slots=2, tokens=1500, **what)
+    L.step([(0, 1290), (1, 77)])
+    L.step([(0, 60), (1, 1210)])
+    L.check_cache()
+
+
+def test_bounded_waits_did_not_expire(pkg, torch_dev):
+    import ctypes
+    st = ctypes.c_int(-1)
+    pkg.check(pkg.lib.cmlb200_attention8_status(ctypes.byref(st), 0))
+    assert st.value == 0
