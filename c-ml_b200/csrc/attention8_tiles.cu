@@ -15,7 +15,6 @@
 // Keys behind a portion's last row are read as that row's (their weights are zero), so nothing other requests left can reach the sums. Every wait is
 // bounded; one that gives up leaves a code in a status word in host memory, the products under way are waited for and tensor memory is freed.
 #include "cache8.cuh"
-#include <type_traits>
 #include "tcgen05_util.cuh"
 
 namespace {
@@ -27,10 +26,21 @@ __device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
     if (a.chunk > 0) return p / a.chunk * a.chunk;
     return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
 }
+// Products whose descriptors differ from one another in their lower halves alone.
+__device__ __forceinline__ void umma_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accum) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n"
+                 ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accum) : "memory");
+}
 // A from tensor memory: 128 rows of 16 fp16 numbers in 8 columns
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accum) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n"
+                 ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accum) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
@@ -39,13 +49,63 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 
 // Shared memory of a CTA: queries, key stages, value stages, then the small things.
+// two numbers at a time
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// nothing that reads the registers moves ahead of this
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[4][32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int j = 0; j < 32; j++) asm volatile("" : "+r"(r[c][j]));
+}
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 struct T8Plan {
     int stages;                                        // of keys and of values
     int splits;
 };
 template <int NM, int SK, int SV>
 struct T8 {
-    static constexpr int kThreads = 32 * (4 * NM + 5);
+    static constexpr int kThreads = 32 * (4 * NM + 8), kSoft = 128 * NM;
+    // registers of a thread: 128 and 168 at launch, then shared out (176 x 256 + 104 x 128 + 56 x 128 = 128 x 512; 232 + 168 + 56 < 3 x 168)
+    static constexpr int kSoftRegs = NM == 2 ? 176 : 232, kConvRegs = NM == 2 ? 104 : 168, kIssueRegs = 56;
     static constexpr int kQ = NM * SK * T8_ROWS * 128, kK = SK * T8_SLAB, kV = SV * T8_SLAB;
     static constexpr int kCols = NM * 128 + NM * SV * 64;                     // tensor memory
     static constexpr int kTmem = kCols <= 256 ? 256 : 512;
@@ -72,8 +132,9 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     auto p_full = [&](int m) { return bars + 80 + 8 * m; };
     auto o_full = [&](int m) { return bars + 96 + 8 * m; };
     const uint32_t drained = bars + 112;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(small + 128);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(small + 136);
+    auto p_more = [&](int m) { return bars + 120 + 8 * m; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(small + 144);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(small + 152);
     float* scales = reinterpret_cast<float*>(small + 256);                    // [4 stages][2][T8_GROUPS]: key scales, log2 of value scales (tile i in i & 3)
     float* unit_s = reinterpret_cast<float*>(small + 2048);                   // [NM * 128] powers of two of the queries; then maxima and sums
     float* c_m = unit_s + NM * T8_ROWS;
@@ -83,7 +144,7 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) { mbar_init(k_full(s), 4); mbar_init(k_empty(s), 1); mbar_init(v_full(s), 4); mbar_init(v_empty(s), 1); }
-        for (int m = 0; m < 2; m++) { mbar_init(s_full(m), 1); mbar_init(p_full(m), 4); mbar_init(o_full(m), 1); }
+        for (int m = 0; m < 2; m++) { mbar_init(s_full(m), 1); mbar_init(p_full(m), 4); mbar_init(p_more(m), 4); mbar_init(o_full(m), 1); }
         mbar_init(drained, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -106,27 +167,34 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     // ---- the queries: row 64 h + i of block m is token i of head hb + 2 m + h, over a power of two of its own
     if (count > 0) {
         const float f = a.scale * kLog2e;
-        for (int r = warp; r < NM * T8_ROWS; r += C::kThreads / 32) {
-            const int i = r & 63, h = hb + (r >> 6);
-            const bool live = i < n && h < group;
-            const float* src = qkv + (size_t)(tl.x + (live ? i : 0)) * ld + (size_t)(kh * group + (live ? h : 0)) * a.dim;
-            float2 x[SK];
-            float most = 0.f;
+        constexpr int kAhead = 16 / SK, kWarps = C::kThreads / 32;            // rows whose loads are under way together
+        for (int r0 = warp; r0 < NM * T8_ROWS; r0 += kAhead * kWarps) {
+            float2 x[kAhead][SK];
 #pragma unroll
-            for (int s = 0; s < SK; s++) {
-                const int d = 64 * s + 2 * lane;
-                x[s].x = live && d < a.dim ? src[d] * f : 0.f;
-                x[s].y = live && d + 1 < a.dim ? src[d + 1] * f : 0.f;
-                most = fmaxf(most, fmaxf(fabsf(x[s].x), fabsf(x[s].y)));
+            for (int b = 0; b < kAhead; b++) {
+                const int r = r0 + b * kWarps, i = r & 63, h = hb + (r >> 6);
+                const bool live = r < NM * T8_ROWS && i < n && h < group;
+                const float* src = qkv + (size_t)(tl.x + (live ? i : 0)) * ld + (size_t)(kh * group + (live ? h : 0)) * a.dim;
+#pragma unroll
+                for (int s = 0; s < SK; s++) {
+                    const int d = 64 * s + 2 * lane;
+                    x[b][s].x = live && d < a.dim ? src[d] : 0.f;
+                    x[b][s].y = live && d + 1 < a.dim ? src[d + 1] : 0.f;
+                }
             }
-            most = lane_max(most);
-            const float unit = most > 0.f ? __uint_as_float(max(min(__float_as_uint(most) & 0x7F800000u, 0x7E000000u), 0x00800000u)) : 1.0f, inv = 1.0f / unit;
-            if (lane == 0) unit_s[r] = unit;
-            uint8_t* dst = smem + (r >> 7) * (SK * T8_ROWS * 128) + (r & 127) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
 #pragma unroll
-            for (int s = 0; s < SK; s++) {
-                const __half2 v = __floats2half2_rn(x[s].x * inv, x[s].y * inv);
-                *reinterpret_cast<__half2*>(dst + s * (T8_ROWS * 128)) = v;
+            for (int b = 0; b < kAhead; b++) {
+                const int r = r0 + b * kWarps;
+                if (r >= NM * T8_ROWS) break;
+                float most = 0.f;
+#pragma unroll
+                for (int s = 0; s < SK; s++) { x[b][s].x *= f; x[b][s].y *= f; most = fmaxf(most, fmaxf(fabsf(x[b][s].x), fabsf(x[b][s].y))); }
+                most = lane_max(most);
+                const float unit = most > 0.f ? __uint_as_float(max(min(__float_as_uint(most) & 0x7F800000u, 0x7E000000u), 0x00800000u)) : 1.0f, inv = 1.0f / unit;
+                if (lane == 0) unit_s[r] = unit;
+                uint8_t* dst = smem + (r >> 7) * (SK * T8_ROWS * 128) + (r & 127) * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+#pragma unroll
+                for (int s = 0; s < SK; s++) *reinterpret_cast<__half2*>(dst + s * (T8_ROWS * 128)) = __floats2half2_rn(x[b][s].x * inv, x[b][s].y * inv);
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -138,10 +206,12 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     dep_trigger();                                     // a launch that allocates tensor memory too may start from here on: every CTA of this one has its own
 
     if (warp < kConv) {                                // ---- softmax
+        more_registers<C::kSoftRegs>();
         const int m = warp >> 2, r = (warp & 3) * 32 + lane, i_tok = r & 63, h = hb + 2 * m + (r >> 6);
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + m * 128, o_at = lanes + NM * 128 + m * (SV * 64);
         const bool live = i_tok < n && h < group;
-        const int p = live ? p0 + i_tok : -1, lo = first_key8(a, max(p, 0)), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
+        // (rows that are none have queries of zero and see what the last one sees; nobody looks at theirs)
+        const int p = live ? p0 + i_tok : p_last, lo = first_key8(a, p), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
         const float unit = unit_s[m * T8_ROWS + r], slope = SLOPES && live ? a.slopes[head] * kLog2e : 0.f;
         float mx_ref = -INFINITY, l = 0.f, vref = -INFINITY;
         bool ok = true;
@@ -150,45 +220,38 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
             ok = __all_sync(0xffffffffu, mbar_wait(s_full(m), i & 1, abort_flag, 1, status));
             if (!ok) break;
             tmem_fence_after();
+            uint32_t v[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32_begin(s_at + 32 * c, v[c]);
             const float* sc = scales + (i & 3) * 2 * T8_GROUPS;
-            // unless every row of the CTA sees every key of the tile
-            const bool edge = n < 64 || h >= group || kt + T8_KEYS - 1 > p0 || (kt < lo_last && kt + T8_KEYS > a.keep);
-            const float far = SLOPES ? slope * (float)(kt - p) : 0.f;        // the part of the bias that all keys share
-            auto seen = [&](int j) { const int key = kt + j; return key <= p && (key >= lo || key < a.keep); };
-            float mx = -INFINITY, vm = vref;
-            if (__any_sync(0xffffffffu, edge)) {
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    uint32_t v[32];
-                    tmem_ld32(s_at + 32 * c, v);
-                    const float f0 = unit * sc[2 * c], f1 = unit * sc[2 * c + 1];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        float s = __uint_as_float(v[j]) * (j < 16 ? f0 : f1);
-                        if (SLOPES) s = fmaf(slope, (float)(32 * c + j), s);
-                        if (seen(32 * c + j)) mx = fmaxf(mx, s);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t v[32];
-                    tmem_ld32(s_at + 32 * c, v);
-                    const float f0 = unit * sc[2 * c], f1 = unit * sc[2 * c + 1];
-                    if (SLOPES) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) mx = fmaxf(mx, fmaf(__uint_as_float(v[j]), j < 16 ? f0 : f1, slope * (float)(32 * c + j)));
-                    } else {
-                        float g0 = __uint_as_float(v[0]), g1 = __uint_as_float(v[16]);
-#pragma unroll
-                        for (int j = 1; j < 16; j++) { g0 = fmaxf(g0, __uint_as_float(v[j])); g1 = fmaxf(g1, __uint_as_float(v[16 + j])); }
-                        mx = fmaxf(mx, fmaxf(g0 * f0, g1 * f1));
-                    }
-                }
-            }
-            mx += far;
+            float vm = vref;
 #pragma unroll
             for (int g = 0; g < T8_GROUPS; g++) vm = fmaxf(vm, sc[T8_GROUPS + g]);
+            const float far = SLOPES ? slope * (float)(kt - p) : 0.f;        // the part of the bias that all keys share
+            // (a scale times a query's power of two that underflows would make NaN of a masked score)
+            auto factor = [&](int g) { return fmaxf(unit * sc[g], 1.17549435e-38f); };
+            tmem_ld_wait(v);
+            // unless every row of the CTA sees every key of the tile
+            if (kt + T8_KEYS - 1 > p0 || (kt < lo_last && kt + T8_KEYS > a.keep)) {
+                const int last = p - kt, begin = lo - kt, kept = a.keep - kt;
+#pragma unroll
+                for (int j = 0; j < T8_KEYS; j++) {
+                    const bool hidden = (j > last) | ((j < begin) & (j >= kept));
+                    v[j >> 5][j & 31] = hidden ? 0xff800000u : v[j >> 5][j & 31];
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < T8_GROUPS; g++) {
+                const float f = factor(g);
+                auto x = [&](int j) { const float y = __uint_as_float(v[g >> 1][16 * (g & 1) + j]); return SLOPES ? fmaf(y, f, slope * (float)(16 * g + j)) : y; };
+                float t0 = x(0), t1 = x(1);
+#pragma unroll
+                for (int j = 2; j < 14; j += 4) { t0 = max3(t0, x(j), x(j + 1)); t1 = max3(t1, x(j + 2), x(j + 3)); }
+                t0 = fmaxf(max3(t0, x(14), x(15)), t1);
+                mx = fmaxf(mx, SLOPES ? t0 : t0 * f);
+            }
+            mx += far;
             if (__any_sync(0xffffffffu, mx > mx_ref + kLazy || vm > vref)) {
                 const float nm = fmaxf(mx_ref, mx), c = nm == -INFINITY ? 1.f : ex2(mx_ref - nm), cv = ex2(vref - vm);
                 mx_ref = nm;
@@ -196,53 +259,50 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
                 l *= c;
                 if (i > 0) {
 #pragma unroll 1
-                    for (int c0 = 0; c0 < dv; c0 += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + c0, o);
+                    for (int c0 = 0; c0 < dv; c0 += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_at + c0, o);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * (c * cv));
-                        tmem_st32(o_at + c0, o);
+                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * (c * cv));
+                        tmem_st16(o_at + c0, o);
                     }
                 }
             }
             const float u = (mx_ref == -INFINITY ? 0.f : mx_ref) - far;
-            // weights of columns 32 c .. 32 c + 31
-            auto weigh = [&](int c, auto masked) {
-                uint32_t v[32], w[16];
-                tmem_ld32(s_at + 32 * c, v);
-                const float f0 = unit * sc[2 * c], f1 = unit * sc[2 * c + 1];
-                const float r0 = fmaxf(sc[T8_GROUPS + 2 * c] - vref, kFarScale) + kWeightBits, r1 = fmaxf(sc[T8_GROUPS + 2 * c + 1] - vref, kFarScale) + kWeightBits;
-                const float b0 = r0 - u, b1 = r1 - u;
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    float s = fmaf(__uint_as_float(v[j]), j < 16 ? f0 : f1, j < 16 ? b0 : b1);
-                    if (SLOPES) s = fmaf(slope, (float)(32 * c + j), s);
-                    if (decltype(masked)::value && !seen(32 * c + j)) s = -INFINITY;
-                    v[j] = __float_as_uint(ex2(s));
+            for (int c = 0; c < 4; c++) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int g = 2 * c + e;
+                    const float f = factor(g), bits = fmaxf(sc[T8_GROUPS + g] - vref, kFarScale) + kWeightBits, b = bits - u;
+                    const uint64_t ff = pair_of(f, f), bb = pair_of(b, b), sl = pair_of(slope, slope);
+                    uint64_t sum = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int k = 16 * e + 2 * j;
+                        uint64_t y = fma_pair(pair_of(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1])), ff, bb);
+                        if (SLOPES) y = fma_pair(sl, pair_of((float)(32 * c + k), (float)(32 * c + k + 1)), y);
+                        float e0, e1;
+                        unpair(y, e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
+                        sum = add_pair(sum, pair_of(e0, e1));
+                        const __half2 x = __floats2half2_rn(e0, e1);
+                        w[8 * e + j] = *reinterpret_cast<const uint32_t*>(&x);
+                    }
+                    float t0, t1;
+                    unpair(sum, t0, t1);
+                    l = fmaf(t0 + t1, ex2(-bits), l);
                 }
-                float t0 = 0.f, t1 = 0.f, t2 = 0.f, t3 = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float e0 = __uint_as_float(v[2 * j]), e1 = __uint_as_float(v[2 * j + 1]), e2 = __uint_as_float(v[16 + 2 * j]), e3 = __uint_as_float(v[17 + 2 * j]);
-                    t0 += e0; t1 += e1; t2 += e2; t3 += e3;
-                    const __half2 a0 = __floats2half2_rn(e0, e1), a1 = __floats2half2_rn(e2, e3);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&a0);
-                    w[8 + j] = *reinterpret_cast<const uint32_t*>(&a1);
+                tmem_st16(s_at + 16 * c, w);           // over the scores, which are all in registers
+                if (c & 1) {                           // half of the tile's keys: their product may begin
+                    tmem_st_wait();
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c == 1 ? p_full(m) : p_more(m));
                 }
-                l = fmaf(t0 + t1, ex2(-r0), fmaf(t2 + t3, ex2(-r1), l));
-                tmem_st16(s_at + 16 * c, w);           // over scores that have been read
-            };
-            if (__any_sync(0xffffffffu, edge)) {
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) weigh(c, std::true_type());
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; c++) weigh(c, std::false_type());
             }
-            tmem_st_wait();
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(m));
         }
         if (ok && count > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_full(m), 0, abort_flag, 2, status));
         tmem_fence_after();
@@ -296,7 +356,56 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
             }
         }
         tmem_fence_before();
+        __syncwarp();
+        if (splits > 1) {
+            cluster_meet();
+            const int quads = dv / 4, width = dv + 4;
+            for (int e = rank * C::kSoft + threadIdx.x; e < NM * T8_ROWS * quads; e += splits * C::kSoft) {
+                const int r = e / quads, c = (e - r * quads) * 4, i = r & 63, h = hb + (r >> 6);
+                if (i >= n || h >= group) continue;
+                float ms[T8_SPLITS], ls[T8_SPLITS], mx = -INFINITY;
+    #pragma unroll
+                for (int s = 0; s < T8_SPLITS; s++) {
+                    ms[s] = -INFINITY;
+                    ls[s] = 0.f;
+                    if (s < splits) {
+                        uint32_t am, al;
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(am) : "r"(smem_addr(c_m + r)), "r"(s));
+                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(al) : "r"(smem_addr(c_l + r)), "r"(s));
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[s]) : "r"(am) : "memory");
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ls[s]) : "r"(al) : "memory");
+                    }
+                    mx = fmaxf(mx, ms[s]);
+                }
+                const int head = kh * group + h;
+                float sum = 0.f;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll
+                for (int s = 0; s < T8_SPLITS; s++) {
+                    if (s >= splits || ms[s] == -INFINITY) continue;             // saw nothing: its values may be anything
+                    uint32_t ax;
+                    float4 y;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ax) : "r"(smem_addr(reinterpret_cast<float*>(smem) + (size_t)r * width + c)), "r"(s));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(ax) : "memory");
+                    const float f = exp2f(ms[s] - mx);
+                    sum = fmaf(ls[s], f, sum);
+                    x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+                }
+                if (a.sink && sum > 0.f) sum += exp2f((a.sinks ? a.sinks[head] : 0.f) * kLog2e - mx);
+                float inv = sum > 0.f ? (a.out_scale == 0.f ? 1.f : a.out_scale) / sum : 0.f;
+                const float* row = qkv + (size_t)(tl.x + i) * ld;
+                if (a.gate_col >= 0 && !a.gate_wide) inv *= sigmoidf(row[a.gate_col + head]);
+                const float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+                __nv_bfloat16* dst = out + (size_t)(tl.x + i) * out_ld + (size_t)head * a.vdim;
+    #pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (c + j < a.vdim) dst[c + j] = __float2bfloat16_rn(a.gate_wide ? v[j] * sigmoidf(row[a.gate_col + head * a.vdim + c + j]) : v[j]);
+            }
+            __syncwarp();
+            cluster_meet();                            // nobody leaves while others read its shared memory
+        }
     } else if (warp < kIssue) {                        // ---- expansion
+        if (NM == 2) fewer_registers<C::kConvRegs>();
         const int tid = threadIdx.x - kConv * 32, w4 = warp - kConv;
         // A slab's 512 pieces of 16 codes: four neighbouring lanes take a key's 64 dimensions, so 64 bytes lie together in a request, and eight lanes' stores,
         // of an even key and the odd one behind it, meet all banks. Piece j of a thread: slab j / 4, key tid / 4 + 32 (j % 4); a batch is kept in registers.
@@ -380,113 +489,77 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
             at = next;
             if (++st == stages) { st = 0; par ^= 1; }
         }
-    } else if (count > 0) {                            // ---- products
-        // fp16 operands, fp32 accumulators, 128 rows; the second one takes V with its columns contiguous
-        const uint32_t is = (1u << 4) | ((uint32_t)(T8_KEYS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(dv >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const int steps = dk >> 4;
-        bool ok = true;
-        auto scores = [&](int m, int st) {
-            if (elect_one()) {
-                const uint64_t ad = make_desc(qs + m * (SK * T8_ROWS * 128)), bd = make_desc(ks + st * C::kK);
-#pragma unroll
-                for (int k = 0; k < 4 * SK; k++)
-                    if (k < steps) umma(tm + m * 128, ad + (uint64_t)((k >> 2) * (T8_ROWS * 128 >> 4) + 2 * (k & 3)), bd + (uint64_t)((k >> 2) * (T8_SLAB >> 4) + 2 * (k & 3)), is, k ? 1u : 0u);
-                if (m == NM - 1) umma_commit(k_empty(st));
-                umma_commit(s_full(m));
-            }
-            __syncwarp();
-        };
-        int kst = 0, kpar = 0, vst = 0, vpar = 0;
-        auto keys = [&]() {
-            const bool got = __all_sync(0xffffffffu, mbar_wait(k_full(kst), kpar, abort_flag, 6, status));
-            tmem_fence_after();
-            return got;
-        };
-        ok = keys();
-        if (ok)
-            for (int m = 0; m < NM; m++) scores(m, kst);
-        if (++kst == stages) { kst = 0; kpar ^= 1; }
-        for (int i = 0; i < count && ok; i++) {
-            ok = __all_sync(0xffffffffu, mbar_wait(v_full(vst), vpar, abort_flag, 7, status));
-            if (!ok) break;
-            for (int m = 0; m < NM && ok; m++) {
-                ok = __all_sync(0xffffffffu, mbar_wait(p_full(m), i & 1, abort_flag, 8, status));
-                if (!ok) break;
-                tmem_fence_after();
+        __syncwarp();
+        if (splits > 1) { cluster_meet(); cluster_meet(); }
+    } else {                                           // ---- products
+        fewer_registers<C::kIssueRegs>();
+        if (warp == kIssue && count > 0) {
+            // fp16 operands, fp32 accumulators, 128 rows; the second one takes V with its columns contiguous
+            const uint32_t is = (1u << 4) | ((uint32_t)(T8_KEYS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(dv >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const int steps = dk >> 4;
+            bool ok = true;
+            auto scores = [&](int m, int st) {
                 if (elect_one()) {
-                    const uint64_t vd = make_desc_mn(vs + vst * C::kV, T8_SLAB);
+                    const uint64_t ad = make_desc(qs + m * (SK * T8_ROWS * 128)), bd = make_desc(ks + st * C::kK);
+                    const uint32_t alo = (uint32_t)ad, blo = (uint32_t)bd, hi = (uint32_t)(ad >> 32);
 #pragma unroll
-                    for (int k = 0; k < T8_KEYS / 16; k++)
-                        umma_ts(tm + NM * 128 + m * (SV * 64), tm + m * 128 + 8 * k, vd + (uint64_t)(k * (2048 >> 4)), io, (i | k) ? 1u : 0u);
-                    if (m == NM - 1) umma_commit(v_empty(vst));
-                    if (i + 1 == count) umma_commit(o_full(m));
+                    for (int k = 0; k < 4 * SK; k++)
+                        if (k < steps) umma_lo(tm + m * 128, alo + (k >> 2) * (T8_ROWS * 128 >> 4) + 2 * (k & 3), blo + (k >> 2) * (T8_SLAB >> 4) + 2 * (k & 3), hi, is, k ? 1u : 0u);
+                    if (m == NM - 1) umma_commit(k_empty(st));
+                    umma_commit(s_full(m));
                 }
                 __syncwarp();
-                if (i + 1 < count) {
-                    if (m == 0) ok = keys();
-                    if (ok) scores(m, kst);
-                }
-            }
-            if (++vst == stages) { vst = 0; vpar ^= 1; }
+            };
+            int kst = 0, kpar = 0, vst = 0, vpar = 0;
+            auto keys = [&]() {
+                const bool got = __all_sync(0xffffffffu, mbar_wait(k_full(kst), kpar, abort_flag, 6, status));
+                tmem_fence_after();
+                return got;
+            };
+            ok = keys();
+            if (ok)
+                for (int m = 0; m < NM; m++) scores(m, kst);
             if (++kst == stages) { kst = 0; kpar ^= 1; }
+            for (int i = 0; i < count && ok; i++) {
+                ok = __all_sync(0xffffffffu, mbar_wait(v_full(vst), vpar, abort_flag, 7, status));
+                if (!ok) break;
+                for (int m = 0; m < NM && ok; m++) {
+                    const uint64_t vd = make_desc_mn(vs + vst * C::kV, T8_SLAB);
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        ok = ok && __all_sync(0xffffffffu, mbar_wait(half ? p_more(m) : p_full(m), i & 1, abort_flag, 8, status));
+                        if (!ok) break;
+                        tmem_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 4 * half; k < 4 * half + 4; k++)
+                                umma_ts(tm + NM * 128 + m * (SV * 64), tm + m * 128 + 8 * k, (uint32_t)vd + k * (2048 >> 4), (uint32_t)(vd >> 32), io, (i | k) ? 1u : 0u);
+                            if (half && m == NM - 1) umma_commit(v_empty(vst));
+                            if (half && i + 1 == count) umma_commit(o_full(m));
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                    if (i + 1 < count) {
+                        if (m == 0) ok = keys();
+                        if (ok) scores(m, kst);
+                    }
+                }
+                if (++vst == stages) { vst = 0; vpar ^= 1; }
+                if (++kst == stages) { kst = 0; kpar ^= 1; }
+            }
+            // nothing that was issued outlives the CTA's tensor memory
+            if (elect_one()) umma_commit(drained);
+            __syncwarp();
+            for (uint32_t it = 0; it < SPIN_LIMIT && !mbar_try(drained, 0); it++) {}
+            __syncwarp();
         }
-        // nothing that was issued outlives the CTA's tensor memory
-        if (elect_one()) umma_commit(drained);
         __syncwarp();
-        for (uint32_t it = 0; it < SPIN_LIMIT && !mbar_try(drained, 0); it++) {}
-        __syncwarp();
+        if (splits > 1) { cluster_meet(); cluster_meet(); }
     }
     __syncthreads();
-    if (splits > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        const int quads = dv / 4, width = dv + 4;
-        for (int e = rank * C::kThreads + threadIdx.x; e < NM * T8_ROWS * quads; e += splits * C::kThreads) {
-            const int r = e / quads, c = (e - r * quads) * 4, i = r & 63, h = hb + (r >> 6);
-            if (i >= n || h >= group) continue;
-            float ms[T8_SPLITS], ls[T8_SPLITS], mx = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < T8_SPLITS; s++) {
-                ms[s] = -INFINITY;
-                ls[s] = 0.f;
-                if (s < splits) {
-                    uint32_t am, al;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(am) : "r"(smem_addr(c_m + r)), "r"(s));
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(al) : "r"(smem_addr(c_l + r)), "r"(s));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[s]) : "r"(am) : "memory");
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ls[s]) : "r"(al) : "memory");
-                }
-                mx = fmaxf(mx, ms[s]);
-            }
-            const int head = kh * group + h;
-            float sum = 0.f;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int s = 0; s < T8_SPLITS; s++) {
-                if (s >= splits || ms[s] == -INFINITY) continue;             // saw nothing: its values may be anything
-                uint32_t ax;
-                float4 y;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ax) : "r"(smem_addr(reinterpret_cast<float*>(smem) + (size_t)r * width + c)), "r"(s));
-                asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(ax) : "memory");
-                const float f = exp2f(ms[s] - mx);
-                sum = fmaf(ls[s], f, sum);
-                x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
-            }
-            if (a.sink && sum > 0.f) sum += exp2f((a.sinks ? a.sinks[head] : 0.f) * kLog2e - mx);
-            float inv = sum > 0.f ? (a.out_scale == 0.f ? 1.f : a.out_scale) / sum : 0.f;
-            const float* row = qkv + (size_t)(tl.x + i) * ld;
-            if (a.gate_col >= 0 && !a.gate_wide) inv *= sigmoidf(row[a.gate_col + head]);
-            const float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-            __nv_bfloat16* dst = out + (size_t)(tl.x + i) * out_ld + (size_t)head * a.vdim;
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (c + j < a.vdim) dst[c + j] = __float2bfloat16_rn(a.gate_wide ? v[j] * sigmoidf(row[a.gate_col + head * a.vdim + c + j]) : v[j]);
-        }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // nobody leaves while others read its shared memory
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
     if (warp == kIssue) {
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::kTmem) : "memory");
