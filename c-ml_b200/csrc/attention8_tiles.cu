@@ -52,7 +52,7 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     const uint32_t pv_done = bars + 96, drained = bars + 104;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(small + 128);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(small + 136);
-    float* scales = reinterpret_cast<float*>(small + 256);                    // [4][2][T8_GROUPS]: key scales, log2 of value scales (tile i in i & 3)
+    float* scales = reinterpret_cast<float*>(small + 256);                    // [4][T8_SCALES] (tile i in i & 3)
     float* unit_s = reinterpret_cast<float*>(small + 1024);                   // [128] powers of two of the queries
     float* meet = unit_s + T8_ROWS;                                           // [2][2][128] the two halves' largest scores, at the end sums
     float* c_m = meet + 4 * T8_ROWS;                                          // [T8_SPLITS][128] maxima and sums of the whole cluster
@@ -107,16 +107,18 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
             ok = ok && __all_sync(0xffffffffu, mbar_wait(s_full(buf), (i >> 1) & 1, abort_flag, 1, status));
             uint32_t v[2][32];
             float mx = -INFINITY, vm = vref;
-            const float* sc = scales + (i & 3) * 2 * T8_GROUPS;
+            const float* sc = scales + (i & 3) * T8_SCALES + 4 * half;
             const float far = SLOPES ? slope * (float)(kt - p) : 0.f;        // the part of the bias that all of its keys share
-            // (a scale times a query's power of two that underflows would make NaN of a masked score)
-            auto factor = [&](int g) { return fmaxf(unit * sc[4 * half + g], 1.17549435e-38f); };
+            float f[4], lv[4];                         // factors of its four groups' scores, log2 of their value scales
             if (ok) {
                 tmem_fence_after();
 #pragma unroll
                 for (int c = 0; c < 2; c++) tmem_ld32_begin(s_at + 64 * half + 32 * c, v[c]);
-#pragma unroll
-                for (int g = 0; g < T8_GROUPS; g++) vm = fmaxf(vm, sc[T8_GROUPS + g]);
+                const float4 s4 = *reinterpret_cast<const float4*>(sc), l4 = *reinterpret_cast<const float4*>(sc + T8_GROUPS);
+                vm = fmaxf(vm, sc[2 * T8_GROUPS - 4 * half]);
+                // (a scale times a query's power of two that underflows would make NaN of a masked score)
+                f[0] = fmaxf(unit * s4.x, 1.17549435e-38f); f[1] = fmaxf(unit * s4.y, 1.17549435e-38f); f[2] = fmaxf(unit * s4.z, 1.17549435e-38f); f[3] = fmaxf(unit * s4.w, 1.17549435e-38f);
+                lv[0] = l4.x; lv[1] = l4.y; lv[2] = l4.z; lv[3] = l4.w;
                 tmem_ld_wait(v);
                 // unless every row of the CTA sees every one of these keys
                 if (kt + 63 > p0 || (kt < lo_last && kt + 64 > a.keep)) {
@@ -128,7 +130,7 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
                     }
                 }
 #pragma unroll
-                for (int g = 0; g < 4; g++) mx = fmaxf(mx, t8_group_max<SLOPES>(v[g >> 1], g & 1, factor(g), slope, 16 * g));
+                for (int g = 0; g < 4; g++) mx = fmaxf(mx, t8_group_max<SLOPES>(v[g >> 1], g & 1, f[g], slope, 16 * g));
                 mx += far;
                 meet[(2 * buf + half) * T8_ROWS + r] = mx;
             }
@@ -157,8 +159,8 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int g = 2 * c + e;
-                    const float bits = fmaxf(sc[T8_GROUPS + 4 * half + g] - vref, kFarScale) + kWeightBits;
-                    l = fmaf(t8_group_weights<SLOPES>(v[c], w, e, factor(g), bits - u, slope, 16 * g), ex2(-bits), l);
+                    const float bits = fmaxf(lv[g] - vref, kFarScale) + kWeightBits;
+                    l = fmaf(t8_group_weights<SLOPES>(v[c], w, e, f[g], bits - u, slope, 16 * g), ex2(-bits), l);
                 }
                 tmem_st16(s_at + 32 * half + 16 * c, w);                      // over scores that both halves have in registers
             }
@@ -254,18 +256,15 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
         if (warp < kIssue) {                           // ---- expansion
             fewer_registers<T8_CONV_REGS>();
             const bool key = warp < kConv + C::kConv;
-            T8Team<I8, S> team;
+            T8Team<I8, S, S == 1 ? 4 : 8> team;
             team.init(key ? a.k_pool : a.v_pool, kh, a.kv_heads, key ? dk : dv, key ? ks : vs, threadIdx.x - (key ? kConv : kConv + C::kConv) * 32);
             const int stage_bytes = key ? C::kK : C::kV;
             bool ok = true;
             int st = 0, par = 1, next = 0, tok[4] = {0, 0, 0, 0};
-            // the first warp of the keys' team looks after the scales: lanes 0 .. 7 a group's key scale, 8 .. 15 its value scale
-            float scale = 0.f;
-            const bool scaler = warp == kConv && lane < 2 * T8_GROUPS;
-            auto scale_at = [&](int token) { return scaler ? (lane < T8_GROUPS ? a.k_scale : a.v_scale)[(size_t)token / kScaleTokens * a.kv_heads + kh] : 0.f; };
+            T8Scaler scaler = {warp == kConv && lane < 2 * T8_GROUPS, lane, kh, 0.f};
             if (count > 0) {
                 const int at = t8_place(a, table, shift, keys, 0, lane);
-                scale = scale_at(at);
+                scaler.fetch(a, at);
                 t8_tokens(tok, at, keys.start(0), p_last, team.g0, team.in_group);
                 team.load(tok, 0);
                 if (count > 1) next = t8_place(a, table, shift, keys, 1, lane);
@@ -274,11 +273,11 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
                 ok = __all_sync(0xffffffffu, mbar_wait(key ? k_empty(st) : v_empty(st), par, abort_flag, key ? 4 : 5, status));
                 if (!ok) break;
                 // (the scores of tile i - 2, which are done, were issued once the softmax of tile i - 4 was)
-                if (scaler) scales[(i & 3) * 2 * T8_GROUPS + lane] = lane < T8_GROUPS ? scale : log2f(fmaxf(scale, 1.17549435e-38f));
+                scaler.put(scales, i);
                 team.store_tile(tok, st * stage_bytes);
                 if (lane == 0) mbar_arrive(key ? k_full(st) : v_full(st));
                 if (i + 1 < count) {
-                    scale = scale_at(next);
+                    scaler.fetch(a, next);
                     t8_tokens(tok, next, keys.start(i + 1), p_last, team.g0, team.in_group);
                     team.load(tok, 0);
                     if (i + 2 < count) next = t8_place(a, table, shift, keys, i + 2, lane);

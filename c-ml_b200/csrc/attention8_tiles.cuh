@@ -144,9 +144,9 @@ __device__ __forceinline__ void t8_queries(const cmlb200_attn& a, const float* _
 // A slab's 512 pieces of 16 codes: four neighbouring lanes take a key's 64 dimensions, so 64 bytes lie together in a request, and eight lanes' stores,
 // of an even key and the odd one behind it, meet all banks. Piece j of a thread: slab j / 4, key tid / 4 + 32 (j % 4), whose group is
 // tid / 64 + 2 (j % 4); a batch is kept in registers.
-template <bool I8, int S>
+template <bool I8, int S, int BATCH>
 struct T8Team {
-    static constexpr int BATCH = S == 1 ? 4 : 8, BATCHES = 4 * S / BATCH;
+    static constexpr int BATCHES = 4 * S / BATCH;
     const uint8_t* base;
     int stride, width, c16, in_group, g0;
     uint32_t to, even;
@@ -195,6 +195,26 @@ struct T8Team {
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
+    }
+};
+// A tile's scales as the softmax finds them: 8 key scales, log2 of 8 value scales, the largest of those; four tiles in turn.
+constexpr int T8_SCALES = 20;
+struct T8Scaler {
+    bool on;                                           // lanes 0 .. 7 of one warp look after key scales, 8 .. 15 after value scales
+    int lane, kh;
+    float scale;
+    __device__ __forceinline__ void fetch(const cmlb200_attn& a, int token) {
+        if (on) scale = (lane < T8_GROUPS ? a.k_scale : a.v_scale)[(size_t)token / kScaleTokens * a.kv_heads + kh];
+    }
+    __device__ __forceinline__ void put(float* scales, int i) const {
+        if (!on) return;
+        const float v = lane < T8_GROUPS ? scale : log2f(fmaxf(scale, 1.17549435e-38f));
+        float m = v;
+#pragma unroll
+        for (int o = 1; o < T8_GROUPS; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFu, m, o));
+        float* s = scales + (i & 3) * T8_SCALES;
+        s[lane] = v;
+        if (lane == T8_GROUPS) s[2 * T8_GROUPS] = m;
     }
 };
 // Where group `lane & 7` of tile i begins in the pools; groups behind the last row's are read as that one.

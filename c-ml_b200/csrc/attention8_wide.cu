@@ -1,23 +1,23 @@
 // Prompt portions over 8-bit caches where there are tiles enough for all SMs: as attention8_tiles.cu, but a CTA takes four query heads of a key/value head, two
 // blocks of 128 rows that share the expansion of the codes. A key tile of a block costs the tensor cores 1,024 cycles and its exponentials as many of the
-// special function units, so the two have to overlap: while one block's softmax runs, the other's products do.
-//   0 .. 7    softmax, a thread a row, warps 0 .. 3 the first block's; a thread holds its 128 scores and hands the weights over in two halves
-//   8 .. 11   expansion of a tile's keys, then of its values (the next tile's keys are requested ahead of this one's values, and the other way round)
-//   12        issues tcgen05.mma, block by block: P V of a tile, then the scores of the next over them. Products are done in order, so that a block's scores being
-//             there means that its O is at rest too
-// Tensor memory: 128 columns of scores a block, then the blocks' O.
+// special function units, so products and softmax have to overlap: a block has two accumulators of scores, 64 keys each, and while the weights of one half tile
+// are made, the scores of the next and the other block's products are.
+//   0 .. 7    softmax, a thread a row, warps 0 .. 3 the first block's
+//   8 .. 15   expansion, four warps for keys and four for values (the next tile's codes are requested once this one's are written)
+//   16, 17    issue tcgen05.mma, a block each: the scores of half tile j + 1, then P V of half tile j
+// Tensor memory: a block's 2 x 64 columns of scores, over which its weights lie, then the blocks' O.
 #include "attention8_tiles.cuh"
 
 namespace {
 
-// S: slabs of 64 dimensions of keys and values. Registers: 128 a thread at launch, then 176 x 256 + 104 x 128 + 56 x 128 = 128 x 512.
+// S: slabs of 64 dimensions of keys and values. Registers: 96 a thread at launch, then 128 x 256 + 80 x 256 + 64 x 128 = 96 x 640.
 template <int S>
 struct W8 {
-    static constexpr int kSoft = 8, kConv = 4, kThreads = 32 * (kSoft + kConv + 4), kRows = 2 * T8_ROWS;
+    static constexpr int kSoft = 8, kConv = 4, kThreads = 32 * (kSoft + 2 * kConv + 4), kRows = 2 * T8_ROWS;
     static constexpr int kQ = 2 * S * T8_ROWS * 128, kK = S * T8_SLAB, kV = S * T8_SLAB, kStages = 2;
     static constexpr int kSmall = 1024 + 4 * kRows, kBytes = 1024 + kQ + kStages * (kK + kV) + kSmall;
 };
-constexpr int W8_TMEM = 512, W8_O_COL = 256, W8_SOFT_REGS = 176, W8_CONV_REGS = 104, W8_ISSUE_REGS = 56;
+constexpr int W8_TMEM = 512, W8_O_COL = 256, W8_SOFT_REGS = 128, W8_CONV_REGS = 80, W8_ISSUE_REGS = 64;
 
 // grid = (kv_heads * blocks, tiles); a block is four query heads.
 template <bool I8, int S, bool SLOPES>
@@ -33,22 +33,22 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
     auto k_empty = [&](int s) { return bars + 16 + 8 * s; };
     auto v_full = [&](int s) { return bars + 32 + 8 * s; };
     auto v_empty = [&](int s) { return bars + 48 + 8 * s; };
-    auto s_full = [&](int m) { return bars + 64 + 8 * m; };
-    auto p_full = [&](int m, int half) { return bars + 80 + 16 * m + 8 * half; };
-    const uint32_t drained = bars + 112;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(small + 128);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(small + 136);
-    float* scales = reinterpret_cast<float*>(small + 256);                    // [4][2][T8_GROUPS]: key scales, log2 of value scales (tile i in i & 3)
+    auto s_full = [&](int m, int half) { return bars + 64 + 16 * m + 8 * half; };
+    auto p_full = [&](int m, int half) { return bars + 96 + 16 * m + 8 * half; };
+    auto pv_done = [&](int m) { return bars + 128 + 8 * m; };
+    auto drained = [&](int m) { return bars + 144 + 8 * m; };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(small + 192);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(small + 200);
+    float* scales = reinterpret_cast<float*>(small + 256);                    // [4][T8_SCALES] (tile i in i & 3)
     float* unit_s = reinterpret_cast<float*>(small + 1024);                   // [256] powers of two of the queries
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kConv = C::kSoft, kIssue = C::kSoft + C::kConv;
+    constexpr int kConv = C::kSoft, kIssue = C::kSoft + 2 * C::kConv;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(k_full(s), C::kConv); mbar_init(k_empty(s), 1); mbar_init(v_full(s), C::kConv); mbar_init(v_empty(s), 1);
-            mbar_init(s_full(s), 1); mbar_init(p_full(s, 0), 4); mbar_init(p_full(s, 1), 4);
+            mbar_init(k_full(s), C::kConv); mbar_init(k_empty(s), 2); mbar_init(v_full(s), C::kConv); mbar_init(v_empty(s), 2);
+            mbar_init(s_full(s, 0), 1); mbar_init(s_full(s, 1), 1); mbar_init(p_full(s, 0), 4); mbar_init(p_full(s, 1), 4); mbar_init(pv_done(s), 1); mbar_init(drained(s), 1);
         }
-        mbar_init(drained, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -62,7 +62,8 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
     const int n = tl.y, p0 = tl.w, p_last = p0 + n - 1, shift = __ffs(a.block_size) - 1;
     const int* table = a.block_table + (size_t)tl.z * a.table_ld;
     const T8Keys keys(a, p0, p_last, 0, 1);
-    const int count = keys.count;
+    // half tiles; the last one is left out where it lies behind the last row
+    const int count = keys.count, halves = 2 * count - (keys.start(count - 1) + 64 > p_last ? 1 : 0);
     t8_queries<S, C::kRows, C::kThreads / 32>(a, qkv, ld, tl, n, kh, hb, group, smem, unit_s);
     tmem_fence_before();
     __syncthreads();
@@ -73,68 +74,74 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
     if (warp < kConv) {                                // ---- softmax
         more_registers<W8_SOFT_REGS>();
         const int m = warp >> 2, r = (warp & 3) * 32 + lane, i_tok = r & 63, h = hb + 2 * m + (r >> 6);
-        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lanes + m * T8_KEYS, o_at = lanes + W8_O_COL + m * (S * 64);
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + W8_O_COL + m * (S * 64);
         const bool live = i_tok < n && h < group;
         // (rows that are none have queries of zero and see what the last one sees; nobody looks at theirs)
         const int p = live ? p0 + i_tok : p_last, lo = first_key8(a, p), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
         const float unit = unit_s[m * T8_ROWS + r], slope = SLOPES && live ? a.slopes[head] * kLog2e : 0.f;
         float ref = -INFINITY, l = 0.f, vref = -INFINITY;
         bool ok = true;
-        for (int i = 0; i < count; i++) {
-            const int kt = keys.start(i);
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full(m), i & 1, abort_flag, 1, status));
+        for (int j = 0; j < halves; j++) {
+            const int half = j & 1, kt = keys.start(j >> 1) + 64 * half;    // the first key
+            const uint32_t s_at = lanes + m * T8_KEYS + 64 * half;
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full(m, half), (j >> 1) & 1, abort_flag, 1, status));
             if (!ok) break;
             tmem_fence_after();
-            uint32_t v[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; c++) tmem_ld32_begin(s_at + 32 * c, v[c]);
-            const float* sc = scales + (i & 3) * 2 * T8_GROUPS;
-            float vm = vref, mx = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < T8_GROUPS; g++) vm = fmaxf(vm, sc[T8_GROUPS + g]);
-            const float far = SLOPES ? slope * (float)(kt - p) : 0.f;        // the part of the bias that all keys share
+            uint32_t v[2][32];
+            tmem_ld32_begin(s_at, v[0]);
+            tmem_ld32_begin(s_at + 32, v[1]);
+            const float* sc = scales + ((j >> 1) & 3) * T8_SCALES + 4 * half;
+            const float4 s4 = *reinterpret_cast<const float4*>(sc), l4 = *reinterpret_cast<const float4*>(sc + T8_GROUPS);
+            const float vm = fmaxf(vref, sc[2 * T8_GROUPS - 4 * half]);
             // (a scale times a query's power of two that underflows would make NaN of a masked score)
-            auto factor = [&](int g) { return fmaxf(unit * sc[g], 1.17549435e-38f); };
+            const float f[4] = {fmaxf(unit * s4.x, 1.17549435e-38f), fmaxf(unit * s4.y, 1.17549435e-38f), fmaxf(unit * s4.z, 1.17549435e-38f), fmaxf(unit * s4.w, 1.17549435e-38f)};
+            const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+            const float far = SLOPES ? slope * (float)(kt - p) : 0.f;        // the part of the bias that all keys share
             tmem_ld_wait(v);
-            // unless every row of the CTA sees every key of the tile
-            if (kt + T8_KEYS - 1 > p0 || (kt < lo_last && kt + T8_KEYS > a.keep)) {
+            // unless every row of the CTA sees every one of these keys
+            if (kt + 63 > p0 || (kt < lo_last && kt + 64 > a.keep)) {
                 const int last = p - kt, begin = lo - kt, kept = a.keep - kt;
 #pragma unroll
-                for (int j = 0; j < T8_KEYS; j++) {
-                    const bool hidden = (j > last) | ((j < begin) & (j >= kept));
-                    v[j >> 5][j & 31] = hidden ? 0xff800000u : v[j >> 5][j & 31];
+                for (int k = 0; k < 64; k++) {
+                    const bool hidden = (k > last) | ((k < begin) & (k >= kept));
+                    v[k >> 5][k & 31] = hidden ? 0xff800000u : v[k >> 5][k & 31];
                 }
             }
+            float mx = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < T8_GROUPS; g++) mx = fmaxf(mx, t8_group_max<SLOPES>(v[g >> 1], g & 1, factor(g), slope, 16 * g));
+            for (int g = 0; g < 4; g++) mx = fmaxf(mx, t8_group_max<SLOPES>(v[g >> 1], g & 1, f[g], slope, 16 * g));
             mx += far;
             if (__any_sync(0xffffffffu, mx > ref + kLazy || vm > vref)) {
                 const float nm = fmaxf(ref, mx), c = nm == -INFINITY ? 1.f : ex2(ref - nm), cv = ex2(vref - vm);
                 ref = nm;
                 vref = vm;
                 l *= c;
-                if (i > 0) t8_scale_o(o_at, 0, 16, dv, c * cv);
+                if (j > 0) {
+                    // (these scores were issued behind P V of half tile j - 2, so that one is done)
+                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done(m), (j - 1) & 1, abort_flag, 3, status));
+                    if (!ok) break;
+                    tmem_fence_after();
+                    t8_scale_o(o_at, 0, 16, dv, c * cv);
+                }
             }
             const float u = (ref == -INFINITY ? 0.f : ref) - far;
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
+            for (int c = 0; c < 2; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int g = 2 * c + e;
-                    const float bits = fmaxf(sc[T8_GROUPS + g] - vref, kFarScale) + kWeightBits;
-                    l = fmaf(t8_group_weights<SLOPES>(v[c], w, e, factor(g), bits - u, slope, 16 * g), ex2(-bits), l);
+                    const float bits = fmaxf(lv[g] - vref, kFarScale) + kWeightBits;
+                    l = fmaf(t8_group_weights<SLOPES>(v[c], w, e, f[g], bits - u, slope, 16 * g), ex2(-bits), l);
                 }
                 tmem_st16(s_at + 16 * c, w);           // over the scores, which are all in registers
-                if (c & 1) {                           // half of the tile's keys: their product may begin
-                    tmem_st_wait();
-                    tmem_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full(m, c >> 1));
-                }
             }
+            tmem_st_wait();
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(m, half));
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(drained, 0, abort_flag, 2, status));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(drained(m), 0, abort_flag, 2, status));
         tmem_fence_after();
         const float* row = qkv + (size_t)(tl.x + (live ? i_tok : 0)) * ld;
         if (a.sink && l > 0.f) l += ex2((a.sinks ? a.sinks[head] : 0.f) * kLog2e - ref);
@@ -144,96 +151,81 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
         tmem_fence_before();
     } else if (warp < kIssue) {                        // ---- expansion
         fewer_registers<W8_CONV_REGS>();
-        const int tid = threadIdx.x - kConv * 32;
-        T8Team<I8, S> k, v;
-        k.init(a.k_pool, kh, a.kv_heads, dk, ks, tid);
-        v.init(a.v_pool, kh, a.kv_heads, dv, vs, tid);
-        // its first warp looks after the scales: lanes 0 .. 7 a group's key scale, 8 .. 15 its value scale
-        const bool scaler = warp == kConv && lane < 2 * T8_GROUPS;
-        auto scale_at = [&](int token) { return scaler ? (lane < T8_GROUPS ? a.k_scale : a.v_scale)[(size_t)token / kScaleTokens * a.kv_heads + kh] : 0.f; };
+        const bool key = warp < kConv + C::kConv;
+        T8Team<I8, S, S == 1 ? 4 : 8> team;
+        team.init(key ? a.k_pool : a.v_pool, kh, a.kv_heads, key ? dk : dv, key ? ks : vs, threadIdx.x - (key ? kConv : kConv + C::kConv) * 32);
+        const int stage_bytes = key ? C::kK : C::kV;
+        T8Scaler scaler = {warp == kConv && lane < 2 * T8_GROUPS, lane, kh, 0.f};
         bool ok = true;
         int next = 0, tok[4];
         const int at = t8_place(a, table, shift, keys, 0, lane);
-        float scale = scale_at(at);
-        t8_tokens(tok, at, keys.start(0), p_last, k.g0, k.in_group);
-        k.load(tok, 0);
-        v.load(tok, 0);
+        scaler.fetch(a, at);
+        t8_tokens(tok, at, keys.start(0), p_last, team.g0, team.in_group);
+        team.load(tok, 0);
         if (count > 1) next = t8_place(a, table, shift, keys, 1, lane);
         for (int i = 0; i < count; i++) {
-            const int st = i & 1, par = ((i >> 1) & 1) ^ 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(k_empty(st), par, abort_flag, 4, status));
+            const int st = i & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(key ? k_empty(st) : v_empty(st), ((i >> 1) & 1) ^ 1, abort_flag, key ? 4 : 5, status));
             if (!ok) break;
-            // (the scores of tile i - 2, which are done, were issued once the softmax of tile i - 3 was)
-            if (scaler) scales[(i & 3) * 2 * T8_GROUPS + lane] = lane < T8_GROUPS ? scale : log2f(fmaxf(scale, 1.17549435e-38f));
-            k.store_tile(tok, st * C::kK);
-            if (lane == 0) mbar_arrive(k_full(st));
+            // (the scores of tile i - 2, which are done, were issued once the softmax of tile i - 4 was)
+            scaler.put(scales, i);
+            team.store_tile(tok, st * stage_bytes);
+            if (lane == 0) mbar_arrive(key ? k_full(st) : v_full(st));
             if (i + 1 < count) {
-                scale = scale_at(next);
-                t8_tokens(tok, next, keys.start(i + 1), p_last, k.g0, k.in_group);
-                k.load(tok, 0);
+                scaler.fetch(a, next);
+                t8_tokens(tok, next, keys.start(i + 1), p_last, team.g0, team.in_group);
+                team.load(tok, 0);
                 if (i + 2 < count) next = t8_place(a, table, shift, keys, i + 2, lane);
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(v_empty(st), par, abort_flag, 5, status));
-            if (!ok) break;
-            v.store_tile(tok, st * C::kV);             // (one batch: `tok` is the next tile's by now)
-            if (lane == 0) mbar_arrive(v_full(st));
-            if (i + 1 < count) v.load(tok, 0);
         }
         __syncwarp();
     } else {                                           // ---- products
         fewer_registers<W8_ISSUE_REGS>();
-        if (warp == kIssue) {
+        if (warp < kIssue + 2) {
             // fp16 operands, fp32 accumulators, 128 rows; the second one takes V with its columns contiguous
-            const uint32_t is = (1u << 4) | ((uint32_t)(T8_KEYS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            const uint32_t is = (1u << 4) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
             const uint32_t io = (1u << 4) | (1u << 16) | ((uint32_t)(dv >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-            const int steps = dk >> 4;
+            const int m = __shfl_sync(0xffffffffu, warp - kIssue, 0), steps = dk >> 4;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), s_at = tm + m * T8_KEYS, o_at = tm + W8_O_COL + m * (S * 64);
             bool ok = true;
-            auto keys_there = [&](int i) {
-                ok = __all_sync(0xffffffffu, mbar_wait(k_full(i & 1), (i >> 1) & 1, abort_flag, 6, status));
+            auto scores = [&](int j) {
+                const int st = (j >> 1) & 1, half = j & 1;
+                if (!half) ok = __all_sync(0xffffffffu, mbar_wait(k_full(st), (j >> 2) & 1, abort_flag, 6, status));
+                if (!ok) return;
                 tmem_fence_after();
-            };
-            auto scores = [&](int m, int i) {
                 if (elect_one()) {
-                    const uint64_t ad = make_desc(qs + m * (S * T8_ROWS * 128)), bd = make_desc(ks + (i & 1) * C::kK);
-                    const uint32_t alo = (uint32_t)ad, blo = (uint32_t)bd, hi = (uint32_t)(ad >> 32);
+                    const uint64_t ad = make_desc(qs + m * (S * T8_ROWS * 128)), bd = make_desc(ks + st * C::kK + half * (64 * 128));
+                    const uint32_t alo = (uint32_t)ad, blo = (uint32_t)bd, hi = (uint32_t)(ad >> 32), d = s_at + 64 * half;
 #pragma unroll
                     for (int k = 0; k < 4 * S; k++)
-                        if (k < steps) umma_lo(tm + m * T8_KEYS, alo + (k >> 2) * (T8_ROWS * 128 >> 4) + 2 * (k & 3), blo + (k >> 2) * (T8_SLAB >> 4) + 2 * (k & 3), hi, is, k ? 1u : 0u);
-                    if (m == 1) umma_commit(k_empty(i & 1));
-                    umma_commit(s_full(m));
+                        if (k < steps) umma_lo(d, alo + (k >> 2) * (T8_ROWS * 128 >> 4) + 2 * (k & 3), blo + (k >> 2) * (T8_SLAB >> 4) + 2 * (k & 3), hi, is, k ? 1u : 0u);
+                    if (half) umma_commit(k_empty(st));
+                    umma_commit(s_full(m, half));
                 }
                 __syncwarp();
             };
-            keys_there(0);
-            for (int m = 0; m < 2 && ok; m++) scores(m, 0);
-            for (int i = 0; i < count && ok; i++) {
-                ok = __all_sync(0xffffffffu, mbar_wait(v_full(i & 1), (i >> 1) & 1, abort_flag, 7, status));
-                for (int m = 0; m < 2 && ok; m++) {
-                    const uint64_t vd = make_desc_mn(vs + (i & 1) * C::kV, T8_SLAB);
+            scores(0);
+            for (int j = 0; j < halves && ok; j++) {
+                const int st = (j >> 1) & 1, half = j & 1;
+                if (j + 1 < halves) scores(j + 1);     // into the accumulator whose weights' product has been issued
+                if (ok && !half) ok = __all_sync(0xffffffffu, mbar_wait(v_full(st), (j >> 2) & 1, abort_flag, 7, status));
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(p_full(m, half), (j >> 1) & 1, abort_flag, 8, status));
+                if (!ok) break;
+                tmem_fence_after();
+                if (elect_one()) {
+                    const uint64_t vd = make_desc_mn(vs + st * C::kV + half * (64 * 128), T8_SLAB);
 #pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        ok = ok && __all_sync(0xffffffffu, mbar_wait(p_full(m, half), i & 1, abort_flag, 8, status));
-                        if (!ok) break;
-                        tmem_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 4 * half; k < 4 * half + 4; k++)
-                                umma_ts(tm + W8_O_COL + m * (S * 64), tm + m * T8_KEYS + 8 * k, (uint32_t)vd + k * (2048 >> 4), (uint32_t)(vd >> 32), io, (i | k) ? 1u : 0u);
-                            if (half && m == 1) umma_commit(v_empty(i & 1));
-                        }
-                        __syncwarp();
-                    }
-                    if (ok && i + 1 < count) {
-                        if (m == 0) keys_there(i + 1);
-                        if (ok) scores(m, i + 1);
-                    }
+                    for (int k = 0; k < 4; k++)
+                        umma_ts(o_at, s_at + 64 * half + 8 * k, (uint32_t)vd + k * (2048 >> 4), (uint32_t)(vd >> 32), io, (j | k) ? 1u : 0u);
+                    if (half) umma_commit(v_empty(st));
+                    umma_commit(pv_done(m));
                 }
+                __syncwarp();
             }
             // nothing that was issued outlives the CTA's tensor memory
-            if (elect_one()) umma_commit(drained);
+            if (elect_one()) umma_commit(drained(m));
             __syncwarp();
-            for (uint32_t it = 0; it < SPIN_LIMIT && !mbar_try(drained, 0); it++) {}
+            for (uint32_t it = 0; it < SPIN_LIMIT && !mbar_try(drained(m), 0); it++) {}
         }
         __syncwarp();
     }
