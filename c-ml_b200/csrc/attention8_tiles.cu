@@ -367,6 +367,24 @@ int status_word8(int** word) {
     return CMLB200_OK;
 }
 
+// Clusters of k such CTAs that run at a time.
+int t8_clusters(const void* kern, int k, int threads, size_t smem) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)k;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(k);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) return n;
+    cudaGetLastError();
+    return max(1, cmlb_num_sms() / k * 3 / 4);
+}
+
 template <bool I8, int S, bool SLOPES>
 int launch_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_tiles, int tiles, __nv_bfloat16* d_out, int out_ld, int* status, cudaStream_t st) {
     using C = T8<S>;
@@ -374,16 +392,27 @@ int launch_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d
     CMLB_REQUIRE((long long)a->kv_heads * blocks <= 65535 && tiles <= 65535, "cmlb200_attention_tiles: %d tiles, %d heads", tiles, a->heads);
     T8Plan plan;
     for (plan.stages = 2; plan.stages > 1 && C::bytes(plan.stages) > 227 * 1024; plan.stages--) {}
-    // few tiles: a cluster shares the keys of each, as far as SMs and keys go (a block table's row holds no more than table_ld blocks)
-    const long long ctas = (long long)tiles * a->kv_heads * blocks, reach = a->chunk > 0 ? a->chunk + 64 : a->window > 0 ? a->window + 64 : 0;
-    long long keys = (long long)a->table_ld * a->block_size;
-    if (reach && reach + a->keep < keys) keys = reach + a->keep;
-    for (plan.splits = 1; plan.splits < T8_SPLITS && ctas * plan.splits * 2 <= cmlb_num_sms() && keys > plan.splits * T8_KEYS; plan.splits *= 2) {}
     // one CTA to an SM: each needs all of the SM's tensor memory, and a cluster's CTAs wait for one another
     const size_t need = (size_t)C::bytes(plan.stages), smem = need > 118 * 1024 ? need : 118 * 1024;
     static size_t attr[kMaxDevices] = {};
+    static int room[kMaxDevices][T8_SPLITS + 1] = {};
     auto kern = attention8_tiles_kernel<I8, S, SLOPES>;
     CMLB_CUDA(cmlb_ensure_smem(kern, smem, attr));
+    // How many CTAs share the keys of a tile: what takes least by an estimate in units of a key tile's time (1.7 us at heads of 128): 5 for a CTA's beginning and end
+    // and 2 for a merge, times the waves, where clusters of a size share the device with as many as fit its groups of SMs. A block table's row bounds the keys.
+    // (64 rows behind 6,000 tokens, 16 tiles of heads: clusters of 8 run in two waves, 43 us.)
+    const long long ctas = (long long)tiles * a->kv_heads * blocks, reach = a->chunk > 0 ? a->chunk + 64 : a->window > 0 ? a->window + 64 : 0;
+    long long keys = (long long)a->table_ld * a->block_size;
+    if (reach && reach + a->keep < keys) keys = reach + a->keep;
+    const long long key_tiles = (keys + T8_KEYS - 1) / T8_KEYS;
+    long long best = 0;
+    plan.splits = 1;
+    for (int k = 1; k <= T8_SPLITS && (k == 1 || (key_tiles >= k && ctas * k <= cmlb_num_sms())); k++) {
+        int* fit = &room[cmlb_device_index()][k];
+        if (!*fit) *fit = k == 1 ? cmlb_num_sms() : t8_clusters((const void*)kern, k, C::kThreads, smem);
+        const long long waves = (ctas + *fit - 1) / *fit, each = (key_tiles + k - 1) / k, t = waves * (5 + each + (k > 1 ? 2 : 0));
+        if (k == 1 || t < best) { best = t; plan.splits = k; }
+    }
     CMLB_CUDA(launch_chain(kern, dim3(plan.splits, a->kv_heads * blocks, tiles), dim3(C::kThreads), smem, plan.splits, st, *a, d_qkv, ld, (const int4*)d_tiles, d_out, out_ld, plan, status));
     return CMLB200_OK;
 }
