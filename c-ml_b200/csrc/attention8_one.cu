@@ -7,7 +7,9 @@
 //                                        a lane's four consecutive codes are its four columns, and no shuffle or shared memory is needed
 //   O^T [16 dims x 8 heads] += V^T P^T   A: a lane holds the same 8, 16 or 32 dimensions of the keys 2t, 2t + 1, 2t + 8, 2t + 9; bytes of two keys are
 //                                        interleaved, which makes the operand's pairs. P^T comes from S^T by movmatrix
-// so the codes go from global memory to registers to the tensor cores. A lane requests the next group's codes before it uses this one's.
+// so the codes go from global memory to registers to the tensor cores. A lane requests the next group's keys as soon as this one's have gone into the products,
+// and its values likewise: 4 KB a warp under way with 32 registers, and 16 warps an SM. int8 keys stay 1,152 too large, as they come out of their conversion: the
+// scores' accumulators begin at -1,152 times the sum of the head's queries, so every term is exact and the fp32 sums are off by no more than the queries' own rounding.
 // A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
 // where m, the warp's reference for the exponentials, moves only when a score has passed it by 7 (powers of two; sums are fp32). Queries are fp16 over
 // a power of two of their own per head, so their size is no matter.
@@ -52,42 +54,60 @@ __device__ __forceinline__ float cluster_load(uint32_t a) {
 }
 
 // KC: 16-code pieces of a key per lane (64 dimensions each). VW: words of a value per lane (32 dimensions each).
-template <int KC, int VW>
-struct Codes {
-    uint32_t k[2][KC][4];                              // keys g, g + 8
-    uint32_t v[4][VW];                                 // keys 2t, 2t + 1, 2t + 8, 2t + 9
-    float ks, vs;
-};
-// from: a group's first token's codes for this key/value head; `last`: its last token that may be read. GLOBAL: the cache, else shared memory.
-template <bool GLOBAL, int KC, int VW>
-__device__ __forceinline__ void load_group(Codes<KC, VW>& x, const uint8_t* k, const uint8_t* v, int kstride, int vstride, int dk, int dv, int last, int lane) {
+template <int KC> struct KeyCodes { uint32_t w[2][KC][4]; };                // keys g, g + 8
+template <int VW> struct ValueCodes { uint32_t w[4][VW]; };                 // keys 2t, 2t + 1, 2t + 8, 2t + 9
+// Where a lane's pieces lie in a group, from its first token's codes for the key/value head on.
+struct Places { int k[2], v[4]; };
+// `last`: the group's last token that may be read
+__device__ __forceinline__ Places places_of(int kstride, int vstride, int piece, int last, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    auto wide = [](const uint8_t* p) { return GLOBAL ? ld_codes(p) : *reinterpret_cast<const uint4*>(p); };
+    Places p;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const uint8_t* r = k + (size_t)min(g + 8 * i, last) * kstride + 16 * t;
+    for (int i = 0; i < 2; i++) p.k[i] = min(g + 8 * i, last) * kstride + 16 * t;
+#pragma unroll
+    for (int i = 0; i < 4; i++) p.v[i] = min(2 * t + (i & 1) + 8 * (i >> 1), last) * vstride + piece * g;
+    return p;
+}
+// GLOBAL: from the cache, else from shared memory
+template <bool GLOBAL, int KC>
+__device__ __forceinline__ void load_keys(KeyCodes<KC>& x, const uint8_t* k, const Places& p, int dk, int lane) {
+    const int t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (64 * c + 16 * t < dk) u = wide(r + 64 * c);
-            x.k[i][c][0] = u.x; x.k[i][c][1] = u.y; x.k[i][c][2] = u.z; x.k[i][c][3] = u.w;
+            if (64 * c + 16 * t < dk) u = GLOBAL ? ld_codes(k + p.k[i] + 64 * c) : *reinterpret_cast<const uint4*>(k + p.k[i] + 64 * c);
+            x.w[i][c][0] = u.x; x.w[i][c][1] = u.y; x.w[i][c][2] = u.z; x.w[i][c][3] = u.w;
         }
-    }
+}
+template <bool GLOBAL, int VW>
+__device__ __forceinline__ void load_values(ValueCodes<VW>& x, const uint8_t* v, const Places& p, int dv, int lane) {
+    const int g = lane >> 2;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint8_t* r = v + (size_t)min(2 * t + (i & 1) + 8 * (i >> 1), last) * vstride;
         if constexpr (VW == 2) {
             uint2 u = make_uint2(0u, 0u);
-            if (8 * g < dv) u = GLOBAL ? ld_codes8(r + 8 * g) : *reinterpret_cast<const uint2*>(r + 8 * g);
-            x.v[i][0] = u.x; x.v[i][1] = u.y;
+            if (8 * g < dv) u = GLOBAL ? ld_codes8(v + p.v[i]) : *reinterpret_cast<const uint2*>(v + p.v[i]);
+            x.w[i][0] = u.x; x.w[i][1] = u.y;
         } else {
 #pragma unroll
             for (int c = 0; c < VW / 4; c++) {
                 uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (128 * c + 16 * g < dv) u = wide(r + 128 * c + 16 * g);
-                x.v[i][4 * c] = u.x; x.v[i][4 * c + 1] = u.y; x.v[i][4 * c + 2] = u.z; x.v[i][4 * c + 3] = u.w;
+                if (128 * c + 16 * g < dv) u = GLOBAL ? ld_codes(v + p.v[i] + 128 * c) : *reinterpret_cast<const uint4*>(v + p.v[i] + 128 * c);
+                x.w[i][4 * c] = u.x; x.w[i][4 * c + 1] = u.y; x.w[i][4 * c + 2] = u.z; x.w[i][4 * c + 3] = u.w;
             }
         }
+    }
+}
+// A word's codes as the keys' operand: int8 codes 1,152 too large, which the accumulators know.
+template <bool I8> __device__ __forceinline__ void unpack_key(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (I8) {
+        const uint32_t u = w ^ 0x80808080u;
+        lo = __byte_perm(u, 0x64646464u, 0x4140);
+        hi = __byte_perm(u, 0x64646464u, 0x4342);
+    } else {
+        unpack8<false>(w, lo, hi);
     }
 }
 
@@ -98,32 +118,35 @@ struct State {
     float vref, vinv;                                  // largest value scale so far, one over it
 };
 
-// S, the weights and O of a group whose first key is `key0` for the row at position p. qs: per head its queries' power of two.
-template <bool I8, int KC, int VW, int NT>
-__device__ __forceinline__ void take_group(State<VW, NT>& st, const Codes<KC, VW>& x, const uint32_t (&q)[NT][KC][4][2], const float (&qs)[NT][2], const float (&slope)[NT][2], int key0, int p,
-                                           int k_lo, int keep, int lane) {
-    const int g = lane >> 2;
-    float s[NT][4];
+// The products of a group's keys with the queries. from: what a head's accumulators begin with.
+template <bool I8, int KC, int NT>
+__device__ __forceinline__ void key_products(float (&s)[NT][4], const KeyCodes<KC>& x, const uint32_t (&q)[NT][KC][4][2], const float (&from)[NT][2]) {
 #pragma unroll
-    for (int n = 0; n < NT; n++) { s[n][0] = 0.f; s[n][1] = 0.f; s[n][2] = 0.f; s[n][3] = 0.f; }
+    for (int n = 0; n < NT; n++) { s[n][0] = from[n][0]; s[n][1] = from[n][1]; s[n][2] = from[n][0]; s[n][3] = from[n][1]; }
 #pragma unroll
     for (int c = 0; c < KC; c++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             uint32_t a[4];
-            unpack8<I8>(x.k[0][c][j], a[0], a[2]);
-            unpack8<I8>(x.k[1][c][j], a[1], a[3]);
+            unpack_key<I8>(x.w[0][c][j], a[0], a[2]);
+            unpack_key<I8>(x.w[1][c][j], a[1], a[3]);
 #pragma unroll
             for (int n = 0; n < NT; n++) mma_f16(s[n], a, q[n][c][j][0], q[n][c][j][1]);
         }
+}
+// Scores and weights of a group whose first key is `key0`, for the row at position p: b is P^T. qs: per head its queries' power of two; ks, vs: the group's scales.
+template <int VW, int NT>
+__device__ __forceinline__ void make_weights(State<VW, NT>& st, float (&s)[NT][4], uint32_t (&b)[NT][2], float ks, float vs, const float (&qs)[NT][2], const float (&slope)[NT][2], int key0, int p,
+                                             int k_lo, int keep, int lane) {
+    const int g = lane >> 2;
     const float back = (float)(p - key0 - g);
     const bool edge = key0 + kScaleTokens - 1 > p || (key0 < k_lo && key0 + kScaleTokens > keep);
-    bool over = x.vs > st.vref;
+    bool over = vs > st.vref;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const float f = qs[n][e] * x.ks;
+            const float f = qs[n][e] * ks;
             s[n][e] = fmaf(s[n][e], f, -slope[n][e] * back);
             s[n][2 + e] = fmaf(s[n][2 + e], f, -slope[n][e] * (back - 8.f));
         }
@@ -143,7 +166,7 @@ __device__ __forceinline__ void take_group(State<VW, NT>& st, const Codes<KC, VW
 #pragma unroll
         for (int e = 0; e < 2; e++) over |= fmaxf(s[n][e], s[n][2 + e]) > st.m[n][e] + 7.f;
     if (__any_sync(0xffffffffu, over)) {
-        const float vnew = fmaxf(st.vref, x.vs), cv = st.vref > 0.f ? st.vref / vnew : 0.f;
+        const float vnew = fmaxf(st.vref, vs), cv = st.vref > 0.f ? st.vref / vnew : 0.f;
         st.vref = vnew;
         st.vinv = vnew > 0.f ? 1.0f / vnew : 0.f;
 #pragma unroll
@@ -162,8 +185,7 @@ __device__ __forceinline__ void take_group(State<VW, NT>& st, const Codes<KC, VW
                 for (int i = 0; i < 2 * VW; i++) { st.o[n][i][e] *= c * cv; st.o[n][i][2 + e] *= c * cv; }
             }
     }
-    const float f = x.vs * st.vinv * kWeightUnit;
-    uint32_t b[NT][2];
+    const float f = vs * st.vinv * kWeightUnit;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         float w[4];
@@ -176,13 +198,16 @@ __device__ __forceinline__ void take_group(State<VW, NT>& st, const Codes<KC, VW
         b[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
         b[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
     }
+}
+template <bool I8, int VW, int NT>
+__device__ __forceinline__ void value_products(State<VW, NT>& st, const ValueCodes<VW>& x, const uint32_t (&b)[NT][2]) {
 #pragma unroll
     for (int i = 0; i < VW; i++) {
         uint32_t a[4], c[4];                           // dimensions 4 i, 4 i + 1 of the lane's piece, then 4 i + 2, 4 i + 3
-        unpack8<I8>(__byte_perm(x.v[0][i], x.v[1][i], 0x5140), a[0], a[1]);
-        unpack8<I8>(__byte_perm(x.v[2][i], x.v[3][i], 0x5140), a[2], a[3]);
-        unpack8<I8>(__byte_perm(x.v[0][i], x.v[1][i], 0x7362), c[0], c[1]);
-        unpack8<I8>(__byte_perm(x.v[2][i], x.v[3][i], 0x7362), c[2], c[3]);
+        unpack8<I8>(__byte_perm(x.w[0][i], x.w[1][i], 0x5140), a[0], a[1]);
+        unpack8<I8>(__byte_perm(x.w[2][i], x.w[3][i], 0x5140), a[2], a[3]);
+        unpack8<I8>(__byte_perm(x.w[0][i], x.w[1][i], 0x7362), c[0], c[1]);
+        unpack8<I8>(__byte_perm(x.w[2][i], x.w[3][i], 0x7362), c[2], c[3]);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             mma_f16(st.o[n][2 * i], a, b[n][0], b[n][1]);
@@ -194,7 +219,7 @@ __device__ __forceinline__ void take_group(State<VW, NT>& st, const Codes<KC, VW
 // grid = (splits, kv_heads * passes, rows), clusters of `splits`. A pass is 8 NT query heads. append: the row's key and value enter the cache here
 // (one pass then), otherwise they are in it.
 template <bool I8, int KC, int VW, int NT>
-__global__ void __launch_bounds__(A1_THREADS)
+__global__ void __launch_bounds__(A1_THREADS, KC == 4 ? 2 : NT == 2 ? 2 : 4)
 attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int ld, const int* __restrict__ row_pos, const int* __restrict__ row_slot, int append,
                       __nv_bfloat16* __restrict__ out, int out_ld) {
     constexpr int HN = 8 * NT, DK = 64 * KC, DV = 32 * VW, PER = DK > DV ? DK / 32 : DV / 32;
@@ -205,7 +230,7 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     uint8_t* tail_v = tail_k + kScaleTokens * DK;
     float* fresh = reinterpret_cast<float*>(tail_v + kScaleTokens * DV);     // [DK], [DV]: the row's own key and value
     float* w_acc = reinterpret_cast<float*>(sm);                             // [A1_WARPS][HN][DV] at the end, over all of the above
-    __shared__ float w_m[A1_WARPS][HN], w_l[A1_WARPS][HN], c_m[HN], c_l[HN], q_unit[HN], tail_scale[2];
+    __shared__ float w_m[A1_WARPS][HN], w_l[A1_WARPS][HN], c_m[HN], c_l[HN], q_unit[HN], q_sum[HN], tail_scale[2];
     __shared__ float2 red[A1_WARPS];
     dep_trigger();
     dep_wait();
@@ -223,17 +248,33 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     const int groups = kept + tail - near + (append ? 0 : 1), step = splits * A1_WARPS;
     auto first_of = [&](int i) { return kScaleTokens * (i < kept ? i : near + i - kept); };
     auto page_of = [&](int i) { return i < groups ? table[first_of(i) >> shift] : 0; };
-    Codes<KC, VW> x[2];
-    auto fetch = [&](Codes<KC, VW>& c, int i, int page) {
-        const int key0 = first_of(i);
-        const size_t token = ((size_t)page << shift) + (key0 & (a.block_size - 1)), sc = token / kScaleTokens * a.kv_heads + kh;
-        load_group<true>(c, static_cast<const uint8_t*>(a.k_pool) + (token * a.kv_heads + kh) * dk, static_cast<const uint8_t*>(a.v_pool) + (token * a.kv_heads + kh) * dv, kstride, vstride, dk, dv,
-                         p - key0, lane);
-        c.ks = a.k_scale[sc];
-        c.vs = a.v_scale[sc];
+    KeyCodes<KC> xk;
+    ValueCodes<VW> xv;
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + (size_t)kh * dk;
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + (size_t)kh * dv;
+    constexpr int PIECE = VW == 2 ? 8 : 16;
+    const Places whole = places_of(kstride, vstride, PIECE, kScaleTokens - 1, lane);
+    // a group's first token in the pools
+    auto token_of = [&](int i, int page) { return ((size_t)page << shift) + (first_of(i) & (a.block_size - 1)); };
+    // (where the row's key is in the cache already, its group may end with it)
+    auto ends = [&](int i) { return !append && first_of(i) + kScaleTokens - 1 > p; };
+    auto fetch_keys = [&](int i, size_t token) {
+        if (ends(i)) load_keys<true>(xk, kp + token * kstride, places_of(kstride, vstride, PIECE, p - first_of(i), lane), dk, lane);
+        else load_keys<true>(xk, kp + token * kstride, whole, dk, lane);
+    };
+    auto fetch_values = [&](int i, size_t token) {
+        if (ends(i)) load_values<true>(xv, vp + token * vstride, places_of(kstride, vstride, PIECE, p - first_of(i), lane), dv, lane);
+        else load_values<true>(xv, vp + token * vstride, whole, dv, lane);
     };
     int i = rank * A1_WARPS + warp, page = page_of(i);
-    if (i < groups) fetch(x[0], i, page);              // under way while the queries are made
+    float ks = 0.f, vs = 0.f;
+    if (i < groups) {                                  // under way while the queries are made
+        const size_t token = token_of(i, page), sc = token / kScaleTokens * a.kv_heads + kh;
+        fetch_keys(i, token);
+        fetch_values(i, token);
+        ks = a.k_scale[sc];
+        vs = a.v_scale[sc];
+    }
     page = page_of(i + step);
 
     // ---- the row's queries, and on rank 0 its key and value
@@ -300,9 +341,15 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
             most = lane_max(most);
             // a power of two that leaves 1 <= largest < 2 (2^-126 at least, so that its inverse is finite)
             const float unit = most > 0.f ? __uint_as_float(max(min(__float_as_uint(most) & 0x7F800000u, 0x7E000000u), 0x00800000u)) : 1.0f, inv = 1.0f / unit;
-            if (lane == 0) q_unit[j] = unit;
+            float sum = 0.f;                           // of the queries as they are rounded
 #pragma unroll
-            for (int e = 0; e < PER; e++) if (lane + 32 * e < DK) q_s[j * DK + lane + 32 * e] = __float2half_rn(y[e] * inv);
+            for (int e = 0; e < PER; e++) {
+                const __half z = __float2half_rn(y[e] * inv);
+                if (lane + 32 * e < DK) q_s[j * DK + lane + 32 * e] = z;
+                sum += __half2float(z);
+            }
+            sum = lane_sum(sum);
+            if (lane == 0) { q_unit[j] = unit; q_sum[j] = sum; }
         } else {
             const bool key = j == HN;
             if (key) prepare(y, row + qw + kh * a.dim, a.dim, a.k_norm ? a.k_norm + (a.head_norm ? 0 : kh * a.dim) : nullptr, ik, a.k_norm && a.head_norm, a.freq != nullptr);
@@ -344,7 +391,7 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
         __syncthreads();
     }
     uint32_t q[NT][KC][4][2];
-    float qs[NT][2], slope[NT][2];
+    float qs[NT][2], slope[NT][2], from[NT][2];
     State<VW, NT> st;
     st.vref = 0.f;
     st.vinv = 0.f;
@@ -362,6 +409,7 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
         for (int e = 0; e < 2; e++) {
             const int j = 8 * n + 2 * t + e;
             qs[n][e] = q_unit[j];
+            from[n][e] = I8 ? -1152.f * q_sum[j] : 0.f;
             slope[n][e] = a.slopes && j < nh ? a.slopes[h0 + j] * kLog2e : 0.f;
             st.m[n][e] = -INFINITY;
             st.l[n][e] = 0.f;
@@ -370,24 +418,32 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
         }
     }
     // ---- the cached groups
+    float sc[NT][4];
+    uint32_t pb[NT][2];
     while (i < groups) {
-#pragma unroll
-        for (int b = 0; b < 2; b++) {
-            if (i >= groups) break;
-            const int next = i + step;
-            if (next < groups) {
-                fetch(x[b ^ 1], next, page);
-                page = page_of(next + step);
-            }
-            take_group<I8, KC, VW, NT>(st, x[b], q, qs, slope, first_of(i), p, k_lo, keep, lane);
-            i = next;
+        const int next = i + step;
+        const bool more = next < groups;
+        const size_t token = more ? token_of(next, page) : 0;
+        key_products<I8, KC, NT>(sc, xk, q, from);
+        if (more) fetch_keys(next, token);
+        make_weights<VW, NT>(st, sc, pb, ks, vs, qs, slope, first_of(i), p, k_lo, keep, lane);
+        if (more) {
+            const size_t at = token / kScaleTokens * a.kv_heads + kh;
+            ks = a.k_scale[at];
+            vs = a.v_scale[at];
+            page = page_of(next + step);
         }
+        value_products<I8, VW, NT>(st, xv, pb);
+        if (more) fetch_values(next, token);
+        i = next;
     }
     if (joins && warp == 0) {
-        load_group<false>(x[0], tail_k, tail_v, DK, DV, dk, dv, off, lane);
-        x[0].ks = tail_scale[0];
-        x[0].vs = tail_scale[1];
-        take_group<I8, KC, VW, NT>(st, x[0], q, qs, slope, tail * kScaleTokens, p, k_lo, keep, lane);
+        const Places mine = places_of(DK, DV, PIECE, off, lane);
+        load_keys<false>(xk, tail_k, mine, dk, lane);
+        load_values<false>(xv, tail_v, mine, dv, lane);
+        key_products<I8, KC, NT>(sc, xk, q, from);
+        make_weights<VW, NT>(st, sc, pb, tail_scale[0], tail_scale[1], qs, slope, tail * kScaleTokens, p, k_lo, keep, lane);
+        value_products<I8, VW, NT>(st, xv, pb);
     }
     // ---- merge the warps, then the CTAs of the cluster
     __syncthreads();                                   // queries and tail are done with
