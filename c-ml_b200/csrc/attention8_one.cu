@@ -7,35 +7,34 @@
 //                                        a lane's four consecutive codes are its four columns, and no shuffle or shared memory is needed
 //   O^T [16 dims x 8 heads] += V^T P^T   A: a lane holds the same 8, 16 or 32 dimensions of the keys 2t, 2t + 1, 2t + 8, 2t + 9; bytes of two keys are
 //                                        interleaved, which makes the operand's pairs. P^T comes from S^T by movmatrix
-// so the codes go from global memory to registers to the tensor cores. A lane requests the next group's keys as soon as this one's have gone into the products,
-// and its values likewise: 4 KB a warp under way with 32 registers, and 16 warps an SM. int8 keys stay 1,152 too large, as they come out of their conversion: the
+// so a lane's operands are its own pieces of the cache. It copies them asynchronously into places of its own in shared memory, three to six groups ahead (groups of 4 KB a
+// warp at heads of 128: 16 warps an SM with one group each under way in registers read 4.1 TB/s). int8 keys stay 1,152 too large, as they come out of their conversion: the
 // scores' accumulators begin at -1,152 times the sum of the head's queries, so every term is exact and the fp32 sums are off by no more than the queries' own rounding.
 // A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
 // where m, the warp's reference for the exponentials, moves only when a score has passed it by 7 (powers of two; sums are fp32). Queries are fp16 over
 // a power of two of their own per head, so their size is no matter.
-// 4 warps a CTA take groups in turn; a cluster of up to 8 CTAs splits a row's keys and merges through distributed shared memory, each CTA a
+// 8 warps a CTA take groups in turn; a cluster of up to 8 CTAs splits a row's keys and merges through distributed shared memory, each CTA a
 // share of the outputs. The group that the row's own token joins belongs to rank 0 alone, which settles its scales, rewrites it where they have grown and
 // attends to it from shared memory; nobody else looks at it.
 #include "cache8.cuh"
 
 namespace {
 
-constexpr int A1_THREADS = 128, A1_WARPS = A1_THREADS / 32, A1_SPLITS = 8;
+constexpr int A1_SPLITS = 8, A1_WARPS = 8, A1_THREADS = 32 * A1_WARPS;
+// groups that a warp has under way: as many as shared memory holds at two CTAs an SM (one where registers allow no more)
+template <int KC, int NT> constexpr int kAhead = KC == 1 ? 6 : (KC == 2 && NT == 2) ? 6 : 3;
+template <int KC, int VW> constexpr int kGroupBytes = 32 * (32 * KC + 16 * VW) + 16;
 constexpr float kWeightUnit = 256.f;
 
 __device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
     if (a.chunk > 0) return p / a.chunk * a.chunk;
     return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
 }
-__device__ __forceinline__ uint4 ld_codes(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ld_codes8(const uint8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+// 16 or 8 bytes into shared memory, or zeros
+template <int BYTES> __device__ __forceinline__ void copy_codes(uint32_t dst, const uint8_t* src, bool there) {
+    const int n = there ? BYTES : 0;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -68,34 +67,76 @@ __device__ __forceinline__ Places places_of(int kstride, int vstride, int piece,
     for (int i = 0; i < 4; i++) p.v[i] = min(2 * t + (i & 1) + 8 * (i >> 1), last) * vstride + piece * g;
     return p;
 }
-// GLOBAL: from the cache, else from shared memory
-template <bool GLOBAL, int KC>
-__device__ __forceinline__ void load_keys(KeyCodes<KC>& x, const uint8_t* k, const Places& p, int dk, int lane) {
-    const int t = lane & 3;
+// A group's pieces on their way into the lane's places: keys' pieces, then values', each 32 lanes' side by side.
+template <int KC, int VW>
+__device__ __forceinline__ void copy_group(uint32_t to, const uint8_t* k, const uint8_t* v, const Places& p, int dk, int dv, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int c = 0; c < KC; c++) copy_codes<16>(to + 512 * (i * KC + c) + 16 * lane, k + p.k[i] + 64 * c, 64 * c + 16 * t < dk);
+    to += 1024 * KC;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (VW == 2) {
+            copy_codes<8>(to + 256 * i + 8 * lane, v + p.v[i], 8 * g < dv);
+        } else {
+#pragma unroll
+            for (int c = 0; c < VW / 4; c++) copy_codes<16>(to + 512 * (i * (VW / 4) + c) + 16 * lane, v + p.v[i] + 128 * c, 128 * c + 16 * g < dv);
+        }
+    }
+}
+template <int KC>
+__device__ __forceinline__ void take_keys(KeyCodes<KC>& x, const uint8_t* from, int lane) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+            const uint4 u = *reinterpret_cast<const uint4*>(from + 512 * (i * KC + c) + 16 * lane);
+            x.w[i][c][0] = u.x; x.w[i][c][1] = u.y; x.w[i][c][2] = u.z; x.w[i][c][3] = u.w;
+        }
+}
+template <int KC, int VW>
+__device__ __forceinline__ void take_values(ValueCodes<VW>& x, const uint8_t* from, int lane) {
+    from += 1024 * KC;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (VW == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(from + 256 * i + 8 * lane);
+            x.w[i][0] = u.x; x.w[i][1] = u.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < VW / 4; c++) {
+                const uint4 u = *reinterpret_cast<const uint4*>(from + 512 * (i * (VW / 4) + c) + 16 * lane);
+                x.w[i][4 * c] = u.x; x.w[i][4 * c + 1] = u.y; x.w[i][4 * c + 2] = u.z; x.w[i][4 * c + 3] = u.w;
+            }
+        }
+    }
+}
+// The same from the row's own group, which lies in shared memory token by token.
+template <int KC, int VW>
+__device__ __forceinline__ void take_tail(KeyCodes<KC>& xk, ValueCodes<VW>& xv, const uint8_t* k, const uint8_t* v, const Places& p, int dk, int dv, int lane) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (64 * c + 16 * t < dk) u = GLOBAL ? ld_codes(k + p.k[i] + 64 * c) : *reinterpret_cast<const uint4*>(k + p.k[i] + 64 * c);
-            x.w[i][c][0] = u.x; x.w[i][c][1] = u.y; x.w[i][c][2] = u.z; x.w[i][c][3] = u.w;
+            if (64 * c + 16 * t < dk) u = *reinterpret_cast<const uint4*>(k + p.k[i] + 64 * c);
+            xk.w[i][c][0] = u.x; xk.w[i][c][1] = u.y; xk.w[i][c][2] = u.z; xk.w[i][c][3] = u.w;
         }
-}
-template <bool GLOBAL, int VW>
-__device__ __forceinline__ void load_values(ValueCodes<VW>& x, const uint8_t* v, const Places& p, int dv, int lane) {
-    const int g = lane >> 2;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if constexpr (VW == 2) {
             uint2 u = make_uint2(0u, 0u);
-            if (8 * g < dv) u = GLOBAL ? ld_codes8(v + p.v[i]) : *reinterpret_cast<const uint2*>(v + p.v[i]);
-            x.w[i][0] = u.x; x.w[i][1] = u.y;
+            if (8 * g < dv) u = *reinterpret_cast<const uint2*>(v + p.v[i]);
+            xv.w[i][0] = u.x; xv.w[i][1] = u.y;
         } else {
 #pragma unroll
             for (int c = 0; c < VW / 4; c++) {
                 uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (128 * c + 16 * g < dv) u = GLOBAL ? ld_codes(v + p.v[i] + 128 * c) : *reinterpret_cast<const uint4*>(v + p.v[i] + 128 * c);
-                x.w[i][4 * c] = u.x; x.w[i][4 * c + 1] = u.y; x.w[i][4 * c + 2] = u.z; x.w[i][4 * c + 3] = u.w;
+                if (128 * c + 16 * g < dv) u = *reinterpret_cast<const uint4*>(v + p.v[i] + 128 * c);
+                xv.w[i][4 * c] = u.x; xv.w[i][4 * c + 1] = u.y; xv.w[i][4 * c + 2] = u.z; xv.w[i][4 * c + 3] = u.w;
             }
         }
     }
@@ -219,16 +260,17 @@ __device__ __forceinline__ void value_products(State<VW, NT>& st, const ValueCod
 // grid = (splits, kv_heads * passes, rows), clusters of `splits`. A pass is 8 NT query heads. append: the row's key and value enter the cache here
 // (one pass then), otherwise they are in it.
 template <bool I8, int KC, int VW, int NT>
-__global__ void __launch_bounds__(A1_THREADS, KC == 4 ? 2 : NT == 2 ? 2 : 4)
+__global__ void __launch_bounds__(A1_THREADS, KC == 4 || NT == 2 ? 1 : 2)
 attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int ld, const int* __restrict__ row_pos, const int* __restrict__ row_slot, int append,
                       __nv_bfloat16* __restrict__ out, int out_ld) {
-    constexpr int HN = 8 * NT, DK = 64 * KC, DV = 32 * VW, PER = DK > DV ? DK / 32 : DV / 32;
+    constexpr int HN = 8 * NT, AHEAD = kAhead<KC, NT>, GROUP = kGroupBytes<KC, VW>, DK = 64 * KC, DV = 32 * VW, PER = DK > DV ? DK / 32 : DV / 32;
     extern __shared__ __align__(16) uint8_t sm[];
     const int dk = a.dim_ld, dv = a.vdim_ld;
     __half* q_s = reinterpret_cast<__half*>(sm);                             // [HN][DK]
     uint8_t* tail_k = sm + HN * DK * 2;                                      // [16][DK], [16][DV]: the row's own group
     uint8_t* tail_v = tail_k + kScaleTokens * DK;
     float* fresh = reinterpret_cast<float*>(tail_v + kScaleTokens * DV);     // [DK], [DV]: the row's own key and value
+    uint8_t* ring = reinterpret_cast<uint8_t*>(fresh + DK + DV) + (threadIdx.x >> 5) * (AHEAD * GROUP);       // the warp's groups under way: codes, then two scales
     float* w_acc = reinterpret_cast<float*>(sm);                             // [A1_WARPS][HN][DV] at the end, over all of the above
     __shared__ float w_m[A1_WARPS][HN], w_l[A1_WARPS][HN], c_m[HN], c_l[HN], q_unit[HN], q_sum[HN], tail_scale[2];
     __shared__ float2 red[A1_WARPS];
@@ -258,24 +300,27 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     auto token_of = [&](int i, int page) { return ((size_t)page << shift) + (first_of(i) & (a.block_size - 1)); };
     // (where the row's key is in the cache already, its group may end with it)
     auto ends = [&](int i) { return !append && first_of(i) + kScaleTokens - 1 > p; };
-    auto fetch_keys = [&](int i, size_t token) {
-        if (ends(i)) load_keys<true>(xk, kp + token * kstride, places_of(kstride, vstride, PIECE, p - first_of(i), lane), dk, lane);
-        else load_keys<true>(xk, kp + token * kstride, whole, dk, lane);
+    // group i into place `at` of the ring; a commit each, whether there is such a group or not
+    auto fetch = [&](int i, int page, int at) {
+        if (i < groups) {
+            const size_t token = token_of(i, page), sc = token / kScaleTokens * a.kv_heads + kh;
+            const uint32_t to = smem_addr(ring) + at * GROUP;
+            const uint8_t *k = kp + token * kstride, *v = vp + token * vstride;
+            if (ends(i)) copy_group<KC, VW>(to, k, v, places_of(kstride, vstride, PIECE, p - first_of(i), lane), dk, dv, lane);
+            else copy_group<KC, VW>(to, k, v, whole, dk, dv, lane);
+            if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + GROUP - 16 + 4 * lane), "l"((lane ? a.v_scale : a.k_scale) + sc) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto fetch_values = [&](int i, size_t token) {
-        if (ends(i)) load_values<true>(xv, vp + token * vstride, places_of(kstride, vstride, PIECE, p - first_of(i), lane), dv, lane);
-        else load_values<true>(xv, vp + token * vstride, whole, dv, lane);
-    };
-    int i = rank * A1_WARPS + warp, page = page_of(i);
-    float ks = 0.f, vs = 0.f;
-    if (i < groups) {                                  // under way while the queries are made
-        const size_t token = token_of(i, page), sc = token / kScaleTokens * a.kv_heads + kh;
-        fetch_keys(i, token);
-        fetch_values(i, token);
-        ks = a.k_scale[sc];
-        vs = a.v_scale[sc];
+    int i = rank * A1_WARPS + warp;
+    {                                                  // under way while the queries are made
+        int pages[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) pages[j] = page_of(i + j * step);
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) fetch(i + j * step, pages[j], j);
     }
-    page = page_of(i + step);
+    int page = page_of(i + AHEAD * step);
 
     // ---- the row's queries, and on rank 0 its key and value
     const size_t own = ((size_t)table[p >> shift] << shift) + (p & (a.block_size - 1)), own_group = own / kScaleTokens * a.kv_heads + kh;
@@ -391,7 +436,7 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
         __syncthreads();
     }
     uint32_t q[NT][KC][4][2];
-    float qs[NT][2], slope[NT][2], from[NT][2];
+    float qs[NT][2], slope[NT][2], from_[NT][2];
     State<VW, NT> st;
     st.vref = 0.f;
     st.vinv = 0.f;
@@ -409,7 +454,7 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
         for (int e = 0; e < 2; e++) {
             const int j = 8 * n + 2 * t + e;
             qs[n][e] = q_unit[j];
-            from[n][e] = I8 ? -1152.f * q_sum[j] : 0.f;
+            from_[n][e] = I8 ? -1152.f * q_sum[j] : 0.f;
             slope[n][e] = a.slopes && j < nh ? a.slopes[h0 + j] * kLog2e : 0.f;
             st.m[n][e] = -INFINITY;
             st.l[n][e] = 0.f;
@@ -420,31 +465,28 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     // ---- the cached groups
     float sc[NT][4];
     uint32_t pb[NT][2];
-    while (i < groups) {
-        const int next = i + step;
-        const bool more = next < groups;
-        const size_t token = more ? token_of(next, page) : 0;
-        key_products<I8, KC, NT>(sc, xk, q, from);
-        if (more) fetch_keys(next, token);
-        make_weights<VW, NT>(st, sc, pb, ks, vs, qs, slope, first_of(i), p, k_lo, keep, lane);
-        if (more) {
-            const size_t at = token / kScaleTokens * a.kv_heads + kh;
-            ks = a.k_scale[at];
-            vs = a.v_scale[at];
-            page = page_of(next + step);
-        }
+    for (int at = 0; i < groups; i += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+        __syncwarp();                                  // (two lanes copied the scales)
+        const uint8_t* from = ring + at * GROUP;
+        const float2 two = *reinterpret_cast<const float2*>(from + GROUP - 16);
+        take_keys<KC>(xk, from, lane);
+        take_values<KC, VW>(xv, from, lane);
+        key_products<I8, KC, NT>(sc, xk, q, from_);
+        make_weights<VW, NT>(st, sc, pb, two.x, two.y, qs, slope, first_of(i), p, k_lo, keep, lane);
         value_products<I8, VW, NT>(st, xv, pb);
-        if (more) fetch_values(next, token);
-        i = next;
+        __syncwarp();
+        fetch(i + AHEAD * step, page, at);
+        page = page_of(i + (AHEAD + 1) * step);
+        at = at + 1 == AHEAD ? 0 : at + 1;
     }
     if (joins && warp == 0) {
-        const Places mine = places_of(DK, DV, PIECE, off, lane);
-        load_keys<false>(xk, tail_k, mine, dk, lane);
-        load_values<false>(xv, tail_v, mine, dv, lane);
-        key_products<I8, KC, NT>(sc, xk, q, from);
+        take_tail<KC, VW>(xk, xv, tail_k, tail_v, places_of(DK, DV, PIECE, off, lane), dk, dv, lane);
+        key_products<I8, KC, NT>(sc, xk, q, from_);
         make_weights<VW, NT>(st, sc, pb, tail_scale[0], tail_scale[1], qs, slope, tail * kScaleTokens, p, k_lo, keep, lane);
         value_products<I8, VW, NT>(st, xv, pb);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     // ---- merge the warps, then the CTAs of the cluster
     __syncthreads();                                   // queries and tail are done with
     const float unit = st.vref / kWeightUnit;
@@ -533,7 +575,7 @@ template <bool I8, int KC, int VW, int NT>
 int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int splits, int passes, int append, __nv_bfloat16* d_out, int out_ld,
                cudaStream_t st) {
     constexpr size_t HN = 8 * NT, DK = 64 * KC, DV = 32 * VW;
-    constexpr size_t before = HN * DK * 2 + kScaleTokens * (DK + DV) + 4 * (DK + DV), after = 4 * A1_WARPS * HN * DV, smem = before > after ? before : after;
+    constexpr size_t before = HN * DK * 2 + kScaleTokens * (DK + DV) + 4 * (DK + DV) + A1_WARPS * kAhead<KC, NT> * kGroupBytes<KC, VW>, after = 4 * A1_WARPS * HN * DV, smem = before > after ? before : after;
     static size_t attr[kMaxDevices] = {};
     auto kern = attention8_one_kernel<I8, KC, VW, NT>;
     CMLB_CUDA(cmlb_ensure_smem(kern, smem, attr));
@@ -556,8 +598,10 @@ int cmlb_attention8_one(const cmlb200_attn* a, const float* d_qkv, int ld, const
     const int reach = a->chunk > 0 ? a->chunk : a->window;
     const int keys = (reach > 0 && reach < max_keys - a->keep) ? reach + a->keep : max_keys;
     const long long base = (long long)rows * a->kv_heads * passes;
-    int splits = 1;
-    while (splits < A1_SPLITS && base * splits < 3 * cmlb_num_sms() && keys > splits * A1_WARPS * kScaleTokens) splits *= 2;
+    // as many CTAs to a row and key/value head as run at a time, while each of their warps has a group (8 rows of 8 heads behind 2,000 tokens: 18.3 us with 4,
+    // 24.4 with 2, 27.7 with 8, which takes two waves)
+    const long long room = (long long)cmlb_num_sms() * (widest > 128 || nt == 2 ? 1 : 2), most = (keys + A1_WARPS * kScaleTokens - 1) / (A1_WARPS * kScaleTokens);
+    const int splits = (int)max(1LL, min(min((long long)A1_SPLITS, room / base), most));
 #define A1_ARGS a, d_qkv, ld, d_row_pos, d_row_slot, rows, splits, passes, append, d_out, out_ld, st
 #define A1_HEADS(I8, KC, VW) return nt == 1 ? launch_one<I8, KC, VW, 1>(A1_ARGS) : launch_one<I8, KC, VW, 2>(A1_ARGS)
 #define A1_SIZES(I8)                            \
