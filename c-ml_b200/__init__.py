@@ -433,6 +433,7 @@ REFERENCE_QUIRKS, KV_FP32, ALL_LOGITS_FP32 = 1, 2, 4
 DT_F32, DT_BF16, DT_F16, DT_I8, DT_E4M3 = 0, 1, 2, 3, 4
 ACT_SILU, ACT_GELU_TANH, ACT_CLAMPED, ACT_GELU_ERF = 0, 1, 2, 3
 DTYPE_FLOAT32, DTYPE_BFLOAT16 = 0, 6
+CACHE_DEFAULT, CACHE_INT8, CACHE_E4M3 = 0, 1, 2
 
 
 class Dense(C.Structure):
@@ -497,7 +498,7 @@ class Pages(C.Structure):
 
 
 class LMOptions(C.Structure):
-    _fields_ = [("dtype", ci), ("max_tokens", ci), ("max_sequences", ci), ("max_step_rows", ci)]
+    _fields_ = [("dtype", ci), ("max_tokens", ci), ("max_sequences", ci), ("max_step_rows", ci), ("cache", ci)]
 
 
 class LMEntry(C.Structure):
@@ -572,6 +573,11 @@ _sig("cml_lm_sequence_close", ci, vp, ci)
 _sig("cml_lm_sequence_length", ci, vp, ci)
 _sig("cml_lm_step", ci, vp, C.POINTER(LMEntry), ci, vp)
 _sig("cml_lm_step_greedy", ci, vp, C.POINTER(LMEntry), ci, vp)
+_sig("cml_lm_sequence_fork", ci, vp, ci)
+_sig("cml_lm_compact", ci, vp)
+_sig("cml_lm_step_scored", ci, vp, C.POINTER(LMEntry), ci, vp, ci, vp, vp, vp, vp)
+_sig("cml_paged_cache_fork", ci, C.POINTER(PagedKVCache), ci, C.POINTER(ci), C.POINTER(ci))
+_sig("cml_paged_cache_compact", ci, C.POINTER(PagedKVCache), vp)
 _sig("cml_lm_decode_greedy", ci, vp, vp, vp, ci, ci, vp, C.POINTER(C.c_float))
 _sig("cml_serving_run_lm", ci, vp, vp, C.POINTER(GenerationConfig), ci, vp, vp)
 _sig("cml_lm_generate", C.POINTER(GenerationResult), vp, vp, ci, C.POINTER(GenerationConfig))
@@ -585,8 +591,8 @@ _sig("cml_paged_cache_release_between", None, C.POINTER(PagedKVCache), ci, ci, c
 class LanguageModel:
     """A model loaded through cml_lm_load, with numpy arrays in and out."""
 
-    def __init__(self, path, dtype=DTYPE_BFLOAT16, max_tokens=2048, max_sequences=8, max_step_rows=0):
-        self.h = lib.cml_lm_load(str(path).encode(), C.byref(LMOptions(dtype, max_tokens, max_sequences, max_step_rows)))
+    def __init__(self, path, dtype=DTYPE_BFLOAT16, max_tokens=2048, max_sequences=8, max_step_rows=0, cache=CACHE_DEFAULT):
+        self.h = lib.cml_lm_load(str(path).encode(), C.byref(LMOptions(dtype, max_tokens, max_sequences, max_step_rows, cache)))
         if not self.h:
             raise CmlB200Error(f"cml_lm_load({path}) failed")
         self.vocab = lib.cml_lm_vocab_size(self.h)
@@ -604,6 +610,33 @@ class LanguageModel:
 
     def end(self, seq):
         check(lib.cml_lm_sequence_close(self.h, seq), "cml_lm_sequence_close")
+
+    def fork(self, seq):
+        s = lib.cml_lm_sequence_fork(self.h, seq)
+        if s < 0:
+            raise CmlB200Error(f"sequence {seq} cannot be forked")
+        return s
+
+    def compact(self):
+        n = lib.cml_lm_compact(self.h)
+        if n < 0:
+            raise CmlB200Error("the pool cannot be compacted")
+        return n
+
+    def scored(self, entries, targets=None, top=0):
+        """entries as for step; targets: a token per wanted place, in their order. (log probabilities or None, entropies, ids [n, top], their log
+        probabilities [n, top]) of all wanted places."""
+        import numpy as np
+        keep = [(np.ascontiguousarray(t, np.int32).ravel(), np.arange(len(t), dtype=np.int32) if w is None else np.ascontiguousarray(w, np.int32).ravel()) for _, t, w in entries]
+        arr = (LMEntry * len(entries))(*(LMEntry(seq, t.ctypes.data, len(t), w.ctypes.data, len(w)) for (seq, _, _), (t, w) in zip(entries, keep)))
+        n = sum(len(w) for _, w in keep)
+        tg = None if targets is None else np.ascontiguousarray(targets, np.int32)
+        if tg is not None and tg.size != n:
+            raise CmlB200Error(f"{tg.size} targets for {n} wanted places")
+        lp, en, ids, best = np.empty(n, np.float32), np.empty(n, np.float32), np.empty((n, top), np.int32), np.empty((n, top), np.float32)
+        check(lib.cml_lm_step_scored(self.h, arr, len(entries), None if tg is None else np_ptr(tg), top, None if tg is None else np_ptr(lp), np_ptr(en), np_ptr(ids) if top else None,
+                                     np_ptr(best) if top else None), "cml_lm_step_scored")
+        return (None if tg is None else lp), en, ids, best
 
     def step(self, entries, greedy=False):
         """entries: (seq, tokens, wanted places or None for all). One list item of logits [n, vocab] (or picks [n]) per entry."""

@@ -20,6 +20,7 @@
 #define SMALL_ROWS 64              /* steps up to this many rows share one compact upload layout, and may be captured */
 #define HEAD_ROWS 256              /* rows of logits per pass of the vocabulary projection */
 #define STAGED_ROWS 32             /* rows of logits that go through page-locked memory */
+#define SCORED_TOP 32              /* likeliest tokens of a scored row at most */
 #define MAX_CLASSES 16
 #define MAX_GRAPHS 32
 
@@ -44,6 +45,11 @@ struct CMLLanguageModel {
     int *d_picked, *h_picked;
     int *d_hist, *d_step;
     size_t hist_cap;
+    int *d_moves, *h_moves;        /* of blocks, and a fork's four numbers; the host side is page-locked */
+    cmlb200_page_pool* d_pools;    /* what a block names, then what a slot names */
+    cmlb200_pages block_pages, slot_pages;
+    char *d_scored, *h_scored;     /* targets and results of scored rows; made by the first scored step */
+    float* d_score_logits;         /* of classes that give logits to the host */
     StepGraph graphs[MAX_GRAPHS];
     unsigned clock;
     unsigned char* in_step;        /* per sequence: already in the entries being checked */
@@ -66,8 +72,33 @@ int cml_lm_known(const char* architecture) { return find_class(architecture) != 
 
 /* ---- load / free ----------------------------------------------------------------------------------- */
 CMLLMOptions cml_lm_default_options(void) {
-    CMLLMOptions o = {.dtype = DTYPE_BFLOAT16, .max_tokens = 8192, .max_sequences = 8, .max_step_rows = 0};
+    CMLLMOptions o = {.dtype = DTYPE_BFLOAT16, .max_tokens = 8192, .max_sequences = 8, .max_step_rows = 0, .cache = CML_LM_CACHE_DEFAULT};
     return o;
+}
+
+/* Descriptions of what block ids and sequence slots name, for forks and compaction. */
+static int make_pages(CMLLanguageModel* lm, int blocks) {
+    const int n[2] = {lm->cls->pools(lm->model, 0, NULL, 0), lm->cls->pools(lm->model, 1, NULL, 0)};
+    const size_t all = (size_t)(n[0] + n[1]);
+    cmlb200_page_pool* h = (cmlb200_page_pool*)calloc(all ? all : 1, sizeof *h);
+    if (!h) return -1;
+    cmlb200_pages* pages[2] = {&lm->block_pages, &lm->slot_pages};
+    int rc = CML_DEV_FAIL(cmlb200_malloc((void**)&lm->d_pools, (all ? all : 1) * sizeof *h), __func__) ? -1 : 0;
+    for (int k = 0; k < 2 && !rc; k++) {
+        cmlb200_page_pool* part = h + (k ? n[0] : 0);
+        lm->cls->pools(lm->model, k, part, n[k]);
+        pages[k]->pools = n[k];
+        pages[k]->pool = lm->d_pools + (k ? n[0] : 0);
+        pages[k]->pages = k ? lm->opt.max_sequences : blocks;
+        for (int i = 0; i < n[k]; i++) if (part[i].bytes > pages[k]->most) pages[k]->most = part[i].bytes;
+    }
+    lm->block_pages.table = lm->d_table;
+    lm->block_pages.slots = lm->opt.max_sequences;
+    lm->block_pages.table_ld = lm->table_ld;
+    if (!rc && all && CML_DEV_FAIL(cmlb200_memcpy_h2d(lm->d_pools, h, all * sizeof *h, lm->stream), __func__)) rc = -1;
+    if (!rc && CML_DEV_FAIL(cmlb200_stream_sync(lm->stream), __func__)) rc = -1;
+    free(h);
+    return rc;
 }
 
 static int make_buffers(CMLLanguageModel* lm) {
@@ -91,7 +122,9 @@ static int make_buffers(CMLLanguageModel* lm) {
     DEV(cmlb200_malloc((void**)&lm->d_picked, HEAD_ROWS * sizeof(int)));
     DEV(cmlb200_host_alloc_pinned((void**)&lm->h_picked, HEAD_ROWS * sizeof(int)));
     DEV(cmlb200_malloc((void**)&lm->d_step, sizeof(int)));
-    return lm->cls->make_pools(lm->model, blocks, BLOCK, lm->opt.max_sequences, lm->table_ld);
+    DEV(cmlb200_host_alloc_pinned((void**)&lm->h_moves, (2 * (size_t)blocks + 8) * sizeof(int)));
+    DEV(cmlb200_malloc((void**)&lm->d_moves, (2 * (size_t)blocks + 8) * sizeof(int)));
+    return lm->cls->make_pools(lm->model, blocks, BLOCK, lm->opt.max_sequences, lm->table_ld) || make_pages(lm, blocks) ? -1 : 0;
 }
 
 CMLLanguageModel* cml_lm_load(const char* path, const CMLLMOptions* options) {
@@ -99,6 +132,7 @@ CMLLanguageModel* cml_lm_load(const char* path, const CMLLMOptions* options) {
     if (!path) { LOG_ERROR("%s: NULL path", who); return NULL; }
     CMLLMOptions o = options ? *options : cml_lm_default_options();
     if (o.dtype != DTYPE_BFLOAT16 && o.dtype != DTYPE_FLOAT32) { LOG_ERROR("%s: dtype must be bfloat16 or float32", who); return NULL; }
+    if (o.cache < CML_LM_CACHE_DEFAULT || o.cache > CML_LM_CACHE_E4M3) { LOG_ERROR("%s: cache %d", who, o.cache); return NULL; }
     if (o.max_tokens <= 0 || o.max_sequences <= 0 || o.max_tokens > (1 << 28)) { LOG_ERROR("%s: max_tokens %d, max_sequences %d", who, o.max_tokens, o.max_sequences); return NULL; }
     if (o.max_step_rows <= 0) o.max_step_rows = o.max_tokens;
     struct stat sb;
@@ -139,12 +173,14 @@ void cml_lm_free(CMLLanguageModel* lm) {
     for (int i = 0; i < MAX_GRAPHS; i++) if (lm->graphs[i].graph) cmlb200_graph_destroy(lm->graphs[i].graph);
     if (lm->model) lm->cls->free(lm->model);
     cml_paged_kv_cache_free(lm->cache);
-    void* dev[] = {lm->d_meta, lm->d_table, lm->d_logits, lm->d_picked, lm->d_hist, lm->d_step};
+    void* dev[] = {lm->d_meta, lm->d_table, lm->d_logits, lm->d_picked, lm->d_hist, lm->d_step, lm->d_moves, lm->d_pools, lm->d_scored, lm->d_score_logits};
     for (size_t i = 0; i < sizeof dev / sizeof dev[0]; i++) cmlb200_free(dev[i]);
     cmlb200_host_free_pinned(lm->h_meta);
     cmlb200_host_free_pinned(lm->h_table);
     cmlb200_host_free_pinned(lm->h_picked);
     cmlb200_host_free_pinned(lm->h_logits);
+    cmlb200_host_free_pinned(lm->h_moves);
+    cmlb200_host_free_pinned(lm->h_scored);
     if (lm->stream) cmlb200_stream_destroy(lm->stream);
     free(lm->in_step);
     free(lm->portions);
@@ -179,6 +215,45 @@ int cml_lm_sequence_close(CMLLanguageModel* lm, int seq) {
 int cml_lm_sequence_length(CMLLanguageModel* lm, int seq) {
     if (!seq_is_open(lm, seq)) return -1;
     return lm->cache ? lm->cache->sequences[seq].seq_len : lm->cls->length(lm->model, seq);
+}
+
+int cml_lm_sequence_fork(CMLLanguageModel* lm, int seq) {
+    static const char* who = "cml_lm_sequence_fork";
+    if (!seq_is_open(lm, seq)) { LOG_ERROR("%s: sequence %d is not open", who, seq); return -1; }
+    if (!lm->cache) { LOG_ERROR("%s: %s models keep no paged cache", who, lm->cls->architecture); return -1; }
+    int from, to;
+    const int child = cml_paged_cache_fork(lm->cache, seq, &from, &to);
+    if (child < 0) return -1;
+    const CMLBlockTable* bt = &lm->cache->sequences[child];
+    const int own = to >= 0, shared = own ? bt->seq_len / BLOCK : bt->num_blocks;
+    const size_t row = (size_t)child * (size_t)lm->table_ld;
+    memcpy(lm->h_table + row, lm->h_table + (size_t)seq * (size_t)lm->table_ld, (size_t)shared * sizeof(int));       /* (places of blocks let go of included) */
+    if (own) lm->h_table[row + (size_t)shared] = to;
+    const int list[6] = {seq, child, shared, to, seq, child};              /* the fork; the move of what the slot keeps */
+    memcpy(lm->h_moves, list, sizeof list);
+    int rc = CML_DEV_FAIL(cmlb200_memcpy_h2d(lm->d_moves, lm->h_moves, sizeof list, lm->stream), who) ||
+             (bt->num_blocks && CML_DEV_FAIL(cmlb200_pages_fork(&lm->block_pages, lm->d_moves, 1, lm->stream), who)) ||
+             (lm->slot_pages.pools && CML_DEV_FAIL(cmlb200_pages_copy(&lm->slot_pages, lm->d_moves + 4, 1, lm->stream), who)) ||
+             CML_DEV_FAIL(cmlb200_stream_sync(lm->stream), who);
+    if (!rc) return child;
+    cml_paged_cache_free_sequence(lm->cache, child);
+    return -1;
+}
+
+int cml_lm_compact(CMLLanguageModel* lm) {
+    static const char* who = "cml_lm_compact";
+    if (!lm || !lm->cache) { LOG_ERROR("%s: no paged cache", who); return -1; }
+    const int moved = cml_paged_cache_compact(lm->cache, lm->h_moves);
+    if (moved <= 0) return moved;
+    for (int s = 0; s < lm->opt.max_sequences; s++) {
+        const CMLBlockTable* bt = &lm->cache->sequences[s];
+        for (int i = 0; bt->block_ids && i < bt->num_blocks; i++)
+            if (bt->block_ids[i] >= 0) lm->h_table[(size_t)s * (size_t)lm->table_ld + (size_t)i] = bt->block_ids[i];
+    }
+    DEV(cmlb200_memcpy_h2d(lm->d_moves, lm->h_moves, 2 * (size_t)moved * sizeof(int), lm->stream));
+    DEV(cmlb200_pages_copy(&lm->block_pages, lm->d_moves, moved, lm->stream));
+    DEV(cmlb200_stream_sync(lm->stream));
+    return moved;
 }
 
 /* Takes the blocks of n further tokens and uploads the new part of the sequence's block table. */
@@ -348,11 +423,37 @@ static int run_captured(CMLLanguageModel* lm, const CMLLMBatch* b, const int* d_
     return 0;
 }
 
-static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, float* logits, int* picked, const char* who) {
+/* What a scored step asks for, per wanted row. */
+typedef struct { const int* targets; int top; float *logprobs, *entropies; int* top_ids; float* top_logprobs; } Scored;
+
+/* Scores k rows of logits on the device and copies what is asked for to places `at` and on. */
+static int score_rows(CMLLanguageModel* lm, const Scored* q, const float* d_logits, int at, int k, void* stream) {
+    /* targets, log probabilities and entropies of HEAD_ROWS rows, then their likeliest tokens and those' log probabilities */
+    const size_t line = HEAD_ROWS * sizeof(int), bytes = 3 * line + 2 * SCORED_TOP * line;
+    if (!lm->d_scored) DEV(cmlb200_malloc((void**)&lm->d_scored, bytes));
+    if (!lm->h_scored) DEV(cmlb200_host_alloc_pinned((void**)&lm->h_scored, bytes));
+    const size_t best = 3 * line + (size_t)k * (size_t)q->top * sizeof(int), used = best + (size_t)k * (size_t)q->top * sizeof(float);
+    char *d = lm->d_scored, *h = lm->h_scored;
+    if (q->targets) {
+        memcpy(h, q->targets + at, (size_t)k * sizeof(int));
+        DEV(cmlb200_memcpy_h2d(d, h, (size_t)k * sizeof(int), stream));
+    }
+    DEV(cmlb200_token_scores(d_logits, CMLB200_DT_F32, lm->info.vocab, k, lm->info.vocab, q->targets ? (const int*)d : NULL, q->top, q->targets ? (float*)(d + line) : NULL,
+                             (float*)(d + 2 * line), q->top ? (int*)(d + 3 * line) : NULL, q->top ? (float*)(d + best) : NULL, stream));
+    DEV(cmlb200_memcpy_d2h(h + line, d + line, used - line, stream));
+    DEV(cmlb200_stream_sync(stream));
+    if (q->logprobs) memcpy(q->logprobs + at, h + line, (size_t)k * sizeof(float));
+    if (q->entropies) memcpy(q->entropies + at, h + 2 * line, (size_t)k * sizeof(float));
+    if (q->top_ids) memcpy(q->top_ids + (size_t)at * (size_t)q->top, h + 3 * line, (size_t)k * (size_t)q->top * sizeof(int));
+    if (q->top_logprobs) memcpy(q->top_logprobs + (size_t)at * (size_t)q->top, h + best, (size_t)k * (size_t)q->top * sizeof(float));
+    return 0;
+}
+
+static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, float* logits, int* picked, const Scored* scored, const char* who) {
     int want = 0;
     const int rows = check_step(lm, entries, n, &want, who), greedy = picked != NULL;
     if (rows < 0) return -1;
-    if (want && !logits && !picked) { LOG_ERROR("%s: no room for the wanted logits", who); return -1; }
+    if (want && !logits && !picked && !scored) { LOG_ERROR("%s: no room for the wanted logits", who); return -1; }
     for (int i = 0; i < n; i++) if (grow_sequence(lm, entries[i].seq, entries[i].num_tokens)) return -1;
     CMLLMBatch b;
     const int* d_want;
@@ -366,7 +467,9 @@ static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, floa
             if (lm->cls->head(lm->model, d_want + at, k, lm->d_logits, lm->stream)) return -1;
             if (greedy) DEV(cmlb200_argmax(lm->d_logits, k, lm->info.vocab, lm->d_picked, lm->stream));
         }
-        if (greedy) {
+        if (scored) {
+            if (score_rows(lm, scored, lm->d_logits, at, k, lm->stream)) return -1;
+        } else if (greedy) {
             DEV(cmlb200_memcpy_d2h(lm->h_picked, lm->d_picked, (size_t)k * sizeof(int), lm->stream));
             DEV(cmlb200_stream_sync(lm->stream));
             memcpy(picked + at, lm->h_picked, (size_t)k * sizeof(int));
@@ -388,7 +491,31 @@ int cml_lm_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries
     static const char* who = "cml_lm_step";
     int want;
     if (lm && !lm->cache) return check_step(lm, entries, num_entries, &want, who) < 0 ? -1 : lm->cls->step(lm->model, entries, num_entries, logits);
-    return run_step(lm, entries, num_entries, logits, NULL, who);
+    return run_step(lm, entries, num_entries, logits, NULL, NULL, who);
+}
+
+int cml_lm_step_scored(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const int* targets, int top, float* logprobs, float* entropies, int* top_ids,
+                       float* top_logprobs) {
+    static const char* who = "cml_lm_step_scored";
+    if (top < 0 || top > SCORED_TOP || (lm && top > lm->info.vocab) || !targets != !logprobs || (top && !top_ids && !top_logprobs) || (!top && (top_ids || top_logprobs))) {
+        LOG_ERROR("%s: targets and log probabilities go together, up to %d likeliest tokens have somewhere to go", who, SCORED_TOP);
+        return -1;
+    }
+    const Scored q = {targets, top, logprobs, entropies, top_ids, top_logprobs};
+    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, NULL, &q, who);
+    /* logits that come to the host go back, HEAD_ROWS rows at a time */
+    int want = 0;
+    if (check_step(lm, entries, num_entries, &want, who) < 0) return -1;
+    const size_t V = (size_t)lm->info.vocab;
+    float* lg = (float*)malloc((size_t)(want ? want : 1) * V * sizeof(float));
+    int rc = lg ? lm->cls->step(lm->model, entries, num_entries, lg) : -1;
+    if (!rc && want && !lm->d_score_logits) rc = CML_DEV_FAIL(cmlb200_malloc((void**)&lm->d_score_logits, HEAD_ROWS * V * sizeof(float)), who) ? -1 : 0;
+    for (int at = 0; at < want && !rc; at += HEAD_ROWS) {
+        const int k = want - at < HEAD_ROWS ? want - at : HEAD_ROWS;
+        rc = CML_DEV_FAIL(cmlb200_memcpy_h2d(lm->d_score_logits, lg + (size_t)at * V, (size_t)k * V * sizeof(float), NULL), who) || score_rows(lm, &q, lm->d_score_logits, at, k, NULL) ? -1 : 0;
+    }
+    free(lg);
+    return rc;
 }
 
 static int argmax_row(const float* row, int n) {
@@ -400,7 +527,7 @@ static int argmax_row(const float* row, int n) {
 int cml_lm_step_greedy(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, int* picked) {
     static const char* who = "cml_lm_step_greedy";
     if (!picked) { LOG_ERROR("%s: invalid arguments", who); return -1; }
-    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, picked, who);
+    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, picked, NULL, who);
     int want = 0;
     if (check_step(lm, entries, num_entries, &want, who) < 0) return -1;
     float* lg = (float*)malloc((size_t)(want ? want : 1) * (size_t)lm->info.vocab * sizeof(float));

@@ -5,6 +5,7 @@
 #include "cml_internal.h"
 #include "cml_json.h"
 #include "cml_lm.h"
+#include "cmlb200.h"
 
 /* One entry's rows that make more than one tile. */
 typedef struct CMLLMPortion {
@@ -46,6 +47,8 @@ typedef struct CMLLMClass {
     int (*make_pools)(void* model, int blocks, int block_size, int slots, int table_ld);
     int (*forward)(void* model, const CMLLMBatch* batch, void* stream);
     int (*head)(void* model, const int* d_rows, int n, float* d_logits, void* stream);
+    /* what a block id names in each layer (per_slot 0), what a sequence slot does (1): up to `max` of them into `pools`; how many there are */
+    int (*pools)(void* model, int per_slot, cmlb200_page_pool* pools, int max);
     int (*check)(void* model, const CMLLMBatch* batch);      /* after the stream drained: -1 when a bounded wait expired */
     /* Classes with caches of their own instead (make_pools == NULL) */
     int (*open)(void* model);

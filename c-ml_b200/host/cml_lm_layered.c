@@ -839,7 +839,7 @@ static int make_expansion(Layered* m, int blocks, int block_size, int slots, int
 
 static int layered_make_pools(void* model, int blocks, int block_size, int slots, int table_ld) {
     Layered* m = (Layered*)model;
-    const size_t es = m->f32 ? 4 : 2, tokens = (size_t)blocks * (size_t)block_size;
+    const size_t es = m->f32 ? 4 : 2, tokens = (size_t)blocks * (size_t)block_size;       /* (of latents; grouped heads have theirs below) */
     for (int i = 0; i < m->num_layers; i++) {
         Layer* l = &m->layers[i];
         const LayerWeights* w = &m->layers[l->source].w;
@@ -856,8 +856,8 @@ static int layered_make_pools(void* model, int blocks, int block_size, int slots
             continue;
         }
         cmlb200_attn* a = &l->attn;
-        const size_t heads = tokens * (size_t)a->kv_heads;
-        a->cache_dtype = m->f32 ? CMLB200_DT_F32 : CMLB200_DT_F16;
+        const size_t heads = tokens * (size_t)a->kv_heads, es = m->f32 ? 4 : m->cache8 ? 1 : 2;
+        a->cache_dtype = m->f32 ? CMLB200_DT_F32 : m->cache8 ? m->cache8 : CMLB200_DT_F16;
         a->block_size = block_size;
         a->q_norm = w->q_norm;
         a->k_norm = w->k_norm;
@@ -867,10 +867,41 @@ static int layered_make_pools(void* model, int blocks, int block_size, int slots
         if (l->kind->form == MIXER_PARALLEL && (l->kind->beside == BESIDE_GRU ? cml_gru_make_state(l, slots) : cml_delta_make_state(m, l, w, slots))) return -1;
         if ((l->kind->grouped.conv || l->kind->grouped.talk) && cml_talk_make_state(l, w, slots)) return -1;
         if (lml_zeroed(&a->k_pool, heads * (size_t)a->dim_ld * es) || lml_zeroed(&a->v_pool, heads * (size_t)a->vdim_ld * es)) return -1;
+        const size_t scales = heads / CMLB200_SCALE_TOKENS * sizeof(float);
+        if (m->cache8 && (lml_zeroed((void**)&a->k_scale, scales) || lml_zeroed((void**)&a->v_scale, scales))) return -1;
     }
+    m->block_size = block_size;
     if (make_expansion(m, blocks, block_size, slots, table_ld) || cml_talk_make_scores(m, slots, table_ld, block_size)) return -1;
     DEV(cmlb200_stream_sync(NULL));
     return 0;
+}
+
+/* Blocks of keys, values, their scales and latents, or what recurrences and convolutions keep for a sequence's slot. */
+static int layered_pools(void* model, int per_slot, cmlb200_page_pool* pools, int max) {
+    const Layered* m = (const Layered*)model;
+    int n = 0;
+#define POOL(base_, bytes_) do { const size_t b_ = (size_t)(bytes_); if ((base_) && b_) { if (n < max) { cmlb200_page_pool p_ = {(base_), b_, b_}; pools[n] = p_; } n++; } } while (0)
+    for (int i = 0; i < m->num_layers; i++) {
+        const Layer* l = &m->layers[i];
+        const cmlb200_attn* a = &l->attn;
+        const cmlb200_delta* d = &l->delta;
+        if (per_slot) {
+            POOL(d->state, (size_t)d->heads * (size_t)d->dim * (size_t)d->vdim_ld * sizeof(float));
+            POOL(d->ring, (size_t)d->taps * (size_t)(2 * d->kv_heads * d->dim + d->heads * d->vdim) * sizeof(float));
+            POOL(l->gru.state, (size_t)l->gru.width * sizeof(float));
+            POOL(a->ring, (size_t)a->taps * (size_t)((a->heads + a->kv_heads) * a->dim + a->kv_heads * a->vdim) * sizeof(float));
+        } else if (l->kind->form == MIXER_LATENT) {
+            if (l->kv_from == i) POOL(l->lat.pool, (size_t)m->block_size * (size_t)l->lat.ld * (m->f32 ? 4 : 2));
+        } else {
+            const size_t heads = (size_t)m->block_size * (size_t)a->kv_heads, es = m->f32 ? 4 : m->cache8 ? 1 : 2;
+            POOL(a->k_pool, heads * (size_t)a->dim_ld * es);
+            POOL(a->v_pool, heads * (size_t)a->vdim_ld * es);
+            POOL(a->k_scale, heads / CMLB200_SCALE_TOKENS * sizeof(float));
+            POOL(a->v_scale, heads / CMLB200_SCALE_TOKENS * sizeof(float));
+        }
+    }
+#undef POOL
+    return n;
 }
 
 /* ---- a step ------------------------------------------------------------------------------------------- */
@@ -1191,6 +1222,8 @@ static int layered_check(void* model, const CMLLMBatch* b) {
     if (m->f32) return 0;
     if (m->q) DEV(cmlb200_attention_latent_status(&status, 1));
     if (status) return -1;
+    if (m->cache8 && b->tiles) DEV(cmlb200_attention8_status(&status, 1));
+    if (status) return -1;
     if (b->rows <= SKINNY_ROWS) return 0;
     DEV(cmlb200_gemm_dense_status(&status, 1));
     return status ? -1 : 0;
@@ -1207,7 +1240,7 @@ static void layered_free(void* model) {
         void* bufs[] = {w->wqkvg.w, w->wo.w, w->wgu.w, w->wd.w, a->norm, a->post, a->in, a->out, a->mix, b->norm, b->post, b->in, b->out, b->mix, w->q_norm, w->k_norm,
                         w->slopes, w->sinks, w->c_norm, w->coef, (void*)w->wqkvg.bias, (void*)w->wo.bias, w->wukt, w->wukv.w, w->router.w, w->experts_gu.w,
                         w->experts_down.w, w->shared_gu.w, w->shared_down.w, w->correction, w->conv, w->rate, w->dt_bias, w->o_norm, w->wa.w, w->wg.w, w->wuq.w, w->wo2.w, w->dq_norm, w->talk, w->left_out, w->right_out, l->attn.ring, l->gru.state, l->freq,
-                        l->attn.k_pool, l->attn.v_pool, l->delta.state, l->delta.ring, l->kv_from == i ? l->lat.pool : NULL};
+                        l->attn.k_pool, l->attn.v_pool, l->attn.k_scale, l->attn.v_scale, l->delta.state, l->delta.ring, l->kv_from == i ? l->lat.pool : NULL};
         for (size_t k = 0; k < sizeof bufs / sizeof bufs[0]; k++) cmlb200_free(bufs[k]);
     }
     const cmlb200_moe* p = &m->plan;
@@ -1228,6 +1261,7 @@ static void* layered_load(const char* path, const CMLJson* config, const CMLLMOp
     m->design = design;
     m->f32 = options->dtype == DTYPE_FLOAT32;
     m->max_sequences = options->max_sequences;
+    m->cache8 = options->cache == CML_LM_CACHE_INT8 ? CMLB200_DT_I8 : options->cache == CML_LM_CACHE_E4M3 ? CMLB200_DT_E4M3 : 0;
     char file[4096];
     snprintf(file, sizeof file, "%s/model.safetensors", path);
     CMLSafetensors* st = NULL;
@@ -1237,6 +1271,13 @@ static void* layered_load(const char* path, const CMLJson* config, const CMLLMOp
         if (!rc) rc = make_rotation(&m->layers[i]);
     }
     cml_safetensors_close(st);
+    for (int i = 0; m->cache8 && !rc && i < m->num_layers; i++) {
+        const Layer* l = &m->layers[i];
+        if (m->f32 || l->kind->form == MIXER_LATENT || l->kind->grouped.conv || l->kind->grouped.talk || l->attn.dim_ld > 256 || l->attn.vdim_ld > 256) {
+            LOG_ERROR("an 8-bit cache goes with bfloat16 and grouped attention of heads up to 256, neither convolved nor with mixed scores: layer %d has another", i);
+            rc = -1;
+        }
+    }
     if (rc || make_activations(m, options->max_step_rows)) { layered_free(m); return NULL; }
     info->vocab = m->vocab;
     for (int i = 0; i < m->num_layers; i++) {
@@ -1249,7 +1290,7 @@ static void* layered_load(const char* path, const CMLJson* config, const CMLLMOp
 }
 
 #define LAYERED_CLASS(name) {.architecture = name, .load = layered_load, .free = layered_free, .make_pools = layered_make_pools, .forward = layered_forward, \
-                             .head = layered_head, .check = layered_check}
+                             .head = layered_head, .pools = layered_pools, .check = layered_check}
 static const CMLLMClass kLayeredClasses[] = {LAYERED_CLASS("Rarolorn"), LAYERED_CLASS("Situlorn"), LAYERED_CLASS("Lenedra"), LAYERED_CLASS("Zevilorn")};
 
 __attribute__((constructor)) static void register_layered(void) {

@@ -110,6 +110,8 @@ typedef struct Layer {             /* a layer of config.json, or one more pass o
 typedef struct Layered {
     const LayeredDesign* design;
     int f32, vocab, width, num_layers;
+    int cache8;                    /* 0, or the CMLB200_DT_ of an 8-bit cache */
+    int block_size;                /* of the pools */
     int streams;                   /* 0: one residual, no streams */
     float eps, embed_scale, cap;
     Layer* layers;

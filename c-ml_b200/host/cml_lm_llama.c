@@ -23,6 +23,7 @@ static void llama_lm_free(void* p) {
 static void* llama_lm_load(const char* path, const CMLJson* config, const CMLLMOptions* options, CMLLMInfo* info) {
     CMLLLaMAConfig c;
     if (config) { LOG_ERROR("llama models are read from GGUF files"); return NULL; }
+    if (options->cache != CML_LM_CACHE_DEFAULT) { LOG_ERROR("llama models keep 16-bit or 32-bit caches"); return NULL; }
     if (options->max_sequences > 32) { LOG_ERROR("llama models serve up to 32 sequences"); return NULL; }
     if (cml_llama_config_from_gguf(path, &c)) return NULL;
     if (options->max_tokens < c.max_seq_len) c.max_seq_len = options->max_tokens;

@@ -9,6 +9,8 @@
  * since the previous one (whole slot ranges per block), then launches cmlb200_paged_gqa_f32 with
  * the sequence's block table. Tokens must be written through cml_paged_cache_append.
  *
+ * Sequences may share blocks (cml_paged_cache_fork): the side table counts a block's owners, and the last one to let go of it returns it to the pool.
+ *
  * cml_paged_kv_cache_create_device makes a cache of bookkeeping alone, for models whose kernels write and
  * read device pools of their own through the block tables (cml_lm.c): blocks are taken with
  * cml_paged_cache_extend and those that every layer's window has passed go back with
@@ -22,9 +24,10 @@
 
 #define FAIL(call, who) CML_DEV_FAIL(call, who)
 
-/* Device side of a cache, found by the cache's address (the public struct has no room for it). */
+/* What the public struct has no room for, found by the cache's address: the owners of blocks, and the device side of a cache with data. */
 typedef struct PagedDev {
     const CMLPagedKVCache* key;
+    int* owners;                      /* per block: sequences that hold it (1 for a block taken by cml_paged_cache_alloc_block alone) */
     float *h_k, *h_v;                 /* host pools the blocks' key_data / value_data point into */
     void *d_k, *d_v;                  /* device pools, NULL until the first forward call */
     int* dev_tokens;                  /* per block: slots already uploaded since it was allocated */
@@ -42,6 +45,14 @@ static PagedDev* pd_find(const CMLPagedKVCache* c) {
     while (p && p->key != c) p = p->next;
     pthread_mutex_unlock(&g_paged_mu);
     return p;
+}
+
+static void pd_register(PagedDev* p, const CMLPagedKVCache* c) {
+    p->key = c;
+    pthread_mutex_lock(&g_paged_mu);
+    p->next = g_paged;
+    g_paged = p;
+    pthread_mutex_unlock(&g_paged_mu);
 }
 
 static size_t token_floats(const CMLPagedKVCache* c) { return (size_t)c->num_kv_heads * c->head_dim; }
@@ -68,9 +79,10 @@ CMLPagedKVCache* cml_paged_kv_cache_create(int max_blocks, int max_sequences, in
     p->h_k = (float*)calloc((size_t)max_blocks * bf, sizeof(float));
     p->h_v = (float*)calloc((size_t)max_blocks * bf, sizeof(float));
     p->dev_tokens = (int*)calloc((size_t)max_blocks, sizeof(int));
-    if (!c->blocks || !c->free_list || !c->sequences || !p->h_k || !p->h_v || !p->dev_tokens) {
+    p->owners = (int*)calloc((size_t)max_blocks, sizeof(int));
+    if (!c->blocks || !c->free_list || !c->sequences || !p->h_k || !p->h_v || !p->dev_tokens || !p->owners) {
         LOG_ERROR("cml_paged_kv_cache_create: allocation failed");
-        free(c->blocks); free(c->free_list); free(c->sequences); free(p->h_k); free(p->h_v); free(p->dev_tokens); free(c); free(p);
+        free(c->blocks); free(c->free_list); free(c->sequences); free(p->h_k); free(p->h_v); free(p->dev_tokens); free(p->owners); free(c); free(p);
         return NULL;
     }
     for (int i = 0; i < max_blocks; i++) {
@@ -80,11 +92,7 @@ CMLPagedKVCache* cml_paged_kv_cache_create(int max_blocks, int max_sequences, in
         c->free_list[i] = i;                               /* top of the stack = last element */
     }
     c->free_count = max_blocks;
-    p->key = c;
-    pthread_mutex_lock(&g_paged_mu);
-    p->next = g_paged;
-    g_paged = p;
-    pthread_mutex_unlock(&g_paged_mu);
+    pd_register(p, c);
     return c;
 }
 
@@ -94,22 +102,25 @@ CMLPagedKVCache* cml_paged_kv_cache_create_device(int max_blocks, int max_sequen
         return NULL;
     }
     CMLPagedKVCache* c = (CMLPagedKVCache*)calloc(1, sizeof *c);
-    if (!c) return NULL;
+    PagedDev* p = (PagedDev*)calloc(1, sizeof *p);
+    if (!c || !p) { LOG_ERROR("cml_paged_kv_cache_create_device: allocation failed"); free(c); free(p); return NULL; }
     c->max_blocks = c->num_blocks = c->free_count = max_blocks;
     c->max_sequences = max_sequences;
     c->block_size = block_size;
     c->blocks = (CMLPageBlock*)calloc((size_t)max_blocks, sizeof(CMLPageBlock));
     c->free_list = (int*)malloc((size_t)max_blocks * sizeof(int));
     c->sequences = (CMLBlockTable*)calloc((size_t)max_sequences, sizeof(CMLBlockTable));
-    if (!c->blocks || !c->free_list || !c->sequences) {
+    p->owners = (int*)calloc((size_t)max_blocks, sizeof(int));
+    if (!c->blocks || !c->free_list || !c->sequences || !p->owners) {
         LOG_ERROR("cml_paged_kv_cache_create_device: allocation failed");
-        free(c->blocks); free(c->free_list); free(c->sequences); free(c);
+        free(c->blocks); free(c->free_list); free(c->sequences); free(p->owners); free(c); free(p);
         return NULL;
     }
     for (int i = 0; i < max_blocks; i++) {
         c->blocks[i].block_id = i;
         c->free_list[i] = max_blocks - 1 - i;              /* block 0 is handed out first */
     }
+    pd_register(p, c);
     return c;
 }
 
@@ -123,7 +134,7 @@ void cml_paged_kv_cache_free(CMLPagedKVCache* cache) {
     pthread_mutex_unlock(&g_paged_mu);
     if (p) {
         cmlb200_free(p->d_k); cmlb200_free(p->d_v); cmlb200_free(p->d_ids); cmlb200_free(p->d_q); cmlb200_free(p->d_o);
-        free(p->h_k); free(p->h_v); free(p->dev_tokens); free(p);
+        free(p->h_k); free(p->h_v); free(p->dev_tokens); free(p->owners); free(p);
     }
     if (cache->sequences) {
         for (int i = 0; i < cache->max_sequences; i++) free(cache->sequences[i].block_ids);
@@ -145,8 +156,9 @@ int cml_paged_cache_alloc_block(CMLPagedKVCache* cache) {
         memset(b->key_data, 0, block_floats(cache) * sizeof(float));
         memset(b->value_data, 0, block_floats(cache) * sizeof(float));
     }
-    PagedDev* p = b->key_data ? pd_find(cache) : NULL;
-    if (p) p->dev_tokens[id] = 0;                          /* nothing of the new owner's tokens is on the device yet */
+    PagedDev* p = pd_find(cache);
+    if (p) p->owners[id] = 1;
+    if (p && b->key_data) p->dev_tokens[id] = 0;           /* nothing of the new owner's tokens is on the device yet */
     cache->total_allocated++;
     return id;
 }
@@ -155,6 +167,8 @@ void cml_paged_cache_free_block(CMLPagedKVCache* cache, int block_id) {
     if (!cache) { LOG_ERROR("cml_paged_cache_free_block: NULL cache"); return; }
     if (block_id < 0 || block_id >= cache->num_blocks) { LOG_ERROR("cml_paged_cache_free_block: invalid block_id %d", block_id); return; }
     if (!cache->blocks[block_id].in_use) { LOG_WARNING("cml_paged_cache_free_block: block %d already free", block_id); return; }
+    PagedDev* p = pd_find(cache);
+    if (p && --p->owners[block_id] > 0) return;            /* other sequences hold it */
     cache->blocks[block_id].in_use = false;
     cache->blocks[block_id].num_tokens = 0;
     cache->free_list[cache->free_count++] = block_id;
@@ -231,6 +245,85 @@ void cml_paged_cache_release_between(CMLPagedKVCache* cache, int seq_id, int fro
     }
 }
 
+int cml_paged_cache_fork(CMLPagedKVCache* cache, int seq_id, int* from, int* to) {
+    static const char* who = "cml_paged_cache_fork";
+    if (from) *from = -1;
+    if (to) *to = -1;
+    CMLBlockTable* bt = live_sequence(cache, seq_id);
+    PagedDev* p = bt ? pd_find(cache) : NULL;
+    if (!bt || !p) { LOG_ERROR("%s: sequence %d is not open", who, seq_id); return -1; }
+    const int data = cache->blocks[0].key_data != NULL, full = bt->seq_len / cache->block_size;
+    const int part = full < bt->num_blocks && bt->block_ids[full] >= 0 && bt->seq_len % cache->block_size;      /* a block that is not full */
+    if (part && !data && (!from || !to)) { LOG_ERROR("%s: nowhere to name the block to copy", who); return -1; }
+    if (part && cache->free_count <= 0) { LOG_ERROR("%s: no free blocks", who); return -1; }
+    int* ids = (int*)malloc((size_t)bt->capacity * sizeof(int));
+    if (!ids) { LOG_ERROR("%s: allocation failed", who); return -1; }
+    const int child = cml_paged_cache_init_sequence(cache);
+    if (child < 0) { free(ids); return -1; }
+    CMLBlockTable* ct = &cache->sequences[child];
+    free(ct->block_ids);
+    ct->block_ids = ids;
+    ct->capacity = bt->capacity;
+    ct->num_blocks = bt->num_blocks;
+    ct->seq_len = bt->seq_len;
+    for (int i = 0; i < bt->num_blocks; i++) {
+        ids[i] = bt->block_ids[i];
+        if (ids[i] < 0 || (part && i == full)) continue;
+        p->owners[ids[i]]++;
+    }
+    if (part) {
+        const int old = bt->block_ids[full], own = cml_paged_cache_alloc_block(cache);
+        ids[full] = own;
+        cache->blocks[own].num_tokens = cache->blocks[old].num_tokens;
+        if (data) {
+            memcpy(cache->blocks[own].key_data, cache->blocks[old].key_data, block_floats(cache) * sizeof(float));
+            memcpy(cache->blocks[own].value_data, cache->blocks[old].value_data, block_floats(cache) * sizeof(float));
+        }
+        if (from) *from = old;
+        if (to) *to = own;
+    }
+    return child;
+}
+
+int cml_paged_cache_compact(CMLPagedKVCache* cache, int* moves) {
+    static const char* who = "cml_paged_cache_compact";
+    PagedDev* p = cache ? pd_find(cache) : NULL;
+    if (!p) { LOG_ERROR("%s: not a cache", who); return -1; }
+    const int data = cache->blocks[0].key_data != NULL, n = cache->num_blocks, used = n - cache->free_count;
+    if (!data && !moves) { LOG_ERROR("%s: nowhere to name the blocks to copy", who); return -1; }
+    int* now = (int*)malloc((size_t)n * sizeof(int));      /* a block's new id */
+    if (!now) { LOG_ERROR("%s: allocation failed", who); return -1; }
+    int count = 0, hole = 0;
+    for (int i = 0; i < n; i++) now[i] = i;
+    for (int i = used; i < n; i++) {
+        if (!cache->blocks[i].in_use) continue;
+        while (cache->blocks[hole].in_use) hole++;
+        CMLPageBlock *a = &cache->blocks[i], *b = &cache->blocks[hole];
+        if (moves) { moves[2 * count] = i; moves[2 * count + 1] = hole; }
+        now[i] = hole;
+        b->in_use = true;
+        b->num_tokens = a->num_tokens;
+        a->in_use = false;
+        a->num_tokens = 0;
+        p->owners[hole] = p->owners[i];
+        p->owners[i] = 0;
+        if (data) {
+            memcpy(b->key_data, a->key_data, block_floats(cache) * sizeof(float));
+            memcpy(b->value_data, a->value_data, block_floats(cache) * sizeof(float));
+            p->dev_tokens[hole] = p->dev_tokens[i] = 0;
+        }
+        count++;
+    }
+    for (int s = 0; count && s < cache->max_sequences; s++) {
+        CMLBlockTable* bt = &cache->sequences[s];
+        for (int i = 0; bt->block_ids && i < bt->num_blocks; i++)
+            if (bt->block_ids[i] >= 0) bt->block_ids[i] = now[bt->block_ids[i]];
+    }
+    free(now);
+    for (int i = 0; count && i < n - used; i++) cache->free_list[i] = n - 1 - i;       /* the lowest is handed out first */
+    return count;
+}
+
 int cml_paged_cache_append(CMLPagedKVCache* cache, int seq_id, const float* key, const float* value) {
     if (!cache || !key || !value) { LOG_ERROR("cml_paged_cache_append: NULL argument"); return -1; }
     if (seq_id < 0 || seq_id >= cache->max_sequences) { LOG_ERROR("cml_paged_cache_append: invalid seq_id %d", seq_id); return -1; }
@@ -289,7 +382,7 @@ Tensor* cml_paged_gqa_forward(CMLPagedKVCache* cache, int seq_id, Tensor* Q, con
     float scale = config->scale;
     if (scale <= 0.0f) scale = 1.0f / sqrtf((float)D);
     PagedDev* p = pd_find(cache);
-    if (!p) { LOG_ERROR("%s: the cache was not created by cml_paged_kv_cache_create", who); return NULL; }
+    if (!p || !p->h_k) { LOG_ERROR("%s: the cache was not created by cml_paged_kv_cache_create", who); return NULL; }
 
     const size_t tf = token_floats(cache), bf = block_floats(cache), pool_bytes = (size_t)cache->num_blocks * bf * sizeof(float);
     if (!p->d_k && (FAIL(cmlb200_malloc(&p->d_k, pool_bytes), who) || FAIL(cmlb200_malloc(&p->d_v, pool_bytes), who))) {

@@ -1,6 +1,6 @@
 /* cml_generate -- generation from the command line, for every model of the registry.
  *
- *   cml_generate --model DIR|FILE.gguf [--dtype bfloat16|float32] [--max-tokens N] [--max-new N]
+ *   cml_generate --model DIR|FILE.gguf [--dtype bfloat16|float32] [--cache default|int8|e4m3] [--max-tokens N] [--max-new N]
  *                [--temperature T --top-k K --top-p P --seed S] [--eos ID]
  *                (--tokens 1,2,3 | --prompt TEXT) ...
  *
@@ -58,6 +58,7 @@ int main(int argc, char** argv) {
         if (!v) return fail("an option without a value", k);
         if (!strcmp(k, "--model")) model = v;
         else if (!strcmp(k, "--dtype")) dtype = v;
+        else if (!strcmp(k, "--cache")) o.cache = !strcmp(v, "int8") ? CML_LM_CACHE_INT8 : !strcmp(v, "e4m3") ? CML_LM_CACHE_E4M3 : !strcmp(v, "default") ? CML_LM_CACHE_DEFAULT : -1;
         else if (!strcmp(k, "--max-tokens")) o.max_tokens = atoi(v);
         else if (!strcmp(k, "--max-new")) max_new = atoi(v);
         else if (!strcmp(k, "--temperature")) { c.temperature = (float)atof(v); c.do_sample = true; }
@@ -72,7 +73,7 @@ int main(int argc, char** argv) {
         } else return fail("unknown option", k);
     }
     if (!model || !requests || (strcmp(dtype, "bfloat16") && strcmp(dtype, "float32")))
-        return fail("usage: cml_generate --model DIR|FILE.gguf [--dtype bfloat16|float32] [--max-tokens N] [--max-new N] [--temperature T] [--top-k K] "
+        return fail("usage: cml_generate --model DIR|FILE.gguf [--dtype bfloat16|float32] [--cache default|int8|e4m3] [--max-tokens N] [--max-new N] [--temperature T] [--top-k K] "
                     "[--top-p P] [--seed S] [--eos ID] (--tokens 1,2,3 | --prompt TEXT) ...", NULL);
     o.dtype = !strcmp(dtype, "float32") ? DTYPE_FLOAT32 : DTYPE_BFLOAT16;
     o.max_sequences = requests < 8 ? requests : 8;

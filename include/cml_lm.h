@@ -26,7 +26,13 @@ typedef struct CMLLMOptions {
     int max_tokens;             /* tokens the cache pool holds, all sequences together */
     int max_sequences;          /* sequences open at a time */
     int max_step_rows;          /* tokens of one step; 0: max_tokens */
+    int cache;                  /* CML_LM_CACHE_DEFAULT: 16-bit keys and values (32-bit in the 32-bit form). _INT8, _E4M3: 8 bits and a scale for
+                                   every 16 tokens and key/value head; serving form of models whose layers all have grouped attention
+                                   with heads up to 256, neither convolved nor with mixed scores */
 } CMLLMOptions;
+#define CML_LM_CACHE_DEFAULT 0
+#define CML_LM_CACHE_INT8 1
+#define CML_LM_CACHE_E4M3 2
 
 /* One sequence's part of a step: its next tokens, and the places among them (ascending) whose logits are
  * asked for. */
@@ -50,6 +56,11 @@ CMLTokenizer* cml_lm_tokenizer(const CMLLanguageModel* lm);      /* owned by the
 int cml_lm_sequence_open(CMLLanguageModel* lm);                  /* id, -1: no free slot */
 int cml_lm_sequence_close(CMLLanguageModel* lm, int seq);
 int cml_lm_sequence_length(CMLLanguageModel* lm, int seq);
+/* A new sequence that goes on from where `seq` stands: it shares the blocks that are full, has a copy of the one that is not, and of a recurrence's state.
+ * Id, -1: no free slot or block (or a class without a paged pool). */
+int cml_lm_sequence_fork(CMLLanguageModel* lm, int seq);
+/* Moves the blocks in use to the lowest ids of the pool. Returns how many moved, -1. */
+int cml_lm_compact(CMLLanguageModel* lm);
 /* Blocks of the pool (cml_lm_block_size tokens each): all of them, and those not in use. */
 int cml_lm_block_size(const CMLLanguageModel* lm);
 int cml_lm_blocks_total(const CMLLanguageModel* lm);
@@ -61,6 +72,11 @@ int cml_lm_blocks_free(const CMLLanguageModel* lm);
 int cml_lm_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, float* logits);
 /* The same, but picks the arg-max of every wanted row on the device: picked[sum of num_want]. */
 int cml_lm_step_greedy(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, int* picked);
+/* The same, but says on the device what the logits of every wanted row mean: the log probability of its token among targets[sum of num_want] (-1: none), the entropy
+ * of the row's distribution in nats, and the `top` (0 .. 32) likeliest tokens with their log probabilities, best first, the lower id first among equals
+ * (top_ids, top_logprobs [sum of num_want][top]). Outputs that are NULL are left out; targets and logprobs go together. See cmlb200_token_scores. */
+int cml_lm_step_scored(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const int* targets, int top, float* logprobs, float* entropies, int* top_ids,
+                       float* top_logprobs);
 /* Greedy decoding that stays on the device: `steps` steps of all sequences, each step's picks the next
  * one's tokens, out_tokens [steps][num_seqs]; *elapsed_ms (optional) is the time of the loop on the device. */
 int cml_lm_decode_greedy(CMLLanguageModel* lm, const int* seqs, const int* first_tokens, int num_seqs, int steps, int* out_tokens,

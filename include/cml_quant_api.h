@@ -329,6 +329,16 @@ int cml_paged_cache_blocks_for(CMLPagedKVCache* cache, int seq_id, int num_token
 int cml_paged_cache_extend(CMLPagedKVCache* cache, int seq_id, int num_tokens);
 void cml_paged_cache_release_before(CMLPagedKVCache* cache, int seq_id, int position);
 void cml_paged_cache_release_between(CMLPagedKVCache* cache, int seq_id, int from, int position);
+/* Additions. A block may belong to several sequences; it returns to the pool when the last of them lets go of it (cml_paged_cache_free_block
+ * takes one owner away).
+ * fork: a new sequence that holds what seq_id holds. Full blocks are shared; the block that is still being filled is doubled: its data
+ * in a cache that has any, otherwise the caller copies block *from to block *to (both -1 when there is none to copy; the pointers may be NULL for
+ * caches with data). -1: no free slot or block, and nothing changes.
+ * compact: blocks in use move to the lowest ids, as few as that takes, in the tables of all sequences (and with their data, where the cache has any; an id from
+ * cml_paged_cache_alloc_block that is in no table may be stale afterwards). moves
+ * [num_blocks][2] gets {from, to} in ascending order of `from`, for callers with pools of their own; may be NULL for caches with data. Returns their number, -1. */
+int cml_paged_cache_fork(CMLPagedKVCache* cache, int seq_id, int* from, int* to);
+int cml_paged_cache_compact(CMLPagedKVCache* cache, int* moves);
 /* Q [1, seq_q, num_heads*head_dim]; query row i sits at position seq_len - seq_q + i of the
  * sequence. Returns a new [1, seq_q, num_heads*head_dim] tensor, NULL on error. */
 Tensor* cml_paged_gqa_forward(CMLPagedKVCache* cache, int seq_id, Tensor* Q, const CMLGQAConfig* config);
