@@ -2,20 +2,28 @@
 //
 //   m = max x, S = sum e^(x - m), Q = sum e^(x - m) (x - m):   log p_t = x_t - m - ln S,   H = ln S - Q / S
 //
-// Both parts of H are positive, so nothing cancels. A row is read once, in 16-byte pieces, by a cluster of 1 to 8 CTAs (more for
-// fewer rows); m, S and Q are carried in fp32 and meet in a fixed order: warp, CTA, cluster. Bound by the bytes of the logits.
+// Both parts of H are positive, so nothing cancels. A row is read once, in 16-byte pieces, by a cluster of 1 to 8 CTAs (more for fewer rows). A thread carries S and Q
+// in fp32, relative to a reference that follows its largest value at a distance: it moves only when a value is above it by more than 6. Q and all exponents are in
+// units of ln 2, so a value costs one multiply-add, one exponential and, two values an instruction, its part of S and Q. Values where that
+// would overflow or lose digits (masked ones, the type's lowest, references beyond a million) are told apart by a piece's range and take a longer way. Threads, warps, CTAs and clusters join in a fixed order.
 //
 // The alternatives need no second pass over the row. A thread remembers the largest of its pieces; the k-th largest of the
 // maxima of the CTA's groups of eight threads is a bound that at least k values reach, and few threads hold anything that does. Their pieces are read
-// again (from L2) and what reaches the bound is collected and ranked by counting. Order: value, then lowest index; as keys, the value's
+// again (from L1 or L2) and what reaches the bound is collected and ranked by counting. Order: value, then lowest index; as keys, the value's
 // bits made monotonic above the index's complement. Should more be collected than there is room for (rows whose large values crowd in a
 // few threads' pieces), the k best are picked one after the other from the same pieces.
+//
+// Many rows are bound by the bytes of the logits and the exponentials beside them, few by the chain of barriers behind the pass. Measured: 2,000 rows of 128,000 bf16
+// 91.5 us (5.6 TB/s; 57 us are exponentials at 16 a clock and SM), 700 of 128,000 fp32 62.6 us (5.7 TB/s), 256 of 32,000 fp32 with the best 20 15.3 us (10.4 without),
+// one of 32,000 with the best 5 5.5 us. Requesting pieces a round ahead cost more registers, and so CTAs under way, than it gave (2,000 rows: 98 to 115 us).
+#include <type_traits>
+
 #include "lm_util.cuh"
 
 namespace {
 
-constexpr int TS_THREADS = 512, TS_WARPS = TS_THREADS / 32, TS_GROUPS = TS_THREADS / 8, TS_MOST = 32, TS_ROOM = 1024;
-static_assert(TS_GROUPS >= TS_MOST, "every group's best could be wanted");
+constexpr float kLn2 = 0.693147180559945f;
+constexpr int TS_MOST = 32, TS_ROOM = 1024;
 
 typedef unsigned long long u64;
 
@@ -29,33 +37,98 @@ __device__ __forceinline__ u64 key_of(float v, uint32_t index) { return v > -INF
 
 template <typename T> constexpr int kPer = 16 / (int)sizeof(T);
 template <typename T> __device__ __forceinline__ void widen_piece(const uint4& u, float (&x)[kPer<T>]) {
-    if constexpr (sizeof(T) == 4) {
-        x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
-    } else {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            T t[2];
-            memcpy(t, &w[i], 4);
-            x[2 * i] = widen(t[0]);
-            x[2 * i + 1] = widen(t[1]);
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            __half2 t;
+            memcpy(&t, &w[i], 4);
+            const float2 f = __half22float2(t);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
         }
     }
 }
-__device__ __forceinline__ uint4 ld_once(const void* p) {
+// largest and smallest of a piece (NaN aside); 16-bit values two at a time
+template <typename T> __device__ __forceinline__ void range_of(const uint4& u, float& most, float& least) {
+    if constexpr (sizeof(T) == 4) {
+        const float a = __uint_as_float(u.x), b = __uint_as_float(u.y), c = __uint_as_float(u.z), d = __uint_as_float(u.w);
+        most = fmaxf(fmaxf(a, b), fmaxf(c, d));
+        least = fminf(fminf(a, b), fminf(c, d));
+    } else {
+        typedef std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162> T2;
+        T2 t[4];
+        memcpy(t, &u, 16);
+        const T2 hi = __hmax2(__hmax2(t[0], t[1]), __hmax2(t[2], t[3])), lo = __hmin2(__hmin2(t[0], t[1]), __hmin2(t[2], t[3]));
+        most = widen(__hmax(hi.x, hi.y));
+        least = widen(__hmin(lo.x, lo.y));
+    }
+}
+__device__ __forceinline__ uint4 ld_row(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+// two fp32 operations an instruction
+__device__ __forceinline__ u64 two(float a, float b) { return ((u64)__float_as_uint(b) << 32) | __float_as_uint(a); }
+__device__ __forceinline__ float first(u64 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float second(u64 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) { u64 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ u64 add2(u64 a, u64 b) { u64 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 
+// S and Q of a part of a row, relative to m; Q and everything that exponents are made of in units of ln 2
 struct Sums { float m, s, q; };
-// what two disjoint parts of a row have together
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, a.s + b.s, a.q + b.q};                     // (NaN in s stays)
-    const float da = fmaxf(a.m - m, -1e30f), db = fmaxf(b.m - m, -1e30f), ca = __expf(da), cb = __expf(db);
-    return {m, a.s * ca + b.s * cb, ca * (a.q + da * a.s) + cb * (b.q + db * b.s)};
+__device__ __forceinline__ float warp_max(float v) { float m; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v)); return m; }
+// what the parts of every `lanes` lanes in turn (a power of two) have together; all lanes' largest is the same
+template <int lanes>
+__device__ __forceinline__ Sums join(const Sums& a) {
+    const float m = warp_max(a.m), d = fmaxf(a.m - m, -1e4f) * kLog2e, c = ex2(d);            // (nothing anywhere: c = 0, and NaN in s stays)
+    float q = c * fmaf(d, a.s, a.q), s = a.s * c;
+#pragma unroll
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    return {m, s, q};
 }
+
+constexpr float TS_TAME = 1048576.f;                   // references up to here: what fl(ref log2(e)) is off by stays below 2^-3
+constexpr float TS_LEAST = -1e37f;                     // values down to here: their products with log2(e) do not overflow
+constexpr float TS_LAZY = 6.f;                         // the reference moves when a value is above it by more than this: e^6 times fewer values than 2^30 fit fp32 easily
+
+// S and Q of a thread's values. The exponent of a value is x log2(e) - fl(ref log2(e)), one rounding; `shift` is what the second product's rounding moved the
+// reference by, and is put right when the reference moves and at the end.
+struct Running {
+    float ref = -INFINITY, minus = 0.f, shift = 0.f;
+    u64 s = 0ull, q = 0ull;
+    __device__ __forceinline__ void scale(float d) {                         // exponents grow by d
+        const float c = ex2(d);
+        const u64 c2 = two(c, c), d2 = two(d, d);
+        q = fma2(c2, fma2(d2, s, q), 0ull);
+        s = fma2(c2, s, 0ull);
+    }
+    __device__ __forceinline__ void move(float to) {
+        const float d = fmaxf(ref - to, -1e4f) * kLog2e - shift;
+        ref = to;
+        minus = fabsf(to) <= TS_TAME ? -(to * kLog2e) : 0.f;
+        shift = fabsf(to) <= TS_TAME ? fmaf(to, kLog2e, minus) : 0.f;
+        scale(d + shift);
+    }
+    // values beside masked ones, or as large as numbers get
+    __device__ __forceinline__ void take_wild(float x) {
+        const float t = fmaf(x - (ref == -INFINITY ? 0.f : ref), kLog2e, shift), e = ex2(t);
+        s = add2(s, two(e, 0.f));
+        q = fma2(two(e, 0.f), two(fmaxf(t, -1e4f), 0.f), q);
+    }
+    __device__ __forceinline__ Sums sums() {
+        scale(-shift);
+        return {ref, first(s) + second(s), first(q) + second(q)};
+    }
+};
 __device__ __forceinline__ uint32_t remote(const void* p, int rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
@@ -67,14 +140,16 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 // grid = rows * splits, clusters of `splits`.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(TS_THREADS)
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS)
 token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int* __restrict__ tokens, int top, int splits, float* __restrict__ logprob, float* __restrict__ entropy,
                     int* __restrict__ top_ids, float* __restrict__ top_logprob) {
-    constexpr int PER = kPer<T>;
-    __shared__ Sums w_sums[TS_WARPS], c_sums[8];
-    __shared__ u64 g_best[TS_GROUPS], bound, room[TS_ROOM], best[8 * TS_MOST], w_best[TS_WARPS];
-    __shared__ int stripes[TS_THREADS], num_stripes, num_room;
+    constexpr int PER = kPer<T>, WARPS = THREADS / 32, GROUPS = THREADS / 8;
+    static_assert(GROUPS >= TS_MOST, "every group's best could be wanted");
+    __shared__ Sums w_sums[WARPS], c_sums[8];
+    __shared__ u64 g_best[GROUPS], bound, room[TS_ROOM], c_best[8 * TS_MOST], last_room[8 * TS_MOST], w_best[WARPS];
+    __shared__ uint8_t holders[WARPS][32];
+    __shared__ int num_room, num_last;
     if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (met below: the cluster's CTAs have begun)
     dep_wait();
     dep_trigger();
@@ -84,88 +159,88 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
     const int head = min(vocab, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T)), pieces = (vocab - head) / PER, tail = vocab - head - pieces * PER;
     const int per = (pieces + splits - 1) / splits, lo = min(pieces, rank * per), hi = min(pieces, lo + per);
     const T* body = row + head;
-    Sums a = {-INFINITY, 0.f, 0.f};
-    u64 mine = 0ull;                                   // largest piece: its value's bits above the complement of its number
-    // n values whose piece has the number `piece` (a single value of head or tail is a piece of its own)
-    auto take = [&](const float* x, int n, uint32_t piece) {
-        float g = x[0];
-        for (int i = 1; i < n; i++) g = fmaxf(g, x[i]);
-        if (TOP) { const u64 k = key_of(g, piece); mine = k > mine ? k : mine; }
-        if (g > a.m) {
-            const float d = fmaxf(a.m - g, -1e30f), c = __expf(d);
-            a.q = c * (a.q + d * a.s);
-            a.s *= c;
-            a.m = g;
-        }
-        const float m = a.m == -INFINITY ? 0.f : a.m;
-        for (int i = 0; i < n; i++) {
-            const float d = x[i] - m, e = ex2(d * kLog2e);
-            a.s += e;
-            a.q = fmaf(e, fmaxf(d, -1e4f), a.q);
+    Running a;
+    float best = -INFINITY;                            // largest value, and the number of its piece
+    uint32_t best_piece = 0;
+    auto note = [&](float most, uint32_t piece) {
+        if (TOP && most > best) { best = most; best_piece = piece; }
+        if (most > a.ref + TS_LAZY) a.move(most);
+    };
+    auto take_one = [&](float x, uint32_t piece) { note(x, piece); a.take_wild(x); };
+    auto take = [&](const uint4& u, uint32_t piece) {
+        float most, least, x[PER];
+        range_of<T>(u, most, least);
+        widen_piece<T>(u, x);
+        note(most, piece);
+        if (least >= TS_LEAST && fabsf(a.ref) <= TS_TAME) {
+            const u64 unit = two(kLog2e, kLog2e), minus = two(a.minus, a.minus);
+#pragma unroll
+            for (int i = 0; i < PER; i += 2) {
+                const u64 t = fma2(two(x[i], x[i + 1]), unit, minus), e = two(ex2(first(t)), ex2(second(t)));
+                a.s = add2(a.s, e);
+                a.q = fma2(e, t, a.q);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++) a.take_wild(x[i]);
         }
     };
     // numbers of pieces ascend along the row: head values, pieces, tail values
     auto single = [&](int i) { return i < head ? (uint32_t)i : (uint32_t)(head + pieces + i); };
     const bool has_head = rank == 0 && (int)threadIdx.x < head, has_tail = rank == splits - 1 && (int)threadIdx.x < tail;
-    if (has_head) { const float x = widen(row[threadIdx.x]); take(&x, 1, single(threadIdx.x)); }
+    if (has_head) take_one(widen(row[threadIdx.x]), single(threadIdx.x));
     int v = lo + threadIdx.x;
-    for (; v + 3 * TS_THREADS < hi; v += 4 * TS_THREADS) {
+    for (; v + 3 * THREADS < hi; v += 4 * THREADS) {
         uint4 u[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) u[j] = ld_once(body + (size_t)(v + j * TS_THREADS) * PER);
+        for (int j = 0; j < 4; j++) u[j] = ld_row(body + (size_t)(v + j * THREADS) * PER);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float x[PER];
-            widen_piece<T>(u[j], x);
-            take(x, PER, (uint32_t)(head + v + j * TS_THREADS));
-        }
+        for (int j = 0; j < 4; j++) take(u[j], (uint32_t)(head + v + j * THREADS));
     }
-    for (; v < hi; v += TS_THREADS) {
-        float x[PER];
-        widen_piece<T>(ld_once(body + (size_t)v * PER), x);
-        take(x, PER, (uint32_t)(head + v));
-    }
-    if (has_tail) { const float x = widen(body[(size_t)pieces * PER + threadIdx.x]); take(&x, 1, single(head + threadIdx.x)); }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.q, o)});
-    if (lane == 0) w_sums[warp] = a;
+    for (; v < hi; v += THREADS) take(ld_row(body + (size_t)v * PER), (uint32_t)(head + v));
+    if (has_tail) take_one(widen(body[(size_t)pieces * PER + threadIdx.x]), single(head + threadIdx.x));
+    const Sums w_part = join<32>(a.sums());
+    if (lane == 0) w_sums[warp] = w_part;
+    const u64 mine = TOP ? key_of(best, best_piece) : 0ull;
     if (TOP) {
         u64 g = mine;
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) { const u64 x = __shfl_xor_sync(0xffffffffu, g, o); g = x > g ? x : g; }
         if ((lane & 7) == 0) g_best[threadIdx.x >> 3] = g;
-        if (threadIdx.x == 0) { bound = 1ull; num_stripes = 0; num_room = 0; }
+        if (threadIdx.x == 0) { bound = 1ull; num_room = 0; num_last = 0; }
     }
     if (splits > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) {
-        Sums t = w_sums[0];
-#pragma unroll
-        for (int w = 1; w < TS_WARPS; w++) t = join(t, w_sums[w]);
+    if (warp == 0) {
+        const Sums none = {-INFINITY, 0.f, 0.f}, t = join<32>(lane < WARPS ? w_sums[lane] : none);
         const uint32_t dst = remote(&c_sums[rank], 0);
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(t.m) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(t.s) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(t.q) : "memory");
+        if (lane == 0) {
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(t.m) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(t.s) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(t.q) : "memory");
+        }
     }
     if (TOP) {
-        if (threadIdx.x < TS_GROUPS) {                 // the bound: the top-th largest of the groups' best, or nothing where fewer have any
-            const u64 k = g_best[threadIdx.x];
-            int above = 0;
-#pragma unroll 8
-            for (int i = 0; i < TS_GROUPS; i++) above += g_best[i] > k;
-            if (k && above == top - 1) bound = k;
-        }
+        // the bound: the top-th largest of the groups' best, or nothing where fewer have any. A group's threads share the comparing
+        const u64 g = g_best[threadIdx.x >> 3];
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < GROUPS / 8; i++) above += g_best[8 * i + (lane & 7)] > g;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (g && above == top - 1) bound = g;          // (all of a group's threads have found the same)
         __syncthreads();
-        if (mine >= bound) stripes[atomicAdd(&num_stripes, 1)] = threadIdx.x;
-        __syncthreads();
-        const int ns = num_stripes, most = (hi - lo + TS_THREADS - 1) / TS_THREADS;        // pieces of a thread, and its head and tail value
         const u64 floor_ = bound;
-        // calls f(value, index, piece) for what the listed threads went through
+        const uint32_t hit = __ballot_sync(0xffffffffu, mine >= floor_);
+        const int ns = __popc(hit), most = (hi - lo + THREADS - 1) / THREADS;        // pieces of a thread, and its head and tail value
+        if (mine >= floor_) holders[warp][__popc(hit & ((1u << lane) - 1))] = (uint8_t)lane;
+        __syncwarp();
+        // calls f(value, index, piece) for what the warp's threads that hold anything went through
         auto again = [&](auto f) {
-            for (int i = threadIdx.x; i < ns * (most + 2); i += TS_THREADS) {
-                const int j = i / ns, t = stripes[i - j * ns];
+            for (int i = lane; i < ns * (most + 2); i += 32) {
+                const int j = i / ns, t = warp * 32 + holders[warp][i - j * ns];
                 if (j < most) {
-                    const int w = lo + t + j * TS_THREADS;
+                    const int w = lo + t + j * THREADS;
                     if (w >= hi) continue;
                     float x[PER];
                     widen_piece<T>(*reinterpret_cast<const uint4*>(body + (size_t)w * PER), x);
@@ -185,9 +260,9 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
         });
         __syncthreads();
         const int nr = num_room;
-        const uint32_t dst = remote(&best[rank * top], 0);
+        const uint32_t dst = remote(&c_best[rank * top], 0);
         if (nr <= TS_ROOM) {
-            for (int i = threadIdx.x; i < nr; i += TS_THREADS) {
+            for (int i = threadIdx.x; i < nr; i += THREADS) {
                 const u64 k = room[i];
                 int above = 0;
                 for (int j = 0; j < nr; j++) above += room[j] > k;
@@ -204,7 +279,7 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
                 __syncthreads();
                 if (lane == 0) w_best[warp] = next;
                 __syncthreads();
-                for (int w = 0; w < TS_WARPS; w++) next = w_best[w] > next ? w_best[w] : next;
+                for (int w = 0; w < WARPS; w++) next = w_best[w] > next ? w_best[w] : next;
                 last = next;
                 if (threadIdx.x == 0) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dst + 8 * n), "l"(next) : "memory");
             }
@@ -213,8 +288,7 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
     if (splits > 1) cluster_sync();
     else __syncthreads();
     if (rank) return;                                  // (nobody reads another CTA's memory from here on)
-    Sums t = c_sums[0];
-    for (int s = 1; s < splits; s++) t = join(t, c_sums[s]);
+    const Sums none = {-INFINITY, 0.f, 0.f}, t = join<8>((lane & 7) < splits ? c_sums[lane & 7] : none);
     const bool nothing = t.m == -INFINITY && t.s == 0.f;
     const float ls = logf(t.s);
     if (threadIdx.x == 0) {
@@ -222,28 +296,44 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
             const int id = tokens[r];
             logprob[r] = nothing || id < 0 || id >= vocab ? -INFINITY : (widen(row[id]) - t.m) - ls;
         }
-        if (entropy) entropy[r] = nothing ? 0.f : ls - t.q / t.s;
+        if (entropy) entropy[r] = nothing ? 0.f : ls - t.q / t.s * kLn2;
     }
-    if (TOP)
-        for (int i = threadIdx.x; i < splits * top; i += TS_THREADS) {
-            const u64 k = best[i];
-            int above = 0;
-            for (int j = 0; j < splits * top; j++) above += best[j] > k || (best[j] == k && j < i);        // (only places without a value are equal)
+    if (TOP) {
+        // what each CTA of the cluster found is in order; nothing below any CTA's last can be wanted
+        const int n = splits * top;
+        u64 least = 0ull;
+        for (int i = 0; i < splits; i++) { const u64 k = c_best[i * top + top - 1]; least = k > least ? k : least; }
+        for (int i = threadIdx.x; i < n; i += THREADS)
+            if (c_best[i] && c_best[i] >= least) last_room[atomicAdd(&num_last, 1)] = c_best[i];
+        __syncthreads();
+        const int found = num_last;
+        for (int i = threadIdx.x; i < max(found, top); i += THREADS) {
+            const u64 k = i < found ? last_room[i] : 0ull;
+            int above = i < found ? 0 : i;             // (places without a value come last)
+            for (int j = 0; i < found && j < found; j++) above += last_room[j] > k;
             if (above >= top) continue;
             const size_t at = (size_t)r * top + above;
             if (top_ids) top_ids[at] = k ? (int)~(uint32_t)k : -1;
             if (top_logprob) top_logprob[at] = k ? (order_value((uint32_t)(k >> 32)) - t.m) - ls : -INFINITY;
         }
+    }
 }
 
 template <typename T>
 int launch_scores(const void* d_logits, long ld, int rows, int vocab, const int* d_tokens, int top, float* d_logprob, float* d_entropy, int* d_top_ids, float* d_top_logprob, cudaStream_t st) {
-    // a cluster's CTAs read at least 8 KB each: more of them while rows are fewer than two CTAs an SM
+    // A cluster's CTAs read at least 8 KB each; more of them share a row while every one has an SM of its own (64 rows of 50,000 bf16, best 20: 8.3 us by
+    // two each, 9.3 by one, 11 by four)
     int splits = 1;
-    while (splits < 8 && (long long)rows * splits < 2 * cmlb_num_sms() && (size_t)vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
+    while (splits < 8 && (long long)rows * splits * 2 <= cmlb_num_sms() && (size_t)vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
+    // Many short rows are a matter of how many CTAs are under way, not of how fast each is: 256 threads for those (2,000 rows of 1,000, best 5: 14.3 us, with
+    // 512 threads 24.8; 256 rows of 32,000, best 20: 19.3 and 15.3)
+    const bool small = (long long)rows >= 4 * cmlb_num_sms() && (size_t)vocab * sizeof(T) <= 65536;
     const dim3 grid((unsigned)rows * splits);
-    if (top) CMLB_CUDA(launch_chain(token_scores_kernel<T, true>, grid, dim3(TS_THREADS), 0, splits, st, (const T*)d_logits, ld, vocab, d_tokens, top, splits, d_logprob, d_entropy, d_top_ids, d_top_logprob));
-    else CMLB_CUDA(launch_chain(token_scores_kernel<T, false>, grid, dim3(TS_THREADS), 0, splits, st, (const T*)d_logits, ld, vocab, d_tokens, top, splits, d_logprob, d_entropy, d_top_ids, d_top_logprob));
+    auto run = [&](auto kernel, int threads) {
+        return launch_chain(kernel, grid, dim3(threads), 0, splits, st, (const T*)d_logits, ld, vocab, d_tokens, top, splits, d_logprob, d_entropy, d_top_ids, d_top_logprob);
+    };
+    if (top) CMLB_CUDA(small ? run(token_scores_kernel<T, true, 256>, 256) : run(token_scores_kernel<T, true, 512>, 512));
+    else CMLB_CUDA(small ? run(token_scores_kernel<T, false, 256>, 256) : run(token_scores_kernel<T, false, 512>, 512));
     return CMLB200_OK;
 }
 

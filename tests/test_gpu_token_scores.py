@@ -145,3 +145,38 @@ def test_streams_and_graphs(pkg, torch_dev):
         assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(out, a))
         x.copy_(torch.randn(3, 5001, device=torch_dev))
         a = call(pkg, torch, x, [1, 2, 3], 5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab,top", [(3, 2), (1000, 32), (5003, 1), (16383, 0)])
+def test_many_short_rows(pkg, torch_dev, dtype, vocab, top):
+    """Enough rows that each is read by few threads; some of special values among them."""
+    import torch
+    x = torch.randn(900, vocab, generator=torch.Generator(device=torch_dev).manual_seed(vocab), device=torch_dev) * 2
+    x[10] = -float("inf")
+    x[20, ::2] = -float("inf")
+    x[30, 1] = float("nan")
+    x[40] = 0
+    x = x.to(getattr(torch, dtype))
+    tokens = np.random.default_rng(vocab).integers(0, vocab, 900)
+    compare(call(pkg, torch, x, tokens, top), want(x.float().cpu().numpy(), tokens, top), vocab)
+
+
+@pytest.mark.parametrize("rows", [1, 900])
+def test_logits_far_from_zero(pkg, torch_dev, rows):
+    """The result knows differences alone. An exponent is off by a rounding of itself, wherever the row lies; numbers whose products overflow included."""
+    import torch
+    vocab = 4099
+    x = np.random.default_rng(rows).standard_normal((rows, vocab)).astype(np.float32)
+    for r, shift in zip(range(rows), [9000.0] * (rows == 1) or np.tile([5e4, -5e4, 1e6, -3e6, 0.0], rows)):
+        x[r] += np.float32(shift)
+    if rows > 1:
+        x[50] = np.float32(-3.4e38); x[50, 7] = np.float32(-1e37)
+        x[51] = np.float32(3e38); x[51, ::3] = np.float32(2.9e38)
+        x[52, ::5] = np.float32(-2e38)
+        x[53] = np.linspace(-1e38, 1e38, vocab, dtype=np.float32)
+        x[54] = np.sort(x[54]); x[54, 4000:] += np.float32(100)
+        x[55] = np.linspace(-50, 50, vocab, dtype=np.float32)             # the reference moves all the way
+    tokens = np.random.default_rng(5).integers(0, vocab, rows)
+    got, ref = call(pkg, torch, torch.from_numpy(x).to(torch_dev), tokens, 7), want(x, tokens, 7)
+    compare(got, ref, vocab)
