@@ -1,6 +1,6 @@
 // Prompt portions over 8-bit caches (cache8.cuh) on the 5th-generation tensor cores.
 //
-// A CTA takes a tile of up to 64 consecutive rows of one sequence and two query heads of a key/value head, 128 rows of the products, and walks key
+// A CTA takes a tile of up to 64 consecutive rows of one sequence and some of a key/value head's query heads, 128 rows of the products, and walks key
 // tiles of 128 tokens: S = Q K^T into one of two accumulators in tensor memory, O += P V with P in tensor memory over the scores it came from. Roles, by warp:
 //   0 .. 7    softmax, two threads a row with 64 keys each (the warps w and w + 4 meet for the row's largest score): all scores in registers, then
 //             exponentials straight into P. The reference of the exponentials moves, and O is scaled, only when a row has grown by more than 8 (powers of two)
@@ -8,7 +8,7 @@
 //             shared memory, keys with the dimensions contiguous, values with theirs as the contiguous non-summed side, both with 128-byte swizzle. Codes are
 //             exact in fp16; scales stay apart: a group's key scale multiplies its scores, its value scale joins the exponent of its weights
 //   16        issues tcgen05.mma: the scores of tile i + 1, then P V of tile i, so that products and softmax overlap
-// Queries are fp16 over a power of two per row and head. Weights are 2^(s - m) times the value scale over the largest so far, times 128: at most 2^15.
+// Rows are (head, token) pairs, one head after the other, so short tiles fill few blocks; queries are fp16 over a power of two of their own. Weights are 2^(s - m) times the value scale over the largest so far, times 128: at most 2^15.
 // Few tiles: a cluster of up to 8 CTAs splits the keys and merges through distributed shared memory.
 // Keys behind a portion's last row are read as that row's (their weights are zero), so nothing other requests left can reach the sums. Every wait is
 // bounded; one that gives up leaves a code in a status word in host memory, the products under way are waited for and tensor memory is freed.
@@ -32,7 +32,7 @@ constexpr int T8_TMEM = 512, T8_O_COL = 256;
 // registers of a thread: 96 at launch, then shared out by role (128 x 256 + 80 x 256 + 64 x 128 = 96 x 640)
 constexpr int T8_SOFT_REGS = 128, T8_CONV_REGS = 80, T8_ISSUE_REGS = 64;
 
-// grid = (splits, kv_heads * blocks, tiles), clusters of `splits`; a block is two query heads.
+// grid = (splits, kv_heads * blocks, tiles), clusters of `splits`; a block is 128 (head, token) rows; those behind a short tile's last end at once.
 template <bool I8, int S, bool SLOPES>
 __global__ void __launch_bounds__(T8<S>::kThreads, 1)
 attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int ld, const int4* __restrict__ tiles, __nv_bfloat16* __restrict__ out, int out_ld, const T8Plan plan,
@@ -76,25 +76,37 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     }
     // first phase of the cluster's barrier: nothing is stored into another CTA before that one runs
     if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    dep_wait();
-    const int4 tl = tiles[gridDim.z - 1 - blockIdx.z];                       // a prompt's last tiles, which see most keys, come first
-    const int group = a.heads / a.kv_heads, blocks = gridDim.y / a.kv_heads, kh = blockIdx.y / blocks, hb = blockIdx.y % blocks * 2;
-    const int n = tl.y, p0 = tl.w, p_last = p0 + n - 1, shift = __ffs(a.block_size) - 1;
-    const int* table = a.block_table + (size_t)tl.z * a.table_ld;
-    const T8Keys keys(a, p0, p_last, rank, splits);
-    const int count = keys.count;
-    if (count > 0) t8_queries<S, T8_ROWS, C::kThreads / 32>(a, qkv, ld, tl, n, kh, hb, group, smem, unit_s);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const int group = a.heads / a.kv_heads, blocks = gridDim.y / a.kv_heads, kh = blockIdx.y / blocks, first_row = (int)(blockIdx.y % blocks) * T8_ROWS, shift = __ffs(a.block_size) - 1;
+    dep_wait();
     dep_trigger();                                     // a launch that allocates tensor memory too may start from here on: every CTA of this one has its own
+    const int4 tl = tiles[gridDim.z - 1 - blockIdx.z];                       // a prompt's last tiles, which see most keys, come first
+    const int n = tl.y, p0 = tl.w, p_last = p0 + n - 1;
+    const T8Rows rows(n, group, first_row);
+    if (rows.none()) {                                 // (the whole cluster's; nothing has been issued)
+        if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp == kIssue) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)T8_TMEM) : "memory");
+        return;
+    }
+    const int* table = a.block_table + (size_t)tl.z * a.table_ld;
+    const T8Keys keys(a, p0, p_last, rank, splits);
+    const int count = keys.count;
+    // the queries, by all warps but those of the expansion, which begin with the first keys meanwhile
+    auto queries = [&](int w) {
+        if (count > 0) t8_queries<S, T8_ROWS, C::kSoft + 4>(a, qkv, ld, tl, rows, kh, smem, unit_s, w);
+        asm volatile("bar.sync 5, %0;" ::"n"(32 * (C::kSoft + 4)) : "memory");
+    };
 
     if (warp < kConv) {                                // ---- softmax
+        queries(warp);
         more_registers<T8_SOFT_REGS>();
-        const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, i_tok = r & 63, h = hb + (r >> 6);
+        const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        int i_tok, h;
+        const bool live = rows.find(r, i_tok, h);
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), o_at = lanes + T8_O_COL;
-        const bool live = i_tok < n && h < group;
         // (rows that are none have queries of zero and see what the last one sees; nobody looks at theirs)
         const int p = live ? p0 + i_tok : p_last, lo = first_key8(a, p), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
         const float unit = unit_s[r], slope = SLOPES && live ? a.slopes[head] * kLog2e : 0.f;
@@ -227,8 +239,9 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
             cluster_meet();
             const int quads = dv / 4;
             for (int e = rank * (32 * C::kSoft) + threadIdx.x; e < T8_ROWS * quads; e += splits * (32 * C::kSoft)) {
-                const int k = e / quads, c = (e - k * quads) * 4, tok = k & 63, hh = hb + (k >> 6);
-                if (tok >= n || hh >= group) continue;
+                const int k = e / quads, c = (e - k * quads) * 4;
+                int tok, hh;
+                if (!rows.find(k, tok, hh)) continue;
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y[T8_SPLITS];
 #pragma unroll
                 for (int s = 0; s < T8_SPLITS; s++) {
@@ -285,6 +298,7 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
                 if (++st == stages) { st = 0; par ^= 1; }
             }
         } else {                                       // ---- products
+            queries(warp - 2 * C::kConv);
             fewer_registers<T8_ISSUE_REGS>();
             if (warp == kIssue && count > 0) {
                 // fp16 operands, fp32 accumulators, 128 rows; the second one takes V with its columns contiguous

@@ -58,13 +58,14 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
     }
     dep_wait();
     const int4 tl = tiles[gridDim.y - 1 - blockIdx.y];                       // a prompt's last tiles, which see most keys, come first
-    const int group = a.heads / a.kv_heads, blocks = gridDim.x / a.kv_heads, kh = blockIdx.x / blocks, hb = blockIdx.x % blocks * 4;
+    const int group = a.heads / a.kv_heads, blocks = gridDim.x / a.kv_heads, kh = blockIdx.x / blocks;
     const int n = tl.y, p0 = tl.w, p_last = p0 + n - 1, shift = __ffs(a.block_size) - 1;
+    const T8Heads rows = {n, group, (int)(blockIdx.x % blocks) * 4};
     const int* table = a.block_table + (size_t)tl.z * a.table_ld;
     const T8Keys keys(a, p0, p_last, 0, 1);
     // half tiles; the last one is left out where it lies behind the last row
     const int count = keys.count, halves = 2 * count - (keys.start(count - 1) + 64 > p_last ? 1 : 0);
-    t8_queries<S, C::kRows, C::kThreads / 32>(a, qkv, ld, tl, n, kh, hb, group, smem, unit_s);
+    t8_queries<S, C::kRows, C::kThreads / 32>(a, qkv, ld, tl, rows, kh, smem, unit_s, warp);
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
@@ -73,9 +74,10 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
 
     if (warp < kConv) {                                // ---- softmax
         more_registers<W8_SOFT_REGS>();
-        const int m = warp >> 2, r = (warp & 3) * 32 + lane, i_tok = r & 63, h = hb + 2 * m + (r >> 6);
+        const int m = warp >> 2, r = (warp & 3) * 32 + lane;
+        int i_tok, h;
+        const bool live = rows.find(m * T8_ROWS + r, i_tok, h);
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), o_at = lanes + W8_O_COL + m * (S * 64);
-        const bool live = i_tok < n && h < group;
         // (rows that are none have queries of zero and see what the last one sees; nobody looks at theirs)
         const int p = live ? p0 + i_tok : p_last, lo = first_key8(a, p), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
         const float unit = unit_s[m * T8_ROWS + r], slope = SLOPES && live ? a.slopes[head] * kLog2e : 0.f;

@@ -356,3 +356,14 @@ def test_bounded_waits_did_not_expire(pkg, torch_dev):
     st = ctypes.c_int(-1)
     pkg.check(pkg.lib.cmlb200_attention8_status(ctypes.byref(st), 0))
     assert st.value == 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("heads,kv_heads", [(12, 1), (7, 1), (14, 2), (64, 2), (5, 5)])
+def test_short_tiles_of_many_heads(pkg, torch_dev, form, heads, kv_heads):
+    """Tiles whose rows and heads share blocks of 128 in every way: few rows of many heads, one less and one more than fill a block, the last tiles of longer portions."""
+    L = Layer(pkg, torch_dev, form, heads, kv_heads, 40, 24, page=16, slopes=heads == 12, sink="own" if heads == 14 else None)
+    L.ld += -L.ld % 4 if heads % 2 == 0 else 0         # rows that begin on 16 bytes, and that do not
+    for parts in ([(0, 2), (1, 3), (2, 18)], [(0, 19), (1, 10), (2, 11)], [(0, 37), (1, 64), (2, 65)], [(0, 5), (1, 77), (2, 63)], [(0, 4), (1, 128), (2, 2)]):
+        L.step(parts)
+    L.check_cache()
