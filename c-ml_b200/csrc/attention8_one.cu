@@ -7,8 +7,10 @@
 //                                        a lane's four consecutive codes are its four columns, and no shuffle or shared memory is needed
 //   O^T [16 dims x 8 heads] += V^T P^T   A: a lane holds the same 8, 16 or 32 dimensions of the keys 2t, 2t + 1, 2t + 8, 2t + 9; bytes of two keys are
 //                                        interleaved, which makes the operand's pairs. P^T comes from S^T by movmatrix
-// so a lane's operands are its own pieces of the cache. It copies them asynchronously into places of its own in shared memory, three to six groups ahead (groups of 4 KB a
-// warp at heads of 128: 16 warps an SM with one group each under way in registers read 4.1 TB/s). int8 keys stay 1,152 too large, as they come out of their conversion: the
+// so a lane's operands are pieces of the cache as they lie there. One TMA copy a group brings 16 tokens of a head (128 bytes of every kv_heads * 128 at heads of 128),
+// three to six groups ahead of the warp that asked for them; group numbers and scales are looked up 32 at a time, one a lane. (32 rows of 8 heads behind 8,192 tokens,
+// 537 MB: 103 us, 5.2 TB/s. With 16-byte copies by the lanes themselves it took 138 us, 133 without any arithmetic; with one group a warp under way in registers 135.)
+// The next group's scores are issued beside one group's value products. int8 keys stay 1,152 too large, as they come out of their conversion: the
 // scores' accumulators begin at -1,152 times the sum of the head's queries, so every term is exact and the fp32 sums are off by no more than the queries' own rounding.
 // A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
 // where m, the warp's reference for the exponentials, moves only when a score has passed it by 7 (powers of two; sums are fp32). Queries are fp16 over
@@ -17,24 +19,24 @@
 // share of the outputs. The group that the row's own token joins belongs to rank 0 alone, which settles its scales, rewrites it where they have grown and
 // attends to it from shared memory; nobody else looks at it.
 #include "cache8.cuh"
+#include "tcgen05_util.cuh"
 
 namespace {
 
 constexpr int A1_SPLITS = 8, A1_WARPS = 8, A1_THREADS = 32 * A1_WARPS;
-// groups that a warp has under way: as many as shared memory holds at two CTAs an SM (one where registers allow no more)
+// groups that a warp has under way: as many as shared memory holds at two CTAs an SM (at one, where registers allow no more)
 template <int KC, int NT> constexpr int kAhead = KC == 1 ? 6 : (KC == 2 && NT == 2) ? 6 : 3;
-template <int KC, int VW> constexpr int kGroupBytes = 32 * (32 * KC + 16 * VW) + 16;
+template <int KC, int VW> constexpr int kGroupBytes = 1024 * KC + 512 * VW;
 constexpr float kWeightUnit = 256.f;
 
 __device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
     if (a.chunk > 0) return p / a.chunk * a.chunk;
     return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
 }
-// 16 or 8 bytes into shared memory, or zeros
-template <int BYTES> __device__ __forceinline__ void copy_codes(uint32_t dst, const uint8_t* src, bool there) {
-    const int n = there ? BYTES : 0;
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+// 16 tokens of one head, `group` of the pool, from dimension d on
+__device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap* map, int d, int head, int group, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(d), "r"(head), "r"(0), "r"(group), "r"(bar) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -67,50 +69,48 @@ __device__ __forceinline__ Places places_of(int kstride, int vstride, int piece,
     for (int i = 0; i < 4; i++) p.v[i] = min(2 * t + (i & 1) + 8 * (i >> 1), last) * vstride + piece * g;
     return p;
 }
-// A group's pieces on their way into the lane's places: keys' pieces, then values', each 32 lanes' side by side.
-template <int KC, int VW>
-__device__ __forceinline__ void copy_group(uint32_t to, const uint8_t* k, const uint8_t* v, const Places& p, int dk, int dv, int lane) {
+// Where piece `chunk` (16 dimensions) of a group's token lies behind the group's copy: rows of 64 or 128 bytes with the copy's swizzle of that width, 128 dimensions
+// after 128.
+template <int SLABS> __device__ __forceinline__ int place_of(int token, int chunk) {
+    if constexpr (SLABS == 1) return 64 * token + ((chunk ^ ((token >> 1) & 3)) << 4);
+    else return (chunk >> 3) * (kScaleTokens * 128) + 128 * token + (((chunk ^ token) & 7) << 4);
+}
+template <int KC>
+__device__ __forceinline__ void take_keys(KeyCodes<KC>& x, const uint8_t* from, int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int c = 0; c < KC; c++) copy_codes<16>(to + 512 * (i * KC + c) + 16 * lane, k + p.k[i] + 64 * c, 64 * c + 16 * t < dk);
-    to += 1024 * KC;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (VW == 2) {
-            copy_codes<8>(to + 256 * i + 8 * lane, v + p.v[i], 8 * g < dv);
-        } else {
-#pragma unroll
-            for (int c = 0; c < VW / 4; c++) copy_codes<16>(to + 512 * (i * (VW / 4) + c) + 16 * lane, v + p.v[i] + 128 * c, 128 * c + 16 * g < dv);
-        }
-    }
-}
-template <int KC>
-__device__ __forceinline__ void take_keys(KeyCodes<KC>& x, const uint8_t* from, int lane) {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
         for (int c = 0; c < KC; c++) {
-            const uint4 u = *reinterpret_cast<const uint4*>(from + 512 * (i * KC + c) + 16 * lane);
+            const uint4 u = *reinterpret_cast<const uint4*>(from + place_of<KC>(g + 8 * i, 4 * c + t));
             x.w[i][c][0] = u.x; x.w[i][c][1] = u.y; x.w[i][c][2] = u.z; x.w[i][c][3] = u.w;
         }
 }
+// `last`: what tokens behind it hold is taken as zero
 template <int KC, int VW>
-__device__ __forceinline__ void take_values(ValueCodes<VW>& x, const uint8_t* from, int lane) {
+__device__ __forceinline__ void take_values(ValueCodes<VW>& x, const uint8_t* from, int last, int lane) {
+    const int g = lane >> 2, t = lane & 3;
     from += 1024 * KC;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
+        const int token = 2 * t + (i & 1) + 8 * (i >> 1);
         if constexpr (VW == 2) {
-            const uint2 u = *reinterpret_cast<const uint2*>(from + 256 * i + 8 * lane);
+            const uint2 u = *reinterpret_cast<const uint2*>(from + place_of<1>(token, g >> 1) + 8 * (g & 1));
             x.w[i][0] = u.x; x.w[i][1] = u.y;
         } else {
 #pragma unroll
             for (int c = 0; c < VW / 4; c++) {
-                const uint4 u = *reinterpret_cast<const uint4*>(from + 512 * (i * (VW / 4) + c) + 16 * lane);
+                const uint4 u = *reinterpret_cast<const uint4*>(from + place_of<2>(token, 8 * c + g));
                 x.w[i][4 * c] = u.x; x.w[i][4 * c + 1] = u.y; x.w[i][4 * c + 2] = u.z; x.w[i][4 * c + 3] = u.w;
             }
         }
+    }
+    if (last < kScaleTokens - 1) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int c = 0; c < VW; c++)
+                if (2 * t + (i & 1) + 8 * (i >> 1) > last) x.w[i][c] = 0u;
     }
 }
 // The same from the row's own group, which lies in shared memory token by token.
@@ -261,19 +261,29 @@ __device__ __forceinline__ void value_products(State<VW, NT>& st, const ValueCod
 // (one pass then), otherwise they are in it.
 template <bool I8, int KC, int VW, int NT>
 __global__ void __launch_bounds__(A1_THREADS, KC == 4 || NT == 2 ? 1 : 2)
-attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int ld, const int* __restrict__ row_pos, const int* __restrict__ row_slot, int append,
-                      __nv_bfloat16* __restrict__ out, int out_ld) {
+attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const cmlb200_attn a, const float* __restrict__ qkv, int ld,
+                      const int* __restrict__ row_pos, const int* __restrict__ row_slot, int append, __nv_bfloat16* __restrict__ out, int out_ld, int* status) {
     constexpr int HN = 8 * NT, AHEAD = kAhead<KC, NT>, GROUP = kGroupBytes<KC, VW>, DK = 64 * KC, DV = 32 * VW, PER = DK > DV ? DK / 32 : DV / 32;
-    extern __shared__ __align__(16) uint8_t sm[];
+    extern __shared__ __align__(16) uint8_t raw[];
+    uint8_t* const groups_s = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+    uint8_t* const ring = groups_s + (threadIdx.x >> 5) * (AHEAD * GROUP);   // the warp's groups under way
+    uint8_t* const sm = groups_s + A1_WARPS * AHEAD * GROUP;
     const int dk = a.dim_ld, dv = a.vdim_ld;
     __half* q_s = reinterpret_cast<__half*>(sm);                             // [HN][DK]
     uint8_t* tail_k = sm + HN * DK * 2;                                      // [16][DK], [16][DV]: the row's own group
     uint8_t* tail_v = tail_k + kScaleTokens * DK;
     float* fresh = reinterpret_cast<float*>(tail_v + kScaleTokens * DV);     // [DK], [DV]: the row's own key and value
-    uint8_t* ring = reinterpret_cast<uint8_t*>(fresh + DK + DV) + (threadIdx.x >> 5) * (AHEAD * GROUP);       // the warp's groups under way: codes, then two scales
-    float* w_acc = reinterpret_cast<float*>(sm);                             // [A1_WARPS][HN][DV] at the end, over all of the above
+    float* w_acc = reinterpret_cast<float*>(groups_s);                       // [A1_WARPS][HN][DV] at the end, over all of the above
+    __shared__ __align__(8) uint64_t full[A1_WARPS][AHEAD];
+    __shared__ int abort_flag;
     __shared__ float w_m[A1_WARPS][HN], w_l[A1_WARPS][HN], c_m[HN], c_l[HN], q_unit[HN], q_sum[HN], tail_scale[2];
     __shared__ float2 red[A1_WARPS];
+    if ((threadIdx.x & 31) == 0) {
+        for (int j = 0; j < AHEAD; j++) mbar_init(smem_addr(&full[threadIdx.x >> 5][j]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 0) abort_flag = 0;
+    __syncthreads();
     dep_trigger();
     dep_wait();
     const int splits = gridDim.x, rank = blockIdx.x, group = a.heads / a.kv_heads, passes = gridDim.y / a.kv_heads, kh = blockIdx.y / passes, pass = blockIdx.y % passes, r = blockIdx.z;
@@ -289,38 +299,35 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     if (kept >= near) { near = 0; kept = 0; }
     const int groups = kept + tail - near + (append ? 0 : 1), step = splits * A1_WARPS;
     auto first_of = [&](int i) { return kScaleTokens * (i < kept ? i : near + i - kept); };
-    auto page_of = [&](int i) { return i < groups ? table[first_of(i) >> shift] : 0; };
     KeyCodes<KC> xk;
     ValueCodes<VW> xv;
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k_pool) + (size_t)kh * dk;
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v_pool) + (size_t)kh * dv;
     constexpr int PIECE = VW == 2 ? 8 : 16;
-    const Places whole = places_of(kstride, vstride, PIECE, kScaleTokens - 1, lane);
-    // a group's first token in the pools
-    auto token_of = [&](int i, int page) { return ((size_t)page << shift) + (first_of(i) & (a.block_size - 1)); };
-    // (where the row's key is in the cache already, its group may end with it)
-    auto ends = [&](int i) { return !append && first_of(i) + kScaleTokens - 1 > p; };
-    // group i into place `at` of the ring; a commit each, whether there is such a group or not
-    auto fetch = [&](int i, int page, int at) {
-        if (i < groups) {
-            const size_t token = token_of(i, page), sc = token / kScaleTokens * a.kv_heads + kh;
-            const uint32_t to = smem_addr(ring) + at * GROUP;
-            const uint8_t *k = kp + token * kstride, *v = vp + token * vstride;
-            if (ends(i)) copy_group<KC, VW>(to, k, v, places_of(kstride, vstride, PIECE, p - first_of(i), lane), dk, dv, lane);
-            else copy_group<KC, VW>(to, k, v, whole, dk, dv, lane);
-            if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + GROUP - 16 + 4 * lane), "l"((lane ? a.v_scale : a.k_scale) + sc) : "memory");
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     int i = rank * A1_WARPS + warp;
-    {                                                  // under way while the queries are made
-        int pages[AHEAD];
+    // Where the warp's groups i, i + step, .. lie in the pools, 32 of them at a time, one a lane: the number of the group there, or -1; and their scales.
+    const int i0 = i, per_page = a.block_size / kScaleTokens;
+    auto look_up = [&](int n) {
+        const int at = i0 + (n + lane) * step;
+        if (at >= groups) return -1;
+        const int first = first_of(at);
+        return table[first >> shift] * per_page + (first & (a.block_size - 1)) / kScaleTokens;
+    };
+    auto scale_of = [&](const float* scales, int where) { return where < 0 ? 0.f : scales[(size_t)where * a.kv_heads + kh]; };
+    int lie = look_up(0), lie_next = -1;
+    // the warp's group number n into place `at` of the ring
+    auto fetch = [&](int n, bool further, int at) {
+        const int where = __shfl_sync(0xffffffffu, further ? lie_next : lie, n & 31);
+        if (where >= 0 && lane == 0) {
+            const uint32_t to = smem_addr(ring) + at * GROUP, bar = smem_addr(&full[warp][at]);
+            mbar_expect_tx(bar, GROUP);
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++) pages[j] = page_of(i + j * step);
+            for (int c = 0; c < (KC + 1) / 2; c++) copy_tokens(to + 2048 * c, &kmap, 128 * c, kh, where, bar);
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++) fetch(i + j * step, pages[j], j);
-    }
-    int page = page_of(i + AHEAD * step);
+            for (int c = 0; c < (VW + 3) / 4; c++) copy_tokens(to + 1024 * KC + 2048 * c, &vmap, 128 * c, kh, where, bar);
+        }
+    };
+#pragma unroll
+    for (int at = 0; at < AHEAD; at++) fetch(at, false, at);       // under way while the queries are made
+    float ks = scale_of(a.k_scale, lie), vs = scale_of(a.v_scale, lie), ks_next = 0.f, vs_next = 0.f;
 
     // ---- the row's queries, and on rank 0 its key and value
     const size_t own = ((size_t)table[p >> shift] << shift) + (p & (a.block_size - 1)), own_group = own / kScaleTokens * a.kv_heads + kh;
@@ -465,20 +472,30 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     // ---- the cached groups
     float sc[NT][4];
     uint32_t pb[NT][2];
-    for (int at = 0; i < groups; i += step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
-        __syncwarp();                                  // (two lanes copied the scales)
-        const uint8_t* from = ring + at * GROUP;
-        const float2 two = *reinterpret_cast<const float2*>(from + GROUP - 16);
-        take_keys<KC>(xk, from, lane);
-        take_values<KC, VW>(xv, from, lane);
+    // The next group's scores are made beside the values' products of one: two chains of MMAs that do not wait for each other. (Behind the last group there are
+    // scores of whatever lies in the ring; nobody looks at them.)
+    uint32_t phase = 0;
+    bool ok = true;
+    auto scores = [&](int at, bool there) {
+        if (there) ok = __all_sync(0xffffffffu, mbar_wait(smem_addr(&full[warp][at]), phase, &abort_flag, 9, status));
+        if (!ok) return;
+        take_keys<KC>(xk, ring + at * GROUP, lane);
         key_products<I8, KC, NT>(sc, xk, q, from_);
-        make_weights<VW, NT>(st, sc, pb, two.x, two.y, qs, slope, first_of(i), p, k_lo, keep, lane);
+    };
+    scores(0, i < groups);
+    int at = 0;
+    for (int n = 0; i < groups && ok; i += step, n++) {
+        make_weights<VW, NT>(st, sc, pb, __shfl_sync(0xffffffffu, ks, n & 31), __shfl_sync(0xffffffffu, vs, n & 31), qs, slope, first_of(i), p, k_lo, keep, lane);
+        take_values<KC, VW>(xv, ring + at * GROUP, append ? kScaleTokens - 1 : p - first_of(i), lane);
+        __syncwarp();                                  // (all lanes have what they need of the place)
+        fetch(n + AHEAD, (n & 31) >= 32 - AHEAD, at);
+        if (++at == AHEAD) { at = 0; phase ^= 1; }
+        // the next 32 groups' places, then their scales, long before they are needed
+        if ((n & 31) == 8) lie_next = look_up((n & ~31) + 32);
+        if ((n & 31) == 16) { ks_next = scale_of(a.k_scale, lie_next); vs_next = scale_of(a.v_scale, lie_next); }
+        if ((n & 31) == 31) { lie = lie_next; ks = ks_next; vs = vs_next; }
+        scores(at, i + step < groups);
         value_products<I8, VW, NT>(st, xv, pb);
-        __syncwarp();
-        fetch(i + AHEAD * step, page, at);
-        page = page_of(i + (AHEAD + 1) * step);
-        at = at + 1 == AHEAD ? 0 : at + 1;
     }
     if (joins && warp == 0) {
         take_tail<KC, VW>(xk, xv, tail_k, tail_v, places_of(DK, DV, PIECE, off, lane), dk, dv, lane);
@@ -486,7 +503,12 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
         make_weights<VW, NT>(st, sc, pb, tail_scale[0], tail_scale[1], qs, slope, tail * kScaleTokens, p, k_lo, keep, lane);
         value_products<I8, VW, NT>(st, xv, pb);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!ok) {                                         // a wait gave up, and has said so: what is under way gets as long again
+        for (int k = 0; k < AHEAD && i + k * step < groups; k++) {
+            for (uint32_t it = 0; it < SPIN_LIMIT && !mbar_try(smem_addr(&full[warp][at]), phase); it++) {}
+            if (++at == AHEAD) { at = 0; phase ^= 1; }
+        }
+    }
     // ---- merge the warps, then the CTAs of the cluster
     __syncthreads();                                   // queries and tail are done with
     const float unit = st.vref / kWeightUnit;
@@ -571,15 +593,35 @@ attention8_one_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int l
     }
 }
 
+// A pool as [groups of 16 tokens][token][head][dimension], its end open: group numbers come from block tables. Rows of up to `width` codes, zeros behind dim_ld.
+int map_pool(CUtensorMap* map, const void* pool, int kv_heads, int dim_ld, int width) {
+    const int row = width < 128 ? width : 128;
+    const cuuint64_t head = (cuuint64_t)dim_ld, token = head * kv_heads, dims[4] = {head, (cuuint64_t)kv_heads, kScaleTokens, 1ull << 31}, strides[3] = {head, token, token * kScaleTokens};
+    const cuuint32_t box[4] = {(cuuint32_t)row, 1, kScaleTokens, 1}, one[4] = {1, 1, 1, 1};
+    EncodeTiledFn encode;
+    const int rc = get_encoder(&encode);
+    if (rc) return rc;
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(pool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CMLB_REQUIRE(r == CUDA_SUCCESS, "cmlb200_attention_one: cuTensorMapEncodeTiled failed with %d for %d heads of %d", (int)r, kv_heads, dim_ld);
+    return CMLB200_OK;
+}
+
 template <bool I8, int KC, int VW, int NT>
 int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int splits, int passes, int append, __nv_bfloat16* d_out, int out_ld,
                cudaStream_t st) {
     constexpr size_t HN = 8 * NT, DK = 64 * KC, DV = 32 * VW;
-    constexpr size_t before = HN * DK * 2 + kScaleTokens * (DK + DV) + 4 * (DK + DV) + A1_WARPS * kAhead<KC, NT> * kGroupBytes<KC, VW>, after = 4 * A1_WARPS * HN * DV, smem = before > after ? before : after;
+    constexpr size_t before = HN * DK * 2 + kScaleTokens * (DK + DV) + 4 * (DK + DV) + A1_WARPS * kAhead<KC, NT> * kGroupBytes<KC, VW>, after = 4 * A1_WARPS * HN * DV, smem = 1024 + (before > after ? before : after);
     static size_t attr[kMaxDevices] = {};
     auto kern = attention8_one_kernel<I8, KC, VW, NT>;
     CMLB_CUDA(cmlb_ensure_smem(kern, smem, attr));
-    CMLB_CUDA(launch_chain(kern, dim3(splits, a->kv_heads * passes, rows), dim3(A1_THREADS), smem, splits, st, *a, d_qkv, ld, d_row_pos, d_row_slot, append, d_out, out_ld));
+    CUtensorMap kmap, vmap;
+    int* status;
+    int rc = map_pool(&kmap, a->k_pool, a->kv_heads, a->dim_ld, DK);
+    if (!rc) rc = map_pool(&vmap, a->v_pool, a->kv_heads, a->vdim_ld, DV);
+    if (!rc) rc = cmlb_attention8_status_word(&status);
+    if (rc) return rc;
+    CMLB_CUDA(launch_chain(kern, dim3(splits, a->kv_heads * passes, rows), dim3(A1_THREADS), smem, splits, st, kmap, vmap, *a, d_qkv, ld, d_row_pos, d_row_slot, append, d_out, out_ld, status));
     return CMLB200_OK;
 }
 
@@ -598,8 +640,8 @@ int cmlb_attention8_one(const cmlb200_attn* a, const float* d_qkv, int ld, const
     const int reach = a->chunk > 0 ? a->chunk : a->window;
     const int keys = (reach > 0 && reach < max_keys - a->keep) ? reach + a->keep : max_keys;
     const long long base = (long long)rows * a->kv_heads * passes;
-    // as many CTAs to a row and key/value head as run at a time, while each of their warps has a group (8 rows of 8 heads behind 2,000 tokens: 18.3 us with 4,
-    // 24.4 with 2, 27.7 with 8, which takes two waves)
+    // as many CTAs to a row and key/value head as run at a time, while each of their warps has a group (8 rows of 8 heads behind 2,000 tokens, when a row's
+    // keys took a third longer: 18.3 us with 4, 24.4 with 2, 27.7 with 8, which takes two waves)
     const long long room = (long long)cmlb_num_sms() * (widest > 128 || nt == 2 ? 1 : 2), most = (keys + A1_WARPS * kScaleTokens - 1) / (A1_WARPS * kScaleTokens);
     const int splits = (int)max(1LL, min(min((long long)A1_SPLITS, room / base), most));
 #define A1_ARGS a, d_qkv, ld, d_row_pos, d_row_slot, rows, splits, passes, append, d_out, out_ld, st

@@ -367,20 +367,6 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
 
 int* g_status8[kMaxDevices] = {};
 
-int status_word8(int** word) {
-    int dev = 0;
-    CMLB_CUDA(cudaGetDevice(&dev));
-    CMLB_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d", dev);
-    if (!g_status8[dev]) {
-        void* p = nullptr;
-        CMLB_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocDefault));
-        *static_cast<int*>(p) = 0;
-        g_status8[dev] = static_cast<int*>(p);
-    }
-    *word = g_status8[dev];
-    return CMLB200_OK;
-}
-
 // Clusters of k such CTAs that run at a time.
 int t8_clusters(const void* kern, int k, int threads, size_t smem) {
     cudaLaunchAttribute attr;
@@ -433,9 +419,28 @@ int launch_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d
 
 }  // namespace
 
+int cmlb_attention8_status_word(int** word) {
+    int dev = 0;
+    CMLB_CUDA(cudaGetDevice(&dev));
+    CMLB_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d", dev);
+    if (!g_status8[dev]) {
+        // (allowed beside a stream that is being captured, in any mode)
+        void* p = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        CMLB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocDefault);
+        CMLB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        CMLB_CUDA(e);
+        *static_cast<int*>(p) = 0;
+        g_status8[dev] = static_cast<int*>(p);
+    }
+    *word = g_status8[dev];
+    return CMLB200_OK;
+}
+
 int cmlb_attention8_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_tiles, int tiles, __nv_bfloat16* d_out, int out_ld, cudaStream_t st) {
     int* status;
-    const int rc = status_word8(&status);
+    const int rc = cmlb_attention8_status_word(&status);
     if (rc) return rc;
     if (cmlb_attention8_wide_fits(a, tiles)) return cmlb_attention8_wide(a, d_qkv, ld, d_tiles, tiles, d_out, out_ld, status, st);
     const int widest = a->dim_ld > a->vdim_ld ? a->dim_ld : a->vdim_ld;
@@ -457,7 +462,7 @@ int cmlb_attention8_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, con
 extern "C" int cmlb200_attention8_status(int* status, int reset) {
     CMLB_REQUIRE(status, "cmlb200_attention8_status: NULL argument");
     int* word;
-    const int rc = status_word8(&word);
+    const int rc = cmlb_attention8_status_word(&word);
     if (rc) return rc;
     *status = *static_cast<volatile int*>(word);
     if (reset) *static_cast<volatile int*>(word) = 0;

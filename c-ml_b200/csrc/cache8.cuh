@@ -66,6 +66,8 @@ __host__ __device__ inline bool is_cache8(int dtype) { return dtype == CMLB200_D
 // `rotate`) in place as well; otherwise the rows are only read.
 int cmlb_cache8_append(const cmlb200_attn* a, float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int first, int rows, bool rotate, bool queries,
                        cudaStream_t st);
+// the current device's word of cmlb200_attention8_status
+int cmlb_attention8_status_word(int** word);
 int cmlb_attention8_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int max_keys, __nv_bfloat16* d_out, int out_ld,
                         cudaStream_t st);
 int cmlb_attention8_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_tiles, int tiles, __nv_bfloat16* d_out, int out_ld, cudaStream_t st);

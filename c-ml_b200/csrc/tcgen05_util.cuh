@@ -97,8 +97,7 @@ __device__ __forceinline__ uint64_t make_desc_mn(uint32_t saddr, uint32_t group)
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// A [rows, cols] matrix of 16-bit elements in boxes of box_cols (128 bytes) by box_rows, 128-byte swizzle, zeros outside.
-inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long rows, int cols, int ld, int box_cols, int box_rows) {
+inline int get_encoder(EncodeTiledFn* out) {
     static EncodeTiledFn fn = nullptr;
     if (!fn) {
         void* p = nullptr;
@@ -107,6 +106,15 @@ inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* ba
         CMLB_REQUIRE(p && q == cudaDriverEntryPointSuccess, "cuTensorMapEncodeTiled is not available in this driver");
         fn = reinterpret_cast<EncodeTiledFn>(p);
     }
+    *out = fn;
+    return CMLB200_OK;
+}
+
+// A [rows, cols] matrix of 16-bit elements in boxes of box_cols (128 bytes) by box_rows, 128-byte swizzle, zeros outside.
+inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long rows, int cols, int ld, int box_cols, int box_rows) {
+    EncodeTiledFn fn;
+    const int rc = get_encoder(&fn);
+    if (rc) return rc;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, one[2] = {1, 1};
     const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

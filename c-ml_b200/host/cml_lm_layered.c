@@ -1222,7 +1222,7 @@ static int layered_check(void* model, const CMLLMBatch* b) {
     if (m->f32) return 0;
     if (m->q) DEV(cmlb200_attention_latent_status(&status, 1));
     if (status) return -1;
-    if (m->cache8 && b->tiles) DEV(cmlb200_attention8_status(&status, 1));
+    if (m->cache8) DEV(cmlb200_attention8_status(&status, 1));
     if (status) return -1;
     if (b->rows <= SKINNY_ROWS) return 0;
     DEV(cmlb200_gemm_dense_status(&status, 1));

@@ -588,7 +588,7 @@ int cmlb200_residual_norm(float* d_x, const float* d_y, int ldy, const float* d_
  * has grown. Numbers beyond 65504 are held there, NaN is cached as 0. Attention is over what the cache then holds, the row's own key and value
  * included. The rows of one sequence follow one another in a call, in order of position, and nothing else of the device writes or reads their
  * groups meanwhile. Entry points: cmlb200_qk_norm_append, cmlb200_rotate_append (no conv), cmlb200_attention_tiles, cmlb200_attention_one;
- * value heads up to 256, key heads up to 256. cmlb200_attention8_status is not 0 once a bounded wait of cmlb200_attention_tiles over such a cache has
+ * value heads up to 256, key heads up to 256. cmlb200_attention8_status is not 0 once a bounded wait of an attention kernel over such a cache has
  * expired (valid when the stream has drained). */
 int cmlb200_attention8_status(int* status, int reset);
 

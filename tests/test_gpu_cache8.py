@@ -367,3 +367,19 @@ def test_short_tiles_of_many_heads(pkg, torch_dev, form, heads, kv_heads):
     for parts in ([(0, 2), (1, 3), (2, 18)], [(0, 19), (1, 10), (2, 11)], [(0, 37), (1, 64), (2, 65)], [(0, 5), (1, 77), (2, 63)], [(0, 4), (1, 128), (2, 2)]):
         L.step(parts)
     L.check_cache()
+
+
+def test_decode_far_into_the_pools(pkg, torch_dev):
+    """Pages beyond the 32-bit offsets of a large pool, read and written through the table."""
+    import torch
+    pages, page, G, D = 70000, 64, 4, 128                                  # 2.3 GB a pool
+    L = Layer(pkg, torch_dev, "i8", 8, G, D, D, page=page, slots=2, tokens=300)
+    big = [torch.full((pages, page, G, D), 0x7F, dtype=torch.int8, device=torch_dev) for _ in range(2)]
+    scales = [torch.full((pages, page // 16, G), float("nan"), device=torch_dev) for _ in range(2)]
+    L.k, L.v, (L.ks, L.vs) = big[0], big[1], scales
+    L.a.k_pool, L.a.v_pool, L.a.k_scale, L.a.v_scale = (x.data_ptr() for x in (*big, *scales))
+    per = -(-300 // page)
+    L.table[:, :per] = pages - 1 - np.arange(2 * per).reshape(2, per) * 3
+    L.d_table.copy_(torch.from_numpy(L.table))
+    for parts in ([(0, 70), (1, 200)], [(0, 1), (1, 1)], [(1, 1)], [(0, 65), (1, 1)]):
+        L.step(parts)
