@@ -15,7 +15,7 @@
 // A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
 // where m, the warp's reference for the exponentials, moves only when a score has passed it by 7 (powers of two; sums are fp32). Queries are fp16 over
 // a power of two of their own per head, so their size is no matter.
-// 8 warps a CTA take groups in turn; a cluster of up to 8 CTAs splits a row's keys and merges through distributed shared memory, each CTA a
+// 8 warps a CTA take groups in turn; a cluster of up to 16 CTAs splits a row's keys and merges through distributed shared memory, each CTA a
 // share of the outputs. The group that the row's own token joins belongs to rank 0 alone, which settles its scales, rewrites it where they have grown and
 // attends to it from shared memory; nobody else looks at it.
 #include "cache8.cuh"
@@ -23,7 +23,7 @@
 
 namespace {
 
-constexpr int A1_SPLITS = 8, A1_WARPS = 8, A1_THREADS = 32 * A1_WARPS;
+constexpr int A1_SPLITS = 16, A1_WARPS = 8, A1_THREADS = 32 * A1_WARPS;
 // groups that a warp has under way: as many as shared memory holds at two CTAs an SM (at one, where registers allow no more)
 template <int KC, int NT> constexpr int kAhead = KC == 1 ? 6 : (KC == 2 && NT == 2) ? 6 : 3;
 template <int KC, int VW> constexpr int kGroupBytes = 1024 * KC + 512 * VW;
@@ -555,25 +555,31 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         const int j = e / DV, d = e - j * DV;
         float v, sum, mx;
         if (splits > 1) {
-            float ms[A1_SPLITS], ls[A1_SPLITS], vs[A1_SPLITS];
+            mx = -INFINITY; v = 0.f; sum = 0.f;
+            for (int s0 = 0; s0 < splits; s0 += 8) {
+                float ms[8], ls[8], vs[8];
 #pragma unroll
-            for (int s = 0; s < A1_SPLITS; s++) {
-                ms[s] = -INFINITY; ls[s] = 0.f; vs[s] = 0.f;
-                if (s < splits) {
-                    ms[s] = cluster_load(cluster_addr(c_m + j, s));
-                    ls[s] = cluster_load(cluster_addr(c_l + j, s));
-                    vs[s] = cluster_load(cluster_addr(w_acc + e, s));
+                for (int s = 0; s < 8; s++) {
+                    ms[s] = -INFINITY; ls[s] = 0.f; vs[s] = 0.f;
+                    if (s0 + s < splits) {
+                        ms[s] = cluster_load(cluster_addr(c_m + j, s0 + s));
+                        ls[s] = cluster_load(cluster_addr(c_l + j, s0 + s));
+                        vs[s] = cluster_load(cluster_addr(w_acc + e, s0 + s));
+                    }
                 }
-            }
-            mx = ms[0];
+                float top = mx;
 #pragma unroll
-            for (int s = 1; s < A1_SPLITS; s++) mx = fmaxf(mx, ms[s]);
-            v = 0.f; sum = 0.f;
+                for (int s = 0; s < 8; s++) top = fmaxf(top, ms[s]);
+                const float was = mx == -INFINITY ? 0.f : exp2f(mx - top);
+                v *= was;
+                sum *= was;
+                mx = top;
 #pragma unroll
-            for (int s = 0; s < A1_SPLITS; s++) {
-                const float c = ms[s] == -INFINITY ? 0.f : exp2f(ms[s] - mx);
-                v = fmaf(vs[s], c, v);
-                sum = fmaf(ls[s], c, sum);
+                for (int s = 0; s < 8; s++) {
+                    const float c = ms[s] == -INFINITY ? 0.f : exp2f(ms[s] - mx);
+                    v = fmaf(vs[s], c, v);
+                    sum = fmaf(ls[s], c, sum);
+                }
             }
         } else {
             v = w_acc[e]; sum = c_l[j]; mx = c_m[j];
@@ -608,13 +614,28 @@ int map_pool(CUtensorMap* map, const void* pool, int kv_heads, int dim_ld, int w
 }
 
 template <bool I8, int KC, int VW, int NT>
-int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int splits, int passes, int append, __nv_bfloat16* d_out, int out_ld,
+int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_row_pos, const int* d_row_slot, int rows, int keys, int passes, int append, __nv_bfloat16* d_out, int out_ld,
                cudaStream_t st) {
     constexpr size_t HN = 8 * NT, DK = 64 * KC, DV = 32 * VW;
     constexpr size_t before = HN * DK * 2 + kScaleTokens * (DK + DV) + 4 * (DK + DV) + A1_WARPS * kAhead<KC, NT> * kGroupBytes<KC, VW>, after = 4 * A1_WARPS * HN * DV, smem = 1024 + (before > after ? before : after);
     static size_t attr[kMaxDevices] = {};
     auto kern = attention8_one_kernel<I8, KC, VW, NT>;
     CMLB_CUDA(cmlb_ensure_smem(kern, smem, attr));
+    // How many CTAs share a row's keys: what takes least by an estimate in units of a warp's time for a group (1.2 us where few are under way): 6 for a CTA's
+    // beginning and end, times the waves, where clusters of a size share the device with as many as fit its groups of SMs. (One row of 8 heads behind 32,000
+    // tokens: 45 us by 8, 35 by 16. 8 behind 2,000, when a group took a third longer: 18.3 us by 4, 24.4 by 2, 27.7 by 8, which takes two waves.)
+    static int room[kMaxDevices][A1_SPLITS + 1] = {};
+    CMLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    const long long base = (long long)rows * a->kv_heads * passes, groups = (keys + kScaleTokens - 1) / kScaleTokens;
+    long long best = 0;
+    int splits = 1;
+    for (int k = 1; k <= A1_SPLITS && (k == 1 || groups > (k - 1) * A1_WARPS); k++) {
+        int* fit = &room[cmlb_device_index()][k];
+        if (!*fit) *fit = cluster_room((const void*)kern, k, A1_THREADS, smem);
+        if (*fit < 0) continue;
+        const long long t = (base + *fit - 1) / *fit * (6 + (groups + k * A1_WARPS - 1) / (k * A1_WARPS));
+        if (k == 1 || t < best) { best = t; splits = k; }
+    }
     CUtensorMap kmap, vmap;
     int* status;
     int rc = map_pool(&kmap, a->k_pool, a->kv_heads, a->dim_ld, DK);
@@ -639,12 +660,7 @@ int cmlb_attention8_one(const cmlb200_attn* a, const float* d_qkv, int ld, const
     }
     const int reach = a->chunk > 0 ? a->chunk : a->window;
     const int keys = (reach > 0 && reach < max_keys - a->keep) ? reach + a->keep : max_keys;
-    const long long base = (long long)rows * a->kv_heads * passes;
-    // as many CTAs to a row and key/value head as run at a time, while each of their warps has a group (8 rows of 8 heads behind 2,000 tokens, when a row's
-    // keys took a third longer: 18.3 us with 4, 24.4 with 2, 27.7 with 8, which takes two waves)
-    const long long room = (long long)cmlb_num_sms() * (widest > 128 || nt == 2 ? 1 : 2), most = (keys + A1_WARPS * kScaleTokens - 1) / (A1_WARPS * kScaleTokens);
-    const int splits = (int)max(1LL, min(min((long long)A1_SPLITS, room / base), most));
-#define A1_ARGS a, d_qkv, ld, d_row_pos, d_row_slot, rows, splits, passes, append, d_out, out_ld, st
+#define A1_ARGS a, d_qkv, ld, d_row_pos, d_row_slot, rows, keys, passes, append, d_out, out_ld, st
 #define A1_HEADS(I8, KC, VW) return nt == 1 ? launch_one<I8, KC, VW, 1>(A1_ARGS) : launch_one<I8, KC, VW, 2>(A1_ARGS)
 #define A1_SIZES(I8)                            \
     do {                                         \

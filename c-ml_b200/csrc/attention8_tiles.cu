@@ -367,24 +367,6 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
 
 int* g_status8[kMaxDevices] = {};
 
-// Clusters of k such CTAs that run at a time.
-int t8_clusters(const void* kern, int k, int threads, size_t smem) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)k;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(k);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) return n;
-    cudaGetLastError();
-    return max(1, cmlb_num_sms() / k * 3 / 4);
-}
-
 template <bool I8, int S, bool SLOPES>
 int launch_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_tiles, int tiles, __nv_bfloat16* d_out, int out_ld, int* status, cudaStream_t st) {
     using C = T8<S>;
@@ -409,7 +391,8 @@ int launch_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d
     plan.splits = 1;
     for (int k = 1; k <= T8_SPLITS && (k == 1 || (key_tiles >= k && ctas * k <= cmlb_num_sms())); k++) {
         int* fit = &room[cmlb_device_index()][k];
-        if (!*fit) *fit = k == 1 ? cmlb_num_sms() : t8_clusters((const void*)kern, k, C::kThreads, smem);
+        if (!*fit) *fit = k == 1 ? cmlb_num_sms() : cluster_room((const void*)kern, k, C::kThreads, smem);
+        if (*fit < 0) continue;
         const long long waves = (ctas + *fit - 1) / *fit, each = (key_tiles + k - 1) / k, t = waves * (5 + each + (k > 1 ? 2 : 0));
         if (k == 1 || t < best) { best = t; plan.splits = k; }
     }

@@ -58,6 +58,24 @@ template <bool I8> __device__ __forceinline__ uint32_t rescale8(uint32_t w, floa
     return pack8<I8>(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
 }
 
+// Clusters of k CTAs of a kernel that run at a time; -1: none.
+inline int cluster_room(const void* kern, int k, int threads, size_t smem) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)k;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(k);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) return n;
+    cudaGetLastError();
+    return k == 1 ? cmlb_num_sms() : -1;
+}
+
 __host__ __device__ inline bool is_cache8(int dtype) { return dtype == CMLB200_DT_I8 || dtype == CMLB200_DT_E4M3; }
 
 }  // namespace
