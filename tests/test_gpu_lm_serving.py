@@ -133,6 +133,26 @@ def test_forks_go_on_as_their_parents_would(synth, tmp_path, load, monkeypatch, 
     assert np.array_equal(r1, r2)
 
 
+@pytest.mark.parametrize("name,dtype,cache", [("mixed", 6, 1), ("latent", 0, 0), ("streams", 6, 0), ("loops", 6, 0)])
+def test_forks_of_what_has_just_begun(synth, tmp_path, load, monkeypatch, name, dtype, cache):
+    """A fork of a sequence without tokens, in slots that others have left their states and tokens in, is another empty one."""
+    cfg, w, folder = build(synth, tmp_path, name, monkeypatch)
+    t = prompt(cfg, 60)
+    m = load(folder, dtype, max_tokens=1024, max_sequences=2, cache=cache)
+    old = [m.open(), m.open()]
+    m.step([(old[0], t[:50], None), (old[1], t[10:], None)])
+    for s in old:
+        m.end(s)
+    a = m.open()
+    b = m.fork(a)
+    got = [m.step([(a, t[:33], None), (b, t[:33], None)]), m.step([(a, t[33:34], None), (b, t[33:34], None)])]
+    want = lm_util.reference(cfg, w, t[:34])
+    for k in range(2):
+        assert np.array_equal(got[0][0], got[0][1]) and np.array_equal(got[1][0], got[1][1])
+        if not cache:
+            assert error(np.concatenate([got[0][k], got[1][k]]), want) < TOL[dtype]
+
+
 def soft(logits):
     z = np.asarray(logits, np.float64)
     z = z - z.max(-1, keepdims=True)
