@@ -81,6 +81,22 @@ def test_a_table_alone_and_many_small_moves(pkg, torch_dev):
     P.check(bufs, name[t].astype(np.int32))
 
 
+@pytest.mark.parametrize("pools", [13, 16])
+def test_many_moves_in_many_pools(pkg, torch_dev, pools):
+    """So many pages that a CTA takes several pools; their number and pages of several pieces do not divide evenly."""
+    sizes = [[(64, 64, 0), (20000, 20016, 16), (36, 48, 4)][k % 3] for k in range(pools)]
+    P = Pools(pkg, torch_dev, sizes, 1700, 9, 50, seed=pools)
+    ids = np.random.default_rng(pools).permutation(1700)
+    pairs = sorted(zip(ids[:800].tolist(), ids[800:1600].tolist()))
+    bufs, t = P.snapshot()
+    name = np.arange(1700)
+    name[[a for a, _ in pairs]] = [b for _, b in pairs]
+    m = P.up(pairs)
+    pkg.check(pkg.lib.cmlb200_pages_copy(P.p, m.data_ptr(), len(pairs), None))
+    P.torch.cuda.synchronize()
+    P.check(P.copied(bufs, pairs), name[t].astype(np.int32))
+
+
 def test_forks(pkg, torch_dev):
     P = Pools(pkg, torch_dev, SIZES, 60, 8, 12)
     bufs, t = P.snapshot()
