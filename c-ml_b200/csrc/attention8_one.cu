@@ -625,7 +625,7 @@ int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_r
     // beginning and end, times the waves, where clusters of a size share the device with as many as fit its groups of SMs. (One row of 8 heads behind 32,000
     // tokens: 45 us by 8, 35 by 16. 8 behind 2,000, when a group took a third longer: 18.3 us by 4, 24.4 by 2, 27.7 by 8, which takes two waves.)
     static int room[kMaxDevices][A1_SPLITS + 1] = {};
-    CMLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    if (!room[cmlb_device_index()][1]) CMLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const long long base = (long long)rows * a->kv_heads * passes, groups = (keys + kScaleTokens - 1) / kScaleTokens;
     long long best = 0;
     int splits = 1;

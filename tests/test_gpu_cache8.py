@@ -383,3 +383,69 @@ def test_decode_far_into_the_pools(pkg, torch_dev):
     L.d_table.copy_(torch.from_numpy(L.table))
     for parts in ([(0, 70), (1, 200)], [(0, 1), (1, 1)], [(1, 1)], [(0, 65), (1, 1)]):
         L.step(parts)
+
+
+CAPTURED_FIRST = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import numpy as np, torch
+import __graft_entry__ as entry
+import test_gpu_cache8 as t
+pkg = entry.load_package()
+dev = torch.device("cuda:0")
+L = t.Layer(pkg, dev, "i8", 8, 2, 64, 64, slots=2)
+for s in range(2):
+    for q in L.seqs[s]:
+        q.append(np.zeros((0,) + q.codes.shape[1:]))
+x, out = torch.randn(2, L.ld, device=dev), torch.zeros(2, 8 * 64, dtype=torch.bfloat16, device=dev)
+pos, slot = torch.zeros(2, dtype=torch.int32, device=dev), torch.arange(2, dtype=torch.int32, device=dev)
+tiles = torch.tensor([[0, 1, 0, 0], [1, 1, 1, 0]], dtype=torch.int32, device=dev)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    if {one}:
+        pkg.check(pkg.lib.cmlb200_attention_one(L.a, x.data_ptr(), L.ld, pos.data_ptr(), slot.data_ptr(), 2, 0, out.data_ptr(), 512, st))
+    else:
+        pkg.check(pkg.lib.cmlb200_qk_norm_append(L.a, x.data_ptr(), L.ld, pos.data_ptr(), slot.data_ptr(), 2, st))
+        pkg.check(pkg.lib.cmlb200_attention_tiles(L.a, x.data_ptr(), L.ld, tiles.data_ptr(), 2, out.data_ptr(), 512, st))
+g.replay()
+torch.cuda.synchronize()
+v = x[:, L.width - 128:L.width].view(2, 2, 1, 64).expand(2, 2, 4, 64).reshape(2, 512)
+assert (out.float() - v).abs().max() < v.abs().max() / 50, (out.float() - v).abs().max()
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("one", [True, False])
+def test_captured_before_anything_else_ran(one):
+    """The first call of a process is one that is being captured (a first token: attention returns its own value, an int8 rounding and bf16's away)."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    tests = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.format(root=str(tests.parent), tests=str(tests), one=one)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_streams_at_once(pkg, torch_dev):
+    """Decoding of two layers at a time, each over its own cache, gives what each gives alone."""
+    import torch
+    L = [Layer(pkg, torch_dev, f, 8, 2, 64, 64, slots=3, seed=k) for k, f in enumerate(("i8", "e4m3"))]
+    for l in L:
+        l.step([(0, 150), (1, 40), (2, 3)])
+    streams = [torch.cuda.Stream(torch_dev) for _ in L]
+    rows = [l.fresh_rows(3) for l in L]
+    put = lambda a, k: torch.from_numpy(np.ascontiguousarray(a, k)).to(torch_dev)
+    pos = [put([len(l.seqs[s][0].codes) for s in range(3)], np.int32) for l in L]
+    slot, x = put([0, 1, 2], np.int32), [put(r, np.float32) for r in rows]
+    out = [[torch.zeros(3, 512, dtype=torch.bfloat16, device=torch_dev) for _ in range(20)] for _ in L]
+    torch.cuda.synchronize()
+    for i in range(20):                                # (the same token again each time: it is the last of its group)
+        for l, st, p, r, o in zip(L, streams, pos, x, out):
+            pkg.check(pkg.lib.cmlb200_attention_one(l.a, r.data_ptr(), l.ld, p.data_ptr(), slot.data_ptr(), 3, 150, o[i].data_ptr(), 512, st.cuda_stream))
+    torch.cuda.synchronize()
+    for l, o, r in zip(L, out, rows):
+        assert all(torch.equal(o[0], y) for y in o)
+        got = l.step([(0, 1), (1, 1), (2, 1)], rows=r)
+        assert np.array_equal(got, o[0].float().cpu().numpy().astype(np.float64))
