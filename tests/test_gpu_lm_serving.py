@@ -153,6 +153,28 @@ def test_forks_of_what_has_just_begun(synth, tmp_path, load, monkeypatch, name, 
             assert error(np.concatenate([got[0][k], got[1][k]]), want) < TOL[dtype]
 
 
+@pytest.mark.parametrize("name,cache", [("mixed", 1), ("streams", 2), ("gated", 1)])
+def test_greedy_decoding_on_the_device(synth, tmp_path, load, monkeypatch, name, cache):
+    """Captured steps over an 8-bit cache, of a sequence, its fork and another: every pick leads the logits of the same step by itself, up to what two ways to split the
+    keys may differ by (each within TOL of the restatement's)."""
+    cfg, w, folder = build(synth, tmp_path, name, monkeypatch)
+    a, b = (load(folder, max_tokens=2048, max_sequences=4, cache=cache) for _ in range(2))
+    t = prompt(cfg, 90)
+    seqs = []
+    for m in (a, b):
+        x, y = m.open(), m.open()
+        feed(m, x, t[:61], [61])
+        feed(m, y, t[61:], [29])
+        seqs.append([x, y, m.fork(x)])
+    first = [int(v) for v in t[:3]]
+    ids, _ = a.decode_greedy(seqs[0], first, 70)
+    tokens = np.concatenate([np.array(first)[None], ids])
+    for k in range(70):
+        logits = b.step([(s, [int(tokens[k, i])], None) for i, s in enumerate(seqs[1])])
+        for i, l in enumerate(logits):
+            assert l[0][ids[k, i]] >= l[0].max() - 2 * TOL[6] * l.std() * np.sqrt(cfg["vocab"])
+
+
 def soft(logits):
     z = np.asarray(logits, np.float64)
     z = z - z.max(-1, keepdims=True)
