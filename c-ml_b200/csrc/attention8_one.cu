@@ -9,7 +9,7 @@
 //                                        interleaved, which makes the operand's pairs. P^T comes from S^T by movmatrix
 // so a lane's operands are pieces of the cache as they lie there. One TMA copy a group brings 16 tokens of a head (128 bytes of every kv_heads * 128 at heads of 128),
 // three to six groups ahead of the warp that asked for them; group numbers and scales are looked up 32 at a time, one a lane. (32 rows of 8 heads behind 8,192 tokens,
-// 537 MB: 103 us, 5.2 TB/s. With 16-byte copies by the lanes themselves it took 138 us, 133 without any arithmetic; with one group a warp under way in registers 135.)
+// 537 MB: 101.5 us, 5.3 TB/s. With 16-byte copies by the lanes themselves it took 138 us, 133 without any arithmetic; with one group a warp under way in registers 135.)
 // The next group's scores are issued beside one group's value products. int8 keys stay 1,152 too large, as they come out of their conversion: the
 // scores' accumulators begin at -1,152 times the sum of the head's queries, so every term is exact and the fp32 sums are off by no more than the queries' own rounding.
 // A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
@@ -290,6 +290,21 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int h0 = kh * group + pass * HN, nh = min(HN, group - pass * HN);
     const float* row = qkv + (size_t)r * ld;
+    const bool joins = append && rank == 0;
+    // heads (queries, then on rank 0 the row's key and value) that a warp prepares: warp, warp + A1_WARPS, .. The first two's entries lane + 32 e are requested before
+    // anything else is looked up
+    auto request = [&](float (&y)[PER], int j) {
+        const float* v = row;
+        int n = 0;
+        if (j < nh) { v = row + (h0 + j) * a.dim; n = a.dim; }
+        else if (j == HN && joins) { v = row + (a.heads + kh) * a.dim; n = a.dim; }
+        else if (j == HN + 1 && joins) { v = row + (a.heads + (a.keys_as_values ? 0 : a.kv_heads)) * a.dim + kh * a.vdim; n = a.vdim; }
+#pragma unroll
+        for (int e = 0; e < PER; e++) { const int d = lane + 32 * e; y[e] = d < n ? v[d] : 0.f; }
+    };
+    float now[PER], after[PER];
+    request(now, warp);
+    request(after, warp + A1_WARPS);
     const int p = row_pos[r], qw = a.heads * a.dim, kw = a.kv_heads * a.dim, shift = __ffs(a.block_size) - 1;
     const int* table = a.block_table + (size_t)row_slot[r] * a.table_ld;
     const int kstride = a.kv_heads * dk, vstride = a.kv_heads * dv;
@@ -313,6 +328,7 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     };
     auto scale_of = [&](const float* scales, int where) { return where < 0 ? 0.f : scales[(size_t)where * a.kv_heads + kh]; };
     int lie = look_up(0), lie_next = -1;
+    const int own_page = table[p >> shift];
     // the warp's group number n into place `at` of the ring
     auto fetch = [&](int n, bool further, int at) {
         const int where = __shfl_sync(0xffffffffu, further ? lie_next : lie, n & 31);
@@ -330,9 +346,8 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     float ks = scale_of(a.k_scale, lie), vs = scale_of(a.v_scale, lie), ks_next = 0.f, vs_next = 0.f;
 
     // ---- the row's queries, and on rank 0 its key and value
-    const size_t own = ((size_t)table[p >> shift] << shift) + (p & (a.block_size - 1)), own_group = own / kScaleTokens * a.kv_heads + kh;
+    const size_t own = ((size_t)own_page << shift) + (p & (a.block_size - 1)), own_group = own / kScaleTokens * a.kv_heads + kh;
     const int off = p & (kScaleTokens - 1);
-    const bool joins = append && rank == 0;
     uint8_t* kd = static_cast<uint8_t*>(a.k_pool) + ((own - off) * a.kv_heads + kh) * dk;
     uint8_t* vd = static_cast<uint8_t*>(a.v_pool) + ((own - off) * a.kv_heads + kh) * dv;
     constexpr int OLD = (kScaleTokens * (DK + DV) / 16 + A1_THREADS - 1) / A1_THREADS;
@@ -355,10 +370,8 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
         if (a.k_norm) ik = 1.0f / sqrtf(ss.y / (float)kw + a.eps);
     }
     const float temp = a.temp_every > 0.f ? 1.0f + a.temp_coef * logf(floorf((float)(p + 1) / a.temp_every) + 1.0f) : 1.0f;
-    // what a warp does with one head: entries lane + 32 j of v, normed and turned
-    auto prepare = [&](float (&y)[PER], const float* v, int n, const float* norm, float inv, bool head_norm, bool turns) {
-#pragma unroll
-        for (int j = 0; j < PER; j++) { const int d = lane + 32 * j; y[j] = d < n ? v[d] : 0.f; }
+    // what a warp does with one head: entries lane + 32 j, normed and turned
+    auto prepare = [&](float (&y)[PER], int n, const float* norm, float inv, bool head_norm, bool turns) {
         if (head_norm) {
             float ss = 0.f;
 #pragma unroll
@@ -381,12 +394,12 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     };
     for (int j = warp; j < HN + (joins ? 2 : 0); j += A1_WARPS) {
         float y[PER], most = 0.f;
+#pragma unroll
+        for (int e = 0; e < PER; e++) { y[e] = now[e]; now[e] = after[e]; }
+        if (HN > A1_WARPS) request(after, j + 2 * A1_WARPS);
         if (j < HN) {
             if (j < nh) {
-                prepare(y, row + (h0 + j) * a.dim, a.dim, a.q_norm ? a.q_norm + (a.head_norm ? 0 : (h0 + j) * a.dim) : nullptr, iq, a.q_norm && a.head_norm, a.freq != nullptr);
-            } else {
-#pragma unroll
-                for (int e = 0; e < PER; e++) y[e] = 0.f;
+                prepare(y, a.dim, a.q_norm ? a.q_norm + (a.head_norm ? 0 : (h0 + j) * a.dim) : nullptr, iq, a.q_norm && a.head_norm, a.freq != nullptr);
             }
 #pragma unroll
             for (int e = 0; e < PER; e++) { y[e] *= temp * a.scale * kLog2e; most = fmaxf(most, fabsf(y[e])); }
@@ -404,8 +417,8 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             if (lane == 0) { q_unit[j] = unit; q_sum[j] = sum; }
         } else {
             const bool key = j == HN;
-            if (key) prepare(y, row + qw + kh * a.dim, a.dim, a.k_norm ? a.k_norm + (a.head_norm ? 0 : kh * a.dim) : nullptr, ik, a.k_norm && a.head_norm, a.freq != nullptr);
-            else prepare(y, row + qw + (a.keys_as_values ? 0 : kw) + kh * a.vdim, a.vdim, nullptr, 1.0f, false, false);
+            if (key) prepare(y, a.dim, a.k_norm ? a.k_norm + (a.head_norm ? 0 : kh * a.dim) : nullptr, ik, a.k_norm && a.head_norm, a.freq != nullptr);
+            else prepare(y, a.vdim, nullptr, 1.0f, false, false);
 #pragma unroll
             for (int e = 0; e < PER; e++) { y[e] = cached8(y[e]); most = fmaxf(most, fabsf(y[e])); }
             most = lane_max(most);
