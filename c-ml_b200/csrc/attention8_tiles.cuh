@@ -35,7 +35,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
 }
 
-// Shared memory of a CTA: queries, key stages, value stages, then the small things.
 // two numbers at a time
 __device__ __forceinline__ uint64_t pair_of(float x, float y) {
     uint64_t r;
