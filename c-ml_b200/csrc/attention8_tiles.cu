@@ -8,7 +8,9 @@
 //             shared memory, keys with the dimensions contiguous, values with theirs as the contiguous non-summed side, both with 128-byte swizzle. Codes are
 //             exact in fp16; scales stay apart: a group's key scale multiplies its scores, its value scale joins the exponent of its weights
 //   16        issues tcgen05.mma: the scores of tile i + 1, then P V of tile i, so that products and softmax overlap
-// Rows are (head, token) pairs, one head after the other, so short tiles fill few blocks; queries are fp16 over a power of two of their own. Weights are 2^(s - m) times the value scale over the largest so far, times 128: at most 2^15.
+// Rows are (head, token) pairs, one head after the other, so short tiles fill few blocks; queries are fp16 over a power of two of their own. A weight is 2^s times its group's value
+// scale, over the largest such product that its row has met, times 128: at most 2^15, and never small because of values that the row does not see or passes over. That
+// largest product and the largest score, which the sum of 2^(s - m) is relative to, are followed apart.
 // Few tiles: a cluster of up to 8 CTAs splits the keys and merges through distributed shared memory.
 // Keys behind a portion's last row are read as that row's (their weights are zero), so nothing other requests left can reach the sums. Every wait is
 // bounded; one that gives up leaves a code in a status word in host memory, the products under way are waited for and tensor memory is freed.
@@ -27,7 +29,7 @@ template <int S>
 struct T8 {
     static constexpr int kSoft = 8, kConv = 4, kThreads = 32 * (kSoft + 2 * kConv + 4);
     static constexpr int kQ = S * T8_ROWS * 128, kK = S * T8_SLAB, kV = S * T8_SLAB;
-    static constexpr int kSmall = 1024 + 4 * T8_ROWS * (1 + 4 + 2 * T8_SPLITS);
+    static constexpr int kSmall = 1024 + 4 * T8_ROWS * (1 + 8 + 2 * T8_SPLITS);
     static int bytes(int stages) { return 1024 + kQ + stages * (kK + kV) + kSmall; }
 };
 constexpr int T8_TMEM = 512, T8_O_COL = 256;
@@ -56,8 +58,8 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     volatile int* abort_flag = reinterpret_cast<volatile int*>(small + 136);
     float* scales = reinterpret_cast<float*>(small + 256);                    // [4][T8_SCALES] (tile i in i & 3)
     float* unit_s = reinterpret_cast<float*>(small + 1024);                   // [128] powers of two of the queries
-    float* meet = unit_s + T8_ROWS;                                           // [2][2][128] the two halves' largest scores, at the end sums
-    float* c_m = meet + 4 * T8_ROWS;                                          // [T8_SPLITS][128] maxima and sums of the whole cluster
+    float2* meet = reinterpret_cast<float2*>(unit_s + T8_ROWS);               // [2][2][128] the two halves' largest scores and products with value scales, at the end sums
+    float* c_m = unit_s + 9 * T8_ROWS;                                         // [T8_SPLITS][128] maxima and sums of the whole cluster
     float* c_l = c_m + T8_SPLITS * T8_ROWS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kConv = C::kSoft, kIssue = C::kSoft + 2 * C::kConv;
@@ -113,14 +115,14 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
         const int p = live ? p0 + i_tok : p_last, lo = first_key8(a, p), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
         const float unit = unit_s[r], slope = SLOPES && live ? a.slopes[head] * kLog2e : 0.f;
         auto pair_meets = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
-        float ref = -INFINITY, l = 0.f, vref = -INFINITY;
+        float ref = -INFINITY, wref = -INFINITY, l = 0.f;                    // references: log2 of scores, log2 of scores times value scales
         bool ok = true;
         for (int i = 0; i < count; i++) {
             const int kt = keys.start(i) + 64 * half, buf = i & 1;          // this thread's first key
             const uint32_t s_at = lanes + buf * T8_KEYS;
             ok = ok && __all_sync(0xffffffffu, mbar_wait(s_full(buf), (i >> 1) & 1, abort_flag, 1, status));
             uint32_t v[2][32];
-            float mx = -INFINITY, vm = vref;
+            float mx = -INFINITY, mw = -INFINITY;
             const float* sc = scales + (i & 3) * T8_SCALES + 4 * half;
             const float far = SLOPES ? slope * (float)(kt - p) : 0.f;        // the part of the bias that all of its keys share
             float f[4], lv[4];                         // factors of its four groups' scores, log2 of their value scales
@@ -129,7 +131,6 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
 #pragma unroll
                 for (int c = 0; c < 2; c++) tmem_ld32_begin(s_at + 64 * half + 32 * c, v[c]);
                 const float4 s4 = *reinterpret_cast<const float4*>(sc), l4 = *reinterpret_cast<const float4*>(sc + T8_GROUPS);
-                vm = fmaxf(vm, sc[2 * T8_GROUPS - 4 * half]);
                 // (a scale times a query's power of two that underflows would make NaN of a masked score)
                 f[0] = fmaxf(unit * s4.x, 1.17549435e-38f); f[1] = fmaxf(unit * s4.y, 1.17549435e-38f); f[2] = fmaxf(unit * s4.z, 1.17549435e-38f); f[3] = fmaxf(unit * s4.w, 1.17549435e-38f);
                 lv[0] = l4.x; lv[1] = l4.y; lv[2] = l4.z; lv[3] = l4.w;
@@ -144,36 +145,43 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
                     }
                 }
 #pragma unroll
-                for (int g = 0; g < 4; g++) mx = fmaxf(mx, t8_group_max<SLOPES>(v[g >> 1], g & 1, f[g], slope, 16 * g));
+                for (int g = 0; g < 4; g++) {
+                    const float m = t8_group_max<SLOPES>(v[g >> 1], g & 1, f[g], slope, 16 * g);
+                    mx = fmaxf(mx, m);
+                    mw = fmaxf(mw, m + lv[g]);
+                }
                 mx += far;
-                meet[(2 * buf + half) * T8_ROWS + r] = mx;
+                mw += far;
+                meet[(2 * buf + half) * T8_ROWS + r] = make_float2(mx, mw);
             }
             tmem_fence_before();
             pair_meets();                              // both halves' scores are in registers, and their largest known
             tmem_fence_after();
             if (!ok) continue;                         // (the other half may have been luckier: the two meet once a tile whatever comes)
-            mx = fmaxf(mx, meet[(2 * buf + (half ^ 1)) * T8_ROWS + r]);
-            if (__any_sync(0xffffffffu, mx > ref + kLazy || vm > vref)) {
-                const float nm = fmaxf(ref, mx), c = nm == -INFINITY ? 1.f : ex2(ref - nm), cv = ex2(vref - vm);
+            const float2 other = meet[(2 * buf + (half ^ 1)) * T8_ROWS + r];
+            mx = fmaxf(mx, other.x);
+            mw = fmaxf(mw, other.y);
+            if (__any_sync(0xffffffffu, mx > ref + kLazy || mw > wref + kLazy)) {
+                const float nm = fmaxf(ref, mx), nw = fmaxf(wref, mw), c = nw == -INFINITY ? 1.f : ex2(wref - nw);
+                l *= nm == -INFINITY ? 1.f : ex2(ref - nm);
                 ref = nm;
-                vref = vm;
-                l *= c;
+                wref = nw;
                 if (i > 0) {
                     // (scores of this tile were issued behind P V of tile i - 2, so that one is done)
                     ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (i - 1) & 1, abort_flag, 2, status));
                     if (!ok) continue;
                     tmem_fence_after();
-                    t8_scale_o(o_at, 16 * half, 32, dv, c * cv);
+                    t8_scale_o(o_at, 16 * half, 32, dv, c);
                 }
             }
-            const float u = (ref == -INFINITY ? 0.f : ref) - far;
+            const float lift = ref == -INFINITY ? 0.f : wref - ref, u = (ref == -INFINITY ? 0.f : ref) - far;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int g = 2 * c + e;
-                    const float bits = fmaxf(lv[g] - vref, kFarScale) + kWeightBits;
+                    const float bits = fmaxf(lv[g] - lift, kFarScale) + kWeightBits;
                     l = fmaf(t8_group_weights<SLOPES>(v[c], w, e, f[g], bits - u, slope, 16 * g), ex2(-bits), l);
                 }
                 tmem_st16(s_at + 32 * half + 16 * c, w);                      // over scores that both halves have in registers
@@ -186,11 +194,12 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
         if (ok && count > 0) ok = __all_sync(0xffffffffu, mbar_wait(drained, 0, abort_flag, 3, status));
         tmem_fence_after();
         if (!ok) { ref = -INFINITY; l = 0.f; }
+        const float lift = wref - ref;
         // a row's two sums (a tile's largest scores have been read before the next one's are written: two pairs of places)
         pair_meets();
-        meet[half * T8_ROWS + r] = l;
+        meet[half * T8_ROWS + r].x = l;
         pair_meets();
-        l += meet[(half ^ 1) * T8_ROWS + r];
+        l += meet[(half ^ 1) * T8_ROWS + r].x;
         const float* row = qkv + (size_t)(tl.x + (live ? i_tok : 0)) * ld;
         float mt = ref, sum = l;
         if (splits > 1) {
@@ -217,7 +226,7 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
         }
         if (a.sink && sum > 0.f) sum += ex2((a.sinks ? a.sinks[head] : 0.f) * kLog2e - mt);
         // what O is multiplied with: its unit, what this CTA's reference lacks of the row's, one over the sum, the gate
-        float inv = ref != -INFINITY && sum > 0.f ? ex2(vref - kWeightBits) * ex2(ref - mt) * (a.out_scale == 0.f ? 1.f : a.out_scale) / sum : 0.f;
+        float inv = ref != -INFINITY && sum > 0.f ? ex2(lift - kWeightBits) * ex2(ref - mt) * (a.out_scale == 0.f ? 1.f : a.out_scale) / sum : 0.f;
         if (a.gate_col >= 0 && !a.gate_wide && live) inv *= sigmoidf(row[a.gate_col + head]);
         if (splits == 1) {
             t8_write_row(a, o_at, 32 * half, 64, live, inv, row, head, out, out_ld, (size_t)tl.x + (live ? i_tok : 0));

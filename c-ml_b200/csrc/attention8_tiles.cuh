@@ -240,8 +240,8 @@ struct T8Team {
         __syncwarp();
     }
 };
-// A tile's scales as the softmax finds them: 8 key scales, log2 of 8 value scales, the largest of those; four tiles in turn.
-constexpr int T8_SCALES = 20;
+// A tile's scales as the softmax finds them: 8 key scales, log2 of 8 value scales; four tiles in turn.
+constexpr int T8_SCALES = 2 * T8_GROUPS;
 struct T8Scaler {
     bool on;                                           // lanes 0 .. 7 of one warp look after key scales, 8 .. 15 after value scales
     int lane, kh;
@@ -250,14 +250,7 @@ struct T8Scaler {
         if (on) scale = (lane < T8_GROUPS ? a.k_scale : a.v_scale)[(size_t)token / kScaleTokens * a.kv_heads + kh];
     }
     __device__ __forceinline__ void put(float* scales, int i) const {
-        if (!on) return;
-        const float v = lane < T8_GROUPS ? scale : log2f(fmaxf(scale, 1.17549435e-38f));
-        float m = v;
-#pragma unroll
-        for (int o = 1; o < T8_GROUPS; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFu, m, o));
-        float* s = scales + (i & 3) * T8_SCALES;
-        s[lane] = v;
-        if (lane == T8_GROUPS) s[2 * T8_GROUPS] = m;
+        if (on) scales[(i & 3) * T8_SCALES + lane] = lane < T8_GROUPS ? scale : log2f(fmaxf(scale, 1.17549435e-38f));
     }
 };
 // Where group `lane & 7` of tile i begins in the pools; groups behind the last row's are read as that one.

@@ -83,7 +83,7 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
         // (rows that are none have queries of zero and see what the last one sees; nobody looks at theirs)
         const int p = live ? p0 + i_tok : p_last, lo = first_key8(a, p), lo_last = first_key8(a, p_last), head = kh * group + (live ? h : 0);
         const float unit = unit_s[m * T8_ROWS + r], slope = SLOPES && live ? a.slopes[head] * kLog2e : 0.f;
-        float ref = -INFINITY, l = 0.f, vref = -INFINITY;
+        float ref = -INFINITY, wref = -INFINITY, l = 0.f;                    // references: log2 of scores, log2 of scores times value scales
         bool ok = true;
         for (int j = 0; j < halves; j++) {
             const int half = j & 1, kt = keys.start(j >> 1) + 64 * half;    // the first key
@@ -96,7 +96,6 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
             tmem_ld32_begin(s_at + 32, v[1]);
             const float* sc = scales + ((j >> 1) & 3) * T8_SCALES + 4 * half;
             const float4 s4 = *reinterpret_cast<const float4*>(sc), l4 = *reinterpret_cast<const float4*>(sc + T8_GROUPS);
-            const float vm = fmaxf(vref, sc[2 * T8_GROUPS - 4 * half]);
             // (a scale times a query's power of two that underflows would make NaN of a masked score)
             const float f[4] = {fmaxf(unit * s4.x, 1.17549435e-38f), fmaxf(unit * s4.y, 1.17549435e-38f), fmaxf(unit * s4.z, 1.17549435e-38f), fmaxf(unit * s4.w, 1.17549435e-38f)};
             const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
@@ -111,31 +110,36 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
                     v[k >> 5][k & 31] = hidden ? 0xff800000u : v[k >> 5][k & 31];
                 }
             }
-            float mx = -INFINITY;
+            float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < 4; g++) mx = fmaxf(mx, t8_group_max<SLOPES>(v[g >> 1], g & 1, f[g], slope, 16 * g));
+            for (int g = 0; g < 4; g++) {
+                const float most = t8_group_max<SLOPES>(v[g >> 1], g & 1, f[g], slope, 16 * g);
+                mx = fmaxf(mx, most);
+                mw = fmaxf(mw, most + lv[g]);
+            }
             mx += far;
-            if (__any_sync(0xffffffffu, mx > ref + kLazy || vm > vref)) {
-                const float nm = fmaxf(ref, mx), c = nm == -INFINITY ? 1.f : ex2(ref - nm), cv = ex2(vref - vm);
+            mw += far;
+            if (__any_sync(0xffffffffu, mx > ref + kLazy || mw > wref + kLazy)) {
+                const float nm = fmaxf(ref, mx), nw = fmaxf(wref, mw), c = nw == -INFINITY ? 1.f : ex2(wref - nw);
+                l *= nm == -INFINITY ? 1.f : ex2(ref - nm);
                 ref = nm;
-                vref = vm;
-                l *= c;
+                wref = nw;
                 if (j > 0) {
                     // (these scores were issued behind P V of half tile j - 2, so that one is done)
                     ok = __all_sync(0xffffffffu, mbar_wait(pv_done(m), (j - 1) & 1, abort_flag, 3, status));
                     if (!ok) break;
                     tmem_fence_after();
-                    t8_scale_o(o_at, 0, 16, dv, c * cv);
+                    t8_scale_o(o_at, 0, 16, dv, c);
                 }
             }
-            const float u = (ref == -INFINITY ? 0.f : ref) - far;
+            const float lift = ref == -INFINITY ? 0.f : wref - ref, u = (ref == -INFINITY ? 0.f : ref) - far;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int g = 2 * c + e;
-                    const float bits = fmaxf(lv[g] - vref, kFarScale) + kWeightBits;
+                    const float bits = fmaxf(lv[g] - lift, kFarScale) + kWeightBits;
                     l = fmaf(t8_group_weights<SLOPES>(v[c], w, e, f[g], bits - u, slope, 16 * g), ex2(-bits), l);
                 }
                 tmem_st16(s_at + 16 * c, w);           // over the scores, which are all in registers
@@ -149,7 +153,7 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
         tmem_fence_after();
         const float* row = qkv + (size_t)(tl.x + (live ? i_tok : 0)) * ld;
         if (a.sink && l > 0.f) l += ex2((a.sinks ? a.sinks[head] : 0.f) * kLog2e - ref);
-        float inv = ok && l > 0.f ? ex2(vref - kWeightBits) * (a.out_scale == 0.f ? 1.f : a.out_scale) / l : 0.f;
+        float inv = ok && l > 0.f ? ex2(wref - ref - kWeightBits) * (a.out_scale == 0.f ? 1.f : a.out_scale) / l : 0.f;
         if (a.gate_col >= 0 && !a.gate_wide && live) inv *= sigmoidf(row[a.gate_col + head]);
         t8_write_row(a, o_at, 0, 32, live, inv, row, head, out, out_ld, (size_t)tl.x + (live ? i_tok : 0));
         tmem_fence_before();
