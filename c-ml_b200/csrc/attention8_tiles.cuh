@@ -87,11 +87,14 @@ template <int N> __device__ __forceinline__ void more_registers() { asm volatile
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 
-// The key tiles of a tile of rows: those of the kept tokens, then from k_lo on (one run from 0 where they meet). A cluster's CTA takes rank, rank + splits, ..
+// The key tiles of a tile of rows: those of the kept tokens, then from k_lo on (one run from 0 where they meet). A cluster's CTA takes rank, rank + splits, .. Groups from
+// hidden_from up to hidden_to lie between the kept tokens and what the first row sees.
 struct T8Keys {
-    int k_lo, kept_tiles, count, p_last, rank, splits;
+    int k_lo, kept_tiles, count, p_last, rank, splits, hidden_from, hidden_to;
     __device__ __forceinline__ T8Keys(const cmlb200_attn& a, int p0, int last, int r, int s) : p_last(last), rank(r), splits(s) {
         k_lo = first_key8(a, p0) & ~(kScaleTokens - 1);
+        hidden_from = a.keep;
+        hidden_to = k_lo;
         kept_tiles = (min(a.keep, k_lo) + T8_KEYS - 1) / T8_KEYS;
         if (kept_tiles * T8_KEYS >= k_lo) { k_lo = 0; kept_tiles = 0; }
         const int total = kept_tiles + (p_last - k_lo) / T8_KEYS + 1;
@@ -253,9 +256,11 @@ struct T8Scaler {
         if (on) scales[(i & 3) * T8_SCALES + lane] = lane < T8_GROUPS ? scale : log2f(fmaxf(scale, 1.17549435e-38f));
     }
 };
-// Where group `lane & 7` of tile i begins in the pools; groups behind the last row's are read as that one.
+// Where group `lane & 7` of tile i begins in the pools; groups behind the last row's are read as that one, and those behind the kept tokens that no row sees as the first: their pages
+// may be anybody's by now.
 __device__ __forceinline__ int t8_place(const cmlb200_attn& a, const int* table, int shift, const T8Keys& keys, int i, int lane) {
-    const int first = min(keys.start(i) + kScaleTokens * (lane & 7), keys.p_last & ~(kScaleTokens - 1));
+    int first = min(keys.start(i) + kScaleTokens * (lane & 7), keys.p_last & ~(kScaleTokens - 1));
+    if (first >= keys.hidden_from && first < keys.hidden_to) first = 0;
     return (table[first >> shift] << shift) + (first & (a.block_size - 1));
 }
 // A thread's four keys of the tile whose groups lie at `at` (t8_place); keys behind the last row are read as that one.

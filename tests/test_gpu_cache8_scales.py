@@ -88,6 +88,26 @@ def test_tokens_in_front_of_the_window_are_larger(pkg, torch_dev, form, tiles):
         run(L, 0, sized(L, 1, [2.0 ** -20]))
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("heads,kv_heads,rows", [(8, 2, 40), (32, 8, 1230)])
+def test_groups_between_kept_tokens_and_window(pkg, torch_dev, form, heads, kv_heads, rows):
+    """Pages that a sequence has let go of belong to somebody else: their scales and codes make no difference, not even one of a bit."""
+    import torch
+    L = Layer(pkg, torch_dev, form, heads, kv_heads, 64, 64, slots=1, tokens=1700, window=48, keep=5)
+    run(L, 0, sized(L, 330, np.full(330, 2.0 ** -6)))
+    state = [t.clone() for t in (L.k, L.v, L.ks, L.vs)]
+    x, had = sized(L, rows, np.full(rows, 2.0 ** -6)), 330
+    pos, given_back, seen = had + np.arange(rows), L.table[0, 1:(had - 47) // 16], []
+    for scale, code in ((2.0 ** -20, 0), (2.0 ** 10, 100), (float("nan"), 0x7F)):                # (the last: what nothing may read)
+        for t, s in zip((L.k, L.v, L.ks, L.vs), state):
+            t.copy_(s)
+        for t, y in ((L.k, code), (L.v, code), (L.ks, scale), (L.vs, scale)):
+            t[torch.from_numpy(given_back.astype(np.int64)).to(torch_dev)] = y
+        seen.append(L.device(x, pos, np.zeros(rows), [(0, rows)], 0, {0: had}))
+        assert np.isfinite(seen[-1]).all()
+    assert all(np.array_equal(seen[0], s) for s in seen[1:])
+
+
 def steered(L, n, group, far):
     """Keys of `group` meet the queries of all rows, the others oppose them; values elsewhere are 2^far times as large."""
     x = sized(L, n, np.where(np.arange(n) // 16 == group, 2.0 ** (14 - far), 2.0 ** 14))
