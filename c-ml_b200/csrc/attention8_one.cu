@@ -12,9 +12,9 @@
 // 537 MB: 101.5 us, 5.3 TB/s. With 16-byte copies by the lanes themselves it took 138 us, 133 without any arithmetic; with one group a warp under way in registers 135.)
 // The next group's scores are issued beside one group's value products. int8 keys stay 1,152 too large, as they come out of their conversion: the
 // scores' accumulators begin at -1,152 times the sum of the head's queries, so every term is exact and the fp32 sums are off by no more than the queries' own rounding.
-// A group's key scale multiplies its scores, its value scale the weights: as fp16 they are e^(s - m) * (scale / largest scale so far) * 256, never above 2^15,
-// where m, the warp's reference for the exponentials, moves only when a score has passed it by 7 (powers of two; sums are fp32). Queries are fp16 over
-// a power of two of their own per head, so their size is no matter.
+// A group's key scale multiplies its scores, its value scale the weights: as fp16 they are 2^s * scale over the largest such product that the head has met, times 256: never above 2^15,
+// and not small because of large values that the softmax passes over. The largest score, which sums of 2^(s - m) are relative to, is followed apart; both references
+// move only when they have been passed by 7 (powers of two; sums are fp32). Queries are fp16 over a power of two of their own per head, so their size is no matter.
 // 8 warps a CTA take groups in turn; a cluster of up to 16 CTAs splits a row's keys and merges through distributed shared memory, each CTA a
 // share of the outputs. The group that the row's own token joins belongs to rank 0 alone, which settles its scales, rewrites it where they have grown and
 // attends to it from shared memory; nobody else looks at it.
@@ -27,7 +27,7 @@ constexpr int A1_SPLITS = 16, A1_WARPS = 8, A1_THREADS = 32 * A1_WARPS;
 // groups that a warp has under way: as many as shared memory holds at two CTAs an SM (at one, where registers allow no more)
 template <int KC, int NT> constexpr int kAhead = KC == 1 ? 6 : (KC == 2 && NT == 2) ? 6 : 3;
 template <int KC, int VW> constexpr int kGroupBytes = 1024 * KC + 512 * VW;
-constexpr float kWeightUnit = 256.f;
+constexpr float kWeightBits = 8.f, kFarScale = -60.f;
 
 __device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
     if (a.chunk > 0) return p / a.chunk * a.chunk;
@@ -152,11 +152,10 @@ template <bool I8> __device__ __forceinline__ void unpack_key(uint32_t w, uint32
     }
 }
 
-// What a warp carries: per head 8 n + 2 t + e the reference m and the sum l (this lane's keys), and O^T.
+// What a warp carries: per head 8 n + 2 t + e the references m (log2 of scores) and w (of scores times value scales), the sum l (this lane's keys), and O^T.
 template <int VW, int NT>
 struct State {
-    float m[NT][2], l[NT][2], o[NT][2 * VW][4];
-    float vref, vinv;                                  // largest value scale so far, one over it
+    float m[NT][2], w[NT][2], l[NT][2], o[NT][2 * VW][4];
 };
 
 // The products of a group's keys with the queries. from: what a head's accumulators begin with.
@@ -182,7 +181,8 @@ __device__ __forceinline__ void make_weights(State<VW, NT>& st, float (&s)[NT][4
     const int g = lane >> 2;
     const float back = (float)(p - key0 - g);
     const bool edge = key0 + kScaleTokens - 1 > p || (key0 < k_lo && key0 + kScaleTokens > keep);
-    bool over = vs > st.vref;
+    const float lv = (float)((int)(__float_as_uint(vs) >> 23) - 127);        // log2 of a power of two
+    bool over = false;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -205,11 +205,11 @@ __device__ __forceinline__ void make_weights(State<VW, NT>& st, float (&s)[NT][4
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) over |= fmaxf(s[n][e], s[n][2 + e]) > st.m[n][e] + 7.f;
+        for (int e = 0; e < 2; e++) {
+            const float mx = fmaxf(s[n][e], s[n][2 + e]);
+            over |= mx > st.m[n][e] + 7.f || mx + lv > st.w[n][e] + 7.f;
+        }
     if (__any_sync(0xffffffffu, over)) {
-        const float vnew = fmaxf(st.vref, vs), cv = st.vref > 0.f ? st.vref / vnew : 0.f;
-        st.vref = vnew;
-        st.vinv = vnew > 0.f ? 1.0f / vnew : 0.f;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -218,24 +218,27 @@ __device__ __forceinline__ void make_weights(State<VW, NT>& st, float (&s)[NT][4
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                mx = fmaxf(st.m[n][e], mx);
-                const float c = mx == -INFINITY ? 1.f : ex2(st.m[n][e] - mx);
-                st.m[n][e] = mx;
-                st.l[n][e] *= c;
+                const float nw = fmaxf(st.w[n][e], mx + lv), nm = fmaxf(st.m[n][e], mx), c = nm == -INFINITY ? 1.f : ex2(st.w[n][e] - nw);
+                st.l[n][e] *= nm == -INFINITY ? 1.f : ex2(st.m[n][e] - nm);
+                st.m[n][e] = nm;
+                st.w[n][e] = nw;
 #pragma unroll
-                for (int i = 0; i < 2 * VW; i++) { st.o[n][i][e] *= c * cv; st.o[n][i][2 + e] *= c * cv; }
+                for (int i = 0; i < 2 * VW; i++) { st.o[n][i][e] *= c; st.o[n][i][2 + e] *= c; }
             }
     }
-    const float f = vs * st.vinv * kWeightUnit;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            w[e] = ex2(s[n][e] - st.m[n][e & 1]);
-            st.l[n][e & 1] += w[e];
+        for (int e = 0; e < 2; e++) {
+            const float m = st.m[n][e] == -INFINITY ? 0.f : st.m[n][e], lift = st.m[n][e] == -INFINITY ? 0.f : st.w[n][e] - m;
+            // (a group this far below the largest product weighs nothing; its part of l is made of the same exponentials)
+            const float bits = fmaxf(lv - lift, kFarScale) + kWeightBits, u = bits - m;
+            w[e] = ex2(s[n][e] + u);
+            w[2 + e] = ex2(s[n][2 + e] + u);
+            st.l[n][e] = fmaf(w[e] + w[2 + e], ex2(-bits), st.l[n][e]);
         }
-        const __half2 h0 = __floats2half2_rn(w[0] * f, w[1] * f), h1 = __floats2half2_rn(w[2] * f, w[3] * f);
+        const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
         b[n][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
         b[n][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
     }
@@ -458,8 +461,6 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     uint32_t q[NT][KC][4][2];
     float qs[NT][2], slope[NT][2], from_[NT][2];
     State<VW, NT> st;
-    st.vref = 0.f;
-    st.vinv = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -477,6 +478,7 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
             from_[n][e] = I8 ? -1152.f * q_sum[j] : 0.f;
             slope[n][e] = a.slopes && j < nh ? a.slopes[h0 + j] * kLog2e : 0.f;
             st.m[n][e] = -INFINITY;
+            st.w[n][e] = -INFINITY;
             st.l[n][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < 2 * VW; k++) { st.o[n][k][e] = 0.f; st.o[n][k][2 + e] = 0.f; }
@@ -524,12 +526,12 @@ attention8_one_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_con
     }
     // ---- merge the warps, then the CTAs of the cluster
     __syncthreads();                                   // queries and tail are done with
-    const float unit = st.vref / kWeightUnit;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             float l = st.l[n][e];
+            const float unit = st.m[n][e] == -INFINITY ? 0.f : ex2(st.w[n][e] - st.m[n][e] - kWeightBits);
             l += __shfl_xor_sync(0xffffffffu, l, 4);
             l += __shfl_xor_sync(0xffffffffu, l, 8);
             l += __shfl_xor_sync(0xffffffffu, l, 16);

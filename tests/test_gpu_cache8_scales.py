@@ -130,6 +130,29 @@ def test_softmax_passes_over_large_values(pkg, torch_dev, form, far, group, tile
     run(L, 0, steered(L, n, group, far))
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("far", [10, 24, 40])
+@pytest.mark.parametrize("dim,heads,kv_heads,tokens", [(64, 4, 2, 70), (128, 32, 8, 300), (128, 16, 1, 70), (256, 4, 1, 600), (64, 20, 1, 70), (16, 320, 320, 300), (64, 160, 160, 300)])
+def test_decoded_tokens_pass_over_large_values(pkg, torch_dev, form, far, dim, heads, kv_heads, tokens):
+    """The same for one row, of few and many heads: a group a warp, and several, the one that counts behind the others."""
+    L = Layer(pkg, torch_dev, form, heads, kv_heads, dim, dim, slots=1, tokens=700, scale=48.0 / dim)
+    x = steered(L, tokens + 3, tokens // 16 - 1, far)
+    run(L, 0, x[:tokens], check=False)
+    for i in range(3):
+        run(L, 0, x[tokens + i:tokens + i + 1])
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_decoded_tokens_behind_values_of_all_sizes(pkg, torch_dev, form):
+    """Groups from 1e-30 to 1e4 in no order, weights alike and steep."""
+    L = Layer(pkg, torch_dev, form, 12, 2, 128, 96, slots=1, tokens=900)
+    run(L, 0, sized(L, 800, np.exp(np.repeat(L.rng.uniform(-69, 9, 50), 16))), check=False)
+    for s in (1, 1, 30, 300):
+        x = sized(L, 1, [1e-12])
+        x[:, :L.H * L.D] *= s
+        run(L, 0, x)
+
+
 @pytest.mark.parametrize("form,heads,kv_heads,dim,vdim,what", [("i8", 15, 5, 80, 64, {}), ("e4m3", 25, 5, 64, 128, dict(slopes=True)), ("i8", 36, 3, 72, 40, dict(gate="head")),
                                                                ("e4m3", 24, 8, 13, 24, dict(window=100)), ("i8", 28, 4, 96, 96, dict(kav=True)), ("e4m3", 36, 3, 128, 80, dict(gate="wide")),
                                                                ("i8", 40, 5, 33, 65, dict(gate="wide", sink="own")), ("e4m3", 15, 5, 128, 128, dict(chunk=200, keep=9))])
