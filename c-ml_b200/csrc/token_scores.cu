@@ -1,11 +1,13 @@
 // Log probabilities of given tokens, entropy, and the best alternatives of rows of logits.
 //
-//   m = max x, S = sum e^(x - m), Q = sum e^(x - m) (x - m):   log p_t = x_t - m - ln S,   H = ln S - Q / S
+//   m = max x, S = sum of the others' e^(x - m), Q = sum e^(x - m) (x - m):   log p_t = (x_t - m) - ln(1 + S),   H = ln(1 + S) - Q / (1 + S)
 //
-// Both parts of H are positive, so nothing cancels. A row is read once, in 16-byte pieces, by a cluster of 1 to 8 CTAs (more for fewer rows). A thread carries S and Q
-// in fp32, relative to a reference that follows its largest value at a distance: it moves only when a value is above it by more than 6. Q and all exponents are in
-// units of ln 2, so a value costs one multiply-add, one exponential and, two values an instruction, its part of S and Q. Values where that
-// would overflow or lose digits (masked ones, the type's lowest, references beyond a million) are told apart by a piece's range and take a longer way. Threads, warps, CTAs and clusters join in a fixed order.
+// S is not below 0 and Q not above, so neither result cancels, no log probability is above 0 and no entropy below, and a row of one value has exactly 0 for both. A row is
+// read once, in 16-byte pieces, by a cluster of 1 to 8 CTAs (more for fewer rows). A thread carries both sums in fp32, the largest value's term among them, relative to a
+// reference that its warp shares and that follows the warp's largest value at a distance: it moves only when a value is above it by more than 1. At the end of the pass the
+// term of the warp's largest value, which is known to the bit, is taken out, and what is left is brought to that value. Q and all exponents are in
+// units of ln 2, so a value costs one multiply-add, one exponential and, two values an instruction, its part of both sums. Values where that
+// would overflow or lose digits (masked ones, the type's lowest, references beyond a million) are told apart by a round's range and take a longer way. Threads, warps, CTAs and clusters join in a fixed order.
 //
 // The alternatives need no second pass over the row. A thread remembers the largest of its pieces; the k-th largest of the
 // maxima of the CTA's groups of eight threads is a bound that at least k values reach, and few threads hold anything that does. Their pieces are read
@@ -80,14 +82,19 @@ __device__ __forceinline__ float second(u64 v) { return __uint_as_float((uint32_
 __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) { u64 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
 __device__ __forceinline__ u64 add2(u64 a, u64 b) { u64 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 
-// S and Q of a part of a row, relative to m; Q and everything that exponents are made of in units of ln 2
+// A part of a row: its largest value m, and S and Q of all the others relative to it (no S where there are none, never below zero; Q, in units of ln 2, never
+// above). The largest value's own term is exactly 1 and 0 and is not in them, so a part of one value has S = Q = 0.
 struct Sums { float m, s, q; };
 __device__ __forceinline__ float warp_max(float v) { float m; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v)); return m; }
-// what the parts of every `lanes` lanes in turn (a power of two) have together; all lanes' largest is the same
+// what the parts of every `lanes` lanes in turn (a power of two) have together, where those of all such sets of lanes are the same. The first lane that has the largest
+// value keeps it out; the other lanes' largest values are values like any other.
 template <int lanes>
 __device__ __forceinline__ Sums join(const Sums& a) {
+    const int lane = (threadIdx.x & 31) & (lanes - 1);
     const float m = warp_max(a.m), d = fmaxf(a.m - m, -1e4f) * kLog2e, c = ex2(d);            // (nothing anywhere: c = 0, and NaN in s stays)
-    float q = c * fmaf(d, a.s, a.q), s = a.s * c;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, a.m == m)) - 1;
+    float s = a.s + (lane == owner || a.m == -INFINITY ? 0.f : 1.f), q = c * fmaf(d, s, a.q);
+    s *= c;
 #pragma unroll
     for (int o = lanes / 2; o > 0; o >>= 1) {
         s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -98,35 +105,55 @@ __device__ __forceinline__ Sums join(const Sums& a) {
 
 constexpr float TS_TAME = 1048576.f;                   // references up to here: what fl(ref log2(e)) is off by stays below 2^-3
 constexpr float TS_LEAST = -1e37f;                     // values down to here: their products with log2(e) do not overflow
-constexpr float TS_LAZY = 6.f;                         // the reference moves when a value is above it by more than this: e^6 times fewer values than 2^30 fit fp32 easily
+constexpr float TS_LAZY = 1.f;                         // the reference moves when a value is above it by more than this, so exponents are below 1.5 and lose no digits of Q
 
-// S and Q of a thread's values. The exponent of a value is x log2(e) - fl(ref log2(e)), one rounding; `shift` is what the second product's rounding moved the
-// reference by, and is put right when the reference moves and at the end.
+// S and Q of a thread's values, relative to a reference that its warp's threads share. The exponent of a value is x log2(e) - fl(ref log2(e)), one rounding; `shift` is what
+// the second product's rounding moved the reference by, and is put right when the reference moves.
 struct Running {
     float ref = -INFINITY, minus = 0.f, shift = 0.f;
     u64 s = 0ull, q = 0ull;
-    __device__ __forceinline__ void scale(float d) {                         // exponents grow by d
-        const float c = ex2(d);
-        const u64 c2 = two(c, c), d2 = two(d, d);
-        q = fma2(c2, fma2(d2, s, q), 0ull);
-        s = fma2(c2, s, 0ull);
-    }
+    __device__ __forceinline__ bool tame() const { return fabsf(ref) <= TS_TAME; }
     __device__ __forceinline__ void move(float to) {
         const float d = fmaxf(ref - to, -1e4f) * kLog2e - shift;
         ref = to;
-        minus = fabsf(to) <= TS_TAME ? -(to * kLog2e) : 0.f;
-        shift = fabsf(to) <= TS_TAME ? fmaf(to, kLog2e, minus) : 0.f;
-        scale(d + shift);
+        minus = tame() ? -(to * kLog2e) : 0.f;
+        shift = tame() ? fmaf(to, kLog2e, minus) : 0.f;
+        const float by = d + shift, c = ex2(by);                             // exponents grow by that
+        const u64 c2 = two(c, c), d2 = two(by, by);
+        q = fma2(c2, fma2(d2, s, q), 0ull);
+        s = fma2(c2, s, 0ull);
     }
+    // of any value; of one at or above TS_LEAST the fast way finds the same bits
+    __device__ __forceinline__ float exponent(float x) const { return tame() ? fmaf(x, kLog2e, minus) : (x - (ref == -INFINITY ? 0.f : ref)) * kLog2e; }
     // values beside masked ones, or as large as numbers get
     __device__ __forceinline__ void take_wild(float x) {
-        const float t = fmaf(x - (ref == -INFINITY ? 0.f : ref), kLog2e, shift), e = ex2(t);
+        const float t = exponent(x), e = ex2(t);
         s = add2(s, two(e, 0.f));
         q = fma2(two(e, 0.f), two(fmaxf(t, -1e4f), 0.f), q);
     }
-    __device__ __forceinline__ Sums sums() {
-        scale(-shift);
-        return {ref, first(s) + second(s), first(q) + second(q)};
+    // The warp's part, `most` being this thread's largest value. What the largest of all put into the sums is taken out again, to the bit (it was met under the present
+    // reference: only a larger value could have moved that since); what rounding leaves on the wrong side of zero is nothing.
+    __device__ __forceinline__ Sums sums(float most) const {
+        const int lane = threadIdx.x & 31;
+        const float m = warp_max(most);
+        const int owner = __ffs(__ballot_sync(0xffffffffu, most == m)) - 1;
+        float ss = first(s) + second(s), qq = first(q) + second(q);
+        const float t = exponent(m);
+        if (lane == owner && m > -INFINITY) {
+            const float e = ex2(t);
+            ss -= e;
+            qq -= __fmul_rn(e, t);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            qq += __shfl_xor_sync(0xffffffffu, qq, o);
+        }
+        if (m == -INFINITY) return {m, ss, qq};        // (nothing, or NaN)
+        const float c = ex2(-t);
+        qq = c * fmaf(-t, ss, qq);
+        ss *= c;
+        return {m, ss < 0.f ? 0.f : ss, qq > 0.f ? 0.f : qq};
     }
 };
 __device__ __forceinline__ uint32_t remote(const void* p, int rank) {
@@ -163,16 +190,16 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
     float best = -INFINITY;                            // largest value, and the number of its piece
     uint32_t best_piece = 0;
     auto note = [&](float most, uint32_t piece) {
-        if (TOP && most > best) { best = most; best_piece = piece; }
-        if (most > a.ref + TS_LAZY) a.move(most);
+        if (most > best) { best = most; best_piece = piece; }
     };
-    auto take_one = [&](float x, uint32_t piece) { note(x, piece); a.take_wild(x); };
-    auto take = [&](const uint4& u, uint32_t piece) {
-        float most, least, x[PER];
-        range_of<T>(u, most, least);
+    // all of a warp come here, before they take values of which this thread's largest is `most`
+    auto prepare = [&](float most) {
+        if (__any_sync(0xffffffffu, most > a.ref + TS_LAZY)) a.move(fmaxf(a.ref, warp_max(most)));
+    };
+    auto take = [&](const uint4& u, bool fast) {
+        float x[PER];
         widen_piece<T>(u, x);
-        note(most, piece);
-        if (least >= TS_LEAST && fabsf(a.ref) <= TS_TAME) {
+        if (fast) {
             const u64 unit = two(kLog2e, kLog2e), minus = two(a.minus, a.minus);
 #pragma unroll
             for (int i = 0; i < PER; i += 2) {
@@ -187,19 +214,49 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
     };
     // numbers of pieces ascend along the row: head values, pieces, tail values
     auto single = [&](int i) { return i < head ? (uint32_t)i : (uint32_t)(head + pieces + i); };
-    const bool has_head = rank == 0 && (int)threadIdx.x < head, has_tail = rank == splits - 1 && (int)threadIdx.x < tail;
-    if (has_head) take_one(widen(row[threadIdx.x]), single(threadIdx.x));
-    int v = lo + threadIdx.x;
-    for (; v + 3 * THREADS < hi; v += 4 * THREADS) {
+    auto take_one = [&](bool on, const T* at, int i) {
+        const float x = on ? widen(*at) : -INFINITY;
+        note(x, single(i));
+        prepare(x);
+        if (on) a.take_wild(x);
+    };
+    if (rank == 0 && warp * 32 < head) take_one((int)threadIdx.x < head, row + threadIdx.x, threadIdx.x);
+    // Four pieces a thread and round, a warp's threads together; the last round has what is left
+    auto round = [&](int v, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
         uint4 u[4];
+        float most = -INFINITY, least = INFINITY;      // one masked value sends all of the round the longer way
 #pragma unroll
-        for (int j = 0; j < 4; j++) u[j] = ld_row(body + (size_t)(v + j * THREADS) * PER);
+        for (int j = 0; j < 4; j++) if (WHOLE || v + j * THREADS < hi) u[j] = ld_row(body + (size_t)(v + j * THREADS) * PER);
 #pragma unroll
-        for (int j = 0; j < 4; j++) take(u[j], (uint32_t)(head + v + j * THREADS));
-    }
-    for (; v < hi; v += THREADS) take(ld_row(body + (size_t)v * PER), (uint32_t)(head + v));
-    if (has_tail) take_one(widen(body[(size_t)pieces * PER + threadIdx.x]), single(head + threadIdx.x));
-    const Sums w_part = join<32>(a.sums());
+        for (int j = 0; j < 4; j++)
+            if (WHOLE || v + j * THREADS < hi) {
+                float m, l;
+                range_of<T>(u[j], m, l);
+                if (!WHOLE) note(m, (uint32_t)(head + v + j * THREADS));
+                most = fmaxf(most, m);
+                least = fminf(least, l);
+            }
+        if (WHOLE && most > best) {                    // (seldom)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (TOP) {
+                    float m, l;
+                    range_of<T>(u[j], m, l);
+                    note(m, (uint32_t)(head + v + j * THREADS));
+                }
+            best = most;
+        }
+        prepare(most);
+        const bool fast = least >= TS_LEAST && a.tame();
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (WHOLE || v + j * THREADS < hi) take(u[j], fast);
+    };
+    int v = lo + warp * 32;
+    for (; v + 3 * THREADS + 32 <= hi; v += 4 * THREADS) round(v + lane, std::true_type());
+    if (v < hi) round(v + lane, std::false_type());
+    if (rank == splits - 1 && warp * 32 < tail) take_one((int)threadIdx.x < tail, body + (size_t)pieces * PER + threadIdx.x, head + threadIdx.x);
+    const Sums w_part = a.sums(best);
     if (lane == 0) w_sums[warp] = w_part;
     const u64 mine = TOP ? key_of(best, best_piece) : 0ull;
     if (TOP) {
@@ -290,13 +347,13 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
     if (rank) return;                                  // (nobody reads another CTA's memory from here on)
     const Sums none = {-INFINITY, 0.f, 0.f}, t = join<8>((lane & 7) < splits ? c_sums[lane & 7] : none);
     const bool nothing = t.m == -INFINITY && t.s == 0.f;
-    const float ls = logf(t.s);
+    const float ls = log1pf(t.s);                      // (t.s is not below 0, so no log probability is above it)
     if (threadIdx.x == 0) {
         if (logprob) {
             const int id = tokens[r];
             logprob[r] = nothing || id < 0 || id >= vocab ? -INFINITY : (widen(row[id]) - t.m) - ls;
         }
-        if (entropy) entropy[r] = nothing ? 0.f : ls - t.q / t.s * kLn2;
+        if (entropy) entropy[r] = nothing ? 0.f : ls - t.q / (1.f + t.s) * kLn2;
     }
     if (TOP) {
         // what each CTA of the cluster found is in order; nothing below any CTA's last can be wanted
