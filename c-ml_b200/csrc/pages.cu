@@ -62,7 +62,7 @@ pages_copy_kernel(const cmlb200_pages p, const int2* __restrict__ moves, int n, 
             if (moves[mid].x < id) lo = mid + 1;
             else hi = mid;
         }
-        if (lo < n && moves[lo].x == id && (unsigned)moves[lo].y < (unsigned)p.pages) p.table[i] = moves[lo].y;
+        if (lo < n && moves[lo].x == id && (unsigned)id < (unsigned)p.pages && (unsigned)moves[lo].y < (unsigned)p.pages) p.table[i] = moves[lo].y;
     }
 }
 
