@@ -73,7 +73,7 @@ pages_fork_kernel(const cmlb200_pages p, const int4* __restrict__ forks) {
     dep_trigger();
     const int4 f = forks[blockIdx.x];
     const bool own = f.w >= 0;
-    if ((unsigned)f.x >= (unsigned)p.slots || (unsigned)f.y >= (unsigned)p.slots || f.x == f.y || f.z < 0 || f.z + own > p.table_ld || f.w >= p.pages) return;
+    if ((unsigned)f.x >= (unsigned)p.slots || (unsigned)f.y >= (unsigned)p.slots || f.x == f.y || f.z < 0 || f.z > p.table_ld - own || f.w >= p.pages) return;
     const int* from = p.table + (size_t)f.x * p.table_ld;
     if ((int)blockIdx.y < p.pools) {
         if (!own) return;

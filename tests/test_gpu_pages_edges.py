@@ -18,3 +18,13 @@ def test_entries_without_a_page_keep_their_value(pkg, torch_dev):
     pkg.check(pkg.lib.cmlb200_pages_copy(P.p, m.data_ptr(), 4, None))
     P.torch.cuda.synchronize()
     P.check(P.copied(bufs, [(7, 8)]), np.where(t == 7, 8, t))
+
+
+def test_forks_of_more_pages_than_numbers_reach(pkg, torch_dev):
+    """One more than the largest number of shared pages would be a negative one."""
+    P = Pools(pkg, torch_dev, SIZES, 60, 8, 12)
+    bufs, t = P.snapshot()
+    f = P.up([(0, 1, 2 ** 31 - 1, 5), (0, 2, 2 ** 31 - 1, -1), (0, 3, 12, 5)])
+    pkg.check(pkg.lib.cmlb200_pages_fork(P.p, f.data_ptr(), 3, None))
+    P.torch.cuda.synchronize()
+    P.check(bufs, t)
