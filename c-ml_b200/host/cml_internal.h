@@ -27,6 +27,11 @@ void* cml_gguf_read_raw(GGUFContext* ctx, const GGUFTensorInfo* info);
 uint16_t cml_f32_to_f16(float f);
 float cml_f16_to_f32(uint16_t h);
 
+/* The two halves of cml_paged_cache_compact, for callers whose own copies may fail: what would move ([num_blocks][2], returns their number), and the bookkeeping of it,
+ * which cannot. */
+int cml_paged_compact_plan(const CMLPagedKVCache* cache, int* moves);
+void cml_paged_compact_apply(CMLPagedKVCache* cache, const int* moves, int count);
+
 /* NCCL, loaded with dlopen (src/distributed/nccl_backend.c:476-479 does the same). */
 int cml_nccl_unique_id(void* id128);
 int cml_nccl_init(void** comm, int nranks, int rank, const void* id128);

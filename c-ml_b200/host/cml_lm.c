@@ -240,19 +240,25 @@ int cml_lm_sequence_fork(CMLLanguageModel* lm, int seq) {
     return -1;
 }
 
+/* The device copies first: their sources stay as they are, so a call that fails leaves every sequence where it was. */
 int cml_lm_compact(CMLLanguageModel* lm) {
     static const char* who = "cml_lm_compact";
     if (!lm || !lm->cache) { LOG_ERROR("%s: no paged cache", who); return -1; }
-    const int moved = cml_paged_cache_compact(lm->cache, lm->h_moves);
-    if (moved <= 0) return moved;
+    const int moved = cml_paged_compact_plan(lm->cache, lm->h_moves);
+    if (!moved) return 0;
+    if (CML_DEV_FAIL(cmlb200_memcpy_h2d(lm->d_moves, lm->h_moves, 2 * (size_t)moved * sizeof(int), lm->stream), who) ||
+        CML_DEV_FAIL(cmlb200_pages_copy(&lm->block_pages, lm->d_moves, moved, lm->stream), who) || CML_DEV_FAIL(cmlb200_stream_sync(lm->stream), who)) {
+        /* (the table may have been renamed by then) */
+        const size_t table = (size_t)lm->opt.max_sequences * (size_t)lm->table_ld * sizeof(int);
+        if (!CML_DEV_FAIL(cmlb200_memcpy_h2d(lm->d_table, lm->h_table, table, lm->stream), who)) CML_DEV_FAIL(cmlb200_stream_sync(lm->stream), who);
+        return -1;
+    }
+    cml_paged_compact_apply(lm->cache, lm->h_moves, moved);
     for (int s = 0; s < lm->opt.max_sequences; s++) {
         const CMLBlockTable* bt = &lm->cache->sequences[s];
         for (int i = 0; bt->block_ids && i < bt->num_blocks; i++)
             if (bt->block_ids[i] >= 0) lm->h_table[(size_t)s * (size_t)lm->table_ld + (size_t)i] = bt->block_ids[i];
     }
-    DEV(cmlb200_memcpy_h2d(lm->d_moves, lm->h_moves, 2 * (size_t)moved * sizeof(int), lm->stream));
-    DEV(cmlb200_pages_copy(&lm->block_pages, lm->d_moves, moved, lm->stream));
-    DEV(cmlb200_stream_sync(lm->stream));
     return moved;
 }
 

@@ -285,42 +285,60 @@ int cml_paged_cache_fork(CMLPagedKVCache* cache, int seq_id, int* from, int* to)
     return child;
 }
 
-int cml_paged_cache_compact(CMLPagedKVCache* cache, int* moves) {
-    static const char* who = "cml_paged_cache_compact";
-    PagedDev* p = cache ? pd_find(cache) : NULL;
-    if (!p) { LOG_ERROR("%s: not a cache", who); return -1; }
-    const int data = cache->blocks[0].key_data != NULL, n = cache->num_blocks, used = n - cache->free_count;
-    if (!data && !moves) { LOG_ERROR("%s: nowhere to name the blocks to copy", who); return -1; }
-    int* now = (int*)malloc((size_t)n * sizeof(int));      /* a block's new id */
-    if (!now) { LOG_ERROR("%s: allocation failed", who); return -1; }
+int cml_paged_compact_plan(const CMLPagedKVCache* cache, int* moves) {
     int count = 0, hole = 0;
-    for (int i = 0; i < n; i++) now[i] = i;
-    for (int i = used; i < n; i++) {
+    for (int i = cache->num_blocks - cache->free_count; i < cache->num_blocks; i++) {
         if (!cache->blocks[i].in_use) continue;
         while (cache->blocks[hole].in_use) hole++;
-        CMLPageBlock *a = &cache->blocks[i], *b = &cache->blocks[hole];
-        if (moves) { moves[2 * count] = i; moves[2 * count + 1] = hole; }
-        now[i] = hole;
+        moves[2 * count] = i;
+        moves[2 * count++ + 1] = hole++;
+    }
+    return count;
+}
+
+void cml_paged_compact_apply(CMLPagedKVCache* cache, const int* moves, int count) {
+    PagedDev* p = pd_find(cache);
+    const int data = cache->blocks[0].key_data != NULL, n = cache->num_blocks, used = n - cache->free_count;
+    if (!count) return;
+    for (int k = 0; k < count; k++) {
+        const int from = moves[2 * k], to = moves[2 * k + 1];
+        CMLPageBlock *a = &cache->blocks[from], *b = &cache->blocks[to];
         b->in_use = true;
         b->num_tokens = a->num_tokens;
         a->in_use = false;
         a->num_tokens = 0;
-        p->owners[hole] = p->owners[i];
-        p->owners[i] = 0;
+        p->owners[to] = p->owners[from];
+        p->owners[from] = 0;
         if (data) {
             memcpy(b->key_data, a->key_data, block_floats(cache) * sizeof(float));
             memcpy(b->value_data, a->value_data, block_floats(cache) * sizeof(float));
-            p->dev_tokens[hole] = p->dev_tokens[i] = 0;
+            p->dev_tokens[to] = p->dev_tokens[from] = 0;
         }
-        count++;
     }
-    for (int s = 0; count && s < cache->max_sequences; s++) {
+    for (int s = 0; s < cache->max_sequences; s++) {
         CMLBlockTable* bt = &cache->sequences[s];
-        for (int i = 0; bt->block_ids && i < bt->num_blocks; i++)
-            if (bt->block_ids[i] >= 0) bt->block_ids[i] = now[bt->block_ids[i]];
+        for (int i = 0; bt->block_ids && i < bt->num_blocks; i++) {
+            int lo = 0, hi = count;                        /* sources ascend */
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (moves[2 * mid] < bt->block_ids[i]) lo = mid + 1;
+                else hi = mid;
+            }
+            if (lo < count && moves[2 * lo] == bt->block_ids[i]) bt->block_ids[i] = moves[2 * lo + 1];
+        }
     }
-    free(now);
-    for (int i = 0; count && i < n - used; i++) cache->free_list[i] = n - 1 - i;       /* the lowest is handed out first */
+    for (int i = 0; i < n - used; i++) cache->free_list[i] = n - 1 - i;      /* the lowest is handed out first */
+}
+
+int cml_paged_cache_compact(CMLPagedKVCache* cache, int* moves) {
+    static const char* who = "cml_paged_cache_compact";
+    if (!cache || !pd_find(cache)) { LOG_ERROR("%s: not a cache", who); return -1; }
+    if (!cache->blocks[0].key_data && !moves) { LOG_ERROR("%s: nowhere to name the blocks to copy", who); return -1; }
+    int* list = moves ? moves : (int*)malloc(2 * (size_t)cache->num_blocks * sizeof(int));
+    if (!list) { LOG_ERROR("%s: allocation failed", who); return -1; }
+    const int count = cml_paged_compact_plan(cache, list);
+    cml_paged_compact_apply(cache, list, count);
+    if (!moves) free(list);
     return count;
 }
 
