@@ -17,6 +17,7 @@
 // Few tiles are bound by latency: what comes before the first scores (table, codes, expansion, queries: 3 to 4 us), 1.2 (heads of 64) to 1.5 us a key tile of which
 // 0.54 are exponentials, and the end. Heads of 128, 8 of 4 queries each: 64 rows 9.2 us, behind 6,000 tokens 24.3, 512 rows 14.5, 1,024 rows 28.5.
 #include "attention8_tiles.cuh"
+#include "status_word.cuh"
 
 namespace {
 
@@ -376,7 +377,7 @@ attention8_tiles_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int
     }
 }
 
-int* g_status8[kMaxDevices] = {};
+StatusWords<kMaxDevices> g_status8;
 
 template <bool I8, int S, bool SLOPES>
 int launch_tiles(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_tiles, int tiles, __nv_bfloat16* d_out, int out_ld, int* status, cudaStream_t st) {
@@ -417,18 +418,7 @@ int cmlb_attention8_status_word(int** word) {
     int dev = 0;
     CMLB_CUDA(cudaGetDevice(&dev));
     CMLB_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d", dev);
-    if (!g_status8[dev]) {
-        // (allowed beside a stream that is being captured, in any mode)
-        void* p = nullptr;
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        CMLB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-        const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocDefault);
-        CMLB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
-        CMLB_CUDA(e);
-        *static_cast<int*>(p) = 0;
-        g_status8[dev] = static_cast<int*>(p);
-    }
-    *word = g_status8[dev];
+    CMLB_CUDA(g_status8.get(dev, word));
     return CMLB200_OK;
 }
 

@@ -19,6 +19,7 @@
 // Every wait is bounded; one that gives up leaves a code in a status word in host memory, and the CTA still drains its
 // copies, meets its cluster and frees its tensor memory.
 #include "tcgen05_util.cuh"
+#include "status_word.cuh"
 
 namespace {
 
@@ -383,19 +384,13 @@ attention_latent_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __gri
     }
 }
 
-int* g_status[kMaxDevices] = {};
+StatusWords<kMaxDevices> g_status;
 
 int status_word(int** word) {
     int dev = 0;
     CMLB_CUDA(cudaGetDevice(&dev));
     CMLB_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d", dev);
-    if (!g_status[dev]) {
-        void* p = nullptr;
-        CMLB_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocDefault));
-        *static_cast<int*>(p) = 0;
-        g_status[dev] = static_cast<int*>(p);
-    }
-    *word = g_status[dev];
+    CMLB_CUDA(g_status.get(dev, word));
     return CMLB200_OK;
 }
 
