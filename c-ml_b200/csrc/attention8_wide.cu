@@ -62,6 +62,11 @@ attention8_wide_kernel(const cmlb200_attn a, const float* __restrict__ qkv, int 
     const int4 tl = tiles[gridDim.y - 1 - blockIdx.y];                       // a prompt's last tiles, which see most keys, come first
     const int group = a.heads / a.kv_heads, blocks = gridDim.x / a.kv_heads, kh = blockIdx.x / blocks;
     const int n = tl.y, p0 = tl.w, p_last = p0 + n - 1, shift = __ffs(a.block_size) - 1;
+    if (n <= 0) {                                      // (as the form for few tiles does)
+        __syncthreads();
+        if (warp == kIssue) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"((uint32_t)W8_TMEM) : "memory");
+        return;
+    }
     const T8Heads rows = {n, group, (int)(blockIdx.x % blocks) * 4};
     const int* table = a.block_table + (size_t)tl.z * a.table_ld;
     const T8Keys keys(a, p0, p_last, 0, 1);
