@@ -29,10 +29,6 @@ template <int KC, int NT> constexpr int kAhead = KC == 1 ? 6 : (KC == 2 && NT ==
 template <int KC, int VW> constexpr int kGroupBytes = 1024 * KC + 512 * VW;
 constexpr float kWeightBits = 8.f, kFarScale = -60.f;
 
-__device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
-    if (a.chunk > 0) return p / a.chunk * a.chunk;
-    return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
-}
 // 16 tokens of one head, `group` of the pool, from dimension d on
 __device__ __forceinline__ void copy_tokens(uint32_t dst, const CUtensorMap* map, int d, int head, int group, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -42,11 +38,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
-}
-__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
-    return a;
 }
 __device__ __forceinline__ float cluster_load(uint32_t a) {
     float v;

@@ -2,6 +2,7 @@
 // rows of one sequence against key tiles of 128 tokens.
 #pragma once
 #include "cache8.cuh"
+#include "pairs.cuh"
 #include "tcgen05_util.cuh"
 
 namespace {
@@ -9,10 +10,6 @@ namespace {
 constexpr int T8_KEYS = 128, T8_SLAB = T8_KEYS * 128, T8_ROWS = 128, T8_GROUPS = T8_KEYS / kScaleTokens, T8_SPLITS = 8;
 constexpr float kLazy = 8.f, kWeightBits = 7.f, kFarScale = -60.f;
 
-__device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
-    if (a.chunk > 0) return p / a.chunk * a.chunk;
-    return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
-}
 // Products whose descriptors differ from one another in their lower halves alone.
 __device__ __forceinline__ void umma_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accum) {
     asm volatile("{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n"
@@ -35,23 +32,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
 }
 
-// two numbers at a time
-__device__ __forceinline__ uint64_t pair_of(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

@@ -12,6 +12,12 @@ namespace {
 
 constexpr int kScaleTokens = 16;
 
+// The first key that the row at position p sees, the kept ones (0 .. keep - 1) aside.
+__device__ __forceinline__ int first_key8(const cmlb200_attn& a, int p) {
+    if (a.chunk > 0) return p / a.chunk * a.chunk;
+    return (a.window > 0 && a.window <= p) ? p - a.window + 1 : 0;
+}
+
 // The smallest allowed power of two that holds `most` (not negative, at most 65504).
 template <bool I8> __device__ __forceinline__ float scale8_for(float most) {
     // most = m 2^x with 1/2 <= m < 1; 127 = 127/128 2^7, 448 = 7/8 2^9

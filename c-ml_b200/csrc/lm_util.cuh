@@ -141,6 +141,12 @@ __device__ __forceinline__ float soft_cap(float v, float cap) { return cap * tan
 // Pieces of the mma.sync kernels.
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// where rank's CTA of the cluster has what lies at p in this one
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }

@@ -21,13 +21,14 @@
 #include <type_traits>
 
 #include "lm_util.cuh"
+#include "pairs.cuh"
 
 namespace {
 
 constexpr float kLn2 = 0.693147180559945f;
 constexpr int TS_MOST = 32, TS_ROOM = 1024;
 
-typedef unsigned long long u64;
+typedef uint64_t u64;
 
 // monotonic in the value; 0 is below everything that can be wanted
 __device__ __forceinline__ uint32_t order_bits(float v) {
@@ -75,13 +76,6 @@ __device__ __forceinline__ uint4 ld_row(const void* p) {
     asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
-// two fp32 operations an instruction
-__device__ __forceinline__ u64 two(float a, float b) { return ((u64)__float_as_uint(b) << 32) | __float_as_uint(a); }
-__device__ __forceinline__ float first(u64 v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float second(u64 v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) { u64 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
-__device__ __forceinline__ u64 add2(u64 a, u64 b) { u64 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
-
 // A part of a row: its largest value m, and S and Q of all the others relative to it (no S where there are none, never below zero; Q, in units of ln 2, never
 // above). The largest value's own term is exactly 1 and 0 and is not in them, so a part of one value has S = Q = 0.
 struct Sums { float m, s, q; };
@@ -119,17 +113,17 @@ struct Running {
         minus = tame() ? -(to * kLog2e) : 0.f;
         shift = tame() ? fmaf(to, kLog2e, minus) : 0.f;
         const float by = d + shift, c = ex2(by);                             // exponents grow by that
-        const u64 c2 = two(c, c), d2 = two(by, by);
-        q = fma2(c2, fma2(d2, s, q), 0ull);
-        s = fma2(c2, s, 0ull);
+        const u64 c2 = pair_of(c, c), d2 = pair_of(by, by);
+        q = fma_pair(c2, fma_pair(d2, s, q), 0ull);
+        s = fma_pair(c2, s, 0ull);
     }
     // of any value; of one at or above TS_LEAST the fast way finds the same bits
     __device__ __forceinline__ float exponent(float x) const { return tame() ? fmaf(x, kLog2e, minus) : (x - (ref == -INFINITY ? 0.f : ref)) * kLog2e; }
     // values beside masked ones, or as large as numbers get
     __device__ __forceinline__ void take_wild(float x) {
         const float t = exponent(x), e = ex2(t);
-        s = add2(s, two(e, 0.f));
-        q = fma2(two(e, 0.f), two(fmaxf(t, -1e4f), 0.f), q);
+        s = add_pair(s, pair_of(e, 0.f));
+        q = fma_pair(pair_of(e, 0.f), pair_of(fmaxf(t, -1e4f), 0.f), q);
     }
     // The warp's part, `most` being this thread's largest value. What the largest of all put into the sums is taken out again, to the bit (it was met under the present
     // reference: only a larger value could have moved that since); what rounding leaves on the wrong side of zero is nothing.
@@ -137,7 +131,10 @@ struct Running {
         const int lane = threadIdx.x & 31;
         const float m = warp_max(most);
         const int owner = __ffs(__ballot_sync(0xffffffffu, most == m)) - 1;
-        float ss = first(s) + second(s), qq = first(q) + second(q);
+        float s0, s1, q0, q1;
+        unpair(s, s0, s1);
+        unpair(q, q0, q1);
+        float ss = s0 + s1, qq = q0 + q1;
         const float t = exponent(m);
         if (lane == owner && m > -INFINITY) {
             const float e = ex2(t);
@@ -156,11 +153,6 @@ struct Running {
         return {m, ss < 0.f ? 0.f : ss, qq > 0.f ? 0.f : qq};
     }
 };
-__device__ __forceinline__ uint32_t remote(const void* p, int rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
-    return a;
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -200,12 +192,15 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
         float x[PER];
         widen_piece<T>(u, x);
         if (fast) {
-            const u64 unit = two(kLog2e, kLog2e), minus = two(a.minus, a.minus);
+            const u64 unit = pair_of(kLog2e, kLog2e), minus = pair_of(a.minus, a.minus);
 #pragma unroll
             for (int i = 0; i < PER; i += 2) {
-                const u64 t = fma2(two(x[i], x[i + 1]), unit, minus), e = two(ex2(first(t)), ex2(second(t)));
-                a.s = add2(a.s, e);
-                a.q = fma2(e, t, a.q);
+                const u64 t = fma_pair(pair_of(x[i], x[i + 1]), unit, minus);
+                float t0, t1;
+                unpair(t, t0, t1);
+                const u64 e = pair_of(ex2(t0), ex2(t1));
+                a.s = add_pair(a.s, e);
+                a.q = fma_pair(e, t, a.q);
             }
         } else {
 #pragma unroll
@@ -270,7 +265,7 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
     __syncthreads();
     if (warp == 0) {
         const Sums none = {-INFINITY, 0.f, 0.f}, t = join<32>(lane < WARPS ? w_sums[lane] : none);
-        const uint32_t dst = remote(&c_sums[rank], 0);
+        const uint32_t dst = cluster_addr(&c_sums[rank], 0);
         if (lane == 0) {
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(t.m) : "memory");
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(t.s) : "memory");
@@ -317,7 +312,7 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
         });
         __syncthreads();
         const int nr = num_room;
-        const uint32_t dst = remote(&c_best[rank * top], 0);
+        const uint32_t dst = cluster_addr(&c_best[rank * top], 0);
         if (nr <= TS_ROOM) {
             for (int i = threadIdx.x; i < nr; i += THREADS) {
                 const u64 k = room[i];
