@@ -9,7 +9,7 @@
 //                                        interleaved, which makes the operand's pairs. P^T comes from S^T by movmatrix
 // so a lane's operands are pieces of the cache as they lie there. One TMA copy a group brings 16 tokens of a head (128 bytes of every kv_heads * 128 at heads of 128),
 // three to six groups ahead of the warp that asked for them; group numbers and scales are looked up 32 at a time, one a lane. (32 rows of 8 heads behind 8,192 tokens,
-// 537 MB: 101.5 us, 5.3 TB/s. With 16-byte copies by the lanes themselves it took 138 us, 133 without any arithmetic; with one group a warp under way in registers 135.)
+// 537 MB: 104 us as int8, 98 as e4m3, 5.2 to 5.5 TB/s. With 16-byte copies by the lanes themselves it took 138 us, 133 without any arithmetic; with one group a warp under way in registers 135.)
 // The next group's scores are issued beside one group's value products. int8 keys stay 1,152 too large, as they come out of their conversion: the
 // scores' accumulators begin at -1,152 times the sum of the head's queries, so every term is exact and the fp32 sums are off by no more than the queries' own rounding.
 // A group's key scale multiplies its scores, its value scale the weights: as fp16 they are 2^s * scale over the largest such product that the head has met, times 256: never above 2^15,
@@ -629,7 +629,7 @@ int launch_one(const cmlb200_attn* a, const float* d_qkv, int ld, const int* d_r
     CMLB_CUDA(cmlb_ensure_smem(kern, smem, attr));
     // How many CTAs share a row's keys: what takes least by an estimate in units of a warp's time for a group (1.2 us where few are under way): 6 for a CTA's
     // beginning and end, times the waves, where clusters of a size share the device with as many as fit its groups of SMs. (One row of 8 heads behind 32,000
-    // tokens: 45 us by 8, 35 by 16. 8 behind 2,000, when a group took a third longer: 18.3 us by 4, 24.4 by 2, 27.7 by 8, which takes two waves.)
+    // tokens: 45 us by 8, 35 by 16. 8 behind 2,000: 15.9 us; when a group took a third longer, 18.3 by 4, 24.4 by 2, 27.7 by 8, which takes two waves.)
     static int room[kMaxDevices][A1_SPLITS + 1] = {};
     if (!room[cmlb_device_index()][1]) CMLB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     const long long base = (long long)rows * a->kv_heads * passes, groups = (keys + kScaleTokens - 1) / kScaleTokens;

@@ -15,7 +15,7 @@
 // Keys behind a portion's last row are read as that row's (their weights are zero), so nothing other requests left can reach the sums. Every wait is
 // bounded; one that gives up leaves a code in a status word in host memory, the products under way are waited for and tensor memory is freed.
 // Few tiles are bound by latency: what comes before the first scores (table, codes, expansion, queries: 3 to 4 us), 1.2 (heads of 64) to 1.5 us a key tile of which
-// 0.54 are exponentials, and the end. Heads of 128, 8 of 4 queries each: 64 rows 9.2 us, behind 6,000 tokens 24.3, 512 rows 14.5, 1,024 rows 28.5.
+// 0.54 are exponentials, and the end. Heads of 128, 8 of 4 queries each: 64 rows 9.3 us, behind 6,000 tokens 24.5, 512 rows 14.2, 1,024 rows 28.3.
 #include "attention8_tiles.cuh"
 #include "status_word.cuh"
 

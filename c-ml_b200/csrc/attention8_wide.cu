@@ -5,8 +5,10 @@
 //   0 .. 7    softmax, a thread a row, warps 0 .. 3 the first block's
 //   8 .. 15   expansion, four warps for keys and four for values (the next tile's codes are requested once this one's are written)
 //   16, 17    issue tcgen05.mma, a block each: the scores of half tile j + 1, then P V of half tile j
-// Measured with 8 heads of 128 and 4 queries each: 4,096 rows behind 4,096 tokens 483 us, 853 TFLOP/s, with softmax and products both under way most of the time;
-// 2,048 rows without a cache 55.6 us.
+// Measured with 8 heads of 128 and 4 queries each: 4,096 rows behind 4,096 tokens 494 us, 835 TFLOP/s (489 as e4m3); 2,048 rows without a cache 55.6 us. Bound by the chain of a softmax
+// warp, and by score products of 64 keys: 6 KB of operands from shared memory are 48 cycles of its 128 bytes, the product itself 32. (Counters: the tensor
+// cores' own pipe active half of the time, products 38 %.) 80 registers a thread of the expansion are a third of what is shared out; with fewer warps there, softmax threads could hold 128 keys.
+// Where a key/value head has 5 or 6 query heads, the second CTA's second block has none and is computed all the same (2,048 rows, 8 key/value heads: 113 us and 115).
 // Tensor memory: a block's 2 x 64 columns of scores, over which its weights lie, then the blocks' O.
 #include "attention8_tiles.cuh"
 

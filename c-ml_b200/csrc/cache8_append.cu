@@ -5,8 +5,9 @@
 // rows, a lane four neighbouring dimensions of each (and of the 128 behind, where heads are that wide): norm and rotation stay in the lane, the largest
 // magnitudes meet in shared memory once, the scales are settled with those of the group's earlier tokens, and a lane's four codes are one store of a
 // row's contiguous ones. Earlier codes are rewritten only where their scale has grown. Everything a CTA needs is requested before its first wait.
-// Bound by the rows' fp32 columns, which are read once (the keys again where a norm spans all heads): 4,096 rows of 8 heads of 128 in 12.9 us (42 MB, 3.3 TB/s), 64 rows
-// in 3.4, most of it a launch and two dependent loads. (With a loop over the rows' positions in place of the one ballot that finds a group's rows: 48.8 and 11.3 us.)
+// Bound by the rows' fp32 columns, which are read once (the keys again where a norm spans all heads), and by how little of it is under way: a CTA serves one group, so 4,096 rows
+// of 8 heads of 128 take three and a half rounds of positions, rows, page and scale, and nothing of the next group is requested meanwhile: 12.7 us (42 MB, 3.3 TB/s; e4m3 13.2), 64 rows
+// in 3.4, most of it a launch and two dependent loads. Queries that are normed or turned are rewritten by one CTA for 16 rows: 4,096 rows of 32 query heads 72 us, 512 25 to 32. (With a loop over the rows' positions in place of the one ballot that finds a group's rows: 48.8 and 11.3 us.)
 #include "cache8.cuh"
 
 namespace {

@@ -3,7 +3,7 @@
 //
 // A page id names the same slot in every pool (a layer's keys, its values, their scales), and pools differ in the size of a page. One launch
 // serves all of them: a CTA moves pieces of 16 KB of one page in one pool or four, four 16-byte loads a thread ahead of their stores, which keeps
-// 64 KB of reads in flight on an SM. Bound by memory: each byte is read once and written once. Measured: 900 pages of 16 layers (keys, values, scales; 946 MB read
+// 96 KB of reads in flight on an SM (six CTAs of 40 registers a thread). Bound by memory: each byte is read once and written once. Measured: 900 pages of 16 layers (keys, values, scales; 946 MB read
 // and written) in 158 us, 6.0 TB/s; four children of a sequence of 777 tokens in 32 layers in 3.0 us.
 #include "lm_util.cuh"
 
@@ -103,7 +103,7 @@ extern "C" int cmlb200_pages_copy(const cmlb200_pages* p, const int* d_moves, in
     CMLB_REQUIRE(((uintptr_t)d_moves & 7) == 0, "%s: the list of moves must be 8-byte aligned", who);
     CMLB_REQUIRE(p->pools > 0 || p->table, "%s: neither pools nor a table", who);
     // Four pools a CTA where CTAs would be many: pools of scales are little work for one (64 pools, 900 moves: 158 us, 168 by one pool a CTA; pages of a quarter: 109 and
-    // 152), one where they are few (40 moves: 6.3 us, 9.7 by four). 8 of them run on an SM at a time.
+    // 152), one where they are few (40 moves: 6.3 us, 9.7 by four).
     const int each = (long long)moves * p->pools >= 64LL * cmlb_num_sms() ? 4 : 1;
     CMLB_CUDA(launch_chain(pages_copy_kernel, dim3(moves, (p->pools + each - 1) / each + (p->table ? 1 : 0), pieces_of(p)), dim3(PG_THREADS), 0, 1, as_stream(stream), *p, (const int2*)d_moves,
                            moves, each));

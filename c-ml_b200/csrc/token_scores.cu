@@ -16,8 +16,8 @@
 // few threads' pieces), the k best are picked one after the other from the same pieces.
 //
 // Many rows are bound by the bytes of the logits and the exponentials beside them, few by the chain of barriers behind the pass. Measured: 2,000 rows of 128,000 bf16
-// 91.5 us (5.6 TB/s; 57 us are exponentials at 16 a clock and SM), 700 of 128,000 fp32 62.6 us (5.7 TB/s), 256 of 32,000 fp32 with the best 20 15.3 us (10.4 without),
-// one of 32,000 with the best 5 5.5 us. Requesting pieces a round ahead cost more registers, and so CTAs under way, than it gave (2,000 rows: 98 to 115 us).
+// 91.5 us (5.6 TB/s; 57 us are exponentials at 16 a clock and SM), 700 of 128,000 fp32 61.8 us (5.8 TB/s), 256 of 32,000 fp32 with the best 20 15.2 us (10.1 without),
+// one of 32,000 with the best 5 5.6 us. Requesting pieces a round ahead cost more registers, and so CTAs under way, than it gave (2,000 rows: 98 to 115 us).
 #include <type_traits>
 
 #include "lm_util.cuh"
@@ -374,11 +374,11 @@ token_scores_kernel(const T* __restrict__ logits, long ld, int vocab, const int*
 template <typename T>
 int launch_scores(const void* d_logits, long ld, int rows, int vocab, const int* d_tokens, int top, float* d_logprob, float* d_entropy, int* d_top_ids, float* d_top_logprob, cudaStream_t st) {
     // A cluster's CTAs read at least 8 KB each; more of them share a row while every one has an SM of its own (64 rows of 50,000 bf16, best 20: 8.3 us by
-    // two each, 9.3 by one, 11 by four)
+    // two each, 9.5 by one, 11.1 by four)
     int splits = 1;
     while (splits < 8 && (long long)rows * splits * 2 <= cmlb_num_sms() && (size_t)vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
-    // Many short rows are a matter of how many CTAs are under way, not of how fast each is: 256 threads for those (2,000 rows of 1,000, best 5: 14.3 us, with
-    // 512 threads 24.8; 256 rows of 32,000, best 20: 19.3 and 15.3)
+    // Many short rows are a matter of how many CTAs are under way, not of how fast each is: 256 threads for those (2,000 rows of 1,000, best 5: 15.7 us, with
+    // 512 threads 27.0; 256 rows of 32,000, best 20: 19.0 and 15.4)
     const bool small = (long long)rows >= 4 * cmlb_num_sms() && (size_t)vocab * sizeof(T) <= 65536;
     const dim3 grid((unsigned)rows * splits);
     auto run = [&](auto kernel, int threads) {

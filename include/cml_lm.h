@@ -59,7 +59,7 @@ int cml_lm_sequence_length(CMLLanguageModel* lm, int seq);
 /* A new sequence that goes on from where `seq` stands: it shares the blocks that are full, has a copy of the one that is not, and of a recurrence's state.
  * Id, -1: no free slot or block (or a class without a paged pool). */
 int cml_lm_sequence_fork(CMLLanguageModel* lm, int seq);
-/* Moves the blocks in use to the lowest ids of the pool. Returns how many moved, -1. */
+/* Moves the blocks in use to the lowest ids of the pool. Returns how many moved, -1: a call of the device failed, and nothing has changed. */
 int cml_lm_compact(CMLLanguageModel* lm);
 /* Blocks of the pool (cml_lm_block_size tokens each): all of them, and those not in use. */
 int cml_lm_block_size(const CMLLanguageModel* lm);

@@ -586,7 +586,9 @@ int cmlb200_residual_norm(float* d_x, const float* d_y, int ldy, const float* d_
  * 2^-126, that holds the largest of the group's new numbers in 127 (int8) or 448 (e4m3) steps, or leaves it as it is where the sequence's
  * earlier tokens in the group have a larger one; codes are numbers over the scale, rounded to even, and earlier codes are rounded to a scale that
  * has grown. Numbers beyond 65504 are held there, NaN is cached as 0. Attention is over what the cache then holds, the row's own key and value
- * included. The rows of one sequence follow one another in a call, in order of position, and nothing else of the device writes or reads their
+ * included. What is narrower than over 16-bit caches: queries are rounded to fp16 over a power of two of their own (2^-11 of the largest number's
+ * binade), and so is a key's weight times its group's value scale, relative to the largest such product of the row (2^-11 of itself down to 2^-21 of that one, 2^-32 of that one below).
+ * Statistics of the softmax, sums and merges are fp32. The rows of one sequence follow one another in a call, in order of position, and nothing else of the device writes or reads their
  * groups meanwhile. Entry points: cmlb200_qk_norm_append, cmlb200_rotate_append (no conv), cmlb200_attention_tiles, cmlb200_attention_one;
  * value heads up to 256, key heads up to 256. cmlb200_attention8_status is not 0 once a bounded wait of an attention kernel over such a cache has
  * expired (valid when the stream has drained). */
@@ -734,7 +736,8 @@ int cmlb200_moe_glu_rows_f32(const float* d_gu, int ld, int rows, int ff, int ac
  * log probabilities: top_ids, top_logprob [rows][top]. tokens and logprob, entropy, and either of the last two may be NULL. Logits of -inf are
  * tokens that cannot come: log probability -inf, no part of the entropy, no alternative (places without one hold id -1 and -inf). A row of
  * nothing but such has log probabilities of -inf, entropy 0 and no alternatives; a token outside the vocabulary has -inf. A row that holds NaN or +inf has NaN
- * for log probabilities and entropy, and its alternatives are those of its other numbers and +inf. Sums are fp32. Stands for the
+ * for log probabilities and entropy, and its alternatives are those of its other numbers and +inf. Sums are fp32, relative to the row's largest value, whose own part in them
+ * is exact: no log probability is above 0, no entropy below, and both are 0 for the only token that can come. Stands for the
  * softmax loops on the host of src/nn/llama.c:662-737. */
 int cmlb200_token_scores(const void* d_logits, int dtype, long ld, int rows, int vocab, const int* d_tokens, int top, float* d_logprob, float* d_entropy, int* d_top_ids,
                          float* d_top_logprob, void* stream);
