@@ -735,7 +735,7 @@ int cmlb200_moe_glu_rows_f32(const float* d_gu, int ld, int rows, int ff, int ac
  * entropy[r] of that distribution in nats, and the `top` (0 .. 32) likeliest tokens of the row, best first, the lower id first among equals, with their
  * log probabilities: top_ids, top_logprob [rows][top]. tokens and logprob, entropy, and either of the last two may be NULL. Logits of -inf are
  * tokens that cannot come: log probability -inf, no part of the entropy, no alternative (places without one hold id -1 and -inf). A row of
- * nothing but such has log probabilities of -inf, entropy 0 and no alternatives; a token outside the vocabulary has -inf. A row that holds NaN or +inf has NaN
+ * nothing but such has log probabilities of -inf, entropy 0 and no alternatives; a token outside the vocabulary has -inf in any row. A row that holds NaN or +inf has NaN
  * for log probabilities and entropy, and its alternatives are those of its other numbers and +inf. Sums are fp32, relative to the row's largest value, whose own part in them
  * is exact: no log probability is above 0, no entropy below, and both are 0 for the only token that can come. Stands for the
  * softmax loops on the host of src/nn/llama.c:662-737. */

@@ -87,3 +87,13 @@ def test_values_five_to_six_apart(pkg, torch_dev, order):
     x[np.arange(2000), at + 4096] = x[np.arange(2000), at] + order * r.uniform(5, 6, 2000).astype(np.float32)
     got, ref = call(pkg, torch, torch.from_numpy(x).to(torch_dev), x.argmax(1), 1), want(x, x.argmax(1), 1)
     assert np.abs(got[0] - ref[0]).max() <= 2.0 ** -22 and np.abs(got[1] - ref[1]).max() <= 2.0 ** -22 and (got[0] <= 0).all() and (got[1] >= 0).all()
+
+
+def test_tokens_outside_the_vocabulary(pkg, torch_dev):
+    """-inf in any row, those of NaN and of nothing among them."""
+    import torch
+    x = torch.randn(6, 77, device=torch_dev)
+    x[1, 5], x[2, 6], x[3] = float("nan"), float("inf"), -float("inf")
+    for bad in (-1, 77, 2 ** 31 - 1, -2 ** 31):
+        lp, en, _, _ = call(pkg, torch, x, [bad] * 6, 0)
+        assert np.isneginf(lp).all() and np.isnan(en[1:3]).all() and en[3] == 0 and np.isfinite(en[[0, 4, 5]]).all()
