@@ -497,6 +497,16 @@ class Pages(C.Structure):
     _fields_ = [("pools", ci), ("pool", vp), ("most", C.c_size_t), ("pages", ci), ("table", vp), ("slots", ci), ("table_ld", ci)]
 
 
+class Dense8(C.Structure):
+    """cmlb200_dense8."""
+    _fields_ = [("rows", ci), ("cols", ci), ("ld", ci), ("w", vp), ("scale", vp), ("bias", vp), ("cap", C.c_float)]
+
+
+class Drafts(C.Structure):
+    """cmlb200_drafts."""
+    _fields_ = [("sequences", ci), ("rows", ci), ("first", vp), ("tokens", vp), ("logits", vp), ("ld", C.c_long), ("temperature", vp), ("random", vp)]
+
+
 class LMOptions(C.Structure):
     _fields_ = [("dtype", ci), ("max_tokens", ci), ("max_sequences", ci), ("max_step_rows", ci), ("cache", ci)]
 
@@ -507,6 +517,13 @@ class LMEntry(C.Structure):
 
 _sig("cmlb200_embed_rows", ci, vp, ci, vp, vp, vp, ci, ci, ci, vp, vp)
 _sig("cmlb200_token_scores", ci, vp, ci, C.c_long, ci, ci, vp, ci, vp, vp, vp, vp, vp)
+_sig("cmlb200_quantize_rows", ci, vp, ci, C.c_long, ci, ci, vp, C.c_long, vp, vp)
+_sig("cmlb200_dense8_work_bytes", sz, ci, ci, ci)
+_sig("cmlb200_linear_dense8", ci, C.POINTER(Dense8), vp, ci, C.c_long, ci, vp, C.c_long, vp, vp)
+_sig("cmlb200_linear_dense8_glu", ci, C.POINTER(Dense8), vp, ci, C.c_long, ci, ci, ci, vp, C.c_long, vp, vp)
+_sig("cmlb200_dense8_status", ci, C.POINTER(ci), ci)
+_sig("cmlb200_verify_work_bytes", sz, ci, ci)
+_sig("cmlb200_verify_drafts", ci, C.POINTER(Drafts), vp, ci, C.c_long, ci, vp, vp, vp, vp)
 _sig("cmlb200_pages_copy", ci, C.POINTER(Pages), vp, ci, vp)
 _sig("cmlb200_pages_fork", ci, C.POINTER(Pages), vp, ci, vp)
 _sig("cmlb200_residual_norm", ci, vp, vp, ci, vp, vp, C.c_float, ci, ci, vp, vp, ci, ci, vp)

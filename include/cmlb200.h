@@ -763,6 +763,55 @@ int cmlb200_pages_copy(const cmlb200_pages* p, const int* d_moves, int moves, vo
  * stays. No child is a parent of the same call, no own page another's page. */
 int cmlb200_pages_fork(const cmlb200_pages* p, const int* d_forks, int forks, void* stream);
 
+/* ---- products in 8-bit integers -------------------------------------------------------------------
+ * Rows of x (tokens) and of a weight (channels) as int8 codes with an fp32 scale each: scale = a / 127 and code = 127 v / a rounded to the nearest, ties to even, where a is the
+ * row's largest magnitude, or 127 * 2^-126 where that is larger. A row that holds NaN or an infinity has codes of 0 and scale NaN, so that all that is made of it is NaN. Rows of
+ * 16-bit floats have the codes of exact arithmetic; of fp32, 127 v is rounded to 32 bits first.
+ * Replaces the per-tensor codes of src/core/quantization.c:8-192, which C-ML has no product for. */
+typedef struct cmlb200_dense8 {
+    int rows, cols, ld;         /* rows = out features; row stride ld bytes, a multiple of 128. Allocated with rows rounded up to 16, the padding zero. cols up to 131071 */
+    void* w;                    /* int8 codes, 16-byte aligned */
+    float* scale;               /* one per row */
+    const float* bias;          /* device, one per row, added to the product; NULL: none */
+    float cap;                  /* > 0: y = cap tanh(y / cap) */
+} cmlb200_dense8;
+/* Quantises rows of x (CMLB200_DT_F32, _BF16 or _F16, row stride ldx elements) into d_q [rows] of stride ldq, a multiple of 128, and d_scale [rows]. Codes behind
+ * the row's end are 0 up to the next multiple of 128. What a model's loader does with a weight, too. */
+int cmlb200_quantize_rows(const void* d_x, int dtype, long ldx, int rows, int cols, int8_t* d_q, long ldq, float* d_scale, void* stream);
+/* y[M, rows] = x[M, cols] . W^T, x quantised in the call: the sums are whole numbers in 32 bits, exact, then y = sum * (x's scale * W's scale) (+ bias, cap) in fp32. x: fp32, bf16 or fp16
+ * rows. _glu: a weight of `ff` gate and `ff` up rows interleaved in groups of 16 (padded with zero rows; bias and cap are not looked at), f = bf16 act(gate) * up with
+ * CMLB200_ACT_SILU, _GELU_TANH or _GELU_ERF. d_work: cmlb200_dense8_work_bytes(M, W->rows, W->cols) bytes, 16-byte aligned, that no other call uses meanwhile; what it holds
+ * before does not matter. Weights and scales are constants, as those of cmlb200_dense: a kernel that writes them is followed by a synchronisation or a copy. _status: not 0 once a
+ * bounded wait expired (valid when the stream has drained). */
+size_t cmlb200_dense8_work_bytes(int M, int rows, int cols);
+int cmlb200_linear_dense8(const cmlb200_dense8* W, const void* d_x, int dtype, long ldx, int M, float* d_y, long ldy, void* d_work, void* stream);
+int cmlb200_linear_dense8_glu(const cmlb200_dense8* W, const void* d_x, int dtype, long ldx, int M, int ff, int act, uint16_t* d_f, long ldf, void* d_work, void* stream);
+int cmlb200_dense8_status(int* status, int reset);
+
+/* ---- drafted tokens, and tokens drawn on the device -------------------------------------------------
+ * Sequence s brings drafts and the target's logits of rows first[s] .. first[s + 1] - 1: a row that each draft is tested against, and one behind the last. With p and q the softmax of the
+ * target's and the drafter's logits over the sequence's temperature (q is 1 at the draft where no drafter's logits are given), draft i is kept while u_i q(draft) < p(draft). The token
+ * behind the kept ones is drawn from p where all were kept, otherwise from what p has above q (from p where that is nothing): kept tokens and the drawn one together are distributed as
+ * tokens drawn from the target one by one. A sequence without drafts has a token drawn. The drawn token has the largest weight / E, E = -ln(1 - v) standard exponentials; ties go to the lower id.
+ * Random numbers come out of Philox4x32-10 with the sequence's 64-bit number as key: v of token j is word j mod 4 of counter (j / 4, 0, 0, 0), u_i word i mod 4 of counter
+ * (i / 4, 1, 0, 0); v = (word + 1/2) / 2^32, u = word / 2^32. A number is used for one call of one sequence. A temperature below 1e-5 is greedy: a draft is kept while it is the
+ * largest logit's token (the lowest such id), which is taken behind the kept ones.
+ * Logits of -inf are tokens that cannot come. A target's row that holds NaN or +inf, or nothing but -inf, ends the sequence: drafts from there on are not kept, and the token is -1. A
+ * drafter's row of that kind counts as none. A draft outside the vocabulary is not kept. Stands for the softmax loops on the host of src/nn/llama.c:662-737 and the
+ * test of drafts in src/nn/speculative.c. */
+typedef struct cmlb200_drafts {
+    int sequences, rows;        /* rows of the target's logits, all sequences together */
+    const int* first;           /* device, [sequences + 1], from 0 to rows: ascending by one more than a sequence's drafts */
+    const int* tokens;          /* device, [rows - sequences]: the drafts, sequence after sequence */
+    const void* logits;         /* device, [rows - sequences] rows that the drafts were drawn from, of the target's type, row stride ld; NULL: drafts were chosen for certain */
+    long ld;
+    const float* temperature;   /* device, [sequences]; NULL: 1 */
+    const uint64_t* random;     /* device, [sequences]; NULL where all temperatures are greedy */
+} cmlb200_drafts;
+/* d_accepted[s]: drafts kept, d_next[s]: the token behind them. d_work: cmlb200_verify_work_bytes(d->rows, d->sequences) bytes, 16-byte aligned, that no other call uses meanwhile. */
+size_t cmlb200_verify_work_bytes(int rows, int sequences);
+int cmlb200_verify_drafts(const cmlb200_drafts* d, const void* d_logits, int dtype, long ld, int vocab, int* d_accepted, int* d_next, void* d_work, void* stream);
+
 /* tokens[i] = picked[i], pos[i] += 1, hist[step * rows + i] = picked[i], step += 1 */
 int cmlb200_advance_tokens(const int* d_picked, int rows, int* d_tokens, int* d_pos, int* d_hist, int* d_step, void* stream);
 
