@@ -9,8 +9,21 @@
 
 #include "lm_util.cuh"
 
+// Where a product's results go, and what makes numbers of its sums
+struct Out8 {
+    const float *wscale, *bias, *xscale;
+    float cap;
+    int act, n_out;
+    void* y;
+    int ldy;
+};
+
+// the product of prompt-sized calls (gemm_dense8.cu)
+int cmlb_gemm_dense8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Out8& out, int glu, cudaStream_t st);
+
 namespace {
 
+constexpr int kSkinny8 = 32;                           // rows of x up to which the decode product is taken
 constexpr int kMaxCols8 = 131071;                      // 128 * 128 * this is the largest sum that 32 bits hold
 constexpr float kLeastMost = 127.f * 1.1754943508222875e-38f;
 

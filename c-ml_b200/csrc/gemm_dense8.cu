@@ -1,0 +1,348 @@
+// Prompt-sized products of int8 weights and int8 rows on the 5th-generation tensor cores: whole numbers in 32 bits in tensor memory, then
+// y = sum * (sx[m] sw[n]) (+ bias, cap), or bf16 act(gate) * up.
+//
+// Weight rows are the MMA's "M" side (operand A), rows of x its "N" side: a lane of tensor memory is a channel, a column a token. A channel's scale and bias are then a lane's own
+// registers, 32 lanes store 32 neighbouring outputs of a token with nothing transposed, a gate row and its up row are 16 lanes apart, and the number of tokens of a
+// tile is any multiple of 16 up to 256.
+//   warp 0      one lane issues TMA loads of both operands (128 columns a slab, 128-byte swizzle) into a ring of stages that runs on across tiles; weights of the first
+//               stages before the launch in front has ended
+//   warp 1      owns tensor memory; an elected lane issues tcgen05.mma kind::i8 (128 or 256 x NX x 32)
+//   warps 2-9   epilogue, two a quarter of tensor memory's lanes
+// Three forms (pick_shape):
+//   pairs       256 channels by up to 256 tokens, a pair of CTAs (cta_group::2): each has 128 channels and half of the tokens' codes. Persistent, two accumulators in turn.
+//   single      128 channels, persistent, the same.
+//   split       where tiles are fewer than SMs a cluster of 2 to 8 CTAs shares the columns of a tile. Their sums meet in distributed shared memory, and since they are whole numbers
+//               the order of adding makes no difference.
+// No load is multicast. Every wait on an mbarrier is bounded; on expiry the CTA raises a status word (cmlb200_dense8_status), waits for its copies and MMAs in flight, frees its tensor
+// memory and returns.
+#include "dense8.cuh"
+#include "tcgen05_util.cuh"
+
+namespace {
+
+constexpr int BK8 = 128, CH = 128;                     // columns of a slab, channels of a CTA
+constexpr int EPI = 8, THREADS8 = 64 + EPI * 32;
+constexpr int A8 = CH * BK8, MOST_STAGES = 8, ROOM8 = 220 * 1024;
+constexpr int BAR_OFF = 0;                             // barriers and words in front of the stages
+constexpr int HEAD8 = 1024;
+
+__device__ int g_dense8_status = 0;
+__device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, &g_dense8_status));
+}
+// for what is under way whoever has given up
+__device__ __forceinline__ void drain8(uint32_t bar, uint32_t parity) {
+    for (uint32_t it = 0; it < SPIN_LIMIT && !mbar_try(bar, parity); ++it)
+        if (it > 1024) __nanosleep(32);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+    if (PAIR)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                     ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                     ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit8(uint32_t bar) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        umma_commit(bar);
+}
+// Arrives at the same barrier of the pair's first CTA. What the arrival stands for lies in this SM's own memory, which its half of the MMA reads: no release for the cluster.
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(bar));
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
+}
+__device__ __forceinline__ void whole_cluster() { asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+struct Gemm8 {
+    Out8 out;
+    int M, N, slabs, NX, tiles_m, tiles, stages, glu;
+};
+
+// Tile number -> token tile, channel tile: groups of 8 token tiles share a sweep over the channels, so that the CTAs working at one time read few distinct slabs.
+__device__ __forceinline__ void tile8(int i, int tiles_m, int tiles, int& tm, int& tn) {
+    const int cols = tiles / tiles_m, per = 8 * cols, gq = i / per, in = i - gq * per, rows = min(8, tiles_m - gq * 8);
+    tm = gq * 8 + in % rows;
+    tn = in / rows;
+}
+
+__device__ __forceinline__ float finish8(int sum, float unit, float bias, float cap) {
+    float y = (float)sum * unit + bias;
+    if (cap > 0.f) y = soft_cap(y, cap);
+    return y;
+}
+
+template <bool PAIR>
+__global__ void __launch_bounds__(THREADS8, 1)
+gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Gemm8 p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t bars = smem_u32(smem), sbase = bars + HEAD8;
+    auto full = [&](int s) { return bars + 8 * s; };
+    auto empty = [&](int s) { return bars + 8 * (MOST_STAGES + s); };
+    auto acc_full = [&](int b) { return bars + 8 * (2 * MOST_STAGES + b); };
+    auto acc_empty = [&](int b) { return bars + 8 * (2 * MOST_STAGES + 2 + b); };
+    const uint32_t drained = bars + 8 * (2 * MOST_STAGES + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 8 * (2 * MOST_STAGES + 5));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank, ranks;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    const int second = PAIR ? (int)rank : 0, first_tile = blockIdx.x / ranks, step = gridDim.x / ranks;
+    if (PAIR) { rank = 0; ranks = 1; }
+    const int kb0 = (int)((long)p.slabs * rank / ranks), nkb = (int)((long)p.slabs * (rank + 1) / ranks) - kb0;
+    const int my_tiles = first_tile < p.tiles ? (p.tiles - first_tile + step - 1) / step : 0, total = my_tiles * nkb;
+    const int b_rows = PAIR ? p.NX / 2 : p.NX, stage = A8 + b_rows * BK8, S = p.stages;
+    const int acc = p.NX <= 32 ? 32 : p.NX <= 64 ? 64 : p.NX <= 128 ? 128 : 256;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) { mbar_init(full(s), PAIR && !second ? 2 : 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), PAIR ? 2 * EPI : EPI); }
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * acc)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)(2 * acc)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    dep_trigger();
+    tmem_fence_before();
+    __syncthreads();
+    if (PAIR) whole_cluster();                         // its barriers and columns, too
+    tmem_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto weights = [&](int it, int s) {
+                int tm, tn;
+                tile8(first_tile + it / nkb * step, p.tiles_m, p.tiles, tm, tn);
+                mbar_expect_tx(full(s), (uint32_t)stage);
+                tma_load_2d(sbase + s * stage, &wmap, (kb0 + it % nkb) * (BK8 / 2), (PAIR ? 2 * CH : CH) * tn + CH * second, full(s));
+            };
+            auto tokens = [&](int it, int s) {
+                int tm, tn;
+                tile8(first_tile + it / nkb * step, p.tiles_m, p.tiles, tm, tn);
+                tma_load_2d(sbase + s * stage + A8, &xmap, (kb0 + it % nkb) * (BK8 / 2), tm * p.NX + second * b_rows, full(s));
+            };
+            const int ahead = min(S, total);
+            for (int it = 0; it < ahead; it++) weights(it, it);
+            dep_wait();
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            for (int it = 0; it < ahead; it++) tokens(it, it);
+            int it = ahead, s = 0;
+            uint32_t phase = 0;
+            for (; it < total; it++) {
+                if (!mbar_wait(empty(s), phase, abort_flag, 1, &g_dense8_status)) break;
+                weights(it, s);
+                tokens(it, s);
+                if (++s == S) { s = 0; phase ^= 1; }
+            }
+            // no copy outlives its CTA (a pair's first CTA: its barriers also wait for the second one's arrivals, which come or are given up)
+            for (int i = max(0, it - S); i < it; i++) drain8(full(i % S), (i / S) & 1);
+        }
+    } else if (warp == 1) {
+        // kind::i8: D s32, A and B signed
+        const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.NX >> 3) << 17) | ((uint32_t)((PAIR ? 2 * CH : CH) >> 4) << 24);
+        int s = 0, done = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        if (PAIR && second) {                          // tells the first CTA what has come to this one
+            for (int it = 0; it < total && ok; it++) {
+                ok = wait8(full(s), phase, abort_flag, 2);
+                if (ok && lane == 0) arrive_first(full(s));
+                __syncwarp();
+                if (++s == S) { s = 0; phase ^= 1; }
+            }
+        } else {
+            for (; done < my_tiles && ok; done++) {
+                const int b = done & 1;
+                ok = wait8(acc_empty(b), ((done >> 1) & 1) ^ 1, abort_flag, 3);
+                if (!ok) break;
+                tmem_fence_after();
+                for (int k = 0; k < nkb; k++) {
+                    ok = wait8(full(s), phase, abort_flag, 4);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    const uint64_t ad = make_desc(sbase + s * stage), bd = make_desc(sbase + s * stage + A8);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < BK8 / 32; kk++)
+                            umma_i8<PAIR>(tmem_base + (uint32_t)(b * acc), ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, (k | kk) ? 1u : 0u);
+                        commit8<PAIR>(empty(s));
+                    }
+                    __syncwarp();
+                    if (++s == S) { s = 0; phase ^= 1; }
+                }
+                if (elect_one()) commit8<PAIR>(acc_full(b));
+                __syncwarp();
+            }
+            if (elect_one()) commit8<PAIR>(drained);   // tensor memory and the stages outlive the MMAs
+            __syncwarp();
+            drain8(drained, 0);
+        }
+    } else {
+        dep_wait();
+        const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane;
+        int* const own = reinterpret_cast<int*>(smem + HEAD8);               // [NX][128]: this CTA's sums, where the stages were
+        for (int done = 0; done < my_tiles; done++) {
+            const int b = done & 1;
+            int tm, tn;
+            tile8(first_tile + done * step, p.tiles_m, p.tiles, tm, tn);
+            const int n = tn * (PAIR ? 2 * CH : CH) + CH * second + ch, m0 = tm * p.NX, most = min(p.NX, p.M - m0);
+            const float sw = n < p.N ? p.out.wscale[n] : 0.f, bias = p.out.bias && n < p.N ? p.out.bias[n] : 0.f;
+            if (!wait8(acc_full(b), (done >> 1) & 1, abort_flag, 5)) break;
+            tmem_fence_after();
+            for (int c0 = half * 32; c0 < p.NX; c0 += 64) {
+                uint32_t v[32];
+                const float sx = c0 + lane < most && ranks == 1 ? p.out.xscale[m0 + c0 + lane] : 0.f;
+                tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * acc + c0), v);
+                if (ranks > 1) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) if (c0 + j < p.NX) own[(c0 + j) * CH + ch] = (int)v[j];
+                } else if (!p.glu) {
+                    float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c0) * p.out.ldy + n;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float unit = __shfl_sync(0xffffffffu, sx, j) * sw;
+                        if (c0 + j < most && n < p.N) y[(size_t)j * p.out.ldy] = finish8((int)v[j], unit, bias, p.out.cap);
+                    }
+                } else {
+                    // 16 gate lanes, 16 up lanes: of two tokens, the lower lanes finish the first and the upper ones the second
+                    const int col = (n >> 5) * 16 + (lane & 15), up = lane >> 4;
+                    __nv_bfloat16* f = static_cast<__nv_bfloat16*>(p.out.y) + (size_t)(m0 + c0 + up) * p.out.ldy + col;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float a = (float)(int)v[j] * (__shfl_sync(0xffffffffu, sx, j) * sw), c = (float)(int)v[j + 1] * (__shfl_sync(0xffffffffu, sx, j + 1) * sw);
+                        const float other = __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
+                        const float r = glu8(p.out.act, up ? other : a, up ? c : other);
+                        if (c0 + j + up < most && col < p.out.n_out) f[(size_t)j * p.out.ldy] = __float2bfloat16_rn(r);
+                    }
+                }
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) arrive_first(acc_empty(b));
+                else mbar_arrive(acc_empty(b));
+            }
+        }
+    }
+    if (ranks > 1) {                                   // one tile, its columns over the cluster: CTA r adds and finishes its share of the tokens
+        __syncwarp();
+        whole_cluster();
+        if (warp >= 2 && !*abort_flag) {
+            int tm, tn;
+            tile8(first_tile, p.tiles_m, p.tiles, tm, tn);
+            const int m0 = tm * p.NX, most = min(p.NX, p.M - m0), per = (most + (int)ranks - 1) / (int)ranks, c_lo = (int)rank * per, c_hi = min(most, c_lo + per);
+            const int quads = p.glu ? 16 : 32;         // four channels each (glu: gate channels, with those 16 on)
+            for (int i = (warp - 2) * 32 + lane; i < (c_hi - c_lo) * quads; i += EPI * 32) {
+                const int c = c_lo + i / quads, k = i % quads, r = p.glu ? (k >> 2) * 32 + (k & 3) * 4 : k * 4, n = tn * CH + r;
+                int a[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
+                for (int w = 0; w < (int)ranks; w++) {
+                    const uint32_t at = cluster_addr(smem + HEAD8 + ((size_t)c * CH + r) * 4, w);
+                    int x0, x1, x2, x3;
+                    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3) : "r"(at) : "memory");
+                    a[0] += x0; a[1] += x1; a[2] += x2; a[3] += x3;
+                    if (p.glu) {
+                        asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3) : "r"(at + 64) : "memory");
+                        u[0] += x0; u[1] += x1; u[2] += x2; u[3] += x3;
+                    }
+                }
+                const float sx = p.out.xscale[m0 + c];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (p.glu) {
+                        const int col = (n >> 5) * 16 + (n & 15) + e;
+                        if (col < p.out.n_out)
+                            static_cast<__nv_bfloat16*>(p.out.y)[(size_t)(m0 + c) * p.out.ldy + col] =
+                                __float2bfloat16_rn(glu8(p.out.act, (float)a[e] * (sx * p.out.wscale[n + e]), (float)u[e] * (sx * p.out.wscale[n + 16 + e])));
+                    } else if (n + e < p.N) {
+                        static_cast<float*>(p.out.y)[(size_t)(m0 + c) * p.out.ldy + n + e] = finish8(a[e], sx * p.out.wscale[n + e], p.out.bias ? p.out.bias[n + e] : 0.f, p.out.cap);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        whole_cluster();                               // nobody leaves while its sums are read
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (PAIR) whole_cluster();                         // nobody reads or arrives there any more
+    if (warp == 1) {
+        tmem_fence_after();
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * acc)) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)(2 * acc)) : "memory");
+    }
+}
+
+struct Shape8 { int NX, ranks; bool pair; };
+
+// Cycles that a form would take, by its waves: a slab takes its MMAs (2 NX) or its bytes (50 a cycle and SM), a tile about 2,500 to start and end, a cluster's sum 1,500 more.
+// How many clusters of 2, 4 and 8 run at once goes by how SMs lie in groups: 74, 33 and 15 on B200.
+Shape8 pick_shape(int M, int N, int slabs) {
+    const int tm = (M + 255) / 256, per = (M + tm - 1) / tm, sms = cmlb_num_sms();
+    const int nx = (per + 15) / 16 * 16, nx2 = (per + 31) / 32 * 32, tn = (N + CH - 1) / CH, tn2 = (N + 2 * CH - 1) / (2 * CH);
+    auto slab = [](int nx, int rows) { const double mma = 2.0 * nx, bytes = (A8 + rows * BK8) / 50.0; return mma > bytes ? mma : bytes; };
+    auto waves = [](long tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); };
+    Shape8 best = {nx, 1, false};
+    double least = waves((long)tm * tn, sms) * (slabs * slab(nx, nx) + 2500);
+    for (int ranks = 2; ranks <= 8 && ranks <= slabs; ranks *= 2) {
+        const int at_once = ranks == 2 ? sms / 2 : ranks == 4 ? sms * 33 / 148 : sms * 15 / 148;
+        const double cost = waves((long)tm * tn, at_once) * ((slabs + ranks - 1) / ranks * slab(nx, nx) + 4000);
+        if (cost < least) { least = cost; best.ranks = ranks; }
+    }
+    const double cost = waves((long)tm * tn2, sms / 2) * (slabs * slab(nx2, nx2 / 2) + 2500);
+    if (cost < least) best = {nx2, 1, true};
+    return best;
+}
+
+template <bool PAIR>
+int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Shape8& shape, const Out8& out, int glu, cudaStream_t st) {
+    const int slabs = (W->cols + BK8 - 1) / BK8, tm = (M + shape.NX - 1) / shape.NX, rows = PAIR ? 2 * CH : CH, tiles = tm * ((W->rows + rows - 1) / rows), box = PAIR ? shape.NX / 2 : shape.NX;
+    // (two codes an element of the maps)
+    CUtensorMap xmap, wmap;
+    int rc = encode_map(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, xq, M, slabs * BK8 / 2, ldq / 2, BK8 / 2, box);
+    if (!rc) rc = encode_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, W->w, W->rows, slabs * BK8 / 2, W->ld / 2, BK8 / 2, CH);
+    if (rc) return rc;
+    const int stage = A8 + box * BK8, sums = shape.ranks > 1 ? shape.NX * CH * 4 : 0;
+    int stages = ROOM8 / stage < MOST_STAGES ? ROOM8 / stage : MOST_STAGES;
+    const Gemm8 p = {out, M, W->rows, slabs, shape.NX, tm, tiles, stages, glu};
+    const size_t smem = 1024 + HEAD8 + (size_t)(stages * stage > sums ? stages * stage : sums);
+    static size_t attr[kMaxDevices] = {};
+    CMLB_CUDA(cmlb_ensure_smem(gemm_dense8_kernel<PAIR>, 1024 + HEAD8 + ROOM8, attr));
+    const int cluster = PAIR ? 2 : shape.ranks, at_once = cmlb_num_sms() / (PAIR ? 2 : 1);
+    const int groups = shape.ranks > 1 || tiles < at_once ? tiles : at_once;
+    CMLB_CUDA(launch_chain(gemm_dense8_kernel<PAIR>, dim3((unsigned)(groups * cluster)), dim3(THREADS8), smem, cluster, st, xmap, wmap, p));
+    return CMLB200_OK;
+}
+
+}  // namespace
+
+int cmlb_gemm_dense8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Out8& out, int glu, cudaStream_t st) {
+    const Shape8 shape = pick_shape(M, W->rows, (W->cols + BK8 - 1) / BK8);
+    return shape.pair ? launch_gemm8<true>(W, xq, ldq, M, shape, out, glu, st) : launch_gemm8<false>(W, xq, ldq, M, shape, out, glu, st);
+}
+
+extern "C" int cmlb200_dense8_status(int* status, int reset) {
+    CMLB_REQUIRE(status, "cmlb200_dense8_status: NULL argument");
+    CMLB_CUDA(cudaDeviceSynchronize());
+    CMLB_CUDA(cudaMemcpyFromSymbol(status, g_dense8_status, sizeof(int)));
+    if (reset) {
+        const int zero = 0;
+        CMLB_CUDA(cudaMemcpyToSymbol(g_dense8_status, &zero, sizeof(int)));
+    }
+    return CMLB200_OK;
+}

@@ -17,14 +17,6 @@ __device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-struct Out8 {
-    const float *wscale, *bias, *xscale;
-    float cap;
-    int act, n_out;
-    void* y;
-    int ldy;
-};
-
 // RT tiles of 16 weight rows per CTA, NB groups of 8 rows of x; blockIdx.y: passes of NB * 8 rows. GLU: tile 0 = 16 gate rows, tile 1 = the 16 up rows that go with them.
 template <int RT, int NB, bool GLU>
 __global__ void __launch_bounds__(GW * 32)
@@ -154,7 +146,7 @@ extern "C" int cmlb200_linear_dense8(const cmlb200_dense8* W, const void* d_x, i
     rc = cmlb200_quantize_rows(d_x, dtype, ldx, M, W->cols, xq, ldq, xs, stream);
     if (rc) return rc;
     const Out8 out = {W->scale, W->bias, xs, W->cap, 0, W->rows, d_y, (int)ldy};
-    return launch_gemv8<1, false>(W, xq, ldq, M, out, as_stream(stream));
+    return M <= kSkinny8 ? launch_gemv8<1, false>(W, xq, ldq, M, out, as_stream(stream)) : cmlb_gemm_dense8(W, xq, ldq, M, out, 0, as_stream(stream));
 }
 
 extern "C" int cmlb200_linear_dense8_glu(const cmlb200_dense8* W, const void* d_x, int dtype, long ldx, int M, int ff, int act, uint16_t* d_f, long ldf, void* d_work, void* stream) {
@@ -169,12 +161,5 @@ extern "C" int cmlb200_linear_dense8_glu(const cmlb200_dense8* W, const void* d_
     rc = cmlb200_quantize_rows(d_x, dtype, ldx, M, W->cols, xq, ldq, xs, stream);
     if (rc) return rc;
     const Out8 out = {W->scale, nullptr, xs, 0.f, act, ff, d_f, (int)ldf};
-    return launch_gemv8<2, true>(W, xq, ldq, M, out, as_stream(stream));
-}
-
-extern "C" int cmlb200_dense8_status(int* status, int reset) {
-    (void)reset;
-    CMLB_REQUIRE(status, "cmlb200_dense8_status: NULL argument");
-    *status = 0;
-    return CMLB200_OK;
+    return M <= kSkinny8 ? launch_gemv8<2, true>(W, xq, ldq, M, out, as_stream(stream)) : cmlb_gemm_dense8(W, xq, ldq, M, out, 1, as_stream(stream));
 }
