@@ -4,8 +4,8 @@
 // Weight rows are the MMA's "M" side (operand A), rows of x its "N" side: a lane of tensor memory is a channel, a column a token. A channel's scale and bias are then a lane's own
 // registers, 32 lanes store 32 neighbouring outputs of a token with nothing transposed, a gate row and its up row are 16 lanes apart, and the number of tokens of a
 // tile is any multiple of 16 up to 256.
-//   warp 0      one lane issues TMA loads of both operands (128 columns a slab, 128-byte swizzle) into a ring of stages that runs on across tiles; weights of the first
-//               stages before the launch in front has ended
+//   warp 0      one lane issues TMA loads of both operands (256 columns a stage, as two blocks of 128 with 128-byte swizzle that one load brings) into a ring of stages that runs
+//               on across tiles; weights of the first stages before the launch in front has ended
 //   warp 1      owns tensor memory; an elected lane issues tcgen05.mma kind::i8 (128 or 256 x NX x 32)
 //   warps 2-9   epilogue, two a quarter of tensor memory's lanes
 // Three forms (pick_shape):
@@ -15,16 +15,17 @@
 //               the order of adding makes no difference.
 // No load is multicast. Every wait on an mbarrier is bounded; on expiry the CTA raises a status word (cmlb200_dense8_status), waits for its copies and MMAs in flight, frees its tensor
 // memory and returns.
+#include <math.h>
+
 #include "dense8.cuh"
 #include "tcgen05_util.cuh"
 
 namespace {
 
-constexpr int BK8 = 128, CH = 128;                     // columns of a slab, channels of a CTA
+constexpr int BK8 = 128, BLOCKS = 2, CH = 128;         // columns of a block, blocks of a stage, channels of a CTA
 constexpr int EPI = 8, THREADS8 = 64 + EPI * 32;
 constexpr int A8 = CH * BK8, MOST_STAGES = 8, ROOM8 = 220 * 1024;
-constexpr int BAR_OFF = 0;                             // barriers and words in front of the stages
-constexpr int HEAD8 = 1024;
+constexpr int HEAD8 = 1024;                            // barriers and words in front of the stages
 
 __device__ int g_dense8_status = 0;
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
@@ -51,6 +52,11 @@ __device__ __forceinline__ void commit8(uint32_t bar) {
     else
         umma_commit(bar);
 }
+// `BLOCKS` blocks of 128 columns of a box of rows
+__device__ __forceinline__ void load_blocks(uint32_t dst, const CUtensorMap* map, int row, int block, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(block), "r"(bar) : "memory");
+}
 // Arrives at the same barrier of the pair's first CTA. What the arrival stands for lies in this SM's own memory, which its half of the MMA reads: no release for the cluster.
 __device__ __forceinline__ void arrive_first(uint32_t bar) {
     uint32_t at;
@@ -61,7 +67,7 @@ __device__ __forceinline__ void whole_cluster() { asm volatile("barrier.cluster.
 
 struct Gemm8 {
     Out8 out;
-    int M, N, slabs, NX, tiles_m, tiles, stages, glu;
+    int M, N, loads, NX, tiles_m, tiles, stages, glu;
 };
 
 // Tile number -> token tile, channel tile: groups of 8 token tiles share a sweep over the channels, so that the CTAs working at one time read few distinct slabs.
@@ -71,10 +77,10 @@ __device__ __forceinline__ void tile8(int i, int tiles_m, int tiles, int& tm, in
     tn = in / rows;
 }
 
+__device__ __noinline__ float far_cap(float y, float cap) { return soft_cap(y, cap); }
 __device__ __forceinline__ float finish8(int sum, float unit, float bias, float cap) {
-    float y = (float)sum * unit + bias;
-    if (cap > 0.f) y = soft_cap(y, cap);
-    return y;
+    const float y = fmaf((float)sum, unit, bias);
+    return cap > 0.f ? far_cap(y, cap) : y;
 }
 
 template <bool PAIR>
@@ -96,17 +102,45 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     const int second = PAIR ? (int)rank : 0, first_tile = blockIdx.x / ranks, step = gridDim.x / ranks;
     if (PAIR) { rank = 0; ranks = 1; }
-    const int kb0 = (int)((long)p.slabs * rank / ranks), nkb = (int)((long)p.slabs * (rank + 1) / ranks) - kb0;
+    const int kb0 = (int)((long)p.loads * rank / ranks), nkb = (int)((long)p.loads * (rank + 1) / ranks) - kb0;
     const int my_tiles = first_tile < p.tiles ? (p.tiles - first_tile + step - 1) / step : 0, total = my_tiles * nkb;
-    const int b_rows = PAIR ? p.NX / 2 : p.NX, stage = A8 + b_rows * BK8, S = p.stages;
+    const int b_rows = PAIR ? p.NX / 2 : p.NX, blocks_a = BLOCKS * A8, stage = blocks_a + BLOCKS * b_rows * BK8, S = p.stages;
     const int acc = p.NX <= 32 ? 32 : p.NX <= 64 ? 64 : p.NX <= 128 ? 128 : 256;
 
+    // places of the next stages to load, counted: with divisions the one thread took 900 cycles a stage
+    struct Place { int tile, k, row; } w = {first_tile, 0, 0}, x = {first_tile, 0, 0};
+    auto tile_row = [&](int tile, bool of_tokens) {
+        int tm, tn;
+        tile8(tile, p.tiles_m, p.tiles, tm, tn);
+        return of_tokens ? tm * p.NX + second * b_rows : (PAIR ? 2 * CH : CH) * tn + CH * second;
+    };
+    auto next = [&](Place& at, bool of_tokens) {
+        if (++at.k == nkb) {
+            at.k = 0;
+            at.tile += step;
+            if (at.tile < p.tiles) at.row = tile_row(at.tile, of_tokens);
+        }
+    };
+    auto weights = [&](uint32_t to, uint32_t bar) {
+        mbar_expect_tx(bar, (uint32_t)stage);
+        load_blocks(to, &wmap, w.row, (kb0 + w.k) * BLOCKS, bar);
+        next(w, false);
+    };
+    auto tokens = [&](uint32_t to, uint32_t bar) {
+        load_blocks(to + blocks_a, &xmap, x.row, (kb0 + x.k) * BLOCKS, bar);
+        next(x, true);
+    };
+    const int ahead = min(S, total);
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) { mbar_init(full(s), PAIR && !second ? 2 : 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < 2; b++) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), PAIR ? 2 * EPI : EPI); }
         mbar_init(drained, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        w.row = tile_row(first_tile, false);
+        x.row = tile_row(first_tile, true);
+        for (int it = 0; it < ahead; it++) weights(sbase + it * stage, full(it));
     }
     if (warp == 1) {
         if (PAIR) {
@@ -126,29 +160,17 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
 
     if (warp == 0) {
         if (lane == 0) {
-            auto weights = [&](int it, int s) {
-                int tm, tn;
-                tile8(first_tile + it / nkb * step, p.tiles_m, p.tiles, tm, tn);
-                mbar_expect_tx(full(s), (uint32_t)stage);
-                tma_load_2d(sbase + s * stage, &wmap, (kb0 + it % nkb) * (BK8 / 2), (PAIR ? 2 * CH : CH) * tn + CH * second, full(s));
-            };
-            auto tokens = [&](int it, int s) {
-                int tm, tn;
-                tile8(first_tile + it / nkb * step, p.tiles_m, p.tiles, tm, tn);
-                tma_load_2d(sbase + s * stage + A8, &xmap, (kb0 + it % nkb) * (BK8 / 2), tm * p.NX + second * b_rows, full(s));
-            };
-            const int ahead = min(S, total);
-            for (int it = 0; it < ahead; it++) weights(it, it);
             dep_wait();
             asm volatile("fence.proxy.async.global;" ::: "memory");
-            for (int it = 0; it < ahead; it++) tokens(it, it);
+            for (int it = 0; it < ahead; it++) tokens(sbase + it * stage, full(it));
             int it = ahead, s = 0;
-            uint32_t phase = 0;
+            uint32_t phase = 0, to = sbase;
             for (; it < total; it++) {
                 if (!mbar_wait(empty(s), phase, abort_flag, 1, &g_dense8_status)) break;
-                weights(it, s);
-                tokens(it, s);
-                if (++s == S) { s = 0; phase ^= 1; }
+                weights(to, full(s));
+                tokens(to, full(s));
+                to += stage;
+                if (++s == S) { s = 0; phase ^= 1; to = sbase; }
             }
             // no copy outlives its CTA (a pair's first CTA: its barriers also wait for the second one's arrivals, which come or are given up)
             for (int i = max(0, it - S); i < it; i++) drain8(full(i % S), (i / S) & 1);
@@ -156,6 +178,8 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
     } else if (warp == 1) {
         // kind::i8: D s32, A and B signed
         const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.NX >> 3) << 17) | ((uint32_t)((PAIR ? 2 * CH : CH) >> 4) << 24);
+        const uint64_t desc0 = make_desc(sbase);
+        const uint32_t b_block = (uint32_t)(b_rows * BK8) >> 4;
         int s = 0, done = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -176,11 +200,12 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
                     ok = wait8(full(s), phase, abort_flag, 4);
                     if (!ok) break;
                     tmem_fence_after();
-                    const uint64_t ad = make_desc(sbase + s * stage), bd = make_desc(sbase + s * stage + A8);
+                    const uint64_t ad = desc0 + (uint64_t)(uint32_t)(s * (stage >> 4)), bd = ad + (uint64_t)(blocks_a >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < BK8 / 32; kk++)
-                            umma_i8<PAIR>(tmem_base + (uint32_t)(b * acc), ad + (uint64_t)(2 * kk), bd + (uint64_t)(2 * kk), idesc, (k | kk) ? 1u : 0u);
+                        for (int kk = 0; kk < BLOCKS * BK8 / 32; kk++)
+                            umma_i8<PAIR>(tmem_base + (uint32_t)(b * acc), ad + (uint64_t)((kk >> 2) * (A8 >> 4) + 2 * (kk & 3)), bd + (uint64_t)((kk >> 2) * b_block + 2 * (kk & 3)), idesc,
+                                          (k | kk) ? 1u : 0u);
                         commit8<PAIR>(empty(s));
                     }
                     __syncwarp();
@@ -207,28 +232,46 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
             tmem_fence_after();
             for (int c0 = half * 32; c0 < p.NX; c0 += 64) {
                 uint32_t v[32];
-                const float sx = c0 + lane < most && ranks == 1 ? p.out.xscale[m0 + c0 + lane] : 0.f;
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * acc + c0), v);
                 if (ranks > 1) {
 #pragma unroll
                     for (int j = 0; j < 32; j++) if (c0 + j < p.NX) own[(c0 + j) * CH + ch] = (int)v[j];
-                } else if (!p.glu) {
+                    continue;
+                }
+                // (scales of tokens behind the last are read, and lie in the workspace, but are not used)
+                const float4* sx = reinterpret_cast<const float4*>(p.out.xscale + m0 + c0);
+                const int left = most - c0;
+                if (!p.glu) {
                     float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c0) * p.out.ldy + n;
+                    const bool mine = n < p.N;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float unit = __shfl_sync(0xffffffffu, sx, j) * sw;
-                        if (c0 + j < most && n < p.N) y[(size_t)j * p.out.ldy] = finish8((int)v[j], unit, bias, p.out.cap);
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s4 = sx[j / 4];
+                        const float su[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float r = finish8((int)v[j + e], su[e] * sw, bias, p.out.cap);
+                            if (mine && j + e < left) *y = r;
+                            y += p.out.ldy;
+                        }
                     }
                 } else {
                     // 16 gate lanes, 16 up lanes: of two tokens, the lower lanes finish the first and the upper ones the second
                     const int col = (n >> 5) * 16 + (lane & 15), up = lane >> 4;
                     __nv_bfloat16* f = static_cast<__nv_bfloat16*>(p.out.y) + (size_t)(m0 + c0 + up) * p.out.ldy + col;
+                    const bool mine = col < p.out.n_out;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float a = (float)(int)v[j] * (__shfl_sync(0xffffffffu, sx, j) * sw), c = (float)(int)v[j + 1] * (__shfl_sync(0xffffffffu, sx, j + 1) * sw);
-                        const float other = __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
-                        const float r = glu8(p.out.act, up ? other : a, up ? c : other);
-                        if (c0 + j + up < most && col < p.out.n_out) f[(size_t)j * p.out.ldy] = __float2bfloat16_rn(r);
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s4 = sx[j / 4];
+                        const float su[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const float a = (float)(int)v[j + e] * (su[e] * sw), c = (float)(int)v[j + e + 1] * (su[e + 1] * sw);
+                            const float other = __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
+                            const float r = glu8(p.out.act, up ? other : a, up ? c : other);
+                            if (mine && j + e + up < left) *f = __float2bfloat16_rn(r);
+                            f += 2 * p.out.ldy;
+                        }
                     }
                 }
             }
@@ -248,35 +291,43 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
             tile8(first_tile, p.tiles_m, p.tiles, tm, tn);
             const int m0 = tm * p.NX, most = min(p.NX, p.M - m0), per = (most + (int)ranks - 1) / (int)ranks, c_lo = (int)rank * per, c_hi = min(most, c_lo + per);
             const int quads = p.glu ? 16 : 32;         // four channels each (glu: gate channels, with those 16 on)
-            for (int i = (warp - 2) * 32 + lane; i < (c_hi - c_lo) * quads; i += EPI * 32) {
-                const int c = c_lo + i / quads, k = i % quads, r = p.glu ? (k >> 2) * 32 + (k & 3) * 4 : k * 4, n = tn * CH + r;
-                int a[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-                for (int w = 0; w < (int)ranks; w++) {
-                    const uint32_t at = cluster_addr(smem + HEAD8 + ((size_t)c * CH + r) * 4, w);
-                    int x0, x1, x2, x3;
-                    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3) : "r"(at) : "memory");
-                    a[0] += x0; a[1] += x1; a[2] += x2; a[3] += x3;
-                    if (p.glu) {
-                        asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(x0), "=r"(x1), "=r"(x2), "=r"(x3) : "r"(at + 64) : "memory");
-                        u[0] += x0; u[1] += x1; u[2] += x2; u[3] += x3;
-                    }
-                }
-                const float sx = p.out.xscale[m0 + c];
+            auto add = [&](auto most_ranks) {
+                constexpr int R = decltype(most_ranks)::value;
+                for (int i = (warp - 2) * 32 + lane; i < (c_hi - c_lo) * quads; i += EPI * 32) {
+                    const int c = c_lo + i / quads, k = i % quads, r = p.glu ? (k >> 2) * 32 + (k & 3) * 4 : k * 4, n = tn * CH + r;
+                    int4 a[R], u[R];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
+                    for (int w = 0; w < R; w++) {
+                        const uint32_t at = cluster_addr(smem + HEAD8 + ((size_t)c * CH + r) * 4, w);
+                        asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(a[w].x), "=r"(a[w].y), "=r"(a[w].z), "=r"(a[w].w) : "r"(at) : "memory");
+                        if (p.glu) asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(u[w].x), "=r"(u[w].y), "=r"(u[w].z), "=r"(u[w].w) : "r"(at + 64) : "memory");
+                    }
+                    const float sx = p.out.xscale[m0 + c];
+                    int sa[4] = {0, 0, 0, 0}, su[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int w = 0; w < R; w++) { sa[0] += a[w].x; sa[1] += a[w].y; sa[2] += a[w].z; sa[3] += a[w].w; }
                     if (p.glu) {
-                        const int col = (n >> 5) * 16 + (n & 15) + e;
-                        if (col < p.out.n_out)
-                            static_cast<__nv_bfloat16*>(p.out.y)[(size_t)(m0 + c) * p.out.ldy + col] =
-                                __float2bfloat16_rn(glu8(p.out.act, (float)a[e] * (sx * p.out.wscale[n + e]), (float)u[e] * (sx * p.out.wscale[n + 16 + e])));
-                    } else if (n + e < p.N) {
-                        static_cast<float*>(p.out.y)[(size_t)(m0 + c) * p.out.ldy + n + e] = finish8(a[e], sx * p.out.wscale[n + e], p.out.bias ? p.out.bias[n + e] : 0.f, p.out.cap);
+#pragma unroll
+                        for (int w = 0; w < R; w++) { su[0] += u[w].x; su[1] += u[w].y; su[2] += u[w].z; su[3] += u[w].w; }
+                        const int col = (n >> 5) * 16 + (n & 15);
+                        __nv_bfloat16* f = static_cast<__nv_bfloat16*>(p.out.y) + (size_t)(m0 + c) * p.out.ldy + col;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (col + e < p.out.n_out) f[e] = __float2bfloat16_rn(glu8(p.out.act, (float)sa[e] * (sx * p.out.wscale[n + e]), (float)su[e] * (sx * p.out.wscale[n + 16 + e])));
+                    } else {
+                        float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c) * p.out.ldy + n;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (n + e < p.N) y[e] = finish8(sa[e], sx * p.out.wscale[n + e], p.out.bias ? p.out.bias[n + e] : 0.f, p.out.cap);
                     }
                 }
-            }
+            };
+            if (ranks == 2) add(std::integral_constant<int, 2>());
+            else if (ranks == 4) add(std::integral_constant<int, 4>());
+            else add(std::integral_constant<int, 8>());
         }
         __syncwarp();
-        whole_cluster();                               // nobody leaves while its sums are read
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");      // nobody leaves while its sums are read (and all of them have been used)
     }
     tmem_fence_before();
     __syncthreads();
@@ -290,36 +341,48 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
 
 struct Shape8 { int NX, ranks; bool pair; };
 
-// Cycles that a form would take, by its waves: a slab takes its MMAs (2 NX) or its bytes (50 a cycle and SM), a tile about 2,500 to start and end, a cluster's sum 1,500 more.
+int encode_blocks(CUtensorMap* map, const void* base, long rows, int blocks, int ld, int box_rows) {
+    EncodeTiledFn fn;
+    const int rc = get_encoder(&fn);
+    if (rc) return rc;
+    const cuuint64_t dims[3] = {BK8 / 2, (cuuint64_t)rows, (cuuint64_t)blocks}, strides[2] = {(cuuint64_t)ld, BK8};       // two codes an element
+    const cuuint32_t box[3] = {BK8 / 2, (cuuint32_t)box_rows, BLOCKS}, one[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CMLB_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with %d for [%ld, %d], stride %d", (int)r, rows, blocks * BK8, ld);
+    return CMLB200_OK;
+}
+
+// Cycles that a form would take, by its waves: a stage takes its MMAs (4 NX) or its bytes (50 a cycle and SM) or its issue (600), a tile about 3,000 to start and end, a cluster's sum
+// 2,000 more.
 // How many clusters of 2, 4 and 8 run at once goes by how SMs lie in groups: 74, 33 and 15 on B200.
-Shape8 pick_shape(int M, int N, int slabs) {
+Shape8 pick_shape(int M, int N, int loads) {
     const int tm = (M + 255) / 256, per = (M + tm - 1) / tm, sms = cmlb_num_sms();
     const int nx = (per + 15) / 16 * 16, nx2 = (per + 31) / 32 * 32, tn = (N + CH - 1) / CH, tn2 = (N + 2 * CH - 1) / (2 * CH);
-    auto slab = [](int nx, int rows) { const double mma = 2.0 * nx, bytes = (A8 + rows * BK8) / 50.0; return mma > bytes ? mma : bytes; };
+    auto stage = [](int nx, int rows) { return fmax(fmax(4.0 * nx, BLOCKS * (A8 + rows * BK8) / 50.0), 600.0); };
     auto waves = [](long tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); };
     Shape8 best = {nx, 1, false};
-    double least = waves((long)tm * tn, sms) * (slabs * slab(nx, nx) + 2500);
-    for (int ranks = 2; ranks <= 8 && ranks <= slabs; ranks *= 2) {
+    double least = waves((long)tm * tn, sms) * (loads * stage(nx, nx) + 3000);
+    for (int ranks = 2; ranks <= 8 && ranks <= loads; ranks *= 2) {
         const int at_once = ranks == 2 ? sms / 2 : ranks == 4 ? sms * 33 / 148 : sms * 15 / 148;
-        const double cost = waves((long)tm * tn, at_once) * ((slabs + ranks - 1) / ranks * slab(nx, nx) + 4000);
+        const double cost = waves((long)tm * tn, at_once) * ((loads + ranks - 1) / ranks * stage(nx, nx) + 5000);
         if (cost < least) { least = cost; best.ranks = ranks; }
     }
-    const double cost = waves((long)tm * tn2, sms / 2) * (slabs * slab(nx2, nx2 / 2) + 2500);
+    const double cost = waves((long)tm * tn2, sms / 2) * (loads * stage(nx2, nx2 / 2) + 3000);
     if (cost < least) best = {nx2, 1, true};
     return best;
 }
 
 template <bool PAIR>
 int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Shape8& shape, const Out8& out, int glu, cudaStream_t st) {
-    const int slabs = (W->cols + BK8 - 1) / BK8, tm = (M + shape.NX - 1) / shape.NX, rows = PAIR ? 2 * CH : CH, tiles = tm * ((W->rows + rows - 1) / rows), box = PAIR ? shape.NX / 2 : shape.NX;
-    // (two codes an element of the maps)
+    const int blocks = (W->cols + BK8 - 1) / BK8, tm = (M + shape.NX - 1) / shape.NX, rows = PAIR ? 2 * CH : CH, tiles = tm * ((W->rows + rows - 1) / rows), box = PAIR ? shape.NX / 2 : shape.NX;
     CUtensorMap xmap, wmap;
-    int rc = encode_map(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, xq, M, slabs * BK8 / 2, ldq / 2, BK8 / 2, box);
-    if (!rc) rc = encode_map(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT16, W->w, W->rows, slabs * BK8 / 2, W->ld / 2, BK8 / 2, CH);
+    int rc = encode_blocks(&xmap, xq, M, blocks, ldq, box);
+    if (!rc) rc = encode_blocks(&wmap, W->w, W->rows, blocks, W->ld, CH);
     if (rc) return rc;
-    const int stage = A8 + box * BK8, sums = shape.ranks > 1 ? shape.NX * CH * 4 : 0;
-    int stages = ROOM8 / stage < MOST_STAGES ? ROOM8 / stage : MOST_STAGES;
-    const Gemm8 p = {out, M, W->rows, slabs, shape.NX, tm, tiles, stages, glu};
+    const int stage = BLOCKS * (A8 + box * BK8), sums = shape.ranks > 1 ? shape.NX * CH * 4 : 0;
+    const int stages = ROOM8 / stage < MOST_STAGES ? ROOM8 / stage : MOST_STAGES;
+    const Gemm8 p = {out, M, W->rows, (blocks + BLOCKS - 1) / BLOCKS, shape.NX, tm, tiles, stages, glu};
     const size_t smem = 1024 + HEAD8 + (size_t)(stages * stage > sums ? stages * stage : sums);
     static size_t attr[kMaxDevices] = {};
     CMLB_CUDA(cmlb_ensure_smem(gemm_dense8_kernel<PAIR>, 1024 + HEAD8 + ROOM8, attr));
@@ -332,7 +395,7 @@ int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, cons
 }  // namespace
 
 int cmlb_gemm_dense8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Out8& out, int glu, cudaStream_t st) {
-    const Shape8 shape = pick_shape(M, W->rows, (W->cols + BK8 - 1) / BK8);
+    const Shape8 shape = pick_shape(M, W->rows, (W->cols + BLOCKS * BK8 - 1) / (BLOCKS * BK8));
     return shape.pair ? launch_gemm8<true>(W, xq, ldq, M, shape, out, glu, st) : launch_gemm8<false>(W, xq, ldq, M, shape, out, glu, st);
 }
 
