@@ -2,12 +2,14 @@
 //
 //   a = max(max |x|, 127 2^-126),   scale = a / 127,   code = 127 x / a rounded to the nearest, ties to even
 //
-// The quotient of a 16-bit number times 127 and a 16-bit number is right to the bit when it is rounded once, ties included, so codes of such rows are those
-// of exact arithmetic. It is a product with 127 / a except next to a tie (closer than that product can be off), where it is a division.
+// The quotient is a product with 127 / a, except next to a tie (closer than that product can be off), where the sign of 127 x - (k + 1/2) a decides. 127 times a number of 16 bits is exact, so
+// codes of such rows are those of exact arithmetic, ties included. Where a's odd part is not a multiple of 127, which is prime, such numbers have no ties but 127 x / a = 63.5, half the
+// largest, and come no closer to one than 2^-20 of themselves: 127 / a a little (2^-22) larger gives every code, and nothing has to be looked at.
 #pragma once
 #include <type_traits>
 
 #include "lm_util.cuh"
+#include "pairs.cuh"
 
 // Where a product's results go, and what makes numbers of its sums
 struct Out8 {
@@ -30,48 +32,87 @@ constexpr float kLeastMost = 127.f * 1.1754943508222875e-38f;
 template <typename T> struct Piece16 { uint4 v[sizeof(T)]; };                // 16 values as they lie (16 bytes hold 16 / sizeof(T) of them)
 
 // value i of a piece of 16-bit or 32-bit floats
-template <typename T> __device__ __forceinline__ void widen16(const Piece16<T>& p, float (&x)[16]) {
+template <typename T> __device__ __forceinline__ float value16(const Piece16<T>& p, int i) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(p.v);
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
-        else if constexpr (std::is_same_v<T, __nv_bfloat16>) x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
-        else x[i] = __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
-    }
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu)));
 }
-// magnitude as a whole number: in the order of the magnitudes, infinities above every number and NaN above those
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t most_of(const float (&x)[16]) {
-    uint32_t m = 0u;
+// The largest magnitude of a piece as a whole number: in the order of the magnitudes, infinities above every number and NaN above those. 16-bit values two at a time
+template <typename T> __device__ __forceinline__ uint32_t most_of(const Piece16<T>& p) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p.v);
+    if constexpr (sizeof(T) == 4) {
+        uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < 16; i++) m = max(m, magnitude(x[i]));
-    return m;
+        for (int i = 0; i < 16; i++) m = max(m, w[i] & 0x7fffffffu);
+        return m;
+    } else {
+        typedef std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162> T2;
+        T2 m, t;
+        memcpy(&m, &w[0], 4);
+        m = __habs2(m);
+#pragma unroll
+        for (int i = 1; i < 8; i++) {
+            memcpy(&t, &w[i], 4);
+            m = __hmax2_nan(m, __habs2(t));
+        }
+        return max(__float_as_uint(widen(m.x)) & 0x7fffffffu, __float_as_uint(widen(m.y)) & 0x7fffffffu);
+    }
 }
 
-struct RowScale {
-    float most, times;                                 // a, 127 / a
+constexpr float kMagic = 12582912.f;                   // a number added to it is rounded to a whole one, in its low bits
+constexpr float kNear = 2.3841858e-7f;                 // 2^-22: four times what 127 / a is off by
+// Next to a tie h: 127 x - h a has the right sign, and is 0 for a tie alone, since it is rounded once
+__device__ __forceinline__ uint32_t settle(float x, float times, float most, float unit) {
+    const float r = __fmul_rn(x, times), k = __fadd_rn(r, kMagic) - kMagic;
+    float whole = k;
+    if (fabsf(r - k) > 0.4375f) {
+        const float h = k + copysignf(0.5f, r - k), d = fmaf(-h, most, __fmul_rn(127.f, x * unit));
+        whole = d == 0.f ? h : h + copysignf(0.5f, d);
+    }
+    return __float_as_uint(whole + kMagic) & 0xffu;
+}
+// not inlined: the kernels' code stays small, which matters where it is fetched anew with every launch
+__device__ __noinline__ uint32_t settled_codes(float4 x, float times, float most, float unit) {
+    return settle(x.x, times, most, unit) | settle(x.y, times, most, unit) << 8 | settle(x.z, times, most, unit) << 16 | settle(x.w, times, most, unit) << 24;
+}
+
+template <typename T> struct RowScale {
+    float most, times, unit;                           // a, what numbers are multiplied with, a power of two that keeps 127 x and a within range
+    bool bad, sure;                                    // a row that holds NaN or an infinity has codes of 0 and scale NaN: whatever is made of it is NaN; a product decides every code
     __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+        bad = bits >= 0x7f800000u;
         most = fmaxf(__uint_as_float(bits), kLeastMost);
-        times = bits >= 0x7f800000u ? 0.f : __fdiv_rn(127.f, most);
-    }
-    // a row that holds NaN or an infinity has codes of 0 and scale NaN: whatever is made of it is NaN
-    __device__ __forceinline__ bool bad(uint32_t bits) const { return bits >= 0x7f800000u; }
-    __device__ __forceinline__ float scale(uint32_t bits) const { return bad(bits) ? __uint_as_float(0x7fffffffu) : __fdiv_rn(most, 127.f); }
-    // the code in the low byte
-    __device__ __forceinline__ uint32_t code(float x) const {
-        const float magic = 12582912.f, r = __fmul_rn(x, times), y = __fadd_rn(r, magic);
-        if (fabsf(r - (y - magic)) > 0.5f - 6.1e-5f) {
-            const float f = most > 1.2676506e30f ? 2.3283064e-10f : 1.f;       // (127 x stays a number)
-            return __float_as_uint(__fadd_rn(__fdiv_rn(__fmul_rn(127.f, x * f), most * f), magic));
+        times = __fdiv_rn(127.f, most);
+        unit = most > 1.2676506e30f ? 2.3283064e-10f : most < 8.6736174e-19f ? 1.8446744e19f : 1.f;
+        sure = false;
+        if (sizeof(T) == 2) {
+            const uint32_t m = (__float_as_uint(most) & 0x7fffffu) | 0x800000u, odd = m >> (__ffs(m) - 1);
+            sure = odd == 127u || odd % 127u != 0u;    // (odd = 127: 127 / a is a power of two)
+            if (odd % 127u != 0u) times *= 1.f + kNear;
         }
-        return __float_as_uint(y);
     }
-    __device__ __forceinline__ uint4 codes(const float (&x)[16], uint32_t bits) const {
+    __device__ __forceinline__ float scale() const { return bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(most, 127.f); }
+    static __device__ __forceinline__ uint32_t bytes(uint64_t y01, uint64_t y23) {
+        return __byte_perm(__byte_perm((uint32_t)y01, (uint32_t)(y01 >> 32), 0x0040), __byte_perm((uint32_t)y23, (uint32_t)(y23 >> 32), 0x0040), 0x5410);
+    }
+    // Four codes in a word, two values an instruction. Not sure: of products with a little less and a little more than 127 / a, which agree except next to a tie
+    __device__ __forceinline__ uint32_t codes(float x0, float x1, float x2, float x3) const {
+        const uint64_t a = pair_of(x0, x1), b = pair_of(x2, x3), magic = pair_of(kMagic, kMagic);
+        if (sizeof(T) == 2 && sure) {
+            const uint64_t f = pair_of(times, times);
+            return bytes(fma_pair(a, f, magic), fma_pair(b, f, magic));
+        }
+        const uint64_t lo = pair_of(times * (1.f - kNear), times * (1.f - kNear)), hi = pair_of(times * (1.f + kNear), times * (1.f + kNear));
+        const uint32_t w = bytes(fma_pair(a, lo, magic), fma_pair(b, lo, magic)), v = bytes(fma_pair(a, hi, magic), fma_pair(b, hi, magic));
+        return w == v ? w : settled_codes(make_float4(x0, x1, x2, x3), times, most * unit, unit);
+    }
+    __device__ __forceinline__ uint4 codes(const Piece16<T>& p) const {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint32_t lo = __byte_perm(code(x[4 * i]), code(x[4 * i + 1]), 0x0040), hi = __byte_perm(code(x[4 * i + 2]), code(x[4 * i + 3]), 0x0040);
-            w[i] = bad(bits) ? 0u : __byte_perm(lo, hi, 0x5410);
+            w[i] = codes(value16(p, 4 * i), value16(p, 4 * i + 1), value16(p, 4 * i + 2), value16(p, 4 * i + 3));
+            if (bad) w[i] = 0u;
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }

@@ -1,72 +1,84 @@
 // Rows (tokens of activations, channels of weights) to int8 codes and a scale each (the arithmetic: dense8.cuh).
 //
-// A CTA has a row: its threads hold 16 values a piece in registers, agree on the largest magnitude and write 16 codes at a time. Rows longer than what
-// the threads hold are read a second time, from L2.
+// A group of warps has a row: its threads hold up to KEEP pieces of 16 values, agree on the largest magnitude and write the codes. Rows longer than what they hold are read a second time,
+// from L2. Few rows: a CTA of as many threads as a row has pieces, so that all of it is under way at once (one row of 4,096 bf16 1.7 us). Many: CTAs of 512 threads that have several short
+// rows or one long one; with a CTA a row, starting CTAs was what took the time (2,048 rows of 4,096: 10.5 us, QT_2048 so).
+// Rows that do not lie on 16-byte boundaries: a thread's 16 values are four times four, 128 apart, so that a warp's loads of single values touch neighbouring bytes.
 #include <type_traits>
 
 #include "dense8.cuh"
 
 namespace {
 
-constexpr int KEEP = 2;
+// Piece c of a row: its 16 values, or, where rows are not on 16-byte boundaries, the warp's block of 512 dealt four values at a time
+template <typename T> __device__ __forceinline__ Piece16<T> load_piece(const T* row, int c, int cols, bool whole) {
+    if (whole) return load16(row, c, cols, true);
+    T t[16];
+    const int at = (c >> 5) * 512 + (c & 31) * 4;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int j = at + (i >> 2) * 128 + (i & 3);
+        t[i] = j < cols ? row[j] : narrow<T>(0.f);
+    }
+    Piece16<T> p;
+    memcpy(&p, t, sizeof p);
+    return p;
+}
+__device__ __forceinline__ void store_piece(int8_t* row, int c, int filled, bool whole, const uint4& v) {
+    if (whole) {
+        if (16 * c < filled) *reinterpret_cast<uint4*>(row + 16 * (size_t)c) = v;
+        return;
+    }
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const int at = (c >> 5) * 512 + (c & 31) * 4;
+#pragma unroll
+    for (int i = 0; i < 4; i++) if (at + i * 128 < filled) *reinterpret_cast<uint32_t*>(row + at + i * 128) = w[i];
+}
 
-template <typename T>
-__global__ void __launch_bounds__(1024)
-quantize_rows_kernel(const T* __restrict__ x, long ldx, int cols, int whole, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
+// grid * (blockDim / (32 group)) rows; group: warps of a row
+template <typename T, int KEEP>
+__global__ void __launch_bounds__(KEEP == 1 ? 1024 : 512)
+quantize_rows_kernel(const T* __restrict__ x, long ldx, int rows, int cols, int whole, int group, int8_t* __restrict__ q, long ldq, float* __restrict__ scale) {
     __shared__ uint32_t red[32];
     dep_trigger();
     dep_wait();
-    const T* row = x + (size_t)blockIdx.x * ldx;
-    const int pieces = (cols + 127) / 128 * 8, step = blockDim.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp / group, step = group * 32, t = threadIdx.x - mine * step, per = (blockDim.x >> 5) / group;
+    const int r = blockIdx.x * per + mine, filled = (cols + 127) / 128 * 128, pieces = (filled / 16 + 31) / 32 * 32;
+    if (r >= rows) return;                             // (whole groups)
+    const T* row = x + (size_t)r * ldx;
     Piece16<T> held[KEEP];
     uint32_t most = 0u;
 #pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-        const int c = threadIdx.x + k * step;
-        if (c < pieces) held[k] = load16(row, c, cols, whole);
-    }
+    for (int k = 0; k < KEEP; k++) if (t + k * step < pieces) held[k] = load_piece(row, t + k * step, cols, whole);
 #pragma unroll
-    for (int k = 0; k < KEEP; k++)
-        if ((int)threadIdx.x + k * step < pieces) {
-            float v[16];
-            widen16<T>(held[k], v);
-            most = max(most, most_of(v));
-        }
-    for (int c = threadIdx.x + KEEP * step; c < pieces; c += step) {
-        float v[16];
-        widen16<T>(load16(row, c, cols, whole), v);
-        most = max(most, most_of(v));
-    }
+    for (int k = 0; k < KEEP; k++) if (t + k * step < pieces) most = max(most, most_of(held[k]));
+    for (int c = t + KEEP * step; c < pieces; c += step) most = max(most, most_of(load_piece(row, c, cols, whole)));
     most = __reduce_max_sync(0xffffffffu, most);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
-    __syncthreads();
-    most = __reduce_max_sync(0xffffffffu, (int)(threadIdx.x & 31) < step / 32 ? red[threadIdx.x & 31] : 0u);
-    const RowScale s(most);
-    uint4* out = reinterpret_cast<uint4*>(q + (size_t)blockIdx.x * ldq);
+    if (group > 1) {
+        if (lane == 0) red[warp] = most;
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + mine), "r"(step) : "memory");
+        most = __reduce_max_sync(0xffffffffu, lane < group ? red[mine * group + lane] : 0u);
+    }
+    const RowScale<T> s(most);
+    int8_t* out = q + (size_t)r * ldq;
 #pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-        const int c = threadIdx.x + k * step;
-        if (c < pieces) {
-            float v[16];
-            widen16<T>(held[k], v);
-            out[c] = s.codes(v, most);
-        }
-    }
-    for (int c = threadIdx.x + KEEP * step; c < pieces; c += step) {
-        float v[16];
-        widen16<T>(load16(row, c, cols, whole), v);
-        out[c] = s.codes(v, most);
-    }
-    if (threadIdx.x == 0) scale[blockIdx.x] = s.scale(most);
+    for (int k = 0; k < KEEP; k++) if (t + k * step < pieces) store_piece(out, t + k * step, filled, whole, s.codes(held[k]));
+    for (int c = t + KEEP * step; c < pieces; c += step) store_piece(out, c, filled, whole, s.codes(load_piece(row, c, cols, whole)));
+    if (t == 0) scale[r] = s.scale();
 }
 
 template <typename T>
 int launch_rows(const void* x, long ldx, int rows, int cols, int8_t* q, long ldq, float* scale, cudaStream_t st) {
-    const int whole = (((uintptr_t)x | ((uintptr_t)ldx * sizeof(T))) & 15) == 0, pieces = (cols + 127) / 128 * 8;
-    // few rows: as many threads as there are pieces, so that all of a row is under way at once
-    const int most = rows <= 2 * cmlb_num_sms() ? 1024 : 256;
-    const int threads = pieces < most ? (pieces + 31) / 32 * 32 : most;
-    CMLB_CUDA(launch_chain(quantize_rows_kernel<T>, dim3(rows), dim3(threads), 0, 1, st, static_cast<const T*>(x), ldx, cols, whole, q, ldq, scale));
+    const int whole = (((uintptr_t)x | ((uintptr_t)ldx * sizeof(T))) & 15) == 0, warps = ((cols + 127) / 128 * 8 + 31) / 32;         // of a thread a piece
+    if (rows <= 2 * cmlb_num_sms()) {
+        const int group = warps < 32 ? warps : 32;
+        CMLB_CUDA(launch_chain(quantize_rows_kernel<T, 1>, dim3(rows), dim3(group * 32), 0, 1, st, static_cast<const T*>(x), ldx, rows, cols, whole, group, q, ldq, scale));
+    } else {
+        constexpr int KEEP = 8 / (int)sizeof(T);
+        int group = 1;
+        while (group < 16 && group * KEEP < warps) group *= 2;
+        CMLB_CUDA(launch_chain(quantize_rows_kernel<T, KEEP>, dim3((rows * (long)group + 15) / 16), dim3(512), 0, 1, st, static_cast<const T*>(x), ldx, rows, cols, whole, group, q, ldq, scale));
+    }
     return CMLB200_OK;
 }
 

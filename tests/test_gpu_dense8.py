@@ -84,6 +84,27 @@ def test_ties_and_ends(pkg, torch_dev, form):
     check_codes(q[ok], s[ok], bad.double().cpu().numpy()[ok], form)
 
 
+@pytest.mark.parametrize("form", ["bfloat16", "float16"])
+def test_every_largest_number(pkg, torch_dev, form):
+    """Rows whose largest number has every mantissa, multiples of 127 among them, and numbers that meet its ties or come next to them."""
+    import torch
+    t = getattr(torch, form)
+    bits = 8 if form == "bfloat16" else 11
+    rows = []
+    for m in range(1 << (bits - 1), 1 << bits):
+        a = float(m)
+        k = torch.arange(0, 128).double()
+        near = ((k + 0.5) * a / 127).to(t).double().clamp_max(a)           # the numbers around every tie
+        rows.append(torch.cat([near, (near * (1 + 2.0 ** -bits)).to(t).double().clamp_max(a), (near * (1 - 2.0 ** -bits)).to(t).double(), torch.tensor([a, a / 2, a / 4, -a / 2])]))
+    x = torch.stack(rows)
+    for scale in (1.0, 2.0 ** -6, 2.0 ** 4 if form == "float16" else 2.0 ** 100, 2.0 ** -14 if form == "float16" else 2.0 ** -130):
+        y = (x * scale).to(t).to(torch_dev)
+        q, s = quantize(pkg, torch, y)
+        check_codes(q, s, y.double().cpu().numpy(), form)
+        q, s = quantize(pkg, torch, y[:200])                              # (few rows: the other shape of CTAs)
+        check_codes(q, s, y[:200].double().cpu().numpy(), form)
+
+
 class Weight:
     """A quantised weight with codes of its own; `half`: gate and up rows in turns of 16."""
 
