@@ -25,7 +25,6 @@ int cmlb_gemm_dense8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, 
 
 namespace {
 
-constexpr int kSkinny8 = 32;                           // rows of x up to which the decode product is taken
 constexpr int kMaxCols8 = 131071;                      // 128 * 128 * this is the largest sum that 32 bits hold
 constexpr float kLeastMost = 127.f * 1.1754943508222875e-38f;
 

@@ -11,8 +11,8 @@
 // Three forms (pick_shape):
 //   pairs       256 channels by up to 256 tokens, a pair of CTAs (cta_group::2): each has 128 channels and half of the tokens' codes. Persistent, two accumulators in turn.
 //   single      128 channels, persistent, the same.
-//   split       where tiles are fewer than SMs a cluster of 2 to 8 CTAs shares the columns of a tile. Their sums meet in distributed shared memory, and since they are whole numbers
-//               the order of adding makes no difference.
+//   split       where tiles are fewer than SMs a cluster of 2 to 8 CTAs shares the columns of a tile. Each finishes its share of the tokens: the others store their sums of those
+//               into its shared memory. Since they are whole numbers the order of adding makes no difference.
 // No load is multicast. Every wait on an mbarrier is bounded; on expiry the CTA raises a status word (cmlb200_dense8_status), waits for its copies and MMAs in flight, frees its tensor
 // memory and returns.
 #include <math.h>
@@ -52,6 +52,14 @@ __device__ __forceinline__ void commit8(uint32_t bar) {
     else
         umma_commit(bar);
 }
+// eight columns of a warp's lanes; there when tmem_there() has returned
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, int (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_there(int (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) : : "memory");
+}
 // `BLOCKS` blocks of 128 columns of a box of rows
 __device__ __forceinline__ void load_blocks(uint32_t dst, const CUtensorMap* map, int row, int block, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -77,7 +85,7 @@ __device__ __forceinline__ void tile8(int i, int tiles_m, int tiles, int& tm, in
     tn = in / rows;
 }
 
-__device__ __noinline__ float far_cap(float y, float cap) { return soft_cap(y, cap); }
+__device__ __noinline__ float far_cap(float y, float cap) { return soft_cap(y, cap); }          // (out of the way)
 __device__ __forceinline__ float finish8(int sum, float unit, float bias, float cap) {
     const float y = fmaf((float)sum, unit, bias);
     return cap > 0.f ? far_cap(y, cap) : y;
@@ -220,58 +228,78 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         }
     } else {
         dep_wait();
-        const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane;
-        int* const own = reinterpret_cast<int*>(smem + HEAD8);               // [NX][128]: this CTA's sums, where the stages were
+        const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane, up = lane >> 4;
+        const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16);
+        // a cluster: rank d finishes tokens d * share .. of the tile; the other ranks' sums of them come to [rank in front of it or behind][share][128] where its stages were
+        const int share = (p.NX + 8 * (int)ranks - 1) / (8 * (int)ranks) * 8;
+        int* const sums = reinterpret_cast<int*>(smem + HEAD8);
         for (int done = 0; done < my_tiles; done++) {
             const int b = done & 1;
             int tm, tn;
             tile8(first_tile + done * step, p.tiles_m, p.tiles, tm, tn);
             const int n = tn * (PAIR ? 2 * CH : CH) + CH * second + ch, m0 = tm * p.NX, most = min(p.NX, p.M - m0);
             const float sw = n < p.N ? p.out.wscale[n] : 0.f, bias = p.out.bias && n < p.N ? p.out.bias[n] : 0.f;
-            if (!wait8(acc_full(b), (done >> 1) & 1, abort_flag, 5)) break;
+            const bool there = wait8(acc_full(b), (done >> 1) & 1, abort_flag, 5);
             tmem_fence_after();
-            for (int c0 = half * 32; c0 < p.NX; c0 += 64) {
-                uint32_t v[32];
-                tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * acc + c0), v);
-                if (ranks > 1) {
+            const uint32_t acc_at = lanes + (uint32_t)(b * acc);
+            if (ranks > 1) {
+                __syncwarp();
+                whole_cluster();                       // everyone's MMAs are through with the stages
+                if (there)
+#pragma unroll 1
+                    for (int d = 1; d < (int)ranks; d++) {
+                        const int to = ((int)rank + d) & ((int)ranks - 1), slot = (int)rank < to ? (int)rank : (int)rank - 1;
+                        const uint32_t base = cluster_addr(sums + (size_t)(slot * share) * CH + ch, to);
+#pragma unroll 1
+                        for (int c = half * 8; c < share && to * share + c < p.NX; c += 16) {
+                            int v[8];
+                            tmem_ld8(acc_at + (uint32_t)(to * share + c), v);
+                            tmem_there(v);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) if (c0 + j < p.NX) own[(c0 + j) * CH + ch] = (int)v[j];
-                    continue;
-                }
-                // (scales of tokens behind the last are read, and lie in the workspace, but are not used)
-                const float4* sx = reinterpret_cast<const float4*>(p.out.xscale + m0 + c0);
-                const int left = most - c0;
-                if (!p.glu) {
-                    float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c0) * p.out.ldy + n;
-                    const bool mine = n < p.N;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 s4 = sx[j / 4];
-                        const float su[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const float r = finish8((int)v[j + e], su[e] * sw, bias, p.out.cap);
-                            if (mine && j + e < left) *y = r;
-                            y += p.out.ldy;
+                            for (int j = 0; j < 8; j++) asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(base + (uint32_t)((c + j) * CH * 4)), "r"(v[j]) : "memory");
                         }
+                    }
+                __syncwarp();
+                whole_cluster();                       // what the others have is here
+            }
+            if (!there) break;
+            // Eight tokens a turn in a small loop: nothing of a kernel's code is cached when it begins, and this is where most of it would be (unrolled over 32 tokens: 4 to 5 us for 128)
+            const int c_lo = (int)rank * share, c_hi = min(most, ranks > 1 ? c_lo + share : p.NX), col = (n >> 5) * 16 + (lane & 15);
+            const bool mine = p.glu ? col < p.out.n_out : n < p.N;
+            int v[8];
+            int c = c_lo + half * 8;
+            if (c < c_hi) tmem_ld8(acc_at + (uint32_t)c, v);
+#pragma unroll 1
+            for (; c < c_hi; c += 16) {
+                // (scales of tokens behind the last are read, and lie in the workspace, but are not used)
+                const float4 s0 = *reinterpret_cast<const float4*>(p.out.xscale + m0 + c), s1 = *reinterpret_cast<const float4*>(p.out.xscale + m0 + c + 4);
+                const float sx[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+                int u[8];
+                tmem_there(v);
+#pragma unroll
+                for (int j = 0; j < 8; j++) u[j] = v[j];
+                if (c + 16 < c_hi) tmem_ld8(acc_at + (uint32_t)(c + 16), v);
+#pragma unroll 1
+                for (int k = 0; k < (int)ranks - 1; k++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) u[j] += sums[(size_t)(k * share + c - c_lo + j) * CH + ch];
+                if (!p.glu) {
+                    float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c) * p.out.ldy + n;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float r = finish8(u[j], sx[j] * sw, bias, p.out.cap);
+                        if (mine && c + j < c_hi) *y = r;
+                        y += p.out.ldy;
                     }
                 } else {
                     // 16 gate lanes, 16 up lanes: of two tokens, the lower lanes finish the first and the upper ones the second
-                    const int col = (n >> 5) * 16 + (lane & 15), up = lane >> 4;
-                    __nv_bfloat16* f = static_cast<__nv_bfloat16*>(p.out.y) + (size_t)(m0 + c0 + up) * p.out.ldy + col;
-                    const bool mine = col < p.out.n_out;
+                    __nv_bfloat16* f = static_cast<__nv_bfloat16*>(p.out.y) + (size_t)(m0 + c + up) * p.out.ldy + col;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 s4 = sx[j / 4];
-                        const float su[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            const float a = (float)(int)v[j + e] * (su[e] * sw), c = (float)(int)v[j + e + 1] * (su[e + 1] * sw);
-                            const float other = __shfl_xor_sync(0xffffffffu, up ? a : c, 16);
-                            const float r = glu8(p.out.act, up ? other : a, up ? c : other);
-                            if (mine && j + e + up < left) *f = __float2bfloat16_rn(r);
-                            f += 2 * p.out.ldy;
-                        }
+                    for (int j = 0; j < 8; j += 2) {
+                        const float a = (float)u[j] * (sx[j] * sw), e = (float)u[j + 1] * (sx[j + 1] * sw), other = __shfl_xor_sync(0xffffffffu, up ? a : e, 16);
+                        const float r = glu8(p.out.act, up ? other : a, up ? e : other);
+                        if (mine && c + j + up < c_hi) *f = __float2bfloat16_rn(r);
+                        f += 2 * p.out.ldy;
                     }
                 }
             }
@@ -283,51 +311,10 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
             }
         }
     }
-    if (ranks > 1) {                                   // one tile, its columns over the cluster: CTA r adds and finishes its share of the tokens
+    if (ranks > 1 && warp < 2) {                       // (the barriers of the sums)
         __syncwarp();
         whole_cluster();
-        if (warp >= 2 && !*abort_flag) {
-            int tm, tn;
-            tile8(first_tile, p.tiles_m, p.tiles, tm, tn);
-            const int m0 = tm * p.NX, most = min(p.NX, p.M - m0), per = (most + (int)ranks - 1) / (int)ranks, c_lo = (int)rank * per, c_hi = min(most, c_lo + per);
-            const int quads = p.glu ? 16 : 32;         // four channels each (glu: gate channels, with those 16 on)
-            auto add = [&](auto most_ranks) {
-                constexpr int R = decltype(most_ranks)::value;
-                for (int i = (warp - 2) * 32 + lane; i < (c_hi - c_lo) * quads; i += EPI * 32) {
-                    const int c = c_lo + i / quads, k = i % quads, r = p.glu ? (k >> 2) * 32 + (k & 3) * 4 : k * 4, n = tn * CH + r;
-                    int4 a[R], u[R];
-#pragma unroll
-                    for (int w = 0; w < R; w++) {
-                        const uint32_t at = cluster_addr(smem + HEAD8 + ((size_t)c * CH + r) * 4, w);
-                        asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(a[w].x), "=r"(a[w].y), "=r"(a[w].z), "=r"(a[w].w) : "r"(at) : "memory");
-                        if (p.glu) asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(u[w].x), "=r"(u[w].y), "=r"(u[w].z), "=r"(u[w].w) : "r"(at + 64) : "memory");
-                    }
-                    const float sx = p.out.xscale[m0 + c];
-                    int sa[4] = {0, 0, 0, 0}, su[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int w = 0; w < R; w++) { sa[0] += a[w].x; sa[1] += a[w].y; sa[2] += a[w].z; sa[3] += a[w].w; }
-                    if (p.glu) {
-#pragma unroll
-                        for (int w = 0; w < R; w++) { su[0] += u[w].x; su[1] += u[w].y; su[2] += u[w].z; su[3] += u[w].w; }
-                        const int col = (n >> 5) * 16 + (n & 15);
-                        __nv_bfloat16* f = static_cast<__nv_bfloat16*>(p.out.y) + (size_t)(m0 + c) * p.out.ldy + col;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (col + e < p.out.n_out) f[e] = __float2bfloat16_rn(glu8(p.out.act, (float)sa[e] * (sx * p.out.wscale[n + e]), (float)su[e] * (sx * p.out.wscale[n + 16 + e])));
-                    } else {
-                        float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c) * p.out.ldy + n;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (n + e < p.N) y[e] = finish8(sa[e], sx * p.out.wscale[n + e], p.out.bias ? p.out.bias[n + e] : 0.f, p.out.cap);
-                    }
-                }
-            };
-            if (ranks == 2) add(std::integral_constant<int, 2>());
-            else if (ranks == 4) add(std::integral_constant<int, 4>());
-            else add(std::integral_constant<int, 8>());
-        }
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");      // nobody leaves while its sums are read (and all of them have been used)
+        whole_cluster();
     }
     tmem_fence_before();
     __syncthreads();
@@ -380,7 +367,7 @@ int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, cons
     int rc = encode_blocks(&xmap, xq, M, blocks, ldq, box);
     if (!rc) rc = encode_blocks(&wmap, W->w, W->rows, blocks, W->ld, CH);
     if (rc) return rc;
-    const int stage = BLOCKS * (A8 + box * BK8), sums = shape.ranks > 1 ? shape.NX * CH * 4 : 0;
+    const int stage = BLOCKS * (A8 + box * BK8), sums = shape.ranks > 1 ? (shape.NX + 8 * shape.ranks) * CH * 4 : 0;
     const int stages = ROOM8 / stage < MOST_STAGES ? ROOM8 / stage : MOST_STAGES;
     const Gemm8 p = {out, M, W->rows, (blocks + BLOCKS - 1) / BLOCKS, shape.NX, tm, tiles, stages, glu};
     const size_t smem = 1024 + HEAD8 + (size_t)(stages * stage > sums ? stages * stage : sums);

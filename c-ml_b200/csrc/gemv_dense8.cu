@@ -1,124 +1,198 @@
-// Decode product of int8 weights and int8 rows, up to 32 rows of x a pass: y[m][n] = sx[m] sw[n] sum_k xq[m][k] wq[n][k], sums in 32-bit integers, exact.
-// The weight streams from HBM once, straight into the A fragments of mma.sync m16n8k32: since any order of the columns will do as long as both operands
-// use the same one, lane t of a quad takes 16 neighbouring bytes of every 64: one 16-byte load a row feeds two MMAs. Codes of x come the same way through L1.
-// The warps of a CTA split K and meet in shared memory; whole numbers, so in any order.
+// Decode products of int8 weights and int8 rows, up to 16 rows of x: y[m][n] = sx[m] sw[n] sum_k xq[m][k] wq[n][k], sums in 32-bit integers, exact; and the entry points of all
+// such products.
 //
-// The first weights are requested before the launch waits for its predecessor: they do not depend on it.
+// One CTA an SM, or two, walks over tiles of 16 weight rows (gate and up rows: 32). The weight streams from HBM once, straight into the A fragments of mma.sync m16n8k32: since any order of the
+// columns will do as long as both operands use the same one, lane t of a quad takes 16 neighbouring bytes of every 64: one 16-byte load a row feeds two MMAs. The warps split K in
+// chunks of 128 columns, each with its next chunks requested RING ahead, across tiles, and the first before the launch waits for its predecessor: weights do not depend on it. Their
+// sums meet in shared memory by atomic additions (whole numbers: the order makes no difference).
+//
+// Rows of x: few of them (M K up to kFused) every CTA quantises itself, into shared memory, while its first weights are on their way: one launch instead of two, and no codes in
+// memory. More come as codes from cmlb200_quantize_rows, through L1, where a warp finds its own columns again with every tile. What is left goes to the tensor-core product of
+// prompts (gemm_dense8.cu).
 #include <type_traits>
 
 #include "dense8.cuh"
 
 namespace {
 
-constexpr int GW = 8;                                  // warps
-
 __device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// RT tiles of 16 weight rows per CTA, NB groups of 8 rows of x; blockIdx.y: passes of NB * 8 rows. GLU: tile 0 = 16 gate rows, tile 1 = the 16 up rows that go with them.
-template <int RT, int NB, bool GLU>
-__global__ void __launch_bounds__(GW * 32)
-gemv_dense8_kernel(const int8_t* __restrict__ W, int ldw, const int8_t* __restrict__ xq, int ldx, int M, int K, const Out8 out) {
-    __shared__ int part[GW][RT * 16][NB * 8 + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * RT * 16, chunks = (K + 127) / 128, m0 = blockIdx.y * NB * 8;
-    const int8_t* wrow[RT][2];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        wrow[i][0] = W + (size_t)(n0 + i * 16 + g) * ldw + 16 * t;
-        wrow[i][1] = wrow[i][0] + (size_t)8 * ldw;
-    }
-    constexpr int RING = 4 / RT;                       // 128-column chunks in flight per warp
+// RT tiles of 16 weight rows a CTA and turn, NB groups of 8 rows of x. GLU: tile 0 = 16 gate rows, tile 1 = the 16 up rows that go with them. T: what x holds; int8_t: codes
+template <typename T, int GW, int RT, int NB, int RING, bool GLU>
+__global__ void __launch_bounds__(GW * 32, 16 / GW)
+gemv_dense8_kernel(const int8_t* __restrict__ W, int ldw, const T* __restrict__ x, long ldx, int M, int K, int whole, int tiles, const Out8 out) {
+    constexpr bool FUSED = sizeof(T) > 1;
+    extern __shared__ __align__(16) uint8_t codes_smem[];
+    __shared__ int sums[2][RT * 16][NB * 8 + 1];
+    __shared__ uint32_t red[GW];
+    __shared__ float sxs[NB * 8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, chunks = (K + 127) / 128;
+    const int lds = chunks * 128 + 64;                 // (rows 64 bytes apart modulo 128: a quarter of a warp reads two of them without a conflict)
     uint4 w[RING][RT][2][2];
-    auto fetch = [&](int u, int c) {
+    int ftile = warp < chunks ? (int)blockIdx.x : tiles, fc = warp;
+    auto fetch = [&](int u) {
+        const int8_t* at = W + (size_t)(ftile * (RT * 16) + g) * ldw + fc * 128 + 16 * t;
 #pragma unroll
         for (int i = 0; i < RT; i++)
 #pragma unroll
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int s = 0; s < 2; s++)
-                    w[u][i][e][s] = c < chunks ? ld_stream(reinterpret_cast<const __nv_bfloat16*>(wrow[i][e] + (size_t)c * 128 + 64 * s)) : make_uint4(0u, 0u, 0u, 0u);
+                    if (ftile < tiles) w[u][i][e][s] = ld_stream(reinterpret_cast<const __nv_bfloat16*>(at + (size_t)(i * 16 + e * 8) * ldw + 64 * s));
+        fc += GW;
+        if (fc >= chunks) { fc = warp; ftile += gridDim.x; }
     };
 #pragma unroll
-    for (int u = 0; u < RING; u++) fetch(u, warp + u * GW);
+    for (int u = 0; u < RING; u++) fetch(u);
+    for (int i = threadIdx.x; i < 2 * RT * 16 * (NB * 8 + 1); i += GW * 32) (&sums[0][0][0])[i] = 0;
     dep_trigger();
     dep_wait();
+    const int8_t* xr[NB];
+    if constexpr (FUSED) {
+        // a row's warps: 16, 8, 4 or 2
+        const int group = M <= 1 ? GW : M <= 2 ? GW / 2 : M <= 4 ? GW / 4 : GW / 8, row = warp / group, step = group * 32, p0 = threadIdx.x - row * step, pieces = chunks * 8;
+        constexpr int KEEP = 2;
+        const bool on = row < M;
+        const T* src = x + (size_t)min(row, M - 1) * ldx;
+        Piece16<T> held[KEEP];
+        uint32_t most = 0u;
+#pragma unroll
+        for (int k = 0; k < KEEP; k++) if (on && p0 + k * step < pieces) held[k] = load16(src, p0 + k * step, K, whole);
+#pragma unroll
+        for (int k = 0; k < KEEP; k++) if (on && p0 + k * step < pieces) most = max(most, most_of(held[k]));
+        for (int c = p0 + KEEP * step; on && c < pieces; c += step) most = max(most, most_of(load16(src, c, K, whole)));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) red[warp] = most;
+        __syncthreads();
+        most = __reduce_max_sync(0xffffffffu, lane < group ? red[row * group + lane] : 0u);
+        const RowScale<T> s(most);
+        uint4* dst = reinterpret_cast<uint4*>(codes_smem + (size_t)row * lds);
+        if (on) {
+#pragma unroll
+            for (int k = 0; k < KEEP; k++) if (p0 + k * step < pieces) dst[p0 + k * step] = s.codes(held[k]);
+            for (int c = p0 + KEEP * step; c < pieces; c += step) dst[c] = s.codes(load16(src, c, K, whole));
+            if (p0 == 0) sxs[row] = s.scale();
+        }
+        xr[0] = reinterpret_cast<const int8_t*>(codes_smem) + (size_t)min(g, M - 1) * lds + 16 * t;
+    } else {
+        if ((int)threadIdx.x < M) sxs[threadIdx.x] = out.xscale[threadIdx.x];
+#pragma unroll
+        for (int b = 0; b < NB; b++) xr[b] = reinterpret_cast<const int8_t*>(x) + (size_t)min(b * 8 + g, M - 1) * ldx + 16 * t;        // rows past M repeat the last, never stored
+    }
+    __syncthreads();
     int acc[RT][NB][4];
 #pragma unroll
     for (int i = 0; i < RT; i++)
 #pragma unroll
         for (int b = 0; b < NB; b++) acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0;
-    const int8_t* xr[NB];
+    int tile = blockIdx.x, c = warp, turn = 0;
+    // The warps' sums meet, and 4 NB warps, others every time, finish 16 outputs of NB * 8 rows. Two buffers in turn; who reads a sum leaves 0 for the turn after the next
+    auto finish = [&]() {
+        int (*mine)[NB * 8 + 1] = sums[turn & 1];
+        if (warp < chunks) {
 #pragma unroll
-    for (int b = 0; b < NB; b++) xr[b] = xq + (size_t)min(m0 + b * 8 + g, M - 1) * ldx + 16 * t;       // rows past M repeat the last, never stored
-    for (int c0 = warp; c0 < chunks; c0 += RING * GW) {
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    atomicAdd(&mine[i * 16 + g][b * 8 + 2 * t], acc[i][b][0]);
+                    atomicAdd(&mine[i * 16 + g][b * 8 + 2 * t + 1], acc[i][b][1]);
+                    atomicAdd(&mine[i * 16 + g + 8][b * 8 + 2 * t], acc[i][b][2]);
+                    atomicAdd(&mine[i * 16 + g + 8][b * 8 + 2 * t + 1], acc[i][b][3]);
+                    acc[i][b][0] = acc[i][b][1] = acc[i][b][2] = acc[i][b][3] = 0;
+                }
+        }
+        __syncthreads();
+        const int i = ((warp - 4 * NB * turn) & (GW - 1)) * 32 + lane, n = i & 15, m = i >> 4;
+        if (m < NB * 8) {
+            const int s = mine[n][m], s2 = GLU ? mine[RT * 16 - 16 + n][m] : 0, r = tile * (RT * 16) + n;
+            mine[n][m] = 0;
+            if (GLU) mine[RT * 16 - 16 + n][m] = 0;
+            if (GLU) {
+                const int col = tile * 16 + n;
+                if (m < M && col < out.n_out)
+                    static_cast<__nv_bfloat16*>(out.y)[(size_t)m * out.ldy + col] = __float2bfloat16_rn(glu8(out.act, (float)s * (sxs[m] * out.wscale[r]), (float)s2 * (sxs[m] * out.wscale[r + 16])));
+            } else if (m < M && r < out.n_out) {
+                float y = (float)s * (sxs[m] * out.wscale[r]);
+                if (out.bias) y += out.bias[r];
+                if (out.cap > 0.f) y = soft_cap(y, out.cap);
+                static_cast<float*>(out.y)[(size_t)m * out.ldy + r] = y;
+            }
+        }
+        turn++;
+        tile += gridDim.x;
+        c = warp;
+    };
+    if (warp >= chunks) {
+        while (tile < tiles) finish();
+        return;
+    }
+    while (tile < tiles) {
 #pragma unroll
         for (int u = 0; u < RING; u++) {
-            const int c = min(c0 + u * GW, chunks - 1);              // past the end: zero weights
+            if (tile >= tiles) break;
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int s = 0; s < 2; s++) {
+                uint4 v[NB];
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(xr[b] + (size_t)c * 128 + 64 * s);
+                for (int b = 0; b < NB; b++) v[b] = *reinterpret_cast<const uint4*>(xr[b] + (size_t)c * 128 + 64 * s);
+#pragma unroll
+                for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
-                        mma_i8(acc[i][b], w[u][i][0][s].x, w[u][i][1][s].x, w[u][i][0][s].y, w[u][i][1][s].y, v.x, v.y);
-                        mma_i8(acc[i][b], w[u][i][0][s].z, w[u][i][1][s].z, w[u][i][0][s].w, w[u][i][1][s].w, v.z, v.w);
+                        mma_i8(acc[i][b], w[u][i][0][s].x, w[u][i][1][s].x, w[u][i][0][s].y, w[u][i][1][s].y, v[b].x, v[b].y);
+                        mma_i8(acc[i][b], w[u][i][0][s].z, w[u][i][1][s].z, w[u][i][0][s].w, w[u][i][1][s].w, v[b].z, v[b].w);
                     }
-                }
-            fetch(u, c0 + (u + RING) * GW);
-        }
-    }
-    // accumulator 0, 1: weight row g, rows 2t, 2t + 1 of x; 2, 3: weight row g + 8
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            part[warp][i * 16 + g][b * 8 + 2 * t] = acc[i][b][0];
-            part[warp][i * 16 + g][b * 8 + 2 * t + 1] = acc[i][b][1];
-            part[warp][i * 16 + g + 8][b * 8 + 2 * t] = acc[i][b][2];
-            part[warp][i * 16 + g + 8][b * 8 + 2 * t + 1] = acc[i][b][3];
-        }
-    __syncthreads();
-    constexpr int OUT = GLU ? 16 : RT * 16;
-    for (int i = threadIdx.x; i < OUT * NB * 8; i += GW * 32) {
-        const int n = i % OUT, m = i / OUT;
-        if (m0 + m >= M) break;
-        int s = 0, s2 = 0;
-#pragma unroll
-        for (int k = 0; k < GW; k++) {
-            s += part[k][n][m];
-            if (GLU) s2 += part[k][RT * 16 - 16 + n][m];
-        }
-        const float sx = out.xscale[m0 + m];
-        if (GLU) {
-            const int c = blockIdx.x * 16 + n;
-            if (c < out.n_out)
-                static_cast<__nv_bfloat16*>(out.y)[(size_t)(m0 + m) * out.ldy + c] = __float2bfloat16_rn(
-                    glu8(out.act, (float)s * (sx * out.wscale[n0 + n]), (float)s2 * (sx * out.wscale[n0 + 16 + n])));
-        } else if (n0 + n < out.n_out) {
-            float y = (float)s * (sx * out.wscale[n0 + n]);
-            if (out.bias) y += out.bias[n0 + n];
-            if (out.cap > 0.f) y = soft_cap(y, out.cap);
-            static_cast<float*>(out.y)[(size_t)(m0 + m) * out.ldy + n0 + n] = y;
+            }
+            fetch(u);
+            c += GW;
+            if (c >= chunks) finish();
         }
     }
 }
 
-template <int RT, bool GLU>
-int launch_gemv8(const cmlb200_dense8* W, const int8_t* xq, int ldx, int M, const Out8& out, cudaStream_t st) {
-    const unsigned tiles = (unsigned)((W->rows + RT * 16 - 1) / (RT * 16));
-#define G8_LAUNCH(NB) CMLB_CUDA(launch_chain(gemv_dense8_kernel<RT, NB, GLU>, dim3(tiles, (unsigned)((M + NB * 8 - 1) / (NB * 8))), dim3(GW * 32), 0, 1, st, static_cast<const int8_t*>(W->w), W->ld, xq, ldx, M, W->cols, out))
-    if (M <= 8) G8_LAUNCH(1);
-    else if (M <= 16) G8_LAUNCH(2);
-    else G8_LAUNCH(4);
-#undef G8_LAUNCH
+// M K up to which the CTAs quantise rows themselves: 4 rows of 4096x4096 5.5 us (two launches 6.2), 8 7.0 (6.4), 2 of 4096x11008 10.6 (11.4), 4 12.3 (11.5)
+constexpr int kFused = 24576;
+// rows * cols of a weight up to which 9 to 16 rows of x are taken here: 16 of 4096x4096 7.8 us (the prompts' product 8.9), of 11008x4096 14.3 (13.5)
+constexpr int kSmall = 20000000;
+
+template <typename T, int GW, int RT, int NB, int RING, bool GLU>
+int launch_gemv8(const cmlb200_dense8* W, const void* x, long ldx, int M, const Out8& out, cudaStream_t st) {
+    const int whole = (((uintptr_t)x | ((uintptr_t)ldx * sizeof(T))) & 15) == 0, chunks = (W->cols + 127) / 128, tiles = (W->rows + RT * 16 - 1) / (RT * 16);
+    const int most = cmlb_num_sms() * (16 / GW);
+    const size_t smem = sizeof(T) > 1 ? (size_t)M * (chunks * 128 + 64) : 0;
+    static size_t attr[kMaxDevices] = {};
+    if (smem) CMLB_CUDA(cmlb_ensure_smem(gemv_dense8_kernel<T, GW, RT, NB, RING, GLU>, smem, attr));
+    CMLB_CUDA(launch_chain(gemv_dense8_kernel<T, GW, RT, NB, RING, GLU>, dim3(tiles < most ? tiles : most), dim3(GW * 32), smem, 1, st, static_cast<const int8_t*>(W->w), W->ld,
+                           static_cast<const T*>(x), ldx, M, W->cols, whole, tiles, out));
     return CMLB200_OK;
 }
 
 size_t codes_bytes(int M, int cols) { return (size_t)M * ((cols + 127) / 128 * 128); }
+
+template <int RT, int RING, bool GLU>
+int product8(const cmlb200_dense8* W, const void* x, int dtype, long ldx, int M, Out8 out, void* work, const char* who, cudaStream_t st) {
+    if (M <= 8 && (long)M * W->cols <= kFused) {
+        CMLB_REQUIRE(ldx >= W->cols && ((uintptr_t)x & (dtype == CMLB200_DT_F32 ? 3 : 1)) == 0, "%s: %d columns, stride %ld, or x is not aligned to its type", who, W->cols, ldx);
+        if (dtype == CMLB200_DT_F32) return launch_gemv8<float, 16, RT, 1, RING, GLU>(W, x, ldx, M, out, st);
+        if (dtype == CMLB200_DT_BF16) return launch_gemv8<__nv_bfloat16, 16, RT, 1, RING, GLU>(W, x, ldx, M, out, st);
+        if (dtype == CMLB200_DT_F16) return launch_gemv8<__half, 16, RT, 1, RING, GLU>(W, x, ldx, M, out, st);
+        CMLB_REQUIRE(false, "%s: dtype %d", who, dtype);
+    }
+    int8_t* xq = static_cast<int8_t*>(work);
+    const int ldq = (W->cols + 127) / 128 * 128;
+    float* xs = reinterpret_cast<float*>(xq + codes_bytes(M, W->cols));
+    const int rc = cmlb200_quantize_rows(x, dtype, ldx, M, W->cols, xq, ldq, xs, st);
+    if (rc) return rc;
+    out.xscale = xs;
+    if (M <= 8 || (M <= 16 && (long)W->rows * W->cols <= kSmall)) {
+        constexpr int G = GLU ? 16 : 8;                // (two CTAs an SM take tiles of 16 weight rows beside one another: 8 rows of 4096x4096 6.95 to 6.4 us, gate and up rows 19.0 and 20.4)
+        return M <= 8 ? launch_gemv8<int8_t, G, RT, 1, RING, GLU>(W, xq, ldq, M, out, st) : launch_gemv8<int8_t, G, RT, 2, RING, GLU>(W, xq, ldq, M, out, st);
+    }
+    return cmlb_gemm_dense8(W, xq, ldq, M, out, GLU, st);
+}
 
 int check8(const cmlb200_dense8* W, const void* x, int M, void* y, void* work, const char* who) {
     CMLB_REQUIRE(W && W->w && W->scale && x && y && work, "%s: NULL argument", who);
@@ -140,13 +214,8 @@ extern "C" int cmlb200_linear_dense8(const cmlb200_dense8* W, const void* d_x, i
     int rc = check8(W, d_x, M, d_y, d_work, who);
     if (rc) return rc;
     CMLB_REQUIRE(ldy >= W->rows && ((uintptr_t)d_y & 3) == 0, "%s: output stride %ld", who, ldy);
-    int8_t* xq = static_cast<int8_t*>(d_work);
-    const int ldq = (W->cols + 127) / 128 * 128;
-    float* xs = reinterpret_cast<float*>(xq + codes_bytes(M, W->cols));
-    rc = cmlb200_quantize_rows(d_x, dtype, ldx, M, W->cols, xq, ldq, xs, stream);
-    if (rc) return rc;
-    const Out8 out = {W->scale, W->bias, xs, W->cap, 0, W->rows, d_y, (int)ldy};
-    return M <= kSkinny8 ? launch_gemv8<1, false>(W, xq, ldq, M, out, as_stream(stream)) : cmlb_gemm_dense8(W, xq, ldq, M, out, 0, as_stream(stream));
+    const Out8 out = {W->scale, W->bias, nullptr, W->cap, 0, W->rows, d_y, (int)ldy};
+    return product8<1, 4, false>(W, d_x, dtype, ldx, M, out, d_work, who, as_stream(stream));
 }
 
 extern "C" int cmlb200_linear_dense8_glu(const cmlb200_dense8* W, const void* d_x, int dtype, long ldx, int M, int ff, int act, uint16_t* d_f, long ldf, void* d_work, void* stream) {
@@ -155,11 +224,6 @@ extern "C" int cmlb200_linear_dense8_glu(const cmlb200_dense8* W, const void* d_
     if (rc) return rc;
     CMLB_REQUIRE(ff > 0 && W->rows == 2 * ((ff + 15) & ~15) && ldf >= ff && ((uintptr_t)d_f & 1) == 0, "%s: %d weight rows for %d outputs, stride %ld", who, W->rows, ff, ldf);
     CMLB_REQUIRE(act == CMLB200_ACT_SILU || act == CMLB200_ACT_GELU_TANH || act == CMLB200_ACT_GELU_ERF, "%s: activation %d", who, act);
-    int8_t* xq = static_cast<int8_t*>(d_work);
-    const int ldq = (W->cols + 127) / 128 * 128;
-    float* xs = reinterpret_cast<float*>(xq + codes_bytes(M, W->cols));
-    rc = cmlb200_quantize_rows(d_x, dtype, ldx, M, W->cols, xq, ldq, xs, stream);
-    if (rc) return rc;
-    const Out8 out = {W->scale, nullptr, xs, 0.f, act, ff, d_f, (int)ldf};
-    return M <= kSkinny8 ? launch_gemv8<2, true>(W, xq, ldq, M, out, as_stream(stream)) : cmlb_gemm_dense8(W, xq, ldq, M, out, 1, as_stream(stream));
+    const Out8 out = {W->scale, nullptr, nullptr, 0.f, act, ff, d_f, (int)ldf};
+    return product8<2, 2, true>(W, d_x, dtype, ldx, M, out, d_work, who, as_stream(stream));
 }
