@@ -25,7 +25,7 @@ namespace {
 constexpr int BK8 = 128, BLOCKS = 2, CH = 128;         // columns of a block, blocks of a stage, channels of a CTA
 constexpr int EPI = 8, THREADS8 = 64 + EPI * 32;
 constexpr int A8 = CH * BK8, MOST_STAGES = 8, ROOM8 = 220 * 1024;
-constexpr int HEAD8 = 1024;                            // barriers and words in front of the stages
+constexpr int SCALES8 = 1024, HEAD8 = SCALES8 + EPI * 512;                    // in front of the stages: barriers and words, then the epilogue warps' scales of tokens
 
 __device__ int g_dense8_status = 0;
 __device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
@@ -139,6 +139,7 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         next(x, true);
     };
     const int ahead = min(S, total);
+    if (threadIdx.x == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&xmap) : "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) { mbar_init(full(s), PAIR && !second ? 2 : 1); mbar_init(empty(s), 1); }
         for (int b = 0; b < 2; b++) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), PAIR ? 2 * EPI : EPI); }
@@ -230,15 +231,24 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         dep_wait();
         const int q = warp & 3, half = (warp - 2) >> 2, ch = q * 32 + lane, up = lane >> 4;
         const uint32_t lanes = tmem_base + ((uint32_t)(q * 32) << 16);
-        // a cluster: rank d finishes tokens d * share .. of the tile; the other ranks' sums of them come to [rank in front of it or behind][share][128] where its stages were
+        // a cluster: rank d finishes tokens d * share .. of the tile; the other ranks' sums of them come to [rank in front of it or behind][share / 4][128][4] where its stages were
         const int share = (p.NX + 8 * (int)ranks - 1) / (8 * (int)ranks) * 8;
         int* const sums = reinterpret_cast<int*>(smem + HEAD8);
+        float* const sxs = reinterpret_cast<float*>(smem + SCALES8) + (warp - 2) * 128;        // of this warp's tokens, in the order it comes to them
         for (int done = 0; done < my_tiles; done++) {
             const int b = done & 1;
             int tm, tn;
             tile8(first_tile + done * step, p.tiles_m, p.tiles, tm, tn);
             const int n = tn * (PAIR ? 2 * CH : CH) + CH * second + ch, m0 = tm * p.NX, most = min(p.NX, p.M - m0);
             const float sw = n < p.N ? p.out.wscale[n] : 0.f, bias = p.out.bias && n < p.N ? p.out.bias[n] : 0.f;
+            const int c_lo = (int)rank * share, c_hi = min(most, ranks > 1 ? c_lo + share : p.NX);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int c = c_lo + half * 8 + (4 * i + (lane >> 3)) * 16 + (lane & 7);
+                sxs[i * 32 + lane] = c < c_hi ? p.out.xscale[m0 + c] : 0.f;
+            }
+            __syncwarp();
             const bool there = wait8(acc_full(b), (done >> 1) & 1, abort_flag, 5);
             tmem_fence_after();
             const uint32_t acc_at = lanes + (uint32_t)(b * acc);
@@ -248,15 +258,20 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
                 if (there)
 #pragma unroll 1
                     for (int d = 1; d < (int)ranks; d++) {
-                        const int to = ((int)rank + d) & ((int)ranks - 1), slot = (int)rank < to ? (int)rank : (int)rank - 1;
-                        const uint32_t base = cluster_addr(sums + (size_t)(slot * share) * CH + ch, to);
+                        const int to = ((int)rank + d) & ((int)ranks - 1), slot = (int)rank < to ? (int)rank : (int)rank - 1, end = min(share, p.NX - to * share);
+                        const uint32_t base = cluster_addr(sums + (size_t)(slot * share) * CH + ch * 4, to);
+                        int v[8], c = half * 8;
+                        if (c < end) tmem_ld8(acc_at + (uint32_t)(to * share + c), v);
 #pragma unroll 1
-                        for (int c = half * 8; c < share && to * share + c < p.NX; c += 16) {
-                            int v[8];
-                            tmem_ld8(acc_at + (uint32_t)(to * share + c), v);
+                        for (; c < end; c += 16) {
+                            int u[8];
                             tmem_there(v);
 #pragma unroll
-                            for (int j = 0; j < 8; j++) asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(base + (uint32_t)((c + j) * CH * 4)), "r"(v[j]) : "memory");
+                            for (int j = 0; j < 8; j++) u[j] = v[j];
+                            if (c + 16 < end) tmem_ld8(acc_at + (uint32_t)(to * share + c + 16), v);
+#pragma unroll
+                            for (int j = 0; j < 8; j += 4)
+                                asm volatile("st.shared::cluster.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(base + (uint32_t)((c + j) * CH * 4)), "r"(u[j]), "r"(u[j + 1]), "r"(u[j + 2]), "r"(u[j + 3]) : "memory");
                         }
                     }
                 __syncwarp();
@@ -264,15 +279,15 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
             }
             if (!there) break;
             // Eight tokens a turn in a small loop: nothing of a kernel's code is cached when it begins, and this is where most of it would be (unrolled over 32 tokens: 4 to 5 us for 128)
-            const int c_lo = (int)rank * share, c_hi = min(most, ranks > 1 ? c_lo + share : p.NX), col = (n >> 5) * 16 + (lane & 15);
+            const int col = (n >> 5) * 16 + (lane & 15);
+            const float4* sx4 = reinterpret_cast<const float4*>(sxs);
             const bool mine = p.glu ? col < p.out.n_out : n < p.N;
             int v[8];
             int c = c_lo + half * 8;
             if (c < c_hi) tmem_ld8(acc_at + (uint32_t)c, v);
 #pragma unroll 1
-            for (; c < c_hi; c += 16) {
-                // (scales of tokens behind the last are read, and lie in the workspace, but are not used)
-                const float4 s0 = *reinterpret_cast<const float4*>(p.out.xscale + m0 + c), s1 = *reinterpret_cast<const float4*>(p.out.xscale + m0 + c + 4);
+            for (; c < c_hi; c += 16, sx4 += 2) {
+                const float4 s0 = sx4[0], s1 = sx4[1];
                 const float sx[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
                 int u[8];
                 tmem_there(v);
@@ -282,7 +297,10 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
 #pragma unroll 1
                 for (int k = 0; k < (int)ranks - 1; k++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) u[j] += sums[(size_t)(k * share + c - c_lo + j) * CH + ch];
+                    for (int j = 0; j < 8; j += 4) {
+                        const int4 o = *reinterpret_cast<const int4*>(sums + (size_t)(k * share + c - c_lo + j) * CH + ch * 4);
+                        u[j] += o.x; u[j + 1] += o.y; u[j + 2] += o.z; u[j + 3] += o.w;
+                    }
                 if (!p.glu) {
                     float* y = static_cast<float*>(p.out.y) + (size_t)(m0 + c) * p.out.ldy + n;
 #pragma unroll
@@ -340,23 +358,24 @@ int encode_blocks(CUtensorMap* map, const void* base, long rows, int blocks, int
     return CMLB200_OK;
 }
 
-// Cycles that a form would take, by its waves: a stage takes its MMAs (4 NX) or its bytes (50 a cycle and SM) or its issue (600), a tile about 3,000 to start and end, a cluster's sum
-// 2,000 more.
-// How many clusters of 2, 4 and 8 run at once goes by how SMs lie in groups: 74, 33 and 15 on B200.
+// Cycles that a form would take, by its waves: a stage takes its MMAs (4 NX) or its bytes (50 a cycle and SM) or its issue (600), a tile about 2,000 to start and end and 8 a token, a
+// cluster's sum 2,000 and 8 a token more. How many clusters of 4 and 8 run at once goes by how SMs lie in groups: 33 and 15 on B200. Tokens are cut into the fewest tiles that hold them, or
+// up to three more, which may fill the last wave better.
 Shape8 pick_shape(int M, int N, int loads) {
-    const int tm = (M + 255) / 256, per = (M + tm - 1) / tm, sms = cmlb_num_sms();
-    const int nx = (per + 15) / 16 * 16, nx2 = (per + 31) / 32 * 32, tn = (N + CH - 1) / CH, tn2 = (N + 2 * CH - 1) / (2 * CH);
+    const int sms = cmlb_num_sms(), fewest = (M + 255) / 256;
     auto stage = [](int nx, int rows) { return fmax(fmax(4.0 * nx, BLOCKS * (A8 + rows * BK8) / 50.0), 600.0); };
     auto waves = [](long tiles, int at_once) { return (double)((tiles + at_once - 1) / at_once); };
-    Shape8 best = {nx, 1, false};
-    double least = waves((long)tm * tn, sms) * (loads * stage(nx, nx) + 3000);
-    for (int ranks = 2; ranks <= 8 && ranks <= loads; ranks *= 2) {
-        const int at_once = ranks == 2 ? sms / 2 : ranks == 4 ? sms * 33 / 148 : sms * 15 / 148;
-        const double cost = waves((long)tm * tn, at_once) * ((loads + ranks - 1) / ranks * stage(nx, nx) + 5000);
-        if (cost < least) { least = cost; best.ranks = ranks; }
+    const long tn = (N + CH - 1) / CH, tn2 = (N + 2 * CH - 1) / (2 * CH);
+    Shape8 best = {};
+    double least = 1e300;
+    for (int tm = fewest; tm <= fewest + 3; tm++) {
+        const int per = (M + tm - 1) / tm, nx = (per + 15) / 16 * 16, nx2 = (per + 31) / 32 * 32;
+        auto take = [&](double cost, const Shape8& s) { if (cost < least) { least = cost; best = s; } };
+        take(waves(tm * tn, sms) * (loads * stage(nx, nx) + 2000 + 8 * nx), {nx, 1, false});
+        take(waves(tm * tn2, sms / 2) * (loads * stage(nx2, nx2 / 2) + 2000 + 8 * nx2), {nx2, 1, true});
+        for (int ranks = 2; ranks <= 8 && ranks <= loads; ranks *= 2)
+            take(waves(tm * tn, ranks == 2 ? sms / 2 : ranks == 4 ? sms * 33 / 148 : sms * 15 / 148) * ((loads + ranks - 1) / ranks * stage(nx, nx) + 4000 + 16 * nx), {nx, ranks, false});
     }
-    const double cost = waves((long)tm * tn2, sms / 2) * (loads * stage(nx2, nx2 / 2) + 3000);
-    if (cost < least) best = {nx2, 1, true};
     return best;
 }
 
