@@ -10,17 +10,20 @@
 //
 // Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: largest value and sum of exponentials, fp32 in a thread and fp64 between threads (or, for
 // greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down, and draws over the one row (and the drafter's)
-// that counts: in fp32 first, then the CTA's candidates within what that can be off by again in fp64, so that which token is drawn does not hang on the order of anything.
+// that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
+// Few rows are bound by the chain of dependent loads and by code that is fetched anew with every launch (hence small loops, and what is seldom needed out of the way), many by memory.
 #include <type_traits>
 
 #include "lm_util.cuh"
 
 namespace {
 
-constexpr int VS_THREADS = 256, VT_THREADS = 512, VS_SPLITS = 16;
+constexpr int VS_THREADS = 256, VT_THREADS = 512, VS_SPLITS = 16, MOST_RANKS = 16;
 constexpr float kGreedy = 1e-5f;                       // colder is greedy
 
-struct Stat { float most; int at; double sum; };       // of a part of a row: largest value, its first place (greedy), sum of e^((x - most) / T)
+// Of a part of a row: largest value, its first place (greedy; otherwise the draft's logit), sum of e^((x - most) / T). A sum that is not a number: the part holds NaN or +inf
+struct Stat { float most; int at; float sum; int pad; };
+static_assert(VS_SPLITS <= 16, "a row's parts are put together by half a warp");
 
 struct Philox { uint32_t w[4]; };
 __device__ __forceinline__ Philox philox(uint64_t key, uint32_t c0, uint32_t c1) {
@@ -42,13 +45,19 @@ __device__ __forceinline__ float lg2(float v) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// log2 of -ln(1 - v), v = (word + 1/2) / 2^32, to about 1e-4: by the series where 1 - v has lost digits of v
-__device__ __forceinline__ float log_wait(uint32_t word) {
-    const float v = ((float)word + 0.5f) * 2.3283064365386963e-10f, rest = ((float)~word + 0.5f) * 2.3283064365386963e-10f;
-    return lg2(v < 0.0625f ? v * fmaf(v, fmaf(v, 0.33333334f, 0.5f), 1.f) : lg2(rest) * -0.6931471805599453f);
+// v = (word + 1/2) / 2^32 to 2^-24 of itself: halves of the word in the low bits of 2^23, which the conversion units have no part in
+__device__ __forceinline__ float uniform_of(uint32_t word) {
+    const float hi = __uint_as_float(__byte_perm(word, 0x4B00u, 0x5432)) - 8388608.f, lo = __uint_as_float(__byte_perm(word, 0x4B00u, 0x5410)) - 8388607.5f;
+    return fmaf(hi, 1.52587890625e-05f, lo * 2.3283064365386963e-10f);
 }
-// ln of the same
-__device__ __forceinline__ double log_wait_exact(uint32_t word) { return log(-log1p(-((double)word + 0.5) * 2.3283064365386963e-10)); }
+// -ln(1 - v), to about 1e-4 of itself: by the series where 1 - v has lost digits of v
+constexpr float kSeries = 0.0625f;
+__device__ __forceinline__ float short_wait(float v) { return v * fmaf(v, fmaf(v, 0.33333334f, 0.5f), 1.f); }
+__device__ __forceinline__ float long_wait(float v) { return lg2(fmaxf(1.f - v, 1.1641532e-10f)) * -0.6931471805599453f; }
+__device__ __noinline__ double far_log(double v) { return log(v); }
+__device__ __noinline__ double far_exp(double v) { return exp(v); }
+// ln of the same: 1 - v is exact in 64 bits
+__device__ __forceinline__ double log_wait_exact(uint32_t word) { return far_log(-far_log(((double)~word + 0.5) * 2.3283064365386963e-10)); }
 
 template <typename T> constexpr int kPer = 16 / (int)sizeof(T);
 template <typename T> __device__ __forceinline__ void widen_piece(const uint4& u, float (&x)[kPer<T>]) {
@@ -57,10 +66,11 @@ template <typename T> __device__ __forceinline__ void widen_piece(const uint4& u
 #pragma unroll
     for (int i = 0; i < kPer<T>; i++) x[i] = widen(t[i]);
 }
-// lowest place of the largest value; NaN (as such) above everything, so that a row with it is known
-__device__ __forceinline__ void better(float& v, int& at, float v2, int at2) {
-    if (v2 > v || (v2 == v && at2 < at)) { v = v2; at = at2; }
-}
+template <typename T> __device__ __forceinline__ T lowest();                 // a logit of a token that cannot come
+template <> __device__ __forceinline__ float lowest<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
+__device__ __forceinline__ float warp_max(float v) { float m; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v)); return m; }
 
 struct Verify {
     cmlb200_drafts d;
@@ -90,95 +100,142 @@ draft_stats_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     if (greedy && side) return;
     const T* row = side ? static_cast<const T*>(v.d.logits) + (size_t)i * v.d.ld : logits + (size_t)(i + s) * v.ld;
     constexpr int PER = kPer<T>;
-    const int V = v.vocab, head = min(V, (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T)), pieces = (V - head) / PER, tail = V - head - pieces * PER;
-    const int per = (pieces + splits - 1) / splits, lo = min(pieces, split * per), hi = min(pieces, lo + per);
-    const T* body = row + head;
+    // pieces of 16 bytes as they lie in memory; the first and the last may begin or end outside the row
+    const int V = v.vocab, lead = (int)(((uintptr_t)row & 15) / sizeof(T)), pieces = (lead + V + PER - 1) / PER, per = (pieces + splits - 1) / splits, lo = split * per, hi = min(pieces, lo + per);
     const float c = greedy ? 0.f : __fdiv_rn(kLog2e, heat);
     float most = -INFINITY, sum = 0.f;
     int at = 0;
-    auto raise = [&](float to) {
-        if (to > most) {
-            sum *= ex2((most - to) * c);               // (from -inf: 0 times 0)
-            most = to;
-        }
-    };
-    auto one = [&](float x, int place) {
-        if (greedy) {
-            if (x > most) { most = x; at = place; }
-            if (x != x) sum = x;
-        } else {
-            raise(x);
-            if (x != -INFINITY) sum += ex2((x - most) * c);
-        }
-    };
-    if (split == 0 && (int)threadIdx.x < head) one(widen(row[threadIdx.x]), threadIdx.x);
     constexpr int U = 4;
+#pragma unroll 1
     for (int p0 = lo + threadIdx.x; p0 < hi; p0 += U * VS_THREADS) {
         uint4 u[U];
 #pragma unroll
-        for (int j = 0; j < U; j++)
-            if (p0 + j * VS_THREADS < hi) u[j] = *reinterpret_cast<const uint4*>(body + (size_t)(p0 + j * VS_THREADS) * PER);
+        for (int j = 0; j < U; j++) {
+            const int e0 = (p0 + j * VS_THREADS) * PER - lead;
+            if (p0 + j * VS_THREADS >= hi) break;
+            if (e0 >= 0 && e0 + PER <= V) u[j] = *reinterpret_cast<const uint4*>(row + e0);
+            else {
+                T t[PER];
+#pragma unroll
+                for (int e = 0; e < PER; e++) t[e] = e0 + e >= 0 && e0 + e < V ? row[e0 + e] : lowest<T>();
+                memcpy(&u[j], t, 16);
+            }
+        }
+        if (greedy) {
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                if (p0 + j * VS_THREADS >= hi) break;
+                float x[PER];
+                widen_piece<T>(u[j], x);
+#pragma unroll
+                for (int e = 0; e < PER; e++) {
+                    if (x[e] > most) { most = x[e]; at = (p0 + j * VS_THREADS) * PER - lead + e; }
+                    if (x[e] != x[e]) sum = x[e];
+                }
+            }
+            continue;
+        }
 #pragma unroll
         for (int j = 0; j < U; j++) {
             if (p0 + j * VS_THREADS >= hi) break;
             float x[PER];
             widen_piece<T>(u[j], x);
-            if (greedy) {
+            float m = x[0];
 #pragma unroll
-                for (int e = 0; e < PER; e++) one(x[e], head + (p0 + j * VS_THREADS) * PER + e);
-            } else {
-                float m = x[0];
-#pragma unroll
-                for (int e = 1; e < PER; e++) m = fmaxf(m, x[e]);
-                raise(m);
-                const float ref = most == -INFINITY ? 0.f : most;          // (a NaN still shows)
-#pragma unroll
-                for (int e = 0; e < PER; e++) sum += ex2((x[e] - ref) * c);
+            for (int e = 1; e < PER; e++) m = fmaxf(m, x[e]);
+            if (m > most) {
+                sum *= ex2((most - m) * c);            // (from -inf: 0 times 0)
+                most = m;
             }
+            const float ref = most == -INFINITY ? 0.f : most;                  // (a NaN still shows)
+#pragma unroll
+            for (int e = 0; e < PER; e++) sum += ex2((x[e] - ref) * c);
         }
     }
-    if (split == splits - 1 && (int)threadIdx.x < tail) one(widen(body[(size_t)pieces * PER + threadIdx.x]), head + pieces * PER + threadIdx.x);
-    auto join = [&](Stat a, const Stat& b) {
-        Stat r = a;
-        better(r.most, r.at, b.most, b.at);
-        if (greedy) r.sum = a.sum + b.sum;
-        else r.sum = (a.most == -INFINITY ? a.sum : a.sum * (double)ex2((a.most - r.most) * c)) + (b.most == -INFINITY ? b.sum : b.sum * (double)ex2((b.most - r.most) * c));
-        return r;
+    // the warp's part, then the CTA's
+    auto together = [&]() {
+        const float top = warp_max(most);
+        if (greedy) {
+            at = (int)__reduce_min_sync(0xffffffffu, most == top ? (uint32_t)at : 0xffffffffu);
+        } else if (most > -INFINITY) sum *= ex2((most - top) * c);
+        most = top;
+        sum = lane_sum(sum);
     };
-    Stat a = {most, at, (double)sum};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const Stat b = {__shfl_xor_sync(0xffffffffu, a.most, o), __shfl_xor_sync(0xffffffffu, a.at, o), __shfl_xor_sync(0xffffffffu, a.sum, o)};
-        a = join(a, b);
-    }
-    if (lane == 0) parts[warp] = a;
+    together();
+    if (lane == 0) parts[warp] = {most, at, sum, 0};
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < VS_THREADS / 32; k++) a = join(a, parts[k]);
-        stats[((size_t)i * sides + side) * splits + split] = a;
+    if (warp) return;
+    const Stat mine_ = lane < VS_THREADS / 32 ? parts[lane] : Stat{-INFINITY, 0x7fffffff, 0.f, 0};
+    most = mine_.most;
+    at = mine_.at;
+    sum = mine_.sum;
+    together();
+    if (lane == 0) {
+        if (!greedy && split == 0) {
+            const int token = v.d.tokens[i];
+            at = __float_as_int(token >= 0 && token < V ? widen(row[token]) : -INFINITY);
+        }
+        stats[((size_t)i * sides + side) * splits + split] = {most, at, sum, 0};
     }
 }
 
-// A row's parts together. most = +inf or a sum that is not a number: no distribution
-__device__ __forceinline__ Stat whole_row(const Stat* parts, int splits, bool greedy, double rate) {
-    Stat a = parts[0];
-    for (int k = 1; k < splits; k++) better(a.most, a.at, parts[k].most, parts[k].at);
-    double sum = 0.0;
-    for (int k = 0; k < splits; k++)
-        sum += greedy || parts[k].most == -INFINITY ? parts[k].sum : parts[k].sum * exp(((double)parts[k].most - (double)a.most) * rate);
-    a.sum = sum;
-    return a;
+// What a draft was tested against, from the parts: the target's row by the lower half of a warp, the drafter's by the upper one
+struct Tested { Stat p, q; };
+__device__ __forceinline__ Tested tested(const Stat* parts, int sides, int splits, float c, bool greedy) {
+    const int lane = threadIdx.x & 31, side = lane >> 4, k = lane & 15;
+    Stat a = {-INFINITY, 0x7fffffff, 0.f, 0};
+    if (side < sides && k < splits) a = parts[side * splits + k];
+    float top = a.most;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    int at = greedy ? (a.most == top ? a.at : 0x7fffffff) : __shfl_sync(0xffffffffu, a.at, lane & 16);
+    float sum = greedy || a.most == -INFINITY ? a.sum : a.sum * ex2((a.most - top) * c);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (greedy) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+    }
+    return {{__shfl_sync(0xffffffffu, top, 0), __shfl_sync(0xffffffffu, at, 0), __shfl_sync(0xffffffffu, sum, 0), 0},
+            {__shfl_sync(0xffffffffu, top, 16), __shfl_sync(0xffffffffu, at, 16), __shfl_sync(0xffffffffu, sum, 16), 0}};
 }
 __device__ __forceinline__ bool holds(const Stat& a) { return a.most > -INFINITY && a.most < INFINITY && a.sum == a.sum; }
 
-// grid = sequences * ranks, clusters of `ranks` (up to 8)
+__device__ __forceinline__ void cluster_all() { asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The best of some tokens and the one behind it, as logarithms to the base 2 relative to a logit `ref` times c; the best's token, the lowest of equals
+struct Best { float z, z2, ref; int at, bad; };
+// of a warp's lanes together
+__device__ __forceinline__ Best best_of_lanes(Best b, float c) {
+    const float top = warp_max(b.ref), by = b.ref == top ? 0.f : (b.ref - top) * c;
+    const float z = b.z + by, most = warp_max(z);      // (-inf where there is nothing)
+    const int at = (int)__reduce_min_sync(0xffffffffu, z == most ? (uint32_t)b.at : 0xffffffffu);
+    const bool it = z == most && b.at == at;           // (a token is one lane's)
+    return {most, warp_max(fmaxf(it ? -INFINITY : z, b.z2 + by)), top, at, (int)__reduce_or_sync(0xffffffffu, (unsigned)b.bad)};
+}
+// logits of tokens 4 g .. 4 g + 3; whole: rows lie on boundaries of four
+template <typename T> __device__ __forceinline__ void load4(const T* row, int g, int vocab, bool whole, float (&x)[4]) {
+    if (whole && 4 * g + 4 <= vocab) {
+        T t[4];
+        if constexpr (sizeof(T) == 4) { const uint4 u = *reinterpret_cast<const uint4*>(row + 4 * (size_t)g); memcpy(t, &u, 16); }
+        else { const uint2 u = *reinterpret_cast<const uint2*>(row + 4 * (size_t)g); memcpy(t, &u, 8); }
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = widen(t[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = 4 * g + e < vocab ? widen(row[4 * (size_t)g + e]) : -INFINITY;
+    }
+}
+
+// grid = sequences * ranks, clusters of `ranks`
 template <typename T>
 __global__ void __launch_bounds__(VT_THREADS)
 draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int splits, const Stat* __restrict__ stats, int ranks, int* __restrict__ accepted, int* __restrict__ next) {
-    struct Best { double z; int at; int bad; };
     __shared__ int stop_at;
-    __shared__ float2 w_most[VT_THREADS / 32];
-    __shared__ Best w_best[VT_THREADS / 32], c_best[8];
+    __shared__ Best w_best[VT_THREADS / 32], c_best[MOST_RANKS];
+    __shared__ double x_best[VT_THREADS / 32 + MOST_RANKS];
+    __shared__ int x_at[VT_THREADS / 32 + MOST_RANKS];
+    constexpr int KEPT = 32;                           // drafts whose rows' parts are kept put together
+    __shared__ Tested kept_stats[KEPT];
     dep_trigger();
     dep_wait();
     const int rank = blockIdx.x % ranks, s = blockIdx.x / ranks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = v.vocab;
@@ -192,29 +249,22 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     const float heat = v.d.temperature ? v.d.temperature[s] : 1.f;
     const bool greedy = !(heat >= kGreedy);
     const double rate = greedy ? 0.0 : 1.0 / (double)heat;
+    const float c = greedy ? 0.f : __fdiv_rn(kLog2e, heat);
     const uint64_t key = v.d.random ? v.d.random[s] : 0ull;
     const int draft0 = first - s;
     if (threadIdx.x == 0) stop_at = n;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += VT_THREADS) {
+    for (int i = warp; i < n; i += VT_THREADS / 32) {          // a warp a draft
         const int token = v.d.tokens[draft0 + i];
-        bool kept = token >= 0 && token < V;
-        if (kept) {
-            const Stat* at = stats + (size_t)(draft0 + i) * sides * splits;
-            const Stat p = whole_row(at, splits, greedy, rate);
-            if (!holds(p)) kept = false;
-            else if (greedy) kept = p.at == token;
-            else {
-                const double chance = exp(((double)widen(logits[(size_t)(first + i) * v.ld + token]) - (double)p.most) * rate) / p.sum;
-                double q = 1.0;
-                if (sides > 1) {
-                    const Stat b = whole_row(at + splits, splits, false, rate);
-                    if (holds(b)) q = exp(((double)widen(static_cast<const T*>(v.d.logits)[(size_t)(draft0 + i) * v.d.ld + token]) - (double)b.most) * rate) / b.sum;
-                }
-                kept = (double)philox(key, (uint32_t)i >> 2, 1u).w[i & 3] * 2.3283064365386963e-10 * q < chance;
-            }
+        const Tested t = tested(stats + (size_t)(draft0 + i) * sides * splits, sides, splits, c, greedy);
+        if (i < KEPT && lane == 0) kept_stats[i] = t;
+        bool kept = token >= 0 && token < V && holds(t.p);
+        if (greedy) kept = kept && t.p.at == token;
+        else if (kept) {
+            const double q = sides > 1 && holds(t.q) ? far_exp(((double)__int_as_float(t.q.at) - (double)t.q.most) * rate) / (double)t.q.sum : 1.0;
+            kept = (double)philox(key, (uint32_t)i >> 2, 1u).w[i & 3] * 2.3283064365386963e-10 * q < far_exp(((double)__int_as_float(t.p.at) - (double)t.p.most) * rate) / (double)t.p.sum;
         }
-        if (!kept) atomicMin(&stop_at, i);
+        if (!kept && lane == 0) atomicMin(&stop_at, i);
     }
     __syncthreads();
     const int stop = stop_at;
@@ -222,109 +272,140 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     // what is taken off: the drafter's chances, or the draft itself
     const T* less = nullptr;
     int without = -1;
-    float p_most = 0.f, q_most = 0.f, p_unit = 1.f, q_unit = 0.f;
-    double p_sum = 1.0, q_sum = 1.0;
+    Tested t = {};
     if (stop < n && !greedy) {
-        const Stat* at = stats + (size_t)(draft0 + stop) * sides * splits;
         if (sides > 1) {
-            const Stat b = whole_row(at + splits, splits, false, rate);
-            if (holds(b)) {
-                const Stat p = whole_row(at, splits, false, rate);
-                less = static_cast<const T*>(v.d.logits) + (size_t)(draft0 + stop) * v.d.ld;
-                p_most = p.most; q_most = b.most;
-                p_sum = p.sum; q_sum = b.sum;
-                p_unit = (float)(1.0 / p.sum); q_unit = (float)(1.0 / b.sum);
-            }
+            t = stop < KEPT ? kept_stats[stop] : tested(stats + (size_t)(draft0 + stop) * sides * splits, sides, splits, c, greedy);
+            if (holds(t.q)) less = static_cast<const T*>(v.d.logits) + (size_t)(draft0 + stop) * v.d.ld;
         }
         if (!less) without = v.d.tokens[draft0 + stop];
     }
-    const float c = greedy ? 1.f : __fdiv_rn(kLog2e, heat);
+    const float p_unit = less ? 1.f / t.p.sum : 0.f, q_unit = less ? 1.f / t.q.sum : 0.f;
+    const bool whole = (((uintptr_t)row | (uintptr_t)less) & (4 * sizeof(T) - 1)) == 0;
     const int groups = (V + 3) / 4, per = (groups + ranks - 1) / ranks, lo = rank * per, hi = min(groups, lo + per);
+    bool first_time = true;
     for (int pass = 0;; pass++) {
-        // log2 of w / E of every token, and the thread's best. Where w is p alone: relative to the largest logit that the thread has met, so that logits far from zero lose no digits
-        float most = -INFINITY, ref = less || greedy ? 0.f : -INFINITY;
+        // The thread's best token: weight over wait, compared as products. Where w is p alone it is relative to the largest logit that the thread has met, so that logits far from zero lose no
+        // digits (greedy: the logit itself, waits of 1). Waits above kSeries are not worked out unless a token would win with that.
+        float best_w = greedy ? -INFINITY : 0.f, best_e = 1.f, ref = less || greedy ? 0.f : -INFINITY;
         int at = 0x7fffffff, bad = 0;
-        for (int g = lo + threadIdx.x; g < hi; g += VT_THREADS) {
-            Philox r;
-            if (!greedy) r = philox(key, (uint32_t)g, 0u);
+        constexpr int U = 2;                           // groups of four tokens under way
+#pragma unroll 1
+        for (int g0 = lo + threadIdx.x; g0 < hi; g0 += U * VT_THREADS) {
+            float x[U][4], y[U][4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = 4 * g + e;
-                if (j >= V) break;
-                const float x = widen(row[j]);
-                if (!(x < INFINITY)) bad = 1;
-                float z;
-                if (greedy) z = x;
-                else if (less) {
-                    const float w = ex2((x - p_most) * c) * p_unit - ex2((widen(less[j]) - q_most) * c) * q_unit;
-                    z = w > 0.f ? lg2(w) - log_wait(r.w[e]) : -INFINITY;
-                } else {
-                    if (x > ref) {
-                        most += (ref - x) * c;         // (nothing yet: -inf)
-                        ref = x;
-                    }
-                    z = j == without ? -INFINITY : (x - ref) * c - log_wait(r.w[e]);           // (-inf beside -inf: NaN, which is never the best)
+            for (int k = 0; k < U; k++)
+                if (g0 + k * VT_THREADS < hi) {
+                    load4(row, g0 + k * VT_THREADS, V, whole, x[k]);
+                    if (less) load4(less, g0 + k * VT_THREADS, V, whole, y[k]);
                 }
-                if (z > most) { most = z; at = j; }
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int g = g0 + k * VT_THREADS;
+                if (g >= hi) break;
+                Philox r;
+                if (!greedy) r = philox(key, (uint32_t)g, 0u);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = 4 * g + e;
+                    const float xe = x[k][e];
+                    if (!(xe < INFINITY)) bad = 1;
+                    if (greedy) {
+                        if (xe > best_w) { best_w = xe; at = j; }
+                        continue;
+                    }
+                    float w;
+                    if (less) w = ex2((xe - t.p.most) * c) * p_unit - ex2((y[k][e] - t.q.most) * c) * q_unit;
+                    else {
+                        if (j == without) continue;
+                        if (xe > ref) {
+                            best_w *= ex2((ref - xe) * c);             // (nothing yet: 0 times 0)
+                            ref = xe;
+                        }
+                        w = ex2((xe - ref) * c);  // (-inf beside -inf: NaN, which is never the best)
+                    }
+                    const float u = uniform_of(r.w[e]);
+                    float wait = u < kSeries ? short_wait(u) : kSeries;
+                    if (w * best_e > best_w * wait) {
+                        if (!(u < kSeries)) wait = long_wait(u);
+                        if (w * best_e > best_w * wait) { best_w = w; best_e = wait; at = j; }
+                    }
+                }
             }
         }
-        auto raise = [&](float& r, float& m, float r2, float m2) {
-            const float top = fmaxf(r, r2);
-            m = fmaxf(m > -INFINITY ? m + (r - top) * c : m, m2 > -INFINITY ? m2 + (r2 - top) * c : m2);
-            r = top;
+        const float most = greedy ? best_w : at == 0x7fffffff ? -INFINITY : lg2(best_w) - lg2(best_e);
+        // CTA and cluster have the best and the one behind it
+        const Best b = {most, -INFINITY, ref, at, bad};
+        auto best_of = [&](Best x) {
+            x = best_of_lanes(x, c);
+            if (lane == 0) w_best[warp] = x;
+            if (first_time) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+            first_time = false;
+            __syncthreads();
+            const Best none = {-INFINITY, -INFINITY, less || greedy ? 0.f : -INFINITY, 0x7fffffff, 0};
+            if (warp == 0) {
+                x = best_of_lanes(lane < VT_THREADS / 32 ? w_best[lane] : none, c);
+                if (lane < ranks) {
+                    const uint32_t dst = cluster_addr(&c_best[rank], lane);
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(x.z) : "memory");
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(x.z2) : "memory");
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(x.ref) : "memory");
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 12), "r"(x.at) : "memory");
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 16), "r"(x.bad) : "memory");
+                }
+            }
+            cluster_all();
+            return best_of_lanes(lane < ranks ? c_best[lane] : none, c);
         };
-        float top = ref, m = most;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) raise(top, m, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) w_most[warp] = make_float2(top, m);
-        __syncthreads();
-        top = w_most[0].x;
-        m = w_most[0].y;
-#pragma unroll
-        for (int k = 1; k < VT_THREADS / 32; k++) raise(top, m, w_most[k].x, w_most[k].y);
-        // candidates again, in 64 bits
-        Best b = {-INFINITY, at, bad};
-        if (most > -INFINITY) {
-            if (greedy) b.z = (double)most;
-            else if (most + (ref - top) * c >= m - (2e-3f + fabsf(m) * 1e-5f)) {
-                double w;
-                if (less) {
-                    const double d = exp(((double)widen(row[at]) - (double)p_most) * rate) / p_sum - exp(((double)widen(less[at]) - (double)q_most) * rate) / q_sum;
-                    w = d > 0.0 ? log(d) : -1e30;              // (what 32 bits took for a weight was their rounding)
-                } else w = (double)widen(row[at]) * rate;
-                b.z = w - log_wait_exact(philox(key, (uint32_t)at >> 2, 0u).w[at & 3]);
+        // the same in 64 bits, over the whole cluster (seldom): warp by warp, then CTA by CTA
+        auto exact_best = [&](double z, int token, Best old) {
+            for (int level = 0; level < 3; level++) {
+#pragma unroll 1
+                for (int o = 16; o > 0; o >>= 1) {
+                    const double z2 = __shfl_xor_sync(0xffffffffu, z, o);
+                    const int t2 = __shfl_xor_sync(0xffffffffu, token, o);
+                    if (z2 > z || (z2 == z && t2 < token)) { z = z2; token = t2; }
+                }
+                if (level == 2) break;
+                if (level == 0) {
+                    if (lane == 0) { x_best[warp] = z; x_at[warp] = token; }
+                    __syncthreads();
+                    z = lane < VT_THREADS / 32 ? x_best[lane] : -INFINITY;
+                    token = lane < VT_THREADS / 32 ? x_at[lane] : 0x7fffffff;
+                } else {
+                    __syncthreads();                   // (everyone has read the warps')
+                    if (warp == 0 && lane < ranks) {
+                        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&x_best[VT_THREADS / 32 + rank], lane)), "d"(z) : "memory");
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&x_at[VT_THREADS / 32 + rank], lane)), "r"(token) : "memory");
+                    }
+                    cluster_all();
+                    z = lane < ranks ? x_best[VT_THREADS / 32 + lane] : -INFINITY;
+                    token = lane < ranks ? x_at[VT_THREADS / 32 + lane] : 0x7fffffff;
+                }
             }
-        }
-        auto join = [](Best& a, const Best& o) {
-            if (o.z > a.z || (o.z == a.z && o.at < a.at)) { a.z = o.z; a.at = o.at; }
-            a.bad |= o.bad;
+            old.at = token;
+            return old;
         };
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Best x = {__shfl_xor_sync(0xffffffffu, b.z, o), __shfl_xor_sync(0xffffffffu, b.at, o), __shfl_xor_sync(0xffffffffu, b.bad, o)};
-            join(b, x);
-        }
-        if (lane == 0) w_best[warp] = b;
-        if (pass == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        __syncthreads();
-        if (warp == 0) {
-            b = lane < VT_THREADS / 32 ? w_best[lane] : Best{-INFINITY, 0x7fffffff, 0};
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) {
-                const Best x = {__shfl_xor_sync(0xffffffffu, b.z, o), __shfl_xor_sync(0xffffffffu, b.at, o), __shfl_xor_sync(0xffffffffu, b.bad, o)};
-                join(b, x);
-            }
-            // every CTA of the cluster learns of every one's best
-            if (lane < ranks) {
-                const uint32_t dst = cluster_addr(&c_best[rank], lane);
-                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst), "d"(b.z) : "memory");
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 8), "r"(b.at) : "memory");
-                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 12), "r"(b.bad) : "memory");
+        Best all = best_of(b);
+        if (!greedy && !all.bad && all.z > -INFINITY) {
+            // What 32 bits are off by at most: 1e-4 of the waits, 1e-5 of logarithms and of products with c (tokens near the best lie within 64 of it). The difference of p and q may lose more
+            // where the two are close; such tokens are seldom drawn. All CTAs know the same: they decide together.
+            constexpr float slack = 1e-3f;
+            if (all.z2 >= all.z - slack) {             // (one call in a thousand)
+                cluster_all();                         // everyone has read what comes now is written over
+                const bool close = most > -INFINITY && most + (ref == all.ref ? 0.f : (ref - all.ref) * c) >= all.z - slack;
+                double z = -INFINITY;
+                if (close) {
+                    double w;
+                    if (less) {
+                        const double d = far_exp(((double)widen(row[at]) - (double)t.p.most) * rate) / (double)t.p.sum - far_exp(((double)widen(less[at]) - (double)t.q.most) * rate) / (double)t.q.sum;
+                        w = d > 0.0 ? far_log(d) : -1e30;      // (what 32 bits took for a weight was their rounding)
+                    } else w = ((double)widen(row[at]) - (double)all.ref) * rate;
+                    z = w - log_wait_exact(philox(key, (uint32_t)at >> 2, 0u).w[at & 3]);
+                }
+                all = exact_best(z, at, all);
             }
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        Best all = c_best[0];
-        for (int k = 1; k < ranks; k++) join(all, c_best[k]);
         // where rounding leaves nothing of p - q (or p is nothing but the draft), p itself
         const bool again = pass == 0 && !all.bad && all.z == -INFINITY && (less || without >= 0);
         if (!again) {
@@ -336,7 +417,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
         }
         less = nullptr;
         without = -1;
-        asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody reads what the next pass writes
+        cluster_all();                                 // nobody reads what the next pass writes
     }
 }
 
@@ -348,8 +429,17 @@ int launch_verify(const Verify& v, const void* logits, int* accepted, int* next,
     while (splits < VS_SPLITS && (long)drafts * sides * splits * 2 <= 4l * cmlb_num_sms() && (size_t)v.vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
     if (drafts)
         CMLB_CUDA(launch_chain(draft_stats_kernel<T>, dim3((unsigned)((long)drafts * sides * splits)), dim3(VS_THREADS), 0, 1, st, v, static_cast<const T*>(logits), sides, splits, stats));
+    // as many CTAs a sequence as find an SM each, but 2,048 tokens at least
     int ranks = 1;
-    while (ranks < 8 && (long)v.d.sequences * ranks * 2 <= 2l * cmlb_num_sms() && v.vocab > ranks * 2048) ranks *= 2;
+    while (ranks < MOST_RANKS && (long)v.d.sequences * ranks * 2 <= (ranks < 8 ? 2l * cmlb_num_sms() : cmlb_num_sms() / 2) && v.vocab > ranks * 2048) ranks *= 2;
+    if (ranks > 8) {
+        static bool allowed[kMaxDevices] = {};
+        const int dev = cmlb_device_index();
+        if (!allowed[dev]) {
+            CMLB_CUDA(cudaFuncSetAttribute(draft_token_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            allowed[dev] = true;
+        }
+    }
     CMLB_CUDA(launch_chain(draft_token_kernel<T>, dim3((unsigned)(v.d.sequences * ranks)), dim3(VT_THREADS), 0, ranks, st, v, static_cast<const T*>(logits), sides, splits, (const Stat*)stats, ranks,
                            accepted, next));
     return CMLB200_OK;

@@ -110,10 +110,46 @@ def test_defaults(pkg, torch_dev):
 
 
 @pytest.mark.parametrize("spread,temperature", [(0.0, 1.0), (0.01, 1.0), (30.0, 1.0), (300.0, 1.0), (2.0, 0.01), (2.0, 1e-4), (2.0, 100.0), (2.0, 9e-6), (2.0, -1.0)])
-def test_flat_and_steep(pkg, torch_dev, spread, temperature):
+@pytest.mark.parametrize("drafter", [True, False])
+def test_flat_and_steep(pkg, torch_dev, spread, temperature, drafter):
     import torch
-    b = Batch(torch, torch_dev, [3, 0, 1, 2] * 5, 3001, 17, temperatures=(temperature,), spread=spread, gap=0.2 * spread)
+    b = Batch(torch, torch_dev, [3, 0, 1, 2] * 5, 3001, 17, drafter=drafter, temperatures=(temperature,), spread=spread, gap=0.2 * spread)
     b.check(b.call(pkg), most_unsure=0.3)
+
+
+def test_far_from_zero(pkg, torch_dev):
+    """Logits that share a large offset lose no digits beyond their own."""
+    import torch
+    b = Batch(torch, torch_dev, [2, 0, 1] * 5, 2000, 71, gap=0.3)
+    b.target += 4096.0
+    b.draft += 1024.0
+    b.check(b.call(pkg), most_unsure=0.2)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 3, 4, 5, 6, 7, 9])
+def test_few_tokens(pkg, torch_dev, vocab):
+    """Waits of all lengths: with one token every one of them wins."""
+    import torch
+    b = Batch(torch, torch_dev, [0] * 3000, vocab, 73 + vocab, spread=0.3)
+    b.check(b.call(pkg))
+
+
+def test_close_calls(pkg, torch_dev):
+    """Tokens whose weights over waits differ by less than 32 bits tell apart: the 64-bit comparison decides. Logits are waits' logarithms, so that all tokens come out nearly equal."""
+    import torch
+    b = Batch(torch, torch_dev, [0] * 64, 1500, 79)
+    rng = np.random.default_rng(9)
+    for s in range(64):
+        z = np.log(drafts_oracle.waits(int(b.key[s]), 1500))
+        keep = rng.permutation(1500)[:40]
+        row = np.full(1500, -40.0)
+        row[keep] = z[keep] + rng.normal(size=40) * 2e-5
+        b.target[s] = torch.from_numpy(row).float()
+    got = b.call(pkg)
+    x = b.target.double().cpu().numpy()
+    for s in range(64):
+        z = x[s] - np.log(drafts_oracle.waits(int(b.key[s]), 1500))
+        assert got[0][s] == 0 and got[1][s] == int(np.argmax(z)), (s, np.sort(z)[-3:], z[got[1][s]])
 
 
 def test_same_logits(pkg, torch_dev):
