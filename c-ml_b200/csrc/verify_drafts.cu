@@ -20,6 +20,7 @@ namespace {
 
 constexpr int VS_THREADS = 256, VT_THREADS = 512, VS_SPLITS = 16, MOST_RANKS = 16;
 constexpr float kGreedy = 1e-5f;                       // colder is greedy
+constexpr float kClose = 0.998f;
 
 // Of a part of a row: largest value, its first place (greedy; otherwise the draft's logit), sum of e^((x - most) / T). A sum that is not a number: the part holds NaN or +inf
 struct Stat { float most; int at; float sum; int pad; };
@@ -50,10 +51,9 @@ __device__ __forceinline__ float uniform_of(uint32_t word) {
     const float hi = __uint_as_float(__byte_perm(word, 0x4B00u, 0x5432)) - 8388608.f, lo = __uint_as_float(__byte_perm(word, 0x4B00u, 0x5410)) - 8388607.5f;
     return fmaf(hi, 1.52587890625e-05f, lo * 2.3283064365386963e-10f);
 }
-// -ln(1 - v), to about 1e-4 of itself: by the series where 1 - v has lost digits of v
-constexpr float kSeries = 0.0625f;
-__device__ __forceinline__ float short_wait(float v) { return v * fmaf(v, fmaf(v, 0.33333334f, 0.5f), 1.f); }
-__device__ __forceinline__ float long_wait(float v) { return lg2(fmaxf(1.f - v, 1.1641532e-10f)) * -0.6931471805599453f; }
+// -ln(1 - v): the first terms of its series, which are never above it, and to about 1e-4 of itself
+__device__ __forceinline__ float least_wait(float v) { return v * fmaf(v, fmaf(v, 0.33333334f, 0.5f), 1.f); }
+__device__ __forceinline__ float wait_of(float v) { return v < 0.0625f ? least_wait(v) : lg2(fmaxf(1.f - v, 1.1641532e-10f)) * -0.6931471805599453f; }
 __device__ __noinline__ double far_log(double v) { return log(v); }
 __device__ __noinline__ double far_exp(double v) { return exp(v); }
 // ln of the same: 1 - v is exact in 64 bits
@@ -212,6 +212,10 @@ __device__ __forceinline__ Best best_of_lanes(Best b, float c) {
     const bool it = z == most && b.at == at;           // (a token is one lane's)
     return {most, warp_max(fmaxf(it ? -INFINITY : z, b.z2 + by)), top, at, (int)__reduce_or_sync(0xffffffffu, (unsigned)b.bad)};
 }
+// the largest of four but number `but`
+__device__ __forceinline__ float most_but(const float (&x)[4], int but) {
+    return fmaxf(fmaxf(but == 0 ? -INFINITY : x[0], but == 1 ? -INFINITY : x[1]), fmaxf(but == 2 ? -INFINITY : x[2], but == 3 ? -INFINITY : x[3]));
+}
 // logits of tokens 4 g .. 4 g + 3; whole: rows lie on boundaries of four
 template <typename T> __device__ __forceinline__ void load4(const T* row, int g, int vocab, bool whole, float (&x)[4]) {
     if (whole && 4 * g + 4 <= vocab) {
@@ -285,55 +289,74 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     const int groups = (V + 3) / 4, per = (groups + ranks - 1) / ranks, lo = rank * per, hi = min(groups, lo + per);
     bool first_time = true;
     for (int pass = 0;; pass++) {
-        // The thread's best token: weight over wait, compared as products. Where w is p alone it is relative to the largest logit that the thread has met, so that logits far from zero lose no
-        // digits (greedy: the logit itself, waits of 1). Waits above kSeries are not worked out unless a token would win with that.
-        float best_w = greedy ? -INFINITY : 0.f, best_e = 1.f, ref = less || greedy ? 0.f : -INFINITY;
-        int at = 0x7fffffff, bad = 0;
+        // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with the least that its wait can be is looked at; there are
+        // few, and only for those a wait is worked out. Where w is p alone it is relative to the largest logit that the warp has met, so that logits far from zero lose no digits (greedy: the logits
+        // themselves).
+        float best = greedy ? -INFINITY : 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY, seen = 0.f;
+        int at = 0x7fffffff;
         constexpr int U = 2;                           // groups of four tokens under way
 #pragma unroll 1
-        for (int g0 = lo + threadIdx.x; g0 < hi; g0 += U * VT_THREADS) {
+        for (int g0 = lo + warp * 32; g0 < hi; g0 += U * VT_THREADS) {
             float x[U][4], y[U][4];
 #pragma unroll
-            for (int k = 0; k < U; k++)
-                if (g0 + k * VT_THREADS < hi) {
-                    load4(row, g0 + k * VT_THREADS, V, whole, x[k]);
-                    if (less) load4(less, g0 + k * VT_THREADS, V, whole, y[k]);
-                }
+            for (int k = 0; k < U; k++) {
+                const int g = g0 + k * VT_THREADS + lane;
+                load4(row, g < hi ? g : groups, V, whole, x[k]);               // (behind the end: -inf)
+                if (less) load4(less, g < hi ? g : groups, V, whole, y[k]);
+            }
 #pragma unroll
             for (int k = 0; k < U; k++) {
-                const int g = g0 + k * VT_THREADS;
-                if (g >= hi) break;
-                Philox r;
-                if (!greedy) r = philox(key, (uint32_t)g, 0u);
+                const int g = g0 + k * VT_THREADS + lane;
+                const float most = fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3]));
+                if (greedy) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (!(x[k][e] < INFINITY)) seen = NAN;
+                        if (x[k][e] > best) { best = x[k][e]; at = 4 * g + e; }
+                    }
+                    continue;
+                }
+                const Philox r = philox(key, (uint32_t)g, 0u);
+                float w[4], u[4];
+                if (less) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - t.p.most) * c) * p_unit - ex2((y[k][e] - t.q.most) * c) * q_unit;
+                } else {
+                    const float top = (uint32_t)(without - 4 * g) < 4u ? most_but(x[k], without - 4 * g) : most;          // (the draft that was turned down sets no reference)
+                    if (__any_sync(0xffffffffu, top > ref)) {
+                        const float to = fmaxf(ref, warp_max(top)), by = ref == -INFINITY ? 0.f : ex2((ref - to) * c);
+                        best *= by;
+                        bound *= by;
+                        ref = to;
+                    }
+                    const float from = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - from) * c);
+                    seen += w[0] * 0.f + w[1] * 0.f;
+                    seen += w[2] * 0.f + w[3] * 0.f;
+                    if ((uint32_t)(without - 4 * g) < 4u) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) if (4 * g + e == without) w[e] = 0.f;
+                    }
+                }
+                bool any = false;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int j = 4 * g + e;
-                    const float xe = x[k][e];
-                    if (!(xe < INFINITY)) bad = 1;
-                    if (greedy) {
-                        if (xe > best_w) { best_w = xe; at = j; }
-                        continue;
+                    u[e] = uniform_of(r.w[e]);
+                    any |= w[e] > bound * kClose * least_wait(u[e]);
+                }
+                if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float score = w[e] > 0.f ? __fdividef(w[e], wait_of(u[e])) : 0.f;
+                        if (score > best) { best = score; at = 4 * g + e; }
                     }
-                    float w;
-                    if (less) w = ex2((xe - t.p.most) * c) * p_unit - ex2((y[k][e] - t.q.most) * c) * q_unit;
-                    else {
-                        if (j == without) continue;
-                        if (xe > ref) {
-                            best_w *= ex2((ref - xe) * c);             // (nothing yet: 0 times 0)
-                            ref = xe;
-                        }
-                        w = ex2((xe - ref) * c);  // (-inf beside -inf: NaN, which is never the best)
-                    }
-                    const float u = uniform_of(r.w[e]);
-                    float wait = u < kSeries ? short_wait(u) : kSeries;
-                    if (w * best_e > best_w * wait) {
-                        if (!(u < kSeries)) wait = long_wait(u);
-                        if (w * best_e > best_w * wait) { best_w = w; best_e = wait; at = j; }
-                    }
+                    bound = warp_max(best);
                 }
             }
         }
-        const float most = greedy ? best_w : at == 0x7fffffff ? -INFINITY : lg2(best_w) - lg2(best_e);
+        const float most = greedy ? best : best > 0.f ? lg2(best) : -INFINITY;
+        const int bad = seen != seen;
         // CTA and cluster have the best and the one behind it
         const Best b = {most, -INFINITY, ref, at, bad};
         auto best_of = [&](Best x) {
@@ -426,7 +449,7 @@ int launch_verify(const Verify& v, const void* logits, int* accepted, int* next,
     const int drafts = v.d.rows - v.d.sequences, sides = v.d.logits ? 2 : 1;
     Stat* stats = static_cast<Stat*>(work);
     int splits = 1;
-    while (splits < VS_SPLITS && (long)drafts * sides * splits * 2 <= 4l * cmlb_num_sms() && (size_t)v.vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
+    while (splits < VS_SPLITS && (long)drafts * sides * splits * 2 <= 8l * cmlb_num_sms() && (size_t)v.vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
     if (drafts)
         CMLB_CUDA(launch_chain(draft_stats_kernel<T>, dim3((unsigned)((long)drafts * sides * splits)), dim3(VS_THREADS), 0, 1, st, v, static_cast<const T*>(logits), sides, splits, stats));
     // as many CTAs a sequence as find an SM each, but 2,048 tokens at least
