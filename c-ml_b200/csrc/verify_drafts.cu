@@ -46,11 +46,8 @@ __device__ __forceinline__ float lg2(float v) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// v = (word + 1/2) / 2^32 to 2^-24 of itself: halves of the word in the low bits of 2^23, which the conversion units have no part in
-__device__ __forceinline__ float uniform_of(uint32_t word) {
-    const float hi = __uint_as_float(__byte_perm(word, 0x4B00u, 0x5432)) - 8388608.f, lo = __uint_as_float(__byte_perm(word, 0x4B00u, 0x5410)) - 8388607.5f;
-    return fmaf(hi, 1.52587890625e-05f, lo * 2.3283064365386963e-10f);
-}
+// v = (word + 1/2) / 2^32 to 2^-23 of itself
+__device__ __forceinline__ float uniform_of(uint32_t word) { return fmaf((float)word, 2.3283064365386963e-10f, 1.1641532e-10f); }
 // -ln(1 - v): the first terms of its series, which are never above it, and to about 1e-4 of itself
 __device__ __forceinline__ float least_wait(float v) { return v * fmaf(v, fmaf(v, 0.33333334f, 0.5f), 1.f); }
 __device__ __forceinline__ float wait_of(float v) { return v < 0.0625f ? least_wait(v) : lg2(fmaxf(1.f - v, 1.1641532e-10f)) * -0.6931471805599453f; }
@@ -70,6 +67,7 @@ template <typename T> __device__ __forceinline__ T lowest();                 // 
 template <> __device__ __forceinline__ float lowest<float>() { return -INFINITY; }
 template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
 template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
+__device__ __forceinline__ float max_nan(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
 __device__ __forceinline__ float warp_max(float v) { float m; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v)); return m; }
 
 struct Verify {
@@ -254,7 +252,9 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     const bool greedy = !(heat >= kGreedy);
     const double rate = greedy ? 0.0 : 1.0 / (double)heat;
     const float c = greedy ? 0.f : __fdiv_rn(kLog2e, heat);
-    const uint64_t key = v.d.random ? v.d.random[s] : 0ull;
+    uint64_t key = v.d.random ? v.d.random[s] : 0ull;
+    // (known to be the same for a warp: its multiples stay in uniform registers)
+    key = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(key >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)key);
     const int draft0 = first - s;
     if (threadIdx.x == 0) stop_at = n;
     __syncthreads();
@@ -292,8 +292,8 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
         // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with the least that its wait can be is looked at; there are
         // few, and only for those a wait is worked out. Where w is p alone it is relative to the largest logit that the warp has met, so that logits far from zero lose no digits (greedy: the logits
         // themselves).
-        float best = greedy ? -INFINITY : 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY, seen = 0.f;
-        int at = 0x7fffffff;
+        float best = greedy ? -INFINITY : 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
+        int at = 0x7fffffff, bad = 0;
         constexpr int U = 2;                           // groups of four tokens under way
 #pragma unroll 1
         for (int g0 = lo + warp * 32; g0 < hi; g0 += U * VT_THREADS) {
@@ -307,11 +307,11 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
 #pragma unroll
             for (int k = 0; k < U; k++) {
                 const int g = g0 + k * VT_THREADS + lane;
-                const float most = fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3]));
+                const float most = max_nan(max_nan(x[k][0], x[k][1]), max_nan(x[k][2], x[k][3]));
+                bad |= !(most < INFINITY);
                 if (greedy) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        if (!(x[k][e] < INFINITY)) seen = NAN;
                         if (x[k][e] > best) { best = x[k][e]; at = 4 * g + e; }
                     }
                     continue;
@@ -332,8 +332,6 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
                     const float from = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
                     for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - from) * c);
-                    seen += w[0] * 0.f + w[1] * 0.f;
-                    seen += w[2] * 0.f + w[3] * 0.f;
                     if ((uint32_t)(without - 4 * g) < 4u) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) if (4 * g + e == without) w[e] = 0.f;
@@ -356,7 +354,6 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
             }
         }
         const float most = greedy ? best : best > 0.f ? lg2(best) : -INFINITY;
-        const int bad = seen != seen;
         // CTA and cluster have the best and the one behind it
         const Best b = {most, -INFINITY, ref, at, bad};
         auto best_of = [&](Best x) {
@@ -449,7 +446,7 @@ int launch_verify(const Verify& v, const void* logits, int* accepted, int* next,
     const int drafts = v.d.rows - v.d.sequences, sides = v.d.logits ? 2 : 1;
     Stat* stats = static_cast<Stat*>(work);
     int splits = 1;
-    while (splits < VS_SPLITS && (long)drafts * sides * splits * 2 <= 8l * cmlb_num_sms() && (size_t)v.vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
+    while (splits < VS_SPLITS && (long)drafts * sides * splits * 2 <= (sizeof(T) == 4 ? 8l : 4l) * cmlb_num_sms() && (size_t)v.vocab * sizeof(T) > (size_t)splits * 8192) splits *= 2;
     if (drafts)
         CMLB_CUDA(launch_chain(draft_stats_kernel<T>, dim3((unsigned)((long)drafts * sides * splits)), dim3(VS_THREADS), 0, 1, st, v, static_cast<const T*>(logits), sides, splits, stats));
     // as many CTAs a sequence as find an SM each, but 2,048 tokens at least
