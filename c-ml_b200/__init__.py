@@ -434,6 +434,7 @@ DT_F32, DT_BF16, DT_F16, DT_I8, DT_E4M3 = 0, 1, 2, 3, 4
 ACT_SILU, ACT_GELU_TANH, ACT_CLAMPED, ACT_GELU_ERF = 0, 1, 2, 3
 DTYPE_FLOAT32, DTYPE_BFLOAT16 = 0, 6
 CACHE_DEFAULT, CACHE_INT8, CACHE_E4M3 = 0, 1, 2
+WEIGHTS_DEFAULT, WEIGHTS_INT8 = 0, 1
 
 
 class Dense(C.Structure):
@@ -508,7 +509,7 @@ class Drafts(C.Structure):
 
 
 class LMOptions(C.Structure):
-    _fields_ = [("dtype", ci), ("max_tokens", ci), ("max_sequences", ci), ("max_step_rows", ci), ("cache", ci)]
+    _fields_ = [("dtype", ci), ("max_tokens", ci), ("max_sequences", ci), ("max_step_rows", ci), ("cache", ci), ("weights", ci)]
 
 
 class LMEntry(C.Structure):
@@ -593,11 +594,16 @@ _sig("cml_lm_step_greedy", ci, vp, C.POINTER(LMEntry), ci, vp)
 _sig("cml_lm_sequence_fork", ci, vp, ci)
 _sig("cml_lm_compact", ci, vp)
 _sig("cml_lm_step_scored", ci, vp, C.POINTER(LMEntry), ci, vp, ci, vp, vp, vp, vp)
+_sig("cml_lm_sequence_truncate", ci, vp, ci, ci)
+_sig("cml_lm_step_sampled", ci, vp, C.POINTER(LMEntry), ci, vp, vp, vp)
+_sig("cml_lm_step_verified", ci, vp, C.POINTER(LMEntry), ci, vp, vp, vp, vp)
+_sig("cml_paged_cache_truncate", ci, C.POINTER(PagedKVCache), ci, ci)
 _sig("cml_paged_cache_fork", ci, C.POINTER(PagedKVCache), ci, C.POINTER(ci), C.POINTER(ci))
 _sig("cml_paged_cache_compact", ci, C.POINTER(PagedKVCache), vp)
 _sig("cml_lm_decode_greedy", ci, vp, vp, vp, ci, ci, vp, C.POINTER(C.c_float))
 _sig("cml_serving_run_lm", ci, vp, vp, C.POINTER(GenerationConfig), ci, vp, vp)
 _sig("cml_lm_generate", C.POINTER(GenerationResult), vp, vp, ci, C.POINTER(GenerationConfig))
+_sig("cml_lm_generate_drafted", C.POINTER(GenerationResult), vp, vp, ci, vp, ci, C.POINTER(GenerationConfig), C.c_uint64, vp)
 _sig("cml_paged_kv_cache_create_device", C.POINTER(PagedKVCache), ci, ci, ci)
 _sig("cml_paged_cache_blocks_for", ci, C.POINTER(PagedKVCache), ci, ci)
 _sig("cml_paged_cache_extend", ci, C.POINTER(PagedKVCache), ci, ci)
@@ -608,8 +614,8 @@ _sig("cml_paged_cache_release_between", None, C.POINTER(PagedKVCache), ci, ci, c
 class LanguageModel:
     """A model loaded through cml_lm_load, with numpy arrays in and out."""
 
-    def __init__(self, path, dtype=DTYPE_BFLOAT16, max_tokens=2048, max_sequences=8, max_step_rows=0, cache=CACHE_DEFAULT):
-        self.h = lib.cml_lm_load(str(path).encode(), C.byref(LMOptions(dtype, max_tokens, max_sequences, max_step_rows, cache)))
+    def __init__(self, path, dtype=DTYPE_BFLOAT16, max_tokens=2048, max_sequences=8, max_step_rows=0, cache=CACHE_DEFAULT, weights=WEIGHTS_DEFAULT):
+        self.h = lib.cml_lm_load(str(path).encode(), C.byref(LMOptions(dtype, max_tokens, max_sequences, max_step_rows, cache, weights)))
         if not self.h:
             raise CmlB200Error(f"cml_lm_load({path}) failed")
         self.vocab = lib.cml_lm_vocab_size(self.h)
@@ -654,6 +660,49 @@ class LanguageModel:
         check(lib.cml_lm_step_scored(self.h, arr, len(entries), None if tg is None else np_ptr(tg), top, None if tg is None else np_ptr(lp), np_ptr(en), np_ptr(ids) if top else None,
                                      np_ptr(best) if top else None), "cml_lm_step_scored")
         return (None if tg is None else lp), en, ids, best
+
+    def truncate(self, seq, length):
+        check(lib.cml_lm_sequence_truncate(self.h, seq, length), "cml_lm_sequence_truncate")
+
+    def _drawn(self, entries, temperatures, random, n):
+        import numpy as np
+        keep = [(np.ascontiguousarray(t, np.int32).ravel(), np.arange(len(t), dtype=np.int32) if w is None else np.ascontiguousarray(w, np.int32).ravel()) for _, t, w in entries]
+        arr = (LMEntry * len(entries))(*(LMEntry(seq, t.ctypes.data, len(t), w.ctypes.data, len(w)) for (seq, _, _), (t, w) in zip(entries, keep)))
+        n = sum(len(w) for _, w in keep) if n is None else n
+        heat = None if temperatures is None else np.ascontiguousarray(np.broadcast_to(np.asarray(temperatures, np.float32), n))
+        rnd = None if random is None else np.ascontiguousarray(random, np.uint64)
+        if rnd is not None and rnd.size != n:
+            raise CmlB200Error(f"{rnd.size} random numbers for {n} draws")
+        return arr, keep, heat, rnd, n
+
+    def sampled(self, entries, temperatures=None, random=None):
+        """entries as for step; a temperature (or one for all) and a random number per wanted place. The tokens drawn, in the order of the places."""
+        import numpy as np
+        arr, keep, heat, rnd, n = self._drawn(entries, temperatures, random, None)
+        out = np.empty(n, np.int32)
+        check(lib.cml_lm_step_sampled(self.h, arr, len(entries), None if heat is None else np_ptr(heat), None if rnd is None else np_ptr(rnd), np_ptr(out)), "cml_lm_step_sampled")
+        return out
+
+    def verified(self, entries, temperatures=None, random=None):
+        """entries: (seq, tokens): the token that the sequence goes on with, then drafts. Drafts kept and the token behind them, per entry."""
+        import numpy as np
+        arr, keep, heat, rnd, n = self._drawn([(q, t, []) for q, t in entries], temperatures, random, len(entries))
+        kept, after = np.empty(n, np.int32), np.empty(n, np.int32)
+        check(lib.cml_lm_step_verified(self.h, arr, len(entries), None if heat is None else np_ptr(heat), None if rnd is None else np_ptr(rnd), np_ptr(kept), np_ptr(after)), "cml_lm_step_verified")
+        return kept, after
+
+    def generate_drafted(self, drafter, drafts, prompt, max_new, temperature=0.0, seed=0, eos=-1):
+        """New tokens, and (steps, drafted, accepted)."""
+        import numpy as np
+        t, stats = np.ascontiguousarray(prompt, np.int32), np.zeros(3, np.int32)
+        cfg = lib.cml_generation_default_config()
+        cfg.do_sample, cfg.temperature, cfg.max_new_tokens, cfg.eos_token_id = temperature > 0, temperature, max_new, eos
+        r = lib.cml_lm_generate_drafted(self.h, drafter.h, drafts, np_ptr(t), len(t), C.byref(cfg), seed, np_ptr(stats))
+        if not r:
+            raise CmlB200Error("cml_lm_generate_drafted failed")
+        out = [r.contents.token_ids[i] for i in range(len(t), r.contents.num_tokens)]
+        lib.cml_generation_result_free(r)
+        return out, tuple(int(x) for x in stats)
 
     def step(self, entries, greedy=False):
         """entries: (seq, tokens, wanted places or None for all). One list item of logits [n, vocab] (or picks [n]) per entry."""

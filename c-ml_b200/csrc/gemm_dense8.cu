@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include "dense8.cuh"
+#include "status_word.cuh"
 #include "tcgen05_util.cuh"
 
 namespace {
@@ -27,9 +28,8 @@ constexpr int EPI = 8, THREADS8 = 64 + EPI * 32;
 constexpr int A8 = CH * BK8, MOST_STAGES = 8, ROOM8 = 220 * 1024;
 constexpr int SCALES8 = 1024, HEAD8 = SCALES8 + EPI * 512;                    // in front of the stages: barriers and words, then the epilogue warps' scales of tokens
 
-__device__ int g_dense8_status = 0;
-__device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, &g_dense8_status));
+__device__ __forceinline__ bool wait8(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code, int* status) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code, status));
 }
 // for what is under way whoever has given up
 __device__ __forceinline__ void drain8(uint32_t bar, uint32_t parity) {
@@ -76,6 +76,7 @@ __device__ __forceinline__ void whole_cluster() { asm volatile("barrier.cluster.
 struct Gemm8 {
     Out8 out;
     int M, N, loads, NX, tiles_m, tiles, stages, glu;
+    int* status;
 };
 
 // Tile number -> token tile, channel tile: groups of 8 token tiles share a sweep over the channels, so that the CTAs working at one time read few distinct slabs.
@@ -175,7 +176,7 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
             int it = ahead, s = 0;
             uint32_t phase = 0, to = sbase;
             for (; it < total; it++) {
-                if (!mbar_wait(empty(s), phase, abort_flag, 1, &g_dense8_status)) break;
+                if (!mbar_wait(empty(s), phase, abort_flag, 1, p.status)) break;
                 weights(to, full(s));
                 tokens(to, full(s));
                 to += stage;
@@ -194,7 +195,7 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         bool ok = true;
         if (PAIR && second) {                          // tells the first CTA what has come to this one
             for (int it = 0; it < total && ok; it++) {
-                ok = wait8(full(s), phase, abort_flag, 2);
+                ok = wait8(full(s), phase, abort_flag, 2, p.status);
                 if (ok && lane == 0) arrive_first(full(s));
                 __syncwarp();
                 if (++s == S) { s = 0; phase ^= 1; }
@@ -202,11 +203,11 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
         } else {
             for (; done < my_tiles && ok; done++) {
                 const int b = done & 1;
-                ok = wait8(acc_empty(b), ((done >> 1) & 1) ^ 1, abort_flag, 3);
+                ok = wait8(acc_empty(b), ((done >> 1) & 1) ^ 1, abort_flag, 3, p.status);
                 if (!ok) break;
                 tmem_fence_after();
                 for (int k = 0; k < nkb; k++) {
-                    ok = wait8(full(s), phase, abort_flag, 4);
+                    ok = wait8(full(s), phase, abort_flag, 4, p.status);
                     if (!ok) break;
                     tmem_fence_after();
                     const uint64_t ad = desc0 + (uint64_t)(uint32_t)(s * (stage >> 4)), bd = ad + (uint64_t)(blocks_a >> 4);
@@ -249,7 +250,7 @@ gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_consta
                 sxs[i * 32 + lane] = c < c_hi ? p.out.xscale[m0 + c] : 0.f;
             }
             __syncwarp();
-            const bool there = wait8(acc_full(b), (done >> 1) & 1, abort_flag, 5);
+            const bool there = wait8(acc_full(b), (done >> 1) & 1, abort_flag, 5, p.status);
             tmem_fence_after();
             const uint32_t acc_at = lanes + (uint32_t)(b * acc);
             if (ranks > 1) {
@@ -380,7 +381,7 @@ Shape8 pick_shape(int M, int N, int loads) {
 }
 
 template <bool PAIR>
-int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Shape8& shape, const Out8& out, int glu, cudaStream_t st) {
+int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Shape8& shape, const Out8& out, int glu, int* status, cudaStream_t st) {
     const int blocks = (W->cols + BK8 - 1) / BK8, tm = (M + shape.NX - 1) / shape.NX, rows = PAIR ? 2 * CH : CH, tiles = tm * ((W->rows + rows - 1) / rows), box = PAIR ? shape.NX / 2 : shape.NX;
     CUtensorMap xmap, wmap;
     int rc = encode_blocks(&xmap, xq, M, blocks, ldq, box);
@@ -388,7 +389,7 @@ int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, cons
     if (rc) return rc;
     const int stage = BLOCKS * (A8 + box * BK8), sums = shape.ranks > 1 ? (shape.NX + 8 * shape.ranks) * CH * 4 : 0;
     const int stages = ROOM8 / stage < MOST_STAGES ? ROOM8 / stage : MOST_STAGES;
-    const Gemm8 p = {out, M, W->rows, (blocks + BLOCKS - 1) / BLOCKS, shape.NX, tm, tiles, stages, glu};
+    const Gemm8 p = {out, M, W->rows, (blocks + BLOCKS - 1) / BLOCKS, shape.NX, tm, tiles, stages, glu, status};
     const size_t smem = 1024 + HEAD8 + (size_t)(stages * stage > sums ? stages * stage : sums);
     static size_t attr[kMaxDevices] = {};
     CMLB_CUDA(cmlb_ensure_smem(gemm_dense8_kernel<PAIR>, 1024 + HEAD8 + ROOM8, attr));
@@ -398,20 +399,31 @@ int launch_gemm8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, cons
     return CMLB200_OK;
 }
 
+StatusWords<kMaxDevices> g_status_words8;
+int status_word8(int** word) {
+    int dev = 0;
+    CMLB_CUDA(cudaGetDevice(&dev));
+    CMLB_REQUIRE(dev >= 0 && dev < kMaxDevices, "device %d", dev);
+    CMLB_CUDA(g_status_words8.get(dev, word));
+    return CMLB200_OK;
+}
+
 }  // namespace
 
 int cmlb_gemm_dense8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Out8& out, int glu, cudaStream_t st) {
+    int* status;
+    const int rc = status_word8(&status);
+    if (rc) return rc;
     const Shape8 shape = pick_shape(M, W->rows, (W->cols + BLOCKS * BK8 - 1) / (BLOCKS * BK8));
-    return shape.pair ? launch_gemm8<true>(W, xq, ldq, M, shape, out, glu, st) : launch_gemm8<false>(W, xq, ldq, M, shape, out, glu, st);
+    return shape.pair ? launch_gemm8<true>(W, xq, ldq, M, shape, out, glu, status, st) : launch_gemm8<false>(W, xq, ldq, M, shape, out, glu, status, st);
 }
 
 extern "C" int cmlb200_dense8_status(int* status, int reset) {
     CMLB_REQUIRE(status, "cmlb200_dense8_status: NULL argument");
-    CMLB_CUDA(cudaDeviceSynchronize());
-    CMLB_CUDA(cudaMemcpyFromSymbol(status, g_dense8_status, sizeof(int)));
-    if (reset) {
-        const int zero = 0;
-        CMLB_CUDA(cudaMemcpyToSymbol(g_dense8_status, &zero, sizeof(int)));
-    }
+    int* word;
+    const int rc = status_word8(&word);
+    if (rc) return rc;
+    *status = *static_cast<volatile int*>(word);
+    if (reset) *static_cast<volatile int*>(word) = 0;
     return CMLB200_OK;
 }

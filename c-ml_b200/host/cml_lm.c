@@ -21,6 +21,13 @@
 #define HEAD_ROWS 256              /* rows of logits per pass of the vocabulary projection */
 #define STAGED_ROWS 32             /* rows of logits that go through page-locked memory */
 #define SCORED_TOP 32              /* likeliest tokens of a scored row at most */
+#define DRAWN_RANDOM 0             /* bytes: what a drawn step uploads (random numbers, first rows, drafts, temperatures), then what comes back */
+#define DRAWN_FIRST (DRAWN_RANDOM + HEAD_ROWS * 8)
+#define DRAWN_TOKENS (DRAWN_FIRST + (HEAD_ROWS + 4) * 4)
+#define DRAWN_TEMPERATURE (DRAWN_TOKENS + HEAD_ROWS * 4)
+#define DRAWN_ACCEPTED (DRAWN_TEMPERATURE + HEAD_ROWS * 4)
+#define DRAWN_NEXT (DRAWN_ACCEPTED + HEAD_ROWS * 4)
+#define DRAWN_BYTES (DRAWN_NEXT + HEAD_ROWS * 4)
 #define MAX_CLASSES 16
 #define MAX_GRAPHS 32
 
@@ -50,6 +57,9 @@ struct CMLLanguageModel {
     cmlb200_pages block_pages, slot_pages;
     char *d_scored, *h_scored;     /* targets and results of scored rows; made by the first scored step */
     float* d_score_logits;         /* of classes that give logits to the host */
+    char *d_drawn, *h_drawn;       /* of rows whose tokens are drawn, and the draws' workspace; made by the first drawn step */
+    void* d_drawn_work;
+    int keep_behind;               /* tokens behind a window that stay in the pool */
     StepGraph graphs[MAX_GRAPHS];
     unsigned clock;
     unsigned char* in_step;        /* per sequence: already in the entries being checked */
@@ -72,7 +82,7 @@ int cml_lm_known(const char* architecture) { return find_class(architecture) != 
 
 /* ---- load / free ----------------------------------------------------------------------------------- */
 CMLLMOptions cml_lm_default_options(void) {
-    CMLLMOptions o = {.dtype = DTYPE_BFLOAT16, .max_tokens = 8192, .max_sequences = 8, .max_step_rows = 0, .cache = CML_LM_CACHE_DEFAULT};
+    CMLLMOptions o = {.dtype = DTYPE_BFLOAT16, .max_tokens = 8192, .max_sequences = 8, .max_step_rows = 0, .cache = CML_LM_CACHE_DEFAULT, .weights = CML_LM_WEIGHTS_DEFAULT};
     return o;
 }
 
@@ -133,6 +143,7 @@ CMLLanguageModel* cml_lm_load(const char* path, const CMLLMOptions* options) {
     CMLLMOptions o = options ? *options : cml_lm_default_options();
     if (o.dtype != DTYPE_BFLOAT16 && o.dtype != DTYPE_FLOAT32) { LOG_ERROR("%s: dtype must be bfloat16 or float32", who); return NULL; }
     if (o.cache < CML_LM_CACHE_DEFAULT || o.cache > CML_LM_CACHE_E4M3) { LOG_ERROR("%s: cache %d", who, o.cache); return NULL; }
+    if (o.weights != CML_LM_WEIGHTS_DEFAULT && o.weights != CML_LM_WEIGHTS_INT8) { LOG_ERROR("%s: weights %d", who, o.weights); return NULL; }
     if (o.max_tokens <= 0 || o.max_sequences <= 0 || o.max_tokens > (1 << 28)) { LOG_ERROR("%s: max_tokens %d, max_sequences %d", who, o.max_tokens, o.max_sequences); return NULL; }
     if (o.max_step_rows <= 0) o.max_step_rows = o.max_tokens;
     struct stat sb;
@@ -173,7 +184,7 @@ void cml_lm_free(CMLLanguageModel* lm) {
     for (int i = 0; i < MAX_GRAPHS; i++) if (lm->graphs[i].graph) cmlb200_graph_destroy(lm->graphs[i].graph);
     if (lm->model) lm->cls->free(lm->model);
     cml_paged_kv_cache_free(lm->cache);
-    void* dev[] = {lm->d_meta, lm->d_table, lm->d_logits, lm->d_picked, lm->d_hist, lm->d_step, lm->d_moves, lm->d_pools, lm->d_scored, lm->d_score_logits};
+    void* dev[] = {lm->d_meta, lm->d_table, lm->d_logits, lm->d_picked, lm->d_hist, lm->d_step, lm->d_moves, lm->d_pools, lm->d_scored, lm->d_score_logits, lm->d_drawn, lm->d_drawn_work};
     for (size_t i = 0; i < sizeof dev / sizeof dev[0]; i++) cmlb200_free(dev[i]);
     cmlb200_host_free_pinned(lm->h_meta);
     cmlb200_host_free_pinned(lm->h_table);
@@ -181,6 +192,7 @@ void cml_lm_free(CMLLanguageModel* lm) {
     cmlb200_host_free_pinned(lm->h_logits);
     cmlb200_host_free_pinned(lm->h_moves);
     cmlb200_host_free_pinned(lm->h_scored);
+    cmlb200_host_free_pinned(lm->h_drawn);
     if (lm->stream) cmlb200_stream_destroy(lm->stream);
     free(lm->in_step);
     free(lm->portions);
@@ -277,7 +289,26 @@ static int grow_sequence(CMLLanguageModel* lm, int seq, int n) {
 
 /* Blocks that every layer's window has passed go back to the pool, those of first tokens that stay in sight aside. */
 static void release_passed(CMLLanguageModel* lm, int seq) {
-    if (lm->info.window > 0) cml_paged_cache_release_between(lm->cache, seq, lm->info.keep_first, lm->cache->sequences[seq].seq_len - lm->info.window + 1);
+    if (lm->info.window > 0) cml_paged_cache_release_between(lm->cache, seq, lm->info.keep_first, lm->cache->sequences[seq].seq_len - lm->info.window + 1 - lm->keep_behind);
+}
+
+void cml_lm_keep_behind(CMLLanguageModel* lm, int tokens) { lm->keep_behind = tokens; }
+const float* cml_lm_logits(const CMLLanguageModel* lm) { return lm->d_logits; }
+int cml_lm_step_rows(const CMLLanguageModel* lm) { return lm->opt.max_step_rows; }
+int cml_lm_takes_drafts(const CMLLanguageModel* lm) { return lm->cache && !lm->slot_pages.pools; }
+
+int cml_lm_sequence_truncate(CMLLanguageModel* lm, int seq, int length) {
+    static const char* who = "cml_lm_sequence_truncate";
+    const int has = cml_lm_sequence_length(lm, seq);
+    if (has < 0) { LOG_ERROR("%s: sequence %d is not open", who, seq); return -1; }
+    if (length == has) return 0;
+    if (!lm->cache) { LOG_ERROR("%s: %s models keep no paged cache", who, lm->cls->architecture); return -1; }
+    if (lm->slot_pages.pools) { LOG_ERROR("%s: %s models keep a state per sequence", who, lm->cls->architecture); return -1; }
+    const CMLBlockTable* bt = &lm->cache->sequences[seq];
+    const int back = lm->info.window > 0 && length + 1 > lm->info.window ? length + 1 - lm->info.window : 0;
+    for (int i = back / BLOCK; length >= 0 && length < has && i < (length + BLOCK - 1) / BLOCK; i++)
+        if (bt->block_ids[i] < 0) { LOG_ERROR("%s: token %d of sequence %d is no longer there", who, i * BLOCK, seq); return -1; }
+    return cml_paged_cache_truncate(lm->cache, seq, length);
 }
 
 /* ---- steps ------------------------------------------------------------------------------------------- */
@@ -455,11 +486,68 @@ static int score_rows(CMLLanguageModel* lm, const Scored* q, const float* d_logi
     return 0;
 }
 
-static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, float* logits, int* picked, const Scored* scored, const char* who) {
+/* What a step draws: a token per wanted row, or, with `accepted`, the drafts of every entry that stay and the token behind them. */
+typedef struct { const float* temperatures; const uint64_t* random; const float* d_drafter; int *accepted, *next; } Drawn;
+
+static int check_drawn(const float* temperatures, const uint64_t* random, int n, const char* who) {
+    int cold = temperatures != NULL;
+    for (int i = 0; temperatures && i < n; i++) {
+        if (!(temperatures[i] >= 1e-5f)) continue;         /* (as the device reads it) */
+        cold = 0;
+        if (temperatures[i] > 1e30f) { LOG_ERROR("%s: temperature %g", who, (double)temperatures[i]); return -1; }
+    }
+    if (!random && !cold) { LOG_ERROR("%s: no random numbers", who); return -1; }
+    return 0;
+}
+
+/* `sequences` of them, their first rows, and drafts in h_drawn already; numbers from place `at` on. */
+static int draw_rows(CMLLanguageModel* lm, const Drawn* q, const float* d_logits, int sequences, int rows, int at, int* accepted, int* next, void* stream) {
+    char *d = lm->d_drawn, *h = lm->h_drawn;
+    for (int i = 0; i < sequences; i++) {
+        ((uint64_t*)(void*)(h + DRAWN_RANDOM))[i] = q->random ? q->random[at + i] : 0;
+        ((float*)(void*)(h + DRAWN_TEMPERATURE))[i] = q->temperatures ? q->temperatures[at + i] : 1.0f;
+    }
+    DEV(cmlb200_memcpy_h2d(d, h, DRAWN_ACCEPTED, stream));
+    const cmlb200_drafts v = {sequences, rows, (const int*)(void*)(d + DRAWN_FIRST), (const int*)(void*)(d + DRAWN_TOKENS), rows > sequences ? q->d_drafter : NULL, lm->info.vocab,
+                              (const float*)(void*)(d + DRAWN_TEMPERATURE), (const uint64_t*)(void*)(d + DRAWN_RANDOM)};
+    DEV(cmlb200_verify_drafts(&v, d_logits, CMLB200_DT_F32, lm->info.vocab, lm->info.vocab, (int*)(void*)(d + DRAWN_ACCEPTED), (int*)(void*)(d + DRAWN_NEXT), lm->d_drawn_work, stream));
+    DEV(cmlb200_memcpy_d2h(h + DRAWN_ACCEPTED, d + DRAWN_ACCEPTED, DRAWN_BYTES - DRAWN_ACCEPTED, stream));
+    DEV(cmlb200_stream_sync(stream));
+    if (accepted) memcpy(accepted, h + DRAWN_ACCEPTED, (size_t)sequences * sizeof(int));
+    memcpy(next, h + DRAWN_NEXT, (size_t)sequences * sizeof(int));
+    return 0;
+}
+static int make_drawn(CMLLanguageModel* lm) {
+    if (!lm->d_drawn) DEV(cmlb200_malloc((void**)&lm->d_drawn, DRAWN_BYTES));
+    if (!lm->h_drawn) {
+        DEV(cmlb200_host_alloc_pinned((void**)&lm->h_drawn, DRAWN_BYTES));
+        memset(lm->h_drawn, 0, DRAWN_BYTES);
+    }
+    if (!lm->d_drawn_work) DEV(cmlb200_malloc(&lm->d_drawn_work, cmlb200_verify_work_bytes(HEAD_ROWS, 1)));
+    return 0;
+}
+/* k rows, a token each */
+static int draw_each(CMLLanguageModel* lm, const Drawn* q, const float* d_logits, int at, int k, void* stream) {
+    if (make_drawn(lm)) return -1;
+    for (int i = 0; i <= k; i++) ((int*)(void*)(lm->h_drawn + DRAWN_FIRST))[i] = i;
+    return draw_rows(lm, q, d_logits, k, k, at, NULL, q->next + at, stream);
+}
+static int draw_behind(CMLLanguageModel* lm, const Drawn* q, const CMLLMEntry* entries, int n, int rows) {
+    if (make_drawn(lm)) return -1;
+    int *first = (int*)(void*)(lm->h_drawn + DRAWN_FIRST), *tokens = (int*)(void*)(lm->h_drawn + DRAWN_TOKENS);
+    first[0] = 0;
+    for (int i = 0; i < n; i++) {
+        memcpy(tokens + first[i] - i, entries[i].tokens + 1, (size_t)(entries[i].num_tokens - 1) * sizeof(int));
+        first[i + 1] = first[i] + entries[i].num_tokens;
+    }
+    return draw_rows(lm, q, lm->d_logits, n, rows, 0, q->accepted, q->next, lm->stream);
+}
+
+static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, float* logits, int* picked, const Scored* scored, const Drawn* drawn, const char* who) {
     int want = 0;
     const int rows = check_step(lm, entries, n, &want, who), greedy = picked != NULL;
     if (rows < 0) return -1;
-    if (want && !logits && !picked && !scored) { LOG_ERROR("%s: no room for the wanted logits", who); return -1; }
+    if (want && !logits && !picked && !scored && !drawn) { LOG_ERROR("%s: no room for the wanted logits", who); return -1; }
     for (int i = 0; i < n; i++) if (grow_sequence(lm, entries[i].seq, entries[i].num_tokens)) return -1;
     CMLLMBatch b;
     const int* d_want;
@@ -473,7 +561,9 @@ static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, floa
             if (lm->cls->head(lm->model, d_want + at, k, lm->d_logits, lm->stream)) return -1;
             if (greedy) DEV(cmlb200_argmax(lm->d_logits, k, lm->info.vocab, lm->d_picked, lm->stream));
         }
-        if (scored) {
+        if (drawn) {
+            if (drawn->accepted ? draw_behind(lm, drawn, entries, n, want) : draw_each(lm, drawn, lm->d_logits, at, k, lm->stream)) return -1;
+        } else if (scored) {
             if (score_rows(lm, scored, lm->d_logits, at, k, lm->stream)) return -1;
         } else if (greedy) {
             DEV(cmlb200_memcpy_d2h(lm->h_picked, lm->d_picked, (size_t)k * sizeof(int), lm->stream));
@@ -489,7 +579,11 @@ static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, floa
     }
     DEV(cmlb200_stream_sync(lm->stream));
     if (lm->cls->check && lm->cls->check(lm->model, &b)) { LOG_ERROR("%s: a bounded device-side wait expired", who); return -1; }
-    for (int i = 0; i < n; i++) release_passed(lm, entries[i].seq);
+    for (int i = 0; i < n; i++) {
+        const int has = lm->cache->sequences[entries[i].seq].seq_len;
+        if (drawn && drawn->accepted && cml_paged_cache_truncate(lm->cache, entries[i].seq, has - entries[i].num_tokens + 1 + drawn->accepted[i])) return -1;
+        release_passed(lm, entries[i].seq);
+    }
     return 0;
 }
 
@@ -497,7 +591,7 @@ int cml_lm_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries
     static const char* who = "cml_lm_step";
     int want;
     if (lm && !lm->cache) return check_step(lm, entries, num_entries, &want, who) < 0 ? -1 : lm->cls->step(lm->model, entries, num_entries, logits);
-    return run_step(lm, entries, num_entries, logits, NULL, NULL, who);
+    return run_step(lm, entries, num_entries, logits, NULL, NULL, NULL, who);
 }
 
 int cml_lm_step_scored(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const int* targets, int top, float* logprobs, float* entropies, int* top_ids,
@@ -508,7 +602,7 @@ int cml_lm_step_scored(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_
         return -1;
     }
     const Scored q = {targets, top, logprobs, entropies, top_ids, top_logprobs};
-    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, NULL, &q, who);
+    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, NULL, &q, NULL, who);
     /* logits that come to the host go back, HEAD_ROWS rows at a time */
     int want = 0;
     if (check_step(lm, entries, num_entries, &want, who) < 0) return -1;
@@ -524,6 +618,54 @@ int cml_lm_step_scored(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_
     return rc;
 }
 
+int cml_lm_step_sampled(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const float* temperatures, const uint64_t* random, int* picked) {
+    static const char* who = "cml_lm_step_sampled";
+    int want = 0;
+    if (!picked) { LOG_ERROR("%s: invalid arguments", who); return -1; }
+    if (check_step(lm, entries, num_entries, &want, who) < 0 || check_drawn(temperatures, random, want, who)) return -1;
+    const Drawn q = {temperatures, random, NULL, NULL, picked};
+    if (lm->cache) return run_step(lm, entries, num_entries, NULL, NULL, NULL, &q, who);
+    /* logits that come to the host go back, HEAD_ROWS rows at a time */
+    const size_t V = (size_t)lm->info.vocab;
+    float* lg = (float*)malloc((size_t)(want ? want : 1) * V * sizeof(float));
+    int rc = lg ? lm->cls->step(lm->model, entries, num_entries, lg) : -1;
+    if (!rc && want && !lm->d_score_logits) rc = CML_DEV_FAIL(cmlb200_malloc((void**)&lm->d_score_logits, HEAD_ROWS * V * sizeof(float)), who) ? -1 : 0;
+    for (int at = 0; at < want && !rc; at += HEAD_ROWS) {
+        const int k = want - at < HEAD_ROWS ? want - at : HEAD_ROWS;
+        rc = CML_DEV_FAIL(cmlb200_memcpy_h2d(lm->d_score_logits, lg + (size_t)at * V, (size_t)k * V * sizeof(float), NULL), who) || draw_each(lm, &q, lm->d_score_logits, at, k, NULL) ? -1 : 0;
+    }
+    free(lg);
+    return rc;
+}
+
+int cml_lm_run_verified(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, const float* temperatures, const uint64_t* random, const float* d_drafter, int* accepted, int* next, const char* who) {
+    if (!lm || !lm->cache || !entries || n <= 0 || n > lm->opt.max_sequences || !accepted || !next) { LOG_ERROR("%s: invalid arguments, or a model without a paged cache", who); return -1; }
+    int all[HEAD_ROWS];
+    long rows = 0;
+    for (int i = 0; i < n; i++) {
+        if (entries[i].num_tokens > 1 && lm->slot_pages.pools) { LOG_ERROR("%s: %s models keep a state per sequence, and take no drafts", who, lm->cls->architecture); return -1; }
+        rows += entries[i].num_tokens > 0 ? entries[i].num_tokens : 0;
+    }
+    if (rows > HEAD_ROWS) { LOG_ERROR("%s: %ld tokens, at most %d", who, rows, HEAD_ROWS); return -1; }
+    if (check_drawn(temperatures, random, n, who)) return -1;
+    CMLLMEntry* e = (CMLLMEntry*)malloc((size_t)n * sizeof *e);
+    if (!e) return -1;
+    for (int i = 0; i < HEAD_ROWS; i++) all[i] = i;
+    for (int i = 0; i < n; i++) {
+        e[i] = entries[i];
+        e[i].want = all;
+        e[i].num_want = e[i].num_tokens;
+    }
+    const Drawn q = {temperatures, random, d_drafter, accepted, next};
+    const int rc = run_step(lm, e, n, NULL, NULL, NULL, &q, who);
+    free(e);
+    return rc;
+}
+
+int cml_lm_step_verified(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const float* temperatures, const uint64_t* random, int* accepted, int* next) {
+    return cml_lm_run_verified(lm, entries, num_entries, temperatures, random, NULL, accepted, next, "cml_lm_step_verified");
+}
+
 static int argmax_row(const float* row, int n) {
     int best = 0;
     for (int i = 1; i < n; i++) if (row[i] > row[best]) best = i;
@@ -533,7 +675,7 @@ static int argmax_row(const float* row, int n) {
 int cml_lm_step_greedy(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, int* picked) {
     static const char* who = "cml_lm_step_greedy";
     if (!picked) { LOG_ERROR("%s: invalid arguments", who); return -1; }
-    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, picked, NULL, who);
+    if (!lm || lm->cache) return run_step(lm, entries, num_entries, NULL, picked, NULL, NULL, who);
     int want = 0;
     if (check_step(lm, entries, num_entries, &want, who) < 0) return -1;
     float* lg = (float*)malloc((size_t)(want ? want : 1) * (size_t)lm->info.vocab * sizeof(float));

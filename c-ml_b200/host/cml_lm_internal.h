@@ -57,6 +57,14 @@ typedef struct CMLLMClass {
     int (*step)(void* model, const CMLLMEntry* entries, int num_entries, float* logits);
 } CMLLMClass;
 
+/* cml_lm.c, for cml_lm_drafts.c. run_verified: cml_lm_step_verified, the drafts having been drawn from d_drafter [all drafts][vocab] (device; NULL: chosen for certain). logits: the device rows
+ * that the last step left, in the order of its wanted rows. keep_behind: so many tokens behind a window stay in the pool, for sequences that are truncated. */
+int cml_lm_run_verified(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, const float* temperatures, const uint64_t* random, const float* d_drafter, int* accepted, int* next, const char* who);
+const float* cml_lm_logits(const CMLLanguageModel* lm);
+void cml_lm_keep_behind(CMLLanguageModel* lm, int tokens);
+int cml_lm_takes_drafts(const CMLLanguageModel* lm);
+int cml_lm_step_rows(const CMLLanguageModel* lm);              /* tokens of a step at most */
+
 /* Classes register themselves before main (a program links those it wants). */
 void cml_lm_register(const CMLLMClass* cls);
 

@@ -904,8 +904,20 @@ static int layered_pools(void* model, int per_slot, cmlb200_page_pool* pools, in
     return n;
 }
 
+/* ---- 8-bit weights ------------------------------------------------------------------------------------ */
+static size_t codes8(const cmlb200_dense* w) { return (size_t)lml_round_up(w->rows, 16) * (size_t)lml_round_up(w->cols, 128); }
+static cmlb200_dense8 view8(const cmlb200_dense* w) {
+    const cmlb200_dense8 v = {w->rows, w->cols, w->ld, w->w, (float*)(void*)((uint8_t*)w->w + codes8(w)), w->bias, w->cap};
+    return v;
+}
+
 /* ---- a step ------------------------------------------------------------------------------------------- */
 int lml_product(const Layered* m, const cmlb200_dense* w, const void* x, int ldx, int rows, float* y, int ldy, void* st) {
+    if (w->dtype == CMLB200_DT_I8) {
+        const cmlb200_dense8 v = view8(w);
+        DEV(cmlb200_linear_dense8(&v, x, CMLB200_DT_BF16, ldx, rows, y, ldy, m->work8, st));
+        return 0;
+    }
     if (m->f32) DEV(cmlb200_linear_dense_f32(w, (const float*)x, ldx, rows, y, ldy, st));
     else if (rows <= SKINNY_ROWS) DEV(cmlb200_gemv_dense(w, (const uint16_t*)x, ldx, rows, y, ldy, st));
     else DEV(cmlb200_gemm_dense(w, (const uint16_t*)x, ldx, rows, y, ldy, st));
@@ -915,7 +927,10 @@ int lml_product(const Layered* m, const cmlb200_dense* w, const void* x, int ldx
 /* y = Wd (act(gate) * up) of the rows in h */
 static int gated_product(const Layered* m, const cmlb200_dense* gu, const cmlb200_dense* down, int ff, int rows, float* y, void* st) {
     const int act = m->design->act;
-    if (m->f32) {
+    if (gu->dtype == CMLB200_DT_I8) {
+        const cmlb200_dense8 v = view8(gu);
+        DEV(cmlb200_linear_dense8_glu(&v, m->h, CMLB200_DT_BF16, m->ld_h, rows, ff, act, (uint16_t*)m->f, m->ld_f, m->work8, st));
+    } else if (m->f32) {
         DEV(cmlb200_linear_dense_f32(gu, (const float*)m->h, m->ld_h, rows, m->gu, m->ld_gu, st));
         DEV(cmlb200_glu_rows_f32(m->gu, m->ld_gu, rows, ff, act, (float*)m->f, m->ld_f, st));
     } else if (rows <= SKINNY_ROWS) {
@@ -1224,9 +1239,44 @@ static int layered_check(void* model, const CMLLMBatch* b) {
     if (status) return -1;
     if (m->cache8) DEV(cmlb200_attention8_status(&status, 1));
     if (status) return -1;
+    if (m->weights8) DEV(cmlb200_dense8_status(&status, 1));
+    if (status) return -1;
     if (b->rows <= SKINNY_ROWS) return 0;
     DEV(cmlb200_gemm_dense_status(&status, 1));
     return status ? -1 : 0;
+}
+
+/* ---- 8-bit weights, made -------------------------------------------------------------------------------- */
+/* A bfloat16 matrix becomes codes and scales of its rows. */
+static int to_int8(cmlb200_dense* w) {
+    if (!w->w) return 0;
+    cmlb200_dense q = *w;
+    q.dtype = CMLB200_DT_I8;
+    q.ld = lml_round_up(w->cols, 128);
+    if (lml_zeroed(&q.w, codes8(w) + (size_t)lml_round_up(w->rows, 16) * sizeof(float))) return -1;
+    if (CML_DEV_FAIL(cmlb200_quantize_rows(w->w, CMLB200_DT_BF16, w->ld, w->rows, w->cols, (int8_t*)q.w, q.ld, (float*)(void*)((uint8_t*)q.w + codes8(w)), NULL), __func__) ||
+        CML_DEV_FAIL(cmlb200_stream_sync(NULL), __func__)) {
+        cmlb200_free(q.w);
+        return -1;
+    }
+    cmlb200_free(w->w);
+    *w = q;
+    return 0;
+}
+
+/* What of a layer (NULL: beside the layers) goes through lml_product and makes no router's logits. A product's workspace holds codes of a step's rows, or of the head's. */
+static int weights8_of(Layered* m, Layer* l, size_t* work) {
+    LayerWeights* w = l ? &l->w : NULL;
+    cmlb200_dense* of_layer[] = {l && m->design->side_by_side && l->ff ? NULL : l ? &w->wqkvg : NULL, l ? &w->wo : &m->head, l ? &w->wo2 : NULL, l ? &w->wuq : NULL, l ? &w->wgu : NULL, l ? &w->wd : NULL,
+                                 l ? &w->shared_gu : NULL, l ? &w->shared_down : NULL};
+    for (size_t k = 0; k < sizeof of_layer / sizeof of_layer[0]; k++) {
+        cmlb200_dense* d = of_layer[k];
+        if (!d || !d->w) continue;
+        if (to_int8(d)) return -1;
+        const size_t bytes = cmlb200_dense8_work_bytes(lml_most(m->max_rows, 256), d->rows, d->cols);
+        if (bytes > *work) *work = bytes;
+    }
+    return 0;
 }
 
 /* ---- class --------------------------------------------------------------------------------------------- */
@@ -1246,7 +1296,7 @@ static void layered_free(void* model) {
     const cmlb200_moe* p = &m->plan;
     void* bufs[] = {m->embed, m->freq, m->final_norm, m->head.w, m->x, m->qkvg, m->y, m->gu, m->h, m->att, m->f, m->q, m->o, m->expand_table, m->expand_k,
                     m->expand_v, m->expand_c, m->xp, m->router, p->ids, p->weight, p->pos, p->src, p->expert, p->start, p->count, p->active, p->num_active,
-                    p->tiles, p->num_tiles, p->self, m->y_shared, m->dec, m->gate, m->low, m->delta_work, m->y_mix, m->y_mix2, m->cq, m->q_rows_out, m->scores};
+                    p->tiles, p->num_tiles, p->self, m->work8, m->y_shared, m->dec, m->gate, m->low, m->delta_work, m->y_mix, m->y_mix2, m->cq, m->q_rows_out, m->scores};
     for (size_t k = 0; k < sizeof bufs / sizeof bufs[0]; k++) cmlb200_free(bufs[k]);
     free(m->layers);
     free(m);
@@ -1262,12 +1312,18 @@ static void* layered_load(const char* path, const CMLJson* config, const CMLLMOp
     m->f32 = options->dtype == DTYPE_FLOAT32;
     m->max_sequences = options->max_sequences;
     m->cache8 = options->cache == CML_LM_CACHE_INT8 ? CMLB200_DT_I8 : options->cache == CML_LM_CACHE_E4M3 ? CMLB200_DT_E4M3 : 0;
+    m->weights8 = options->weights == CML_LM_WEIGHTS_INT8;
     char file[4096];
     snprintf(file, sizeof file, "%s/model.safetensors", path);
     CMLSafetensors* st = NULL;
-    int rc = read_config(config, m) || !(st = cml_safetensors_open(file)) || load_shared(m, st);
+    if (m->weights8 && m->f32) LOG_ERROR("8-bit weights go with bfloat16");
+    int rc = (m->weights8 && m->f32) || read_config(config, m) || !(st = cml_safetensors_open(file)) || load_shared(m, st);
+    size_t work8 = 0;
+    m->max_rows = options->max_step_rows;
+    if (m->weights8 && !rc) rc = weights8_of(m, NULL, &work8);
     for (int i = 0; i < m->num_layers && !rc; i++) {
         if (m->layers[i].source == i) rc = load_layer(m, st, i);
+        if (m->layers[i].source == i && m->weights8 && !rc) rc = weights8_of(m, &m->layers[i], &work8);
         if (!rc) rc = make_rotation(&m->layers[i]);
     }
     cml_safetensors_close(st);
@@ -1278,7 +1334,7 @@ static void* layered_load(const char* path, const CMLJson* config, const CMLLMOp
             rc = -1;
         }
     }
-    if (rc || make_activations(m, options->max_step_rows)) { layered_free(m); return NULL; }
+    if (rc || (work8 && lml_zeroed(&m->work8, work8)) || make_activations(m, options->max_step_rows)) { layered_free(m); return NULL; }
     info->vocab = m->vocab;
     for (int i = 0; i < m->num_layers; i++) {
         const int window = window_of(&m->layers[i]);

@@ -111,6 +111,8 @@ typedef struct Layered {
     const LayeredDesign* design;
     int f32, vocab, width, num_layers;
     int cache8;                    /* 0, or the CMLB200_DT_ of an 8-bit cache */
+    int weights8;                  /* matrices that lml_product alone reads are int8: dtype CMLB200_DT_I8, codes with a stride of whole 128 bytes, the rows' scales behind them */
+    void* work8;                   /* of their products */
     int block_size;                /* of the pools */
     int streams;                   /* 0: one residual, no streams */
     float eps, embed_scale, cap;

@@ -245,6 +245,26 @@ void cml_paged_cache_release_between(CMLPagedKVCache* cache, int seq_id, int fro
     }
 }
 
+int cml_paged_cache_truncate(CMLPagedKVCache* cache, int seq_id, int length) {
+    static const char* who = "cml_paged_cache_truncate";
+    CMLBlockTable* bt = live_sequence(cache, seq_id);
+    PagedDev* p = bt ? pd_find(cache) : NULL;
+    if (!bt || !p || cache->blocks[0].key_data) { LOG_ERROR("%s: sequence %d is not open, or its cache holds host data", who, seq_id); return -1; }
+    if (length < 0 || length > bt->seq_len) { LOG_ERROR("%s: %d tokens of %d", who, length, bt->seq_len); return -1; }
+    const int part = length % cache->block_size ? length / cache->block_size : -1;
+    if (length < bt->seq_len && part >= 0 && (bt->block_ids[part] < 0 || p->owners[bt->block_ids[part]] > 1)) {
+        LOG_ERROR("%s: the block of token %d of sequence %d is gone, or shared", who, length - 1, seq_id);
+        return -1;
+    }
+    const int keep = (length + cache->block_size - 1) / cache->block_size;
+    while (bt->num_blocks > keep) {
+        const int id = bt->block_ids[--bt->num_blocks];
+        if (id >= 0) cml_paged_cache_free_block(cache, id);
+    }
+    bt->seq_len = length;
+    return 0;
+}
+
 int cml_paged_cache_fork(CMLPagedKVCache* cache, int seq_id, int* from, int* to) {
     static const char* who = "cml_paged_cache_fork";
     if (from) *from = -1;

@@ -323,12 +323,15 @@ int cml_paged_cache_append(CMLPagedKVCache* cache, int seq_id, const float* key,
  * that a model's kernels own (key_data / value_data are NULL; append and cml_paged_gqa_forward refuse it).
  * blocks_for: blocks the next num_tokens tokens of a sequence take; extend: takes them, all or none;
  * release_before: gives back the blocks that lie wholly before `position` (their block_ids become -1),
- * for models in which no layer looks further back; release_between: the same, but keeps the blocks that hold tokens before `from`. */
+ * for models in which no layer looks further back; release_between: the same, but keeps the blocks that hold tokens before `from`;
+ * truncate: the sequence ends after `length` tokens, blocks behind them go back to the pool; refused (-1, nothing changes) where `length` is beyond its end, or inside a
+ * block that was let go of or that another sequence shares. */
 CMLPagedKVCache* cml_paged_kv_cache_create_device(int max_blocks, int max_sequences, int block_size);
 int cml_paged_cache_blocks_for(CMLPagedKVCache* cache, int seq_id, int num_tokens);
 int cml_paged_cache_extend(CMLPagedKVCache* cache, int seq_id, int num_tokens);
 void cml_paged_cache_release_before(CMLPagedKVCache* cache, int seq_id, int position);
 void cml_paged_cache_release_between(CMLPagedKVCache* cache, int seq_id, int from, int position);
+int cml_paged_cache_truncate(CMLPagedKVCache* cache, int seq_id, int length);
 /* Additions. A block may belong to several sequences; it returns to the pool when the last of them lets go of it (cml_paged_cache_free_block
  * takes one owner away).
  * fork: a new sequence that holds what seq_id holds. Full blocks are shared; the block that is still being filled is doubled: its data

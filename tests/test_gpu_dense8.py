@@ -297,3 +297,37 @@ def test_streams_and_graphs(pkg, torch_dev, m):
         graph.replay()
         torch.cuda.synchronize()
         assert (y.double().cpu().numpy() == want[i]).all()
+
+
+CAPTURED_FIRST = """
+import ctypes, sys
+sys.path.insert(0, {root!r})
+import torch
+import __graft_entry__ as entry
+pkg = entry.load_package()
+m, n, k = {m}, 300, 500
+x, codes, scale = torch.ones(m, k, device="cuda", dtype=torch.bfloat16), torch.ones(304, 512, device="cuda", dtype=torch.int8), torch.ones(304, device="cuda")
+codes[:, k:] = 0
+y, work = torch.zeros(m, n, device="cuda"), torch.zeros(pkg.lib.cmlb200_dense8_work_bytes(m, n, k), device="cuda", dtype=torch.uint8)
+w = pkg.Dense8(rows=n, cols=k, ld=512, w=codes.data_ptr(), scale=scale.data_ptr())
+torch.cuda.synchronize()
+g, status = torch.cuda.CUDAGraph(), ctypes.c_int(-1)
+with torch.cuda.graph(g):
+    pkg.check(pkg.lib.cmlb200_linear_dense8(w, x.data_ptr(), pkg.DT_BF16, k, m, y.data_ptr(), n, work.data_ptr(), torch.cuda.current_stream().cuda_stream), "linear_dense8")
+    pkg.check(pkg.lib.cmlb200_dense8_status(ctypes.byref(status), 0))
+assert status.value == 0
+g.replay()
+torch.cuda.synchronize()
+assert ((y - k).abs() <= 5 * 2.0 ** -24 * k).all(), y
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("m", [1, 12, 40, 600])
+def test_captured_before_anything_else_ran(m):
+    """The first call of a process is one that is being captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.format(root=str(Path(__file__).resolve().parents[1]), m=m)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
