@@ -17,7 +17,7 @@ struct Out8 {
     float cap;
     int act, n_out;
     void* y;
-    int ldy;
+    long ldy;
 };
 
 // the product of prompt-sized calls (gemm_dense8.cu)

@@ -153,7 +153,7 @@ gemv_dense8_kernel(const int8_t* __restrict__ W, int ldw, const T* __restrict__ 
     }
 }
 
-// M K up to which the CTAs quantise rows themselves: 4 rows of 4096x4096 5.5 us (two launches 6.2), 8 7.0 (6.4), 2 of 4096x11008 10.6 (11.4), 4 12.3 (11.5)
+// M K up to which the CTAs quantise several rows themselves (a single one always: 8192x28672 41.3 us, two launches 44.2): 4 rows of 4096x4096 5.5 us (two launches 6.2), 8 7.0 (6.4), 2 of 4096x11008 10.6 (11.4), 4 12.3 (11.5)
 constexpr int kFused = 24576;
 // rows * cols of a weight up to which 9 to 16 rows of x are taken here: 16 of 4096x4096 7.8 us (the prompts' product 8.9), of 11008x4096 14.3 (13.5)
 constexpr int kSmall = 20000000;
@@ -174,7 +174,7 @@ size_t codes_bytes(int M, int cols) { return (size_t)M * ((cols + 127) / 128 * 1
 
 template <int RT, int RING, bool GLU>
 int product8(const cmlb200_dense8* W, const void* x, int dtype, long ldx, int M, Out8 out, void* work, const char* who, cudaStream_t st) {
-    if (M <= 8 && (long)M * W->cols <= kFused) {
+    if (M == 1 || (M <= 8 && (long)M * W->cols <= kFused)) {
         CMLB_REQUIRE(ldx >= W->cols && ((uintptr_t)x & (dtype == CMLB200_DT_F32 ? 3 : 1)) == 0, "%s: %d columns, stride %ld, or x is not aligned to its type", who, W->cols, ldx);
         if (dtype == CMLB200_DT_F32) return launch_gemv8<float, 16, RT, 1, RING, GLU>(W, x, ldx, M, out, st);
         if (dtype == CMLB200_DT_BF16) return launch_gemv8<__nv_bfloat16, 16, RT, 1, RING, GLU>(W, x, ldx, M, out, st);
@@ -206,7 +206,7 @@ int check8(const cmlb200_dense8* W, const void* x, int M, void* y, void* work, c
 
 extern "C" size_t cmlb200_dense8_work_bytes(int M, int rows, int cols) {
     if (M <= 0 || rows <= 0 || cols <= 0) return 0;
-    return codes_bytes(M, cols) + ((size_t)M + 275) / 4 * 16;      // (the prompts' kernel reads scales of whole tiles)
+    return codes_bytes(M, cols) + ((size_t)M * 4 + 15) / 16 * 16;
 }
 
 extern "C" int cmlb200_linear_dense8(const cmlb200_dense8* W, const void* d_x, int dtype, long ldx, int M, float* d_y, long ldy, void* d_work, void* stream) {
@@ -214,7 +214,7 @@ extern "C" int cmlb200_linear_dense8(const cmlb200_dense8* W, const void* d_x, i
     int rc = check8(W, d_x, M, d_y, d_work, who);
     if (rc) return rc;
     CMLB_REQUIRE(ldy >= W->rows && ((uintptr_t)d_y & 3) == 0, "%s: output stride %ld", who, ldy);
-    const Out8 out = {W->scale, W->bias, nullptr, W->cap, 0, W->rows, d_y, (int)ldy};
+    const Out8 out = {W->scale, W->bias, nullptr, W->cap, 0, W->rows, d_y, ldy};
     return product8<1, 4, false>(W, d_x, dtype, ldx, M, out, d_work, who, as_stream(stream));
 }
 
@@ -224,6 +224,6 @@ extern "C" int cmlb200_linear_dense8_glu(const cmlb200_dense8* W, const void* d_
     if (rc) return rc;
     CMLB_REQUIRE(ff > 0 && W->rows == 2 * ((ff + 15) & ~15) && ldf >= ff && ((uintptr_t)d_f & 1) == 0, "%s: %d weight rows for %d outputs, stride %ld", who, W->rows, ff, ldf);
     CMLB_REQUIRE(act == CMLB200_ACT_SILU || act == CMLB200_ACT_GELU_TANH || act == CMLB200_ACT_GELU_ERF, "%s: activation %d", who, act);
-    const Out8 out = {W->scale, nullptr, nullptr, 0.f, act, ff, d_f, (int)ldf};
+    const Out8 out = {W->scale, nullptr, nullptr, 0.f, act, ff, d_f, ldf};
     return product8<2, 2, true>(W, d_x, dtype, ldx, M, out, d_work, who, as_stream(stream));
 }

@@ -12,6 +12,7 @@
 // greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down, and draws over the one row (and the drafter's)
 // that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
 // Few rows are bound by the chain of dependent loads and by code that is fetched anew with every launch (hence small loops, and what is seldom needed out of the way), many by memory.
+#include <atomic>
 #include <type_traits>
 
 #include "lm_util.cuh"
@@ -441,6 +442,30 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     }
 }
 
+// 16 where the device can place a cluster of so many, otherwise 8
+template <typename T>
+int most_ranks() {
+    static std::atomic<int> known[kMaxDevices] = {};
+    std::atomic<int>& n = known[cmlb_device_index()];
+    if (!n.load()) {
+        int clusters = 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(MOST_RANKS);
+        cfg.blockDim = dim3(VT_THREADS);
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = MOST_RANKS;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        const bool fits = cudaFuncSetAttribute(draft_token_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                          cudaOccupancyMaxActiveClusters(&clusters, draft_token_kernel<T>, &cfg) == cudaSuccess && clusters > 0;
+        if (!fits) cudaGetLastError();
+        n.store(fits ? MOST_RANKS : 8);
+    }
+    return n.load();
+}
+
 template <typename T>
 int launch_verify(const Verify& v, const void* logits, int* accepted, int* next, void* work, cudaStream_t st) {
     const int drafts = v.d.rows - v.d.sequences, sides = v.d.logits ? 2 : 1;
@@ -450,16 +475,9 @@ int launch_verify(const Verify& v, const void* logits, int* accepted, int* next,
     if (drafts)
         CMLB_CUDA(launch_chain(draft_stats_kernel<T>, dim3((unsigned)((long)drafts * sides * splits)), dim3(VS_THREADS), 0, 1, st, v, static_cast<const T*>(logits), sides, splits, stats));
     // as many CTAs a sequence as find an SM each, but 2,048 tokens at least
+    const int most = most_ranks<T>();
     int ranks = 1;
-    while (ranks < MOST_RANKS && (long)v.d.sequences * ranks * 2 <= (ranks < 8 ? 2l * cmlb_num_sms() : cmlb_num_sms() / 2) && v.vocab > ranks * 2048) ranks *= 2;
-    if (ranks > 8) {
-        static bool allowed[kMaxDevices] = {};
-        const int dev = cmlb_device_index();
-        if (!allowed[dev]) {
-            CMLB_CUDA(cudaFuncSetAttribute(draft_token_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            allowed[dev] = true;
-        }
-    }
+    while (ranks < most && (long)v.d.sequences * ranks * 2 <= (ranks < 8 ? 2l * cmlb_num_sms() : cmlb_num_sms() / 2) && v.vocab > ranks * 2048) ranks *= 2;
     CMLB_CUDA(launch_chain(draft_token_kernel<T>, dim3((unsigned)(v.d.sequences * ranks)), dim3(VT_THREADS), 0, ranks, st, v, static_cast<const T*>(logits), sides, splits, (const Stat*)stats, ranks,
                            accepted, next));
     return CMLB200_OK;

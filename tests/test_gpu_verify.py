@@ -293,3 +293,35 @@ def test_draws_are_distributed(pkg, torch_dev):
         count = np.bincount(token, minlength=V)
         chi = ((count - S * p) ** 2 / (S * p)).sum()
         assert chi < 8 + 6 * np.sqrt(16) + 6, (count / S, p)
+
+
+CAPTURED_FIRST = """
+import sys
+sys.path.insert(0, {root!r})
+sys.path.insert(0, {tests!r})
+import torch
+import __graft_entry__ as entry
+from test_gpu_verify import Batch
+pkg = entry.load_package()
+b = Batch(torch, torch.device("cuda:0"), {counts}, 40000, 5)
+k = {{}}
+b.call(pkg, keep=k)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    k["run"](torch.cuda.current_stream().cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+b.check(k["out"][:, :len(b.counts)].cpu().numpy())
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("counts", [[3], [0, 2] * 20])
+def test_captured_before_anything_else_ran(counts):
+    import subprocess
+    import sys
+    from pathlib import Path
+    tests = Path(__file__).resolve().parent
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.format(root=str(tests.parent), tests=str(tests), counts=counts)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
