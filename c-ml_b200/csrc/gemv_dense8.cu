@@ -7,7 +7,9 @@
 // sums meet in shared memory by atomic additions (whole numbers: the order makes no difference).
 //
 // Rows of x: few of them (M K up to kFused) every CTA quantises itself, into shared memory, while its first weights are on their way: one launch instead of two, and no codes in
-// memory. More come as codes from cmlb200_quantize_rows, through L1, where a warp finds its own columns again with every tile. What is left goes to the tensor-core product of
+// memory. (A warp's work for an output is a few instructions a weight byte, so what bounds these calls is memory, or a launch and its prologue: gate and up rows of 11008x4096 15.7 us for one row of x, 5.7 TB/s;
+// 32000x8192 for 4 rows 44 us, 6.0 TB/s; 4096x4096 5.0 us, of which the bytes are 2.6. With CTAs of 16 weight rows each and a launch of its own for the codes: 19.7, 49 and 5.6.)
+// More rows come as codes from cmlb200_quantize_rows, through L1, where a warp finds its own columns again with every tile. What is left goes to the tensor-core product of
 // prompts (gemm_dense8.cu).
 #include <type_traits>
 

@@ -2,7 +2,9 @@
 //
 // A group of warps has a row: its threads hold up to KEEP pieces of 16 values, agree on the largest magnitude and write the codes. Rows longer than what they hold are read a second time,
 // from L2. Few rows: a CTA of as many threads as a row has pieces, so that all of it is under way at once (one row of 4,096 bf16 1.7 us). Many: CTAs of 512 threads that have several short
-// rows or one long one; with a CTA a row, starting CTAs was what took the time (2,048 rows of 4,096: 10.5 us, QT_2048 so).
+// rows or one long one; with a CTA a row, starting CTAs was what took the time (2,048 rows of 4,096: 10.5 us, 7.3 so).
+// 4,096 rows of 28,672 bf16 60 to 79 us (4.5 to 5.8 TB/s: memory), 22,016 of 4,096 44 us (6.1 TB/s). A branch for every value next to a tie, or a division, cost more than the bytes: with those the same
+// rows took 122 and 116 us, since one word in seven of a warp holds half of its row's largest number.
 // Rows that do not lie on 16-byte boundaries: a thread's 16 values are four times four, 128 apart, so that a warp's loads of single values touch neighbouring bytes.
 #include <type_traits>
 
