@@ -24,6 +24,12 @@ namespace {
 constexpr int VS_THREADS = 256, VT_THREADS = 512, VS_SPLITS = 16, MOST_RANKS = 16;
 constexpr float kGreedy = 1e-5f;                       // colder is greedy
 constexpr float kClose = 0.998f;
+constexpr int MOST_VOCAB = 1 << 28;
+// (infinite ones would make no number of the logits of tokens that cannot come; no number at all stays that, which is greedy)
+__device__ __forceinline__ float heat_of(const cmlb200_drafts& d, int s) {
+    const float t = d.temperature ? d.temperature[s] : 1.f;
+    return t > 1e30f ? 1e30f : t;
+}
 
 // Of a part of a row: largest value, its first place (greedy; otherwise the draft's logit), sum of e^((x - most) / T). A sum that is not a number: the part holds NaN or +inf
 struct Stat { float most; int at; float sum; int pad; };
@@ -96,7 +102,7 @@ draft_stats_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     __syncthreads();
     const int s = mine;
     if (s < 0) return;                                 // (rows that no sequence has)
-    const float heat = v.d.temperature ? v.d.temperature[s] : 1.f;
+    const float heat = heat_of(v.d, s);
     const bool greedy = !(heat >= kGreedy);
     if (greedy && side) return;
     const T* row = side ? static_cast<const T*>(v.d.logits) + (size_t)i * v.d.ld : logits + (size_t)(i + s) * v.ld;
@@ -251,7 +257,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     }
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (met below: the cluster's CTAs have begun)
     const int n = end - first - 1;
-    const float heat = v.d.temperature ? v.d.temperature[s] : 1.f;
+    const float heat = heat_of(v.d, s);
     const bool greedy = !(heat >= kGreedy);
     const double rate = greedy ? 0.0 : 1.0 / (double)heat;
     const float c = greedy ? 0.f : __fdiv_rn(kLog2e, heat);
@@ -496,7 +502,7 @@ extern "C" int cmlb200_verify_drafts(const cmlb200_drafts* d, const void* d_logi
     static const char* who = "cmlb200_verify_drafts";
     CMLB_REQUIRE(d && d_logits && d_accepted && d_next && d_work && d->first, "%s: NULL argument", who);
     CMLB_REQUIRE(d->sequences > 0 && d->rows >= d->sequences && d->rows <= (1 << 20), "%s: %d rows of %d sequences", who, d->rows, d->sequences);
-    CMLB_REQUIRE(vocab > 0 && ld >= vocab && (!d->logits || d->ld >= vocab), "%s: %d logits, strides %ld and %ld", who, vocab, ld, d->ld);
+    CMLB_REQUIRE(vocab > 0 && vocab <= MOST_VOCAB && ld >= vocab && (!d->logits || d->ld >= vocab), "%s: %d logits, strides %ld and %ld", who, vocab, ld, d->ld);
     CMLB_REQUIRE(d->tokens || d->rows == d->sequences, "%s: %d drafts without tokens", who, d->rows - d->sequences);
     CMLB_REQUIRE(d->random || d->temperature, "%s: no random numbers, and no temperatures that could do without", who);
     CMLB_REQUIRE((((uintptr_t)d_logits | (uintptr_t)d->logits) & (dtype == CMLB200_DT_F32 ? 3 : 1)) == 0 && ((uintptr_t)d_work & 15) == 0 && ((uintptr_t)d->random & 7) == 0,

@@ -163,6 +163,22 @@ def test_same_logits(pkg, torch_dev):
 
 
 @pytest.mark.parametrize("form", FORMS)
+def test_without_end(pkg, torch_dev, form):
+    """Infinite temperatures: any token that can come is as likely as any other, and those that cannot still do not. What is no temperature is greedy."""
+    import torch
+    b = Batch(torch, torch_dev, [4] * 30, 300, 8, form, True)
+    b.target[:, ::3] = b.draft[:, ::3] = -float("inf")
+    b.tokens = (b.tokens // 3 * 3 + 1).astype(np.int32)
+    got = []
+    for t in (np.inf, 1e38, 1e30, np.nan, 0.0):
+        b.t[:] = t
+        got.append(b.call(pkg))
+    assert (got[0] == got[2]).all() and (got[1] == got[2]).all() and (got[3] == got[4]).all()
+    assert (got[0][0] == 4).all()                      # p = q: u p < p
+    assert (got[0][1] % 3 != 0).all() and len(set(got[0][1])) > 20
+
+
+@pytest.mark.parametrize("form", FORMS)
 def test_masked(pkg, torch_dev, form):
     """Tokens that cannot come: never drawn; a draft that the target rules out is turned down, one that the drafter ruled out is kept where the target allows it."""
     import torch

@@ -63,7 +63,7 @@ def test_drafts(pkg, bad):
     assert pkg.lib.cmlb200_verify_drafts(drafts(pkg, **bad), P, 0, 50, 50, P, P, P, None) == -1 and pkg.last_error()
 
 
-@pytest.mark.parametrize("args", [(None, 0, 50, 50, P, P, P), (P, 0, 49, 50, P, P, P), (P, 0, 50, 0, P, P, P), (P, 0, 50, 50, None, P, P), (P, 0, 50, 50, P, None, P), (P, 0, 50, 50, P, P, None),
+@pytest.mark.parametrize("args", [(None, 0, 50, 50, P, P, P), (P, 0, 49, 50, P, P, P), (P, 0, 50, 0, P, P, P), (P, 0, (1 << 28) + 1, (1 << 28) + 1, P, P, P), (P, 0, 50, 50, None, P, P), (P, 0, 50, 50, P, None, P), (P, 0, 50, 50, P, P, None),
                                   (P, 0, 50, 50, P, P, P + 8), (P + 2, 0, 50, 50, P, P, P), (P, 3, 50, 50, P, P, P), (P + 1, 1, 50, 50, P, P, P)])
 def test_verify(pkg, args):
     assert pkg.lib.cmlb200_verify_drafts(drafts(pkg), *args, None) == -1
