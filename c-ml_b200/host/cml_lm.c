@@ -295,6 +295,7 @@ static void release_passed(CMLLanguageModel* lm, int seq) {
 void cml_lm_keep_behind(CMLLanguageModel* lm, int tokens) { lm->keep_behind = tokens; }
 const float* cml_lm_logits(const CMLLanguageModel* lm) { return lm->d_logits; }
 int cml_lm_step_rows(const CMLLanguageModel* lm) { return lm->opt.max_step_rows; }
+long cml_lm_longest(const CMLLanguageModel* lm) { return (long)lm->table_ld * BLOCK; }
 int cml_lm_takes_drafts(const CMLLanguageModel* lm) { return lm->cache && !lm->slot_pages.pools; }
 
 int cml_lm_sequence_truncate(CMLLanguageModel* lm, int seq, int length) {

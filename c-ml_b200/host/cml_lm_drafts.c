@@ -24,11 +24,11 @@ typedef struct Drafting {
     size_t row;                    /* bytes */
 } Drafting;
 
-/* The prompt into a model, as many tokens as a step takes at a time; picked: the token drawn behind it (NULL: none). */
-static int read_prompt(Drafting* d, CMLLanguageModel* lm, int seq, int portion, const int* prompt, int n, int* picked) {
+/* Tokens into a model, as many tokens as a step takes at a time; picked: the token drawn behind it (NULL: none). */
+static int read_prompt(Drafting* d, CMLLanguageModel* lm, int seq, int portion, const int* tokens, int n, int* picked) {
     for (int at = 0; at < n; at += portion) {
         const int k = n - at < portion ? n - at : portion, last = k - 1, ask = picked && at + k == n;
-        const CMLLMEntry e = {seq, prompt + at, k, &last, ask};
+        const CMLLMEntry e = {seq, tokens + at, k, &last, ask};
         const uint64_t r = ask ? next_random(&d->random) : 0;
         if (ask ? cml_lm_step_sampled(lm, &e, 1, &d->temperature, &r, picked) : cml_lm_step(lm, &e, 1, NULL)) return -1;
     }
@@ -39,10 +39,7 @@ static int read_prompt(Drafting* d, CMLLanguageModel* lm, int seq, int portion, 
 static int draw_drafts(Drafting* d, const int* tokens, int n, int count, int* drafts) {
     const int has = cml_lm_sequence_length(d->drafter, d->draft_seq);
     for (int i = 0; i < count; i++) {
-        const int k = i ? 1 : n - has, last = k - 1;
-        const CMLLMEntry e = {d->draft_seq, i ? drafts + i - 1 : tokens + has, k, &last, 1};
-        const uint64_t r = next_random(&d->random);
-        if (cml_lm_step_sampled(d->drafter, &e, 1, &d->temperature, &r, drafts + i)) return -1;
+        if (read_prompt(d, d->drafter, d->draft_seq, cml_lm_step_rows(d->drafter), i ? drafts + i - 1 : tokens + has, i ? 1 : n - has, drafts + i)) return -1;
         if (drafts[i] < 0) return i;                       /* (no distribution: the drafts end here) */
         if (CML_DEV_FAIL(cmlb200_memcpy_d2d((char*)d->d_probabilities + (size_t)i * d->row, cml_lm_logits(d->drafter), d->row, NULL), __func__) || CML_DEV_FAIL(cmlb200_stream_sync(NULL), __func__))
             return -1;
@@ -61,6 +58,11 @@ CMLGenerationResult* cml_lm_generate_drafted(CMLLanguageModel* lm, CMLLanguageMo
     c.eos_token_id = -1;
     if (config) c = *config;
     if (c.max_new_tokens <= 0) c.max_new_tokens = 256;
+    if ((long)num_tokens + c.max_new_tokens > cml_lm_longest(lm) || (long)num_tokens + c.max_new_tokens > cml_lm_longest(drafter)) {
+        LOG_ERROR("%s: %d tokens behind %d, sequences of %ld and %ld", who, c.max_new_tokens, num_tokens, cml_lm_longest(lm), cml_lm_longest(drafter));
+        return NULL;
+    }
+    if (drafts > cml_lm_step_rows(lm) - 1) drafts = cml_lm_step_rows(lm) - 1;
     Drafting d = {lm, drafter, -1, -1, c.do_sample ? c.temperature : 0.0f, seed, NULL, (size_t)cml_lm_vocab_size(lm) * sizeof(float)};
     CMLLMDraftStats s = {0, 0, 0};
     struct timespec t0, t1;
@@ -72,7 +74,7 @@ CMLGenerationResult* cml_lm_generate_drafted(CMLLanguageModel* lm, CMLLanguageMo
     if (ok) memcpy(res->token_ids, prompt, (size_t)num_tokens * sizeof(int));
     /* what a rejected draft took may be behind a window by then */
     cml_lm_keep_behind(drafter, drafts + 1);
-    ok = ok && !CML_DEV_FAIL(cmlb200_malloc((void**)&d.d_probabilities, (size_t)drafts * d.row), who) && (d.seq = cml_lm_sequence_open(lm)) >= 0 && (d.draft_seq = cml_lm_sequence_open(drafter)) >= 0 &&
+    ok = ok && !CML_DEV_FAIL(cmlb200_malloc((void**)&d.d_probabilities, (size_t)(drafts + 1) * d.row), who) && (d.seq = cml_lm_sequence_open(lm)) >= 0 && (d.draft_seq = cml_lm_sequence_open(drafter)) >= 0 &&
          !read_prompt(&d, lm, d.seq, cml_lm_step_rows(lm), prompt, num_tokens, &token) && !read_prompt(&d, drafter, d.draft_seq, cml_lm_step_rows(drafter), prompt, num_tokens, NULL);
     if (ok && token < 0) { LOG_ERROR("%s: the prompt's logits hold no distribution", who); ok = 0; }
     if (ok) {

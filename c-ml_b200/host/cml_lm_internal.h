@@ -64,6 +64,7 @@ const float* cml_lm_logits(const CMLLanguageModel* lm);
 void cml_lm_keep_behind(CMLLanguageModel* lm, int tokens);
 int cml_lm_takes_drafts(const CMLLanguageModel* lm);
 int cml_lm_step_rows(const CMLLanguageModel* lm);              /* tokens of a step at most */
+long cml_lm_longest(const CMLLanguageModel* lm);                /* tokens of a sequence at most, of models with a paged cache */
 
 /* Classes register themselves before main (a program links those it wants). */
 void cml_lm_register(const CMLLMClass* cls);

@@ -107,7 +107,7 @@ CMLGenerationResult* cml_lm_generate(CMLLanguageModel* lm, const int* prompt, in
 /* Generates from a prompt with drafts of another model of the same vocabulary, on the same device: it draws `drafts` (1 .. 32) tokens one by one, of which a step of `lm` keeps what fits its own
  * distribution (cml_lm_step_verified, with the drafter's own probabilities): the result is distributed as cml_lm_step_sampled's, whatever the drafter is, and equals it where config is greedy (up to
  * rounding: a step of several tokens multiplies in other kernels than one of a single token). The same folder loaded with 8-bit weights is a drafter. config NULL: greedy, 256 tokens; its top_k and
- * top_p are not looked at. Neither model may keep a state per sequence. stats may be NULL. */
+ * top_p are not looked at. Steps that are shorter than drafts + 1 bring as many drafts as they hold. Neither model may keep a state per sequence, and both hold the prompt and max_new_tokens. stats may be NULL. */
 typedef struct CMLLMDraftStats {
     int steps, drafted, accepted;
 } CMLLMDraftStats;

@@ -200,6 +200,27 @@ def test_generation_ends(synth, tmp_path, load):  # noqa: F811
         assert m.generate_drafted(d, 4, t, 40, eos=eos)[0] == whole[:whole.index(eos) + 1]
 
 
+def test_short_steps(synth, tmp_path, load):  # noqa: F811
+    """Steps of a few tokens: as many drafts as go into one, a drafter that takes what it has not seen one by one, and no drafts where a step is a single token."""
+    cfg, w, folder = lm_util.build(synth, tmp_path, "plain")
+    t = list(prompt(cfg, 20))
+    for rows, draft_rows in ((3, 1), (1, 1), (2, 2), (1, 40)):
+        m, d = load(folder, max_step_rows=rows), load(folder, max_step_rows=draft_rows)
+        got, (steps, drafted, accepted) = m.generate_drafted(d, 4, t, 30)
+        assert len(got) == 30 and drafted <= steps * (rows - 1) and (drafted > 0) == (rows > 1)
+        logits = lm_util.reference(cfg, w, t + got)[len(t) - 1:-1]
+        assert (logits.max(1) - logits[np.arange(30), got] <= 6 * lm_util.TOL[6] * logits.std()).all()
+
+
+def test_lengths_out_of_range(pkg, synth, tmp_path, load):  # noqa: F811
+    cfg, w, folder = lm_util.build(synth, tmp_path, "plain")
+    m, d = load(folder), load(folder)
+    for n in (2 ** 31 - 1, 2 ** 31 - 40, 20000):        # (more than numbers, or the pool, hold: what was taken is given back)
+        with pytest.raises(pkg.CmlB200Error):
+            m.generate_drafted(d, 4, list(prompt(cfg, 30)), n)
+        assert pkg_free(m) and pkg_free(d)
+
+
 def test_sampled_generation(synth, tmp_path, load):  # noqa: F811
     """Drafted generation has the model's own distribution: third tokens of many runs, beside what the model's probabilities say of them, with a drafter that is another model."""
     cfg, w, folder = lm_util.build(synth, tmp_path, "plain")
