@@ -301,8 +301,8 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
         // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with the least that its wait can be is looked at; there are
         // few, and only for those a wait is worked out. Where w is p alone it is relative to the largest logit that the warp has met, so that logits far from zero lose no digits (greedy: the logits
         // themselves).
-        float best = greedy ? -INFINITY : 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
-        int at = 0x7fffffff, bad = 0;
+        float best = greedy ? -INFINITY : 0.f, second = 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
+        int at = 0x7fffffff, at2 = 0x7fffffff, bad = 0;
         constexpr int U = 2;                           // groups of four tokens under way
 #pragma unroll 1
         for (int g0 = lo + warp * 32; g0 < hi; g0 += U * VT_THREADS) {
@@ -335,6 +335,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
                     if (__any_sync(0xffffffffu, top > ref)) {
                         const float to = fmaxf(ref, warp_max(top)), by = ref == -INFINITY ? 0.f : ex2((ref - to) * c);
                         best *= by;
+                        second *= by;
                         bound *= by;
                         ref = to;
                     }
@@ -356,15 +357,22 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const float score = w[e] > 0.f ? __fdividef(w[e], wait_of(u[e])) : 0.f;
-                        if (score > best) { best = score; at = 4 * g + e; }
+                        if (score > second) { second = score; at2 = 4 * g + e; }
+                        if (second > best) {
+                            const float was = best;
+                            const int was_at = at;
+                            best = second; at = at2;
+                            second = was; at2 = was_at;
+                        }
                     }
                     bound = warp_max(best);
                 }
             }
         }
         const float most = greedy ? best : best > 0.f ? lg2(best) : -INFINITY;
-        // CTA and cluster have the best and the one behind it
-        const Best b = {most, -INFINITY, ref, at, bad};
+        // thread, CTA and cluster have the best and the one behind it
+        const float behind = second > 0.f ? lg2(second) : -INFINITY;
+        const Best b = {most, behind, ref, at, bad};
         auto best_of = [&](Best x) {
             x = best_of_lanes(x, c);
             if (lane == 0) w_best[warp] = x;
@@ -422,17 +430,23 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
             constexpr float slack = 1e-3f;
             if (all.z2 >= all.z - slack) {             // (one call in a thousand)
                 cluster_all();                         // everyone has read what comes now is written over
-                const bool close = most > -INFINITY && most + (ref == all.ref ? 0.f : (ref - all.ref) * c) >= all.z - slack;
+                const float by = ref == all.ref ? 0.f : (ref - all.ref) * c;
                 double z = -INFINITY;
-                if (close) {
+                int token = 0x7fffffff;
+#pragma unroll 1
+                for (int k = 0; k < 2; k++) {
+                    const float m = k ? behind : most;
+                    const int j = k ? at2 : at;
+                    if (!(m > -INFINITY && m + by >= all.z - slack)) continue;
                     double w;
                     if (less) {
-                        const double d = far_exp(((double)widen(row[at]) - (double)t.p.most) * rate) / (double)t.p.sum - far_exp(((double)widen(less[at]) - (double)t.q.most) * rate) / (double)t.q.sum;
+                        const double d = far_exp(((double)widen(row[j]) - (double)t.p.most) * rate) / (double)t.p.sum - far_exp(((double)widen(less[j]) - (double)t.q.most) * rate) / (double)t.q.sum;
                         w = d > 0.0 ? far_log(d) : -1e30;      // (what 32 bits took for a weight was their rounding)
-                    } else w = ((double)widen(row[at]) - (double)all.ref) * rate;
-                    z = w - log_wait_exact(philox(key, (uint32_t)at >> 2, 0u).w[at & 3]);
+                    } else w = ((double)widen(row[j]) - (double)all.ref) * rate;
+                    w -= log_wait_exact(philox(key, (uint32_t)j >> 2, 0u).w[j & 3]);
+                    if (w > z || (w == z && j < token)) { z = w; token = j; }
                 }
-                all = exact_best(z, at, all);
+                all = exact_best(z, token, all);
             }
         }
         // where rounding leaves nothing of p - q (or p is nothing but the draft), p itself

@@ -152,6 +152,22 @@ def test_close_calls(pkg, torch_dev):
         assert got[0][s] == 0 and got[1][s] == int(np.argmax(z)), (s, np.sort(z)[-3:], z[got[1][s]])
 
 
+@pytest.mark.parametrize("vocab,at", [(2, (0, 1)), (4, (0, 3)), (4, (1, 2)), (50, (49, 48)), (5000, (2049, 2051)), (40000, (12, 2060)), (40000, (12, 4108))])
+def test_close_neighbours(pkg, torch_dev, vocab, at):
+    """The same where the two tokens are a thread's: of one group of four, or of groups that it looks at one after another."""
+    import torch
+    b = Batch(torch, torch_dev, [0] * 400, vocab, 80)
+    rng, at = np.random.default_rng(vocab), list(at)
+    x = np.full((400, vocab), -40.0)
+    for s in range(400):
+        x[s, at] = np.log(drafts_oracle.waits(int(b.key[s]), vocab))[at] + rng.normal(size=2) * 2e-6
+    b.target[:] = torch.from_numpy(x).float()
+    got, x = b.call(pkg), b.target.double().cpu().numpy()
+    for s in range(400):
+        z = x[s] - np.log(drafts_oracle.waits(int(b.key[s]), vocab))
+        assert got[0][s] == 0 and got[1][s] == int(np.argmax(z)), (s, z[at] - z.max(), got[1][s])
+
+
 def test_same_logits(pkg, torch_dev):
     """A drafter whose logits are the target's: everything is kept."""
     import torch
