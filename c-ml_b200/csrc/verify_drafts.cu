@@ -11,8 +11,8 @@
 // Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: largest value and sum of exponentials, fp32 in a thread and fp64 between threads (or, for
 // greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down, and draws over the one row (and the drafter's)
 // that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
-// Measured: four drafts of one sequence over 32,000 tokens 8.6 us, of 32 sequences over 128,000 40 (22.5 for the bytes: 25 for the tested rows, 15 for the draws, which are 50 instructions a token, a third of
-// them Philox, on 256 CTAs), one draw over 32,000 4.4, 64 over 128,000 23.
+// Measured: four drafts of one sequence over 32,000 tokens 8.7 us, of 32 sequences over 128,000 41 (22.5 for the bytes: 25 for the tested rows, 15 for the draws, which are 45 instructions a token, a third of
+// them Philox, on 256 CTAs), one draw over 32,000 4.6, 64 over 128,000 23.5.
 // Few rows are bound by the chain of dependent loads and by code that is fetched anew with every launch (hence small loops, and what is seldom needed out of the way), many by memory.
 #include <atomic>
 #include <type_traits>
@@ -298,7 +298,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     const int groups = (V + 3) / 4, per = (groups + ranks - 1) / ranks, lo = rank * per, hi = min(groups, lo + per);
     bool first_time = true;
     for (int pass = 0;; pass++) {
-        // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with the least that its wait can be is looked at; there are
+        // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with v, which is never above its wait, is looked at; there are
         // few, and only for those a wait is worked out. Where w is p alone it is relative to the largest logit that the warp has met, so that logits far from zero lose no digits (greedy: the logits
         // themselves).
         float best = greedy ? -INFINITY : 0.f, second = 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
@@ -326,7 +326,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
                     continue;
                 }
                 const Philox r = philox(key, (uint32_t)g, 0u);
-                float w[4], u[4];
+                float w[4];
                 if (less) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - t.p.most) * c) * p_unit - ex2((y[k][e] - t.q.most) * c) * q_unit;
@@ -349,14 +349,11 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
                 }
                 bool any = false;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    u[e] = uniform_of(r.w[e]);
-                    any |= w[e] > bound * kClose * least_wait(u[e]);
-                }
+                for (int e = 0; e < 4; e++) any |= w[e] > bound * (float)r.w[e];
                 if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float score = w[e] > 0.f ? __fdividef(w[e], wait_of(u[e])) : 0.f;
+                        const float score = w[e] > 0.f ? __fdividef(w[e], wait_of(uniform_of(r.w[e]))) : 0.f;
                         if (score > second) { second = score; at2 = 4 * g + e; }
                         if (second > best) {
                             const float was = best;
@@ -365,7 +362,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
                             second = was; at2 = was_at;
                         }
                     }
-                    bound = warp_max(best);
+                    bound = warp_max(best) * (kClose * 2.3283064365386963e-10f);
                 }
             }
         }
