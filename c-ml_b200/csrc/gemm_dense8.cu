@@ -15,7 +15,7 @@
 //               into its shared memory. Since they are whole numbers the order of adding makes no difference.
 // What bounds it. Many tokens: an SM reads 64 KB from L2 for the 1,024 cycles of MMAs of a stage of 256 x 256 x 256, and gets them in about 1,250 (13.5 TB/s in all): tensor cores 85 % busy, 4,096 tokens of
 // 8192x8192 175 us; for seconds on end the power limit, 4,096 of 8192x28672 640 us and 3.0 POP/s. Few tokens: the weight's bytes, and beside them the codes' launch, 0.7 us from its end to the first
-// MMA, 0.4 us behind the last, 0.6 to 2.5 us of epilogue (77 of 11008x4096 13.7 us, the bytes 7.3; 500 of 6144x4096 18.4; 256 of 4096x4096 11.4).
+// MMA, 0.4 us behind the last, 0.6 to 2.5 us of epilogue (77 of 11008x4096 13.7 us, the bytes 7.3; 500 of 6144x4096 18.1; 256 of 4096x4096 11.5).
 // The one thread that loads and the warp that issues MMAs were what took the time before: places found by division 900 cycles a block, a wait, a fence and a commit for every 128 columns 500.
 // No load is multicast. Every wait on an mbarrier is bounded; on expiry the CTA raises a status word (cmlb200_dense8_status), waits for its copies and MMAs in flight, frees its tensor
 // memory and returns.

@@ -2,7 +2,8 @@
 //
 // A group of warps has a row: its threads hold up to KEEP pieces of 16 values, agree on the largest magnitude and write the codes. Rows longer than what they hold are read a second time,
 // from L2. Few rows: a CTA of as many threads as a row has pieces, so that all of it is under way at once (one row of 4,096 bf16 1.7 us). Many: CTAs of 512 threads that have several short
-// rows or one long one; with a CTA a row, starting CTAs was what took the time (2,048 rows of 4,096: 10.5 us, 7.3 so).
+// rows or one long one; with a CTA a row, starting CTAs was what took the time (2,048 rows of 4,096: 10.5 us, 7.3 so), with fewer CTAs than SMs the chain of a thread's pieces (500 rows of 4,096 4.5 us, a CTA each 3.1; 333 of 777 3.1
+// and 2.0; 1,000 of 4,096 with four warps each instead of two 5.8 to 4.8).
 // 4,096 rows of 28,672 bf16 60 to 79 us (4.5 to 5.8 TB/s: memory), 22,016 of 4,096 44 us (6.1 TB/s). A branch for every value next to a tie, or a division, cost more than the bytes: with those the same
 // rows took 122 and 116 us, since one word in seven of a warp holds half of its row's largest number.
 // Rows that do not lie on 16-byte boundaries: a thread's 16 values are four times four, 128 apart, so that a warp's loads of single values touch neighbouring bytes.
@@ -72,13 +73,14 @@ quantize_rows_kernel(const T* __restrict__ x, long ldx, int rows, int cols, int 
 template <typename T>
 int launch_rows(const void* x, long ldx, int rows, int cols, int8_t* q, long ldq, float* scale, cudaStream_t st) {
     const int whole = (((uintptr_t)x | ((uintptr_t)ldx * sizeof(T))) & 15) == 0, warps = ((cols + 127) / 128 * 8 + 31) / 32;         // of a thread a piece
-    if (rows <= 2 * cmlb_num_sms()) {
+    // a CTA a row where they are few, or all resident at once; otherwise as many warps a row as its pieces need, or as give every SM a CTA
+    if (rows <= 2 * cmlb_num_sms() || (rows <= 4 * cmlb_num_sms() && (long)rows * warps <= 64l * cmlb_num_sms())) {
         const int group = warps < 32 ? warps : 32;
         CMLB_CUDA(launch_chain(quantize_rows_kernel<T, 1>, dim3(rows), dim3(group * 32), 0, 1, st, static_cast<const T*>(x), ldx, rows, cols, whole, group, q, ldq, scale));
     } else {
         constexpr int KEEP = 8 / (int)sizeof(T);
         int group = 1;
-        while (group < 16 && group * KEEP < warps) group *= 2;
+        while (group < 16 && (group * KEEP < warps || (group < warps && rows * (long)group < 16l * cmlb_num_sms()))) group *= 2;
         CMLB_CUDA(launch_chain(quantize_rows_kernel<T, KEEP>, dim3((rows * (long)group + 15) / 16), dim3(512), 0, 1, st, static_cast<const T*>(x), ldx, rows, cols, whole, group, q, ldq, scale));
     }
     return CMLB200_OK;

@@ -63,6 +63,13 @@ def test_rows(pkg, torch_dev, form, rows, cols):
 
 
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("rows,cols", [(593, 777), (600, 4097), (1100, 2050), (2500, 130), (1200, 9000), (7000, 33)])
+def test_many_rows(pkg, torch_dev, form, rows, cols):
+    """CTAs of several rows, in every number of warps."""
+    test_rows(pkg, torch_dev, form, rows, cols)
+
+
+@pytest.mark.parametrize("form", FORMS)
 def test_ties_and_ends(pkg, torch_dev, form):
     """Ties that a scale rounded to 32 bits would miss; zeros; the smallest and largest numbers; rows that are not numbers."""
     import torch
