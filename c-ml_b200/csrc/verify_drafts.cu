@@ -11,8 +11,8 @@
 // Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: largest value and sum of exponentials, fp32 in a thread and fp64 between threads (or, for
 // greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down, and draws over the one row (and the drafter's)
 // that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
-// Measured: four drafts of one sequence over 32,000 tokens 8.7 us, of 32 sequences over 128,000 41 (22.5 for the bytes: 25 for the tested rows, 15 for the draws, which are 45 instructions a token, a third of
-// them Philox, on 256 CTAs), one draw over 32,000 4.6, 64 over 128,000 23.5.
+// Measured: four drafts of one sequence over 32,000 tokens 8.7 us, of 32 sequences over 128,000 40 (22.5 for the bytes: 25 for the tested rows, 14 for the draws, which are some 45 instructions a token, a third of
+// them Philox, on 256 CTAs), one draw over 32,000 4.6, 64 over 128,000 22 (with the waits of all four tokens worked out where one could win: 23.5).
 // Few rows are bound by the chain of dependent loads and by code that is fetched anew with every launch (hence small loops, and what is seldom needed out of the way), many by memory.
 #include <atomic>
 #include <type_traits>
@@ -353,7 +353,8 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
                 if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float score = w[e] > 0.f ? __fdividef(w[e], wait_of(uniform_of(r.w[e]))) : 0.f;
+                        if (!(w[e] > bound * (float)r.w[e])) continue;
+                        const float score = __fdividef(w[e], wait_of(uniform_of(r.w[e])));
                         if (score > second) { second = score; at2 = 4 * g + e; }
                         if (second > best) {
                             const float was = best;
