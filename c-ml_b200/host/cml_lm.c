@@ -316,7 +316,7 @@ int cml_lm_sequence_truncate(CMLLanguageModel* lm, int seq, int length) {
 /* Everything that can be wrong with a step, before anything changes. Returns the number of rows, -1. */
 static int check_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, int* want, const char* who) {
     if (!lm || !entries || n <= 0) { LOG_ERROR("%s: invalid arguments", who); return -1; }
-    long rows = 0, blocks = 0;
+    long rows = 0, blocks = 0, wanted = 0;
     int bad = 0;
     *want = 0;
     memset(lm->in_step, 0, (size_t)lm->opt.max_sequences);
@@ -339,11 +339,13 @@ static int check_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, in
             blocks += cml_paged_cache_blocks_for(lm->cache, e->seq, e->num_tokens);
         }
         rows += e->num_tokens;
-        *want += e->num_want;
+        wanted += e->num_want;
         bad = 0;
     }
     if (bad) return -1;
     if (rows > lm->opt.max_step_rows) { LOG_ERROR("%s: %ld tokens in a step of at most %d", who, rows, lm->opt.max_step_rows); return -1; }
+    if (wanted > lm->opt.max_step_rows && wanted > SMALL_ROWS) { LOG_ERROR("%s: %ld places wanted in a step of at most %d tokens", who, wanted, lm->opt.max_step_rows); return -1; }
+    *want = (int)wanted;
     if (lm->cache && blocks > lm->cache->free_count) { LOG_ERROR("%s: %ld blocks needed, %d free", who, blocks, lm->cache->free_count); return -1; }
     return (int)rows;
 }
@@ -355,8 +357,8 @@ static int round_keys(int keys) {
 }
 
 /* Fills the packed row array from the entries (whose sequences have grown already) and uploads it. */
-static int upload_rows(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, int rows, CMLLMBatch* b, const int** d_want) {
-    const int stride = rows <= SMALL_ROWS ? SMALL_ROWS : (lm->opt.max_step_rows + 3) & ~3;
+static int upload_rows(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, int rows, int wanted, CMLLMBatch* b, const int** d_want) {
+    const int stride = rows <= SMALL_ROWS && wanted <= SMALL_ROWS ? SMALL_ROWS : (lm->opt.max_step_rows + 3) & ~3;
     int *tok = lm->h_meta, *pos = tok + stride, *slot = pos + stride, *want = slot + stride, *runs = want + stride;
     int *tiles = runs + 4 * lm->opt.max_sequences, num_runs = 0;
     int one = 0, one_keys = 0, w = 0, t = 0, short_rows = 0, short_tiles = 0, short_keys = 0, portions = 0;
@@ -552,7 +554,7 @@ static int run_step(CMLLanguageModel* lm, const CMLLMEntry* entries, int n, floa
     for (int i = 0; i < n; i++) if (grow_sequence(lm, entries[i].seq, entries[i].num_tokens)) return -1;
     CMLLMBatch b;
     const int* d_want;
-    if (upload_rows(lm, entries, n, rows, &b, &d_want)) return -1;
+    if (upload_rows(lm, entries, n, rows, want, &b, &d_want)) return -1;
     const size_t V = (size_t)lm->info.vocab;
     const int first = want < HEAD_ROWS ? want : HEAD_ROWS;
     if ((b.one_rows == rows && rows <= SMALL_ROWS) ? run_captured(lm, &b, d_want, first, greedy) : enqueue_step(lm, &b, d_want, first, greedy)) return -1;
@@ -715,7 +717,7 @@ int cml_lm_decode_greedy(CMLLanguageModel* lm, const int* seqs, const int* first
     CMLLMBatch b;
     const int* d_want;
     for (int i = 0; i < num_seqs; i++) if (grow_sequence(lm, seqs[i], 1)) return -1;
-    if (upload_rows(lm, e, num_seqs, num_seqs, &b, &d_want)) return -1;
+    if (upload_rows(lm, e, num_seqs, num_seqs, num_seqs, &b, &d_want)) return -1;
     for (int i = 0; i < num_seqs; i++) if (steps > 1 && grow_sequence(lm, seqs[i], steps - 1)) return -1;
     b.max_keys = round_keys(max_len);
     DEV(cmlb200_memset(lm->d_step, 0, sizeof(int), lm->stream));

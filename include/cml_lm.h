@@ -42,7 +42,7 @@ typedef struct CMLLMOptions {
 #define CML_LM_CACHE_E4M3 2
 
 /* One sequence's part of a step: its next tokens, and the places among them (ascending) whose logits are
- * asked for. */
+ * asked for: of all entries together no more than a step may have tokens (or 64, where that is more). */
 typedef struct CMLLMEntry {
     int seq;
     const int* tokens;
