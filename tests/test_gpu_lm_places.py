@@ -22,12 +22,13 @@ def test_draws_of_one_row(pkg, synth, tmp_path, load, name, tokens, places):  # 
     line = rng.integers(0, cfg["vocab"], tokens)
     b = m.fork(a)
     logits = m.step([(b, line, None)])[0]
-    c, d = m.fork(a), m.fork(other)
+    d = m.fork(other)
     single = m.step([(d, [5], None)])[0]
     for turn in range(3):                               # (a shape's second step is captured, its third replayed)
         at = np.sort(rng.integers(0, tokens, places))
         key = rng.integers(0, 2 ** 64, places + 1, dtype=np.uint64)
-        got = m.sampled([(c, line, at), (other, [5], [0])], 1.0, key)
+        c, e = m.fork(a), m.fork(other)
+        got = m.sampled([(c, line, at), (e, [5], [0])], 1.0, key)
         rows = np.concatenate([logits[at], single])
         unsure = 0
         for i in range(places + 1):
@@ -37,8 +38,8 @@ def test_draws_of_one_row(pkg, synth, tmp_path, load, name, tokens, places):  # 
             unsure += got[i] != want[1]
             assert z.max() - z[got[i]] <= 6 * lm_util.TOL[6] * rows[i].std(), (turn, i)
         assert unsure <= 1 + 0.1 * places
-        m.truncate(c, 30)
-        m.truncate(other, 9)
+        m.end(c)
+        m.end(e)
 
 
 def test_no_more_than_there_is_room_for(pkg, synth, tmp_path, load):  # noqa: F811
