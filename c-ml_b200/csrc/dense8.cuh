@@ -20,6 +20,8 @@ struct Out8 {
     long ldy;
 };
 
+// cmlb200_quantize_rows; ahead: launches behind it begin before it has written anything (quantize_rows.cu)
+int cmlb_quantize_rows(const void* d_x, int dtype, long ldx, int rows, int cols, int8_t* d_q, long ldq, float* d_scale, int ahead, cudaStream_t st);
 // the product of prompt-sized calls (gemm_dense8.cu)
 int cmlb_gemm_dense8(const cmlb200_dense8* W, const int8_t* xq, int ldq, int M, const Out8& out, int glu, cudaStream_t st);
 

@@ -186,7 +186,7 @@ int product8(const cmlb200_dense8* W, const void* x, int dtype, long ldx, int M,
     int8_t* xq = static_cast<int8_t*>(work);
     const int ldq = (W->cols + 127) / 128 * 128;
     float* xs = reinterpret_cast<float*>(xq + codes_bytes(M, W->cols));
-    const int rc = cmlb200_quantize_rows(x, dtype, ldx, M, W->cols, xq, ldq, xs, st);
+    const int rc = cmlb_quantize_rows(x, dtype, ldx, M, W->cols, xq, ldq, xs, 1, st);
     if (rc) return rc;
     out.xscale = xs;
     if (M <= 8 || (M <= 16 && (long)W->rows * W->cols <= kSmall)) {

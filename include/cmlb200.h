@@ -776,12 +776,12 @@ typedef struct cmlb200_dense8 {
     float cap;                  /* > 0: y = cap tanh(y / cap) */
 } cmlb200_dense8;
 /* Quantises rows of x (CMLB200_DT_F32, _BF16 or _F16, row stride ldx elements) into d_q [rows] of stride ldq, a multiple of 128, and d_scale [rows]. Codes behind
- * the row's end are 0 up to the next multiple of 128. What a model's loader does with a weight, too. */
+ * the row's end are 0 up to the next multiple of 128. What a model's loader does with a weight, too: a product with it may be the next call on the stream. */
 int cmlb200_quantize_rows(const void* d_x, int dtype, long ldx, int rows, int cols, int8_t* d_q, long ldq, float* d_scale, void* stream);
 /* y[M, rows] = x[M, cols] . W^T, x quantised in the call: the sums are whole numbers in 32 bits, exact, then y = sum * (x's scale * W's scale) (+ bias, cap) in fp32. x: fp32, bf16 or fp16
  * rows. _glu: a weight of `ff` gate and `ff` up rows interleaved in groups of 16 (padded with zero rows; bias and cap are not looked at), f = bf16 act(gate) * up with
  * CMLB200_ACT_SILU, _GELU_TANH or _GELU_ERF. d_work: cmlb200_dense8_work_bytes(M, W->rows, W->cols) bytes, 16-byte aligned, that no other call uses meanwhile; what it holds
- * before does not matter. Weights and scales are constants, as those of cmlb200_dense: a kernel that writes them is followed by a synchronisation or a copy. _status: not 0 once a
+ * before does not matter. Weights and scales are constants, as those of cmlb200_dense: a kernel that writes them, but for cmlb200_quantize_rows, is followed by a synchronisation or a copy. _status: not 0 once a
  * bounded wait expired (valid when the stream has drained). */
 size_t cmlb200_dense8_work_bytes(int M, int rows, int cols);
 int cmlb200_linear_dense8(const cmlb200_dense8* W, const void* d_x, int dtype, long ldx, int M, float* d_y, long ldy, void* d_work, void* stream);
