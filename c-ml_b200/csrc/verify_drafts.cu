@@ -8,9 +8,9 @@
 // (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, 2011) keyed by the sequence's 64-bit number: v of token j is word j mod 4 of
 // counter (j / 4, 0, 0, 0), u_i word i mod 4 of counter (i / 4, 1, 0, 0).
 //
-// Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: largest value and sum of exponentials, fp32 in a thread and fp64 between threads (or, for
-// greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down, and draws over the one row (and the drafter's)
-// that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
+// Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: sums of exponentials in fp32, 16 or 32 at a time (or, for
+// greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down (where u q and p lie closer than such sums are sure, sums in 64 bits
+// throughout decide), and draws over the one row (and the drafter's) that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
 // Measured: four drafts of one sequence over 32,000 tokens 8.7 us, of 32 sequences over 128,000 40 (22.5 for the bytes: 25 for the tested rows, 14 for the draws, which are some 45 instructions a token, a third of
 // them Philox, on 256 CTAs), one draw over 32,000 4.6, 64 over 128,000 22 (with the waits of all four tokens worked out where one could win: 23.5).
 // Few rows are bound by the chain of dependent loads and by code that is fetched anew with every launch (hence small loops, and what is seldom needed out of the way), many by memory.
@@ -24,6 +24,11 @@ namespace {
 constexpr int VS_THREADS = 256, VT_THREADS = 512, VS_SPLITS = 16, MOST_RANKS = 16;
 constexpr float kGreedy = 1e-5f;                       // colder is greedy
 constexpr float kClose = 0.998f;
+// What two chances from 32-bit exponentials may be off by together, relative to themselves: an exponential 2^-22 and 2^-23 of its exponent (142 at most); a row's sum 4e-6 for that (of exponents
+// that are 30 at most where they weigh anything), 2e-6 for 32 values added, 3e-6 for parts put together three times, and 2^-24 for each of a thread's 32 values or more, of which there are V / 4096 at
+// most. Closer calls are decided in 64 bits.
+__device__ __forceinline__ double doubt_of(int vocab) { return 3.0517578125e-5 + 2.9103830456733704e-11 * (double)vocab; }
+constexpr float kLazy = 16.f;                          // a sum's reference is changed where a value is 2^16 times as large
 constexpr int MOST_VOCAB = 1 << 28;
 // (infinite ones would make no number of the logits of tokens that cannot come; no number at all stays that, which is greedy)
 __device__ __forceinline__ float heat_of(const cmlb200_drafts& d, int s) {
@@ -31,7 +36,8 @@ __device__ __forceinline__ float heat_of(const cmlb200_drafts& d, int s) {
     return t > 1e30f ? 1e30f : t;
 }
 
-// Of a part of a row: largest value, its first place (greedy; otherwise the draft's logit), sum of e^((x - most) / T). A sum that is not a number: the part holds NaN or +inf
+// Of a part of a row: largest value and its first place (greedy), or a value that none is far above, the draft's logit and the sum of e^((x - most) / T). A sum that is not a number:
+// the part holds NaN or +inf
 struct Stat { float most; int at; float sum; int pad; };
 static_assert(VS_SPLITS <= 16, "a row's parts are put together by half a warp");
 
@@ -64,6 +70,8 @@ __device__ __forceinline__ float wait_of(uint32_t word) {
     const float v = uniform_of(word);
     return v < 0.0625f ? least_wait(v) : lg2(uniform_of(~word)) * -0.6931471805599453f;
 }
+// u of draft i
+__device__ __forceinline__ double coin(uint64_t key, int i) { return (double)philox(key, (uint32_t)i >> 2, 1u).w[i & 3] * 2.3283064365386963e-10; }
 __device__ __noinline__ double far_log(double v) { return log(v); }
 __device__ __noinline__ double far_exp(double v) { return exp(v); }
 // ln of the same: 1 - v is exact in 64 bits
@@ -82,6 +90,12 @@ template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { r
 template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
 __device__ __forceinline__ float max_nan(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
 __device__ __forceinline__ float warp_max(float v) { float m; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v)); return m; }
+
+__device__ __forceinline__ double lane_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 
 struct Verify {
     cmlb200_drafts d;
@@ -146,6 +160,7 @@ draft_stats_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
             }
             continue;
         }
+        float part = 0.f;                              // of 16 or 32 values
 #pragma unroll
         for (int j = 0; j < U; j++) {
             if (p0 + j * VS_THREADS >= hi) break;
@@ -154,14 +169,17 @@ draft_stats_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
             float m = x[0];
 #pragma unroll
             for (int e = 1; e < PER; e++) m = fmaxf(m, x[e]);
-            if (m > most) {
-                sum *= ex2((most - m) * c);            // (from -inf: 0 times 0)
+            if ((m - most) * c > kLazy) {              // (what was there before weighs 2^-16 at most, and so does what its factor is off by)
+                const float by = ex2((most - m) * c);  // (from -inf: 0 times 0)
+                sum *= by;
+                part *= by;
                 most = m;
             }
             const float ref = most == -INFINITY ? 0.f : most;                  // (a NaN still shows)
 #pragma unroll
-            for (int e = 0; e < PER; e++) sum += ex2((x[e] - ref) * c);
+            for (int e = 0; e < PER; e++) part += ex2((x[e] - ref) * c);
         }
+        sum += part;
     }
     // the warp's part, then the CTA's
     auto together = [&]() {
@@ -211,6 +229,19 @@ __device__ __forceinline__ Tested tested(const Stat* parts, int sides, int split
 }
 __device__ __forceinline__ bool holds(const Stat& a) { return a.most > -INFINITY && a.most < INFINITY && a.sum == a.sum; }
 
+// The sum of e^((x - from) rate) over a row that holds numbers, in 64 bits throughout, by a CTA together
+template <typename T> __device__ __noinline__ double exact_sum(const T* row, int vocab, double from, double rate) {
+    __shared__ double warps[VT_THREADS / 32];
+    double sum = 0.0;
+#pragma unroll 1
+    for (int j = threadIdx.x; j < vocab; j += VT_THREADS) sum += exp(((double)widen(row[j]) - from) * rate);
+    sum = lane_sum64(sum);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    return lane_sum64((threadIdx.x & 31) < VT_THREADS / 32 ? warps[threadIdx.x & 31] : 0.0);
+}
+
 __device__ __forceinline__ void cluster_all() { asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // The best of some tokens and the one behind it, as logarithms to the base 2 relative to a logit `ref` times c; the best's token, the lowest of equals
@@ -241,15 +272,33 @@ template <typename T> __device__ __forceinline__ void load4(const T* row, int g,
     }
 }
 
+constexpr int KEPT = 32;                               // drafts whose rows' parts are kept put together
+__device__ __forceinline__ double chance(const Stat& a, double rate) { return far_exp(((double)__int_as_float(a.at) - (double)a.most) * rate); }
+// Draft `from` and those behind it, up to `stop`, of which some lie closer than their rows' sums are sure: with sums in 64 bits throughout. The first that is turned down, or `stop`; a CTA together
+template <typename T>
+__device__ __noinline__ int settle(const T* rows, long ld, const T* drafter, long drafter_ld, const Stat* stats, int splits, int vocab, float heat, uint64_t key, int from, int stop) {
+    const double rate = 1.0 / (double)heat;
+    const float c = __fdiv_rn(kLog2e, heat);
+    const int sides = drafter ? 2 : 1;
+    for (int i = from; i < stop; i++) {
+        const Tested t = tested(stats + (size_t)i * sides * splits, sides, splits, c, false);
+        const bool beside = drafter && holds(t.q);
+        const double u = coin(key, i), p = chance(t.p, rate), q = beside ? chance(t.q, rate) : 1.0;
+        if (!(fabs(u * (beside ? q / (double)t.q.sum : q) - p / (double)t.p.sum) < doubt_of(vocab) * p / (double)t.p.sum)) continue;
+        const double p_sum = exact_sum(rows + (size_t)i * ld, vocab, t.p.most, rate), q_sum = beside ? exact_sum(drafter + (size_t)i * drafter_ld, vocab, t.q.most, rate) : 1.0;
+        if (!(u * (q / q_sum) < p / p_sum)) return i;
+    }
+    return stop;
+}
+
 // grid = sequences * ranks, clusters of `ranks`. Two CTAs an SM: with 71 registers a thread, which leave room for one, 32 sequences of 4 drafts over 128,000 tokens took 56 us instead of 41
 template <typename T>
 __global__ void __launch_bounds__(VT_THREADS, 2)
 draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int splits, const Stat* __restrict__ stats, int ranks, int* __restrict__ accepted, int* __restrict__ next) {
-    __shared__ int stop_at;
+    __shared__ int stop_at, doubt_at;
     __shared__ Best w_best[VT_THREADS / 32], c_best[MOST_RANKS];
     __shared__ double x_best[VT_THREADS / 32 + MOST_RANKS];
     __shared__ int x_at[VT_THREADS / 32 + MOST_RANKS];
-    constexpr int KEPT = 32;                           // drafts whose rows' parts are kept put together
     __shared__ Tested kept_stats[KEPT];
     dep_trigger();
     dep_wait();
@@ -269,7 +318,7 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
     // (known to be the same for a warp: its multiples stay in uniform registers)
     key = (uint64_t)__reduce_or_sync(0xffffffffu, (uint32_t)(key >> 32)) << 32 | __reduce_or_sync(0xffffffffu, (uint32_t)key);
     const int draft0 = first - s;
-    if (threadIdx.x == 0) stop_at = n;
+    if (threadIdx.x == 0) stop_at = doubt_at = n;
     __syncthreads();
     for (int i = warp; i < n; i += VT_THREADS / 32) {          // a warp a draft
         const int token = v.d.tokens[draft0 + i];
@@ -278,13 +327,20 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
         bool kept = token >= 0 && token < V && holds(t.p);
         if (greedy) kept = kept && t.p.at == token;
         else if (kept) {
-            const double q = sides > 1 && holds(t.q) ? far_exp(((double)__int_as_float(t.q.at) - (double)t.q.most) * rate) / (double)t.q.sum : 1.0;
-            kept = (double)philox(key, (uint32_t)i >> 2, 1u).w[i & 3] * 2.3283064365386963e-10 * q < far_exp(((double)__int_as_float(t.p.at) - (double)t.p.most) * rate) / (double)t.p.sum;
+            const double q = sides > 1 && holds(t.q) ? chance(t.q, rate) / (double)t.q.sum : 1.0, p = chance(t.p, rate) / (double)t.p.sum, uq = coin(key, i) * q;
+            kept = uq < p;
+            if (fabs(uq - p) < doubt_of(V) * p) {
+                kept = true;
+                if (lane == 0) atomicMin(&doubt_at, i);
+            }
         }
         if (!kept && lane == 0) atomicMin(&stop_at, i);
     }
     __syncthreads();
-    const int stop = stop_at;
+    int stop = stop_at;
+    if (doubt_at < stop)                               // one draft in some ten thousand
+        stop = settle<T>(logits + (size_t)first * v.ld, v.ld, v.d.logits ? static_cast<const T*>(v.d.logits) + (size_t)draft0 * v.d.ld : nullptr, v.d.ld, stats + (size_t)draft0 * sides * splits, splits, V, heat,
+                         key, doubt_at, stop);
     const T* row = logits + (size_t)(first + stop) * v.ld;
     // what is taken off: the drafter's chances, or the draft itself
     const T* less = nullptr;

@@ -44,3 +44,97 @@ def test_waits_of_numbers_next_to_one(pkg, torch_dev):
         z = x[s] - np.log(drafts_oracle.waits(key, vocab))
         assert int(np.argmax(z)) == (j if off > 0 else other[s])
         assert got[1][s] == int(np.argmax(z)), (s, off, got[1][s])
+
+
+def first_coins(keys):
+    """u of the first draft, for many keys at once: Philox4x32-10 at counter (0, 1, 0, 0)."""
+    u64 = np.uint64
+    mask, sh = u64(0xFFFFFFFF), u64(32)
+    a, b, c, d = (np.full(keys.shape, x, u64) for x in (0, 1, 0, 0))
+    k0, k1 = keys & mask, keys >> sh
+    for _ in range(10):
+        p, q = a * u64(0xD2511F53), c * u64(0xCD9E8D57)
+        a, b, c, d = (q >> sh) ^ b ^ k0, q & mask, (p >> sh) ^ d ^ k1, p & mask
+        k0, k1 = (k0 + u64(0x9E3779B9)) & mask, (k1 + u64(0xBB67AE85)) & mask
+    return a.astype(np.float64) / 2.0 ** 32
+
+
+@pytest.fixture(scope="module")
+def pool():
+    """A few million keys by their first coins."""
+    keys = np.random.default_rng(8).integers(0, 2 ** 64, 1 << 22, dtype=np.uint64)
+    assert np.array_equal(first_coins(keys[:50]), [drafts_oracle.coins(int(k), 1)[0] for k in keys[:50]])
+    u = first_coins(keys)
+    order = np.argsort(u)
+    return u[order], keys[order]
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7, 2.5])
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("form,vocab,lead", [("float32", 32000, 0), ("float32", 100003, 1), ("float32", 37, 0), ("bfloat16", 32000, 3), ("float16", 5001, 0)])
+def test_coins_next_to_the_chance(pkg, torch_dev, pool, form, vocab, lead, drafter, temperature):
+    """Random numbers right below and right above the one at which a draft is turned down: sums of exponentials that hold 32 bits would take one for the other."""
+    import torch
+    n = 64
+    b = Batch(torch, torch_dev, [1] * n, vocab, vocab + n, form, drafter, (temperature,), gap=0.3, lead=lead)
+    x = b.target.double().cpu().numpy()
+    d = b.draft.double().cpu().numpy() if drafter else None
+    t, u, keys = float(b.t[0]), *pool
+    want, close = [], 0
+    for s in range(n):
+        j = int(np.argsort(x[2 * s])[-1 - s % 5])       # a likely token that the drafter finds likelier, so that a coin decides
+        b.tokens[s] = j
+        p = drafts_oracle.chances(x[2 * s], t)[j]
+        q = drafts_oracle.chances(d[s], t)[j] if drafter else 1.0
+        i = int(np.searchsorted(u, p / q)) - (s % 2)
+        if not 0 <= i < len(u):
+            i = 0                                        # (p above q: kept, whatever u is)
+        b.key[s] = keys[i]
+        assert abs(u[i] * q - p) > 1e-12 * p             # (as far as 64 bits are sure)
+        close += abs(u[i] * q - p) < 2e-6 * p
+        want.append(int(u[i] * q < p))
+    assert (close > n // 8 or not drafter) and 0 < sum(want) < n          # (without a drafter coins of small chances lie further apart)
+    got = b.call(pkg)
+    assert got[0].tolist() == want
+    again = b.call(pkg)
+    assert (got == again).all()
+
+
+def test_every_draft_is_close(pkg, torch_dev, pool):
+    """A run of drafts whose chances are exactly the coins of certain words is decided one after another."""
+    import torch
+    vocab, n = 64, 40
+    b = Batch(torch, torch_dev, [n, 3, n], vocab, 4)
+    x = b.target.double().cpu().numpy()
+    key = [int(k) for k in b.key]
+    # two tokens, p of the draft next to the coin: p = 1 / (1 + e^-z), the nearest 32-bit z and the ones beside it
+    rows, drafts, kept = [], [], []
+    for s, count in enumerate(b.counts):
+        u = drafts_oracle.coins(key[s], count)
+        done = None
+        for i in range(count):
+            z = np.float32(np.log(u[i] / (1 - u[i])))
+            stop_here = (s, i) in ((0, 37), (1, 1), (2, 33))
+            for step in range(-3, 4):                    # the lowest that is kept, or the highest that is not
+                y = z
+                for _ in range(abs(step)):
+                    y = np.nextafter(y, np.float32(np.inf if step > 0 else -np.inf))
+                p = 1.0 / (1.0 + np.exp(-float(y)))
+                if (u[i] < p) != stop_here and not stop_here:
+                    break
+                if stop_here and not u[i] < p:
+                    chosen = y
+            y = chosen if stop_here else y
+            row = np.full(vocab, -np.inf)
+            row[3], row[9] = float(y), 0.0
+            rows.append(row)
+            drafts.append(3)
+            if done is None and not u[i] < 1.0 / (1.0 + np.exp(-float(y))):
+                done = i
+        rows.append(x[0])
+        kept.append(count if done is None else done)
+    b.draft = None
+    b.tokens = np.array(drafts, np.int32)
+    b.target[:] = torch.from_numpy(np.array(rows)).float()
+    assert kept == [37, 1, 33]
+    assert b.call(pkg)[0].tolist() == kept
