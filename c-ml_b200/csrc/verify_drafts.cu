@@ -8,11 +8,13 @@
 // (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, 2011) keyed by the sequence's 64-bit number: v of token j is word j mod 4 of
 // counter (j / 4, 0, 0, 0), u_i word i mod 4 of counter (i / 4, 1, 0, 0).
 //
-// Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: sums of exponentials in fp32, 16 or 32 at a time (or, for
-// greedy sequences, the place of the largest). draft_token: a cluster a sequence finds the first draft that is turned down (where u q and p lie closer than such sums are sure, sums in 64 bits
-// throughout decide), and draws over the one row (and the drafter's) that counts, in fp32; tokens that come closer to the best than that can be off by are weighed again in fp64, so that which token is drawn does not hang on the order of anything.
-// Measured: four drafts of one sequence over 32,000 tokens 8.7 us, of 32 sequences over 128,000 40 (22.5 for the bytes: 25 for the tested rows, 14 for the draws, which are some 45 instructions a token, a third of
-// them Philox, on 256 CTAs), one draw over 32,000 4.6, 64 over 128,000 22 (with the waits of all four tokens worked out where one could win: 23.5).
+// Two launches. draft_stats: the rows that drafts are tested against, several CTAs a row: sums of exponentials in fp32, 16 or 32 values at a time (or, for greedy sequences, the place of the largest).
+// draft_token: a cluster a sequence finds the first draft that is turned down, and draws over the one row (and the drafter's) that counts, in fp32. What fp32 cannot tell is decided in fp64, sums of the
+// rows included, so that neither hangs on the order of anything: u q and p that lie closer than the sums are sure; a best token that is not above all others by more than they can be off by, where a
+// token of p - q, which may lose all its digits, has a least and a most. It is seldom, and kept out of the way of the loops: 5 to 11 us more for a draw over 32,000 or
+// 128,000 tokens, 12 to 26 with a drafter's row.
+// Measured: four drafts of one sequence over 32,000 tokens 9.2 us, of 32 sequences over 128,000 41.7 (22.5 for the bytes: 25 for the tested rows, the rest for the draws, which are some 45 instructions a token,
+// a third of them Philox, on 256 CTAs), one draw over 32,000 5.0, 64 over 128,000 21.0 (with one loop for all kinds of rows: 22.6).
 // Few rows are bound by the chain of dependent loads and by code that is fetched anew with every launch (hence small loops, and what is seldom needed out of the way), many by memory.
 #include <atomic>
 #include <type_traits>
@@ -229,30 +231,39 @@ __device__ __forceinline__ Tested tested(const Stat* parts, int sides, int split
 }
 __device__ __forceinline__ bool holds(const Stat& a) { return a.most > -INFINITY && a.most < INFINITY && a.sum == a.sum; }
 
-// The sum of e^((x - from) rate) over a row that holds numbers, in 64 bits throughout, by a CTA together
-template <typename T> __device__ __noinline__ double exact_sum(const T* row, int vocab, double from, double rate) {
-    __shared__ double warps[VT_THREADS / 32];
-    double sum = 0.0;
-#pragma unroll 1
-    for (int j = threadIdx.x; j < vocab; j += VT_THREADS) sum += exp(((double)widen(row[j]) - from) * rate);
-    sum = lane_sum64(sum);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    return lane_sum64((threadIdx.x & 31) < VT_THREADS / 32 ? warps[threadIdx.x & 31] : 0.0);
-}
-
 __device__ __forceinline__ void cluster_all() { asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// The best of some tokens and the one behind it, as logarithms to the base 2 relative to a logit `ref` times c; the best's token, the lowest of equals
-struct Best { float z, z2, ref; int at, bad; };
+// What a cluster's CTAs tell one another where 64 bits decide
+struct Weighed {
+    double best[VT_THREADS / 32 + MOST_RANKS];
+    int at[VT_THREADS / 32 + MOST_RANKS];
+    double warps[VT_THREADS / 32], sums[2][MOST_RANKS];
+};
+// Sum of e^((x - from) rate) over a row that holds numbers, in 64 bits throughout, by a cluster together, in an order that is always the same. Two calls one after another are turn 0 and turn 1
+template <typename T> __device__ __noinline__ double exact_sum(const T* row, int vocab, double from, double rate, int ranks, int turn, Weighed* in) {
+    const int rank = blockIdx.x % ranks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, end = (int)((long)vocab * (rank + 1) / ranks);
+    double sum = 0.0;
+#pragma unroll 2
+    for (int j = (int)((long)vocab * rank / ranks) + threadIdx.x; j < end; j += VT_THREADS) sum += exp(((double)widen(row[j]) - from) * rate);
+    sum = lane_sum64(sum);
+    __syncthreads();
+    if (lane == 0) in->warps[warp] = sum;
+    __syncthreads();
+    sum = lane_sum64(lane < VT_THREADS / 32 ? in->warps[lane] : 0.0);
+    if (warp == 0 && lane < ranks) asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&in->sums[turn][rank], lane)), "d"(sum) : "memory");
+    cluster_all();                                     // (and all have read what the turn before the last left)
+    return lane_sum64(lane < ranks ? in->sums[turn][lane] : 0.0);
+}
+
+// What the best of some tokens has at most and at least, and the most that any of the others has, as logarithms to the base 2 relative to a logit `ref` times c; the best's token, the lowest of equals
+struct Best { float z, least, others, ref; int at, bad; };
 // of a warp's lanes together
 __device__ __forceinline__ Best best_of_lanes(Best b, float c) {
     const float top = warp_max(b.ref), by = b.ref == top ? 0.f : (b.ref - top) * c;
     const float z = b.z + by, most = warp_max(z);      // (-inf where there is nothing)
     const int at = (int)__reduce_min_sync(0xffffffffu, z == most ? (uint32_t)b.at : 0xffffffffu);
     const bool it = z == most && b.at == at;           // (a token is one lane's)
-    return {most, warp_max(fmaxf(it ? -INFINITY : z, b.z2 + by)), top, at, (int)__reduce_or_sync(0xffffffffu, (unsigned)b.bad)};
+    return {most, warp_max(it ? b.least + by : -INFINITY), warp_max(fmaxf(it ? -INFINITY : z, b.others + by)), top, at, (int)__reduce_or_sync(0xffffffffu, (unsigned)b.bad)};
 }
 // the largest of four but number `but`
 __device__ __forceinline__ float most_but(const float (&x)[4], int but) {
@@ -274,31 +285,101 @@ template <typename T> __device__ __forceinline__ void load4(const T* row, int g,
 
 constexpr int KEPT = 32;                               // drafts whose rows' parts are kept put together
 __device__ __forceinline__ double chance(const Stat& a, double rate) { return far_exp(((double)__int_as_float(a.at) - (double)a.most) * rate); }
-// Draft `from` and those behind it, up to `stop`, of which some lie closer than their rows' sums are sure: with sums in 64 bits throughout. The first that is turned down, or `stop`; a CTA together
+// What is asked for seldom is worked out anew from memory, out of the way of the loops: held for it, things would have no registers there.
+__device__ __forceinline__ uint64_t key_of(const cmlb200_drafts& d, int s) { return d.random ? d.random[s] : 0ull; }
+// The first draft that is turned down, from number `from` on, or their number: with sums in 64 bits throughout where u q and p lie closer than their rows' sums are sure. A cluster together
 template <typename T>
-__device__ __noinline__ int settle(const T* rows, long ld, const T* drafter, long drafter_ld, const Stat* stats, int splits, int vocab, float heat, uint64_t key, int from, int stop) {
+__device__ __noinline__ int settle(const Verify& v, const T* logits, const Stat* stats, int splits, int ranks, int from, Weighed* in) {
+    const int s = blockIdx.x / ranks, first = v.d.first[s], n = v.d.first[s + 1] - first - 1, sides = v.d.logits ? 2 : 1;
+    const float heat = heat_of(v.d, s), c = __fdiv_rn(kLog2e, heat);
     const double rate = 1.0 / (double)heat;
-    const float c = __fdiv_rn(kLog2e, heat);
-    const int sides = drafter ? 2 : 1;
-    for (int i = from; i < stop; i++) {
-        const Tested t = tested(stats + (size_t)i * sides * splits, sides, splits, c, false);
-        const bool beside = drafter && holds(t.q);
-        const double u = coin(key, i), p = chance(t.p, rate), q = beside ? chance(t.q, rate) : 1.0;
-        if (!(fabs(u * (beside ? q / (double)t.q.sum : q) - p / (double)t.p.sum) < doubt_of(vocab) * p / (double)t.p.sum)) continue;
-        const double p_sum = exact_sum(rows + (size_t)i * ld, vocab, t.p.most, rate), q_sum = beside ? exact_sum(drafter + (size_t)i * drafter_ld, vocab, t.q.most, rate) : 1.0;
-        if (!(u * (q / q_sum) < p / p_sum)) return i;
+    for (int i = from; i < n; i++) {
+        const int d = first - s + i, token = v.d.tokens[d];
+        const Tested t = tested(stats + (size_t)d * sides * splits, sides, splits, c, false);
+        if (token < 0 || token >= v.vocab || !holds(t.p)) return i;
+        const bool beside = sides > 1 && holds(t.q);
+        const double u = coin(key_of(v.d, s), i), p = chance(t.p, rate), q = beside ? chance(t.q, rate) : 1.0, p_near = p / (double)t.p.sum, uq_near = beside ? u * (q / (double)t.q.sum) : u;
+        bool kept = uq_near < p_near;
+        if (fabs(uq_near - p_near) < doubt_of(v.vocab) * p_near) {
+            const double p_sum = exact_sum(logits + (size_t)(first + i) * v.ld, v.vocab, t.p.most, rate, ranks, 0, in);
+            const double q_sum = beside ? exact_sum(static_cast<const T*>(v.d.logits) + (size_t)d * v.d.ld, v.vocab, t.q.most, rate, ranks, 1, in) : 1.0;
+            kept = u * (q / q_sum) < p / p_sum;
+            cluster_all();                             // (turn 0 again)
+        }
+        if (!kept) return i;
     }
-    return stop;
+    return n;
 }
 
-// grid = sequences * ranks, clusters of `ranks`. Two CTAs an SM: with 71 registers a thread, which leave room for one, 32 sequences of 4 drafts over 128,000 tokens took 56 us instead of 41
+// A draw behind `stop` drafts whose best tokens lie closer than 32 bits tell: every token of these groups that could be the best is weighed in 64 bits, sums of its rows included. A
+// cluster together. kind: 0 p itself, 1 p without the draft, 2 p - q
+template <typename T>
+__device__ __noinline__ int weigh(const Verify& v, const T* logits, const Stat* stats, int splits, int ranks, int stop, int kind, float ref, float least, Weighed* in) {
+    const int rank = blockIdx.x % ranks, s = blockIdx.x / ranks, first = v.d.first[s], d = first - s + stop, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = v.vocab;
+    const int groups = (V + 3) / 4, per = (groups + ranks - 1) / ranks, lo = rank * per, hi = min(groups, lo + per), without = kind == 1 ? v.d.tokens[d] : -1;
+    const float heat = heat_of(v.d, s), c = __fdiv_rn(kLog2e, heat), doubt = (float)doubt_of(V), bound = ex2(least) * (kClose * 2.3283064365386963e-10f);
+    const uint64_t key = key_of(v.d, s);
+    const double rate = 1.0 / (double)heat;
+    const T *row = logits + (size_t)(first + stop) * v.ld, *less = kind == 2 ? static_cast<const T*>(v.d.logits) + (size_t)d * v.d.ld : nullptr;
+    Tested t = {};
+    double p_sum = 1.0, q_sum = 1.0;
+    if (less) {
+        t = tested(stats + (size_t)d * 2 * splits, 2, splits, c, false);
+        p_sum = exact_sum(row, V, t.p.most, rate, ranks, 0, in);
+        q_sum = exact_sum(less, V, t.q.most, rate, ranks, 1, in);
+    }
+    const float p_unit = (1.f + doubt) / t.p.sum, q_unit = (1.f - doubt) / t.q.sum;
+    double z = -INFINITY;
+    int token = 0x7fffffff;
+#pragma unroll 1
+    for (int j = 4 * lo + threadIdx.x; j < min(V, 4 * hi); j += VT_THREADS) {
+        const float x = widen(row[j]), y = less ? widen(less[j]) : 0.f;
+        const uint32_t word = philox(key, (uint32_t)j >> 2, 0u).w[j & 3];
+        const float w = less ? ex2((x - t.p.most) * c) * p_unit - ex2((y - t.q.most) * c) * q_unit : ex2((x - ref) * c);
+        if (!(w > bound * (float)word) || j == without) continue;
+        double l;
+        if (less) {
+            const double p = far_exp(((double)x - (double)t.p.most) * rate) / p_sum, more = p - far_exp(((double)y - (double)t.q.most) * rate) / q_sum;
+            if (!(more > 5.8207660913467407e-11 * p)) continue;                // (2^-34: what 64 bits' sums may be off by; the same distribution from shifted logits is nothing above itself)
+            l = far_log(more);
+        } else l = ((double)x - (double)ref) * rate;
+        l -= log_wait_exact(word);
+        if (l > z) { z = l; token = j; }               // (a thread's tokens ascend)
+    }
+    for (int level = 0; level < 3; level++) {
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) {
+            const double z2 = __shfl_xor_sync(0xffffffffu, z, o);
+            const int t2 = __shfl_xor_sync(0xffffffffu, token, o);
+            if (z2 > z || (z2 == z && t2 < token)) { z = z2; token = t2; }
+        }
+        if (level == 2) break;
+        if (level == 0) {
+            __syncthreads();
+            if (lane == 0) { in->best[warp] = z; in->at[warp] = token; }
+            __syncthreads();
+            z = lane < VT_THREADS / 32 ? in->best[lane] : -INFINITY;
+            token = lane < VT_THREADS / 32 ? in->at[lane] : 0x7fffffff;
+        } else {
+            if (warp == 0 && lane < ranks) {
+                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&in->best[VT_THREADS / 32 + rank], lane)), "d"(z) : "memory");
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&in->at[VT_THREADS / 32 + rank], lane)), "r"(token) : "memory");
+            }
+            cluster_all();
+            z = lane < ranks ? in->best[VT_THREADS / 32 + lane] : -INFINITY;
+            token = lane < ranks ? in->at[VT_THREADS / 32 + lane] : 0x7fffffff;
+        }
+    }
+    return token;
+}
+
+// grid = sequences * ranks, clusters of `ranks`. Two CTAs an SM: with more than 64 registers a thread, which leave room for one, 32 sequences of 4 drafts over 128,000 tokens took 56 us instead of 42
 template <typename T>
 __global__ void __launch_bounds__(VT_THREADS, 2)
-draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int splits, const Stat* __restrict__ stats, int ranks, int* __restrict__ accepted, int* __restrict__ next) {
+draft_token_kernel(const __grid_constant__ Verify v, const T* __restrict__ logits, int sides, int splits, const Stat* __restrict__ stats, int ranks, int* __restrict__ accepted, int* __restrict__ next) {
     __shared__ int stop_at, doubt_at;
     __shared__ Best w_best[VT_THREADS / 32], c_best[MOST_RANKS];
-    __shared__ double x_best[VT_THREADS / 32 + MOST_RANKS];
-    __shared__ int x_at[VT_THREADS / 32 + MOST_RANKS];
+    __shared__ Weighed far;
     __shared__ Tested kept_stats[KEPT];
     dep_trigger();
     dep_wait();
@@ -329,196 +410,165 @@ draft_token_kernel(const Verify v, const T* __restrict__ logits, int sides, int 
         else if (kept) {
             const double q = sides > 1 && holds(t.q) ? chance(t.q, rate) / (double)t.q.sum : 1.0, p = chance(t.p, rate) / (double)t.p.sum, uq = coin(key, i) * q;
             kept = uq < p;
-            if (fabs(uq - p) < doubt_of(V) * p) {
-                kept = true;
-                if (lane == 0) atomicMin(&doubt_at, i);
-            }
+            if (fabs(uq - p) < doubt_of(V) * p && lane == 0) atomicMin(&doubt_at, i);
         }
         if (!kept && lane == 0) atomicMin(&stop_at, i);
     }
     __syncthreads();
     int stop = stop_at;
-    if (doubt_at < stop)                               // one draft in some ten thousand
-        stop = settle<T>(logits + (size_t)first * v.ld, v.ld, v.d.logits ? static_cast<const T*>(v.d.logits) + (size_t)draft0 * v.d.ld : nullptr, v.d.ld, stats + (size_t)draft0 * sides * splits, splits, V, heat,
-                         key, doubt_at, stop);
-    const T* row = logits + (size_t)(first + stop) * v.ld;
-    // what is taken off: the drafter's chances, or the draft itself
-    const T* less = nullptr;
-    int without = -1;
-    Tested t = {};
-    if (stop < n && !greedy) {
-        if (sides > 1) {
-            t = stop < KEPT ? kept_stats[stop] : tested(stats + (size_t)(draft0 + stop) * sides * splits, sides, splits, c, greedy);
-            if (holds(t.q)) less = static_cast<const T*>(v.d.logits) + (size_t)(draft0 + stop) * v.d.ld;
-        }
-        if (!less) without = v.d.tokens[draft0 + stop];
-    }
-    const float p_unit = less ? 1.f / t.p.sum : 0.f, q_unit = less ? 1.f / t.q.sum : 0.f;
-    const bool whole = (((uintptr_t)row | (uintptr_t)less) & (4 * sizeof(T) - 1)) == 0;
+    bool unsettled = doubt_at <= stop && doubt_at < n, plain = false;
     const int groups = (V + 3) / 4, per = (groups + ranks - 1) / ranks, lo = rank * per, hi = min(groups, lo + per);
     bool first_time = true;
-    for (int pass = 0;; pass++) {
+    for (;;) {
+        const int s = blockIdx.x / ranks, first = v.d.first[s], n = v.d.first[s + 1] - first - 1, draft0 = first - s;
+        const T* row = logits + (size_t)(first + stop) * v.ld;
+        // what is taken off: the drafter's chances, or the draft itself
+        const T* less = nullptr;
+        int without = -1;
+        Tested t = {};
+        if (stop < n && !greedy && !plain) {
+            if (sides > 1) {
+                t = stop < KEPT ? kept_stats[stop] : tested(stats + (size_t)(draft0 + stop) * sides * splits, sides, splits, c, greedy);
+                if (holds(t.q)) less = static_cast<const T*>(v.d.logits) + (size_t)(draft0 + stop) * v.d.ld;
+            }
+            if (!less) without = v.d.tokens[draft0 + stop];
+        }
+        // of p - q at most
+        const float doubt = (float)doubt_of(V), p_unit = less ? (1.f + doubt) / t.p.sum : 0.f, q_unit = less ? (1.f - doubt) / t.q.sum : 0.f;
+        const bool whole = (((uintptr_t)row | (uintptr_t)less) & (4 * sizeof(T) - 1)) == 0;
         // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with v, which is never above its wait, is looked at; there are
         // few, and only for those a wait is worked out. Where w is p alone it is relative to the largest logit that the warp has met, so that logits far from zero lose no digits (greedy: the logits
-        // themselves).
-        float best = greedy ? -INFINITY : 0.f, second = 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
-        int at = 0x7fffffff, at2 = 0x7fffffff, bad = 0;
-        constexpr int U = 2;                           // groups of four tokens under way
+        // themselves). p - q may lose all of its digits: a token counts with what it is at most, the bound is what the best is at least.
+        float best = greedy ? -INFINITY : 0.f, least = 0.f, others = 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
+        int at = 0x7fffffff, bad = 0;
+        // one loop for each kind of row: none holds registers for another
+        auto scan = [&](auto greedy_, auto residual_) {
+            constexpr bool GREEDY = decltype(greedy_)::value, RESIDUAL = decltype(residual_)::value;
+            constexpr int U = 2;                           // groups of four tokens under way
 #pragma unroll 1
-        for (int g0 = lo + warp * 32; g0 < hi; g0 += U * VT_THREADS) {
-            float x[U][4], y[U][4];
+            for (int g0 = lo + warp * 32; g0 < hi; g0 += U * VT_THREADS) {
+                float x[U][4], y[U][4];
 #pragma unroll
-            for (int k = 0; k < U; k++) {
-                const int g = g0 + k * VT_THREADS + lane;
-                load4(row, g < hi ? g : groups, V, whole, x[k]);               // (behind the end: -inf)
-                if (less) load4(less, g < hi ? g : groups, V, whole, y[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < U; k++) {
-                const int g = g0 + k * VT_THREADS + lane;
-                const float most = max_nan(max_nan(x[k][0], x[k][1]), max_nan(x[k][2], x[k][3]));
-                bad |= !(most < INFINITY);
-                if (greedy) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (x[k][e] > best) { best = x[k][e]; at = 4 * g + e; }
-                    }
-                    continue;
+                for (int k = 0; k < U; k++) {
+                    const int g = g0 + k * VT_THREADS + lane;
+                    load4(row, g < hi ? g : groups, V, whole, x[k]);               // (behind the end: -inf)
+                    if (RESIDUAL) load4(less, g < hi ? g : groups, V, whole, y[k]);
                 }
-                const Philox r = philox(key, (uint32_t)g, 0u);
-                float w[4];
-                if (less) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - t.p.most) * c) * p_unit - ex2((y[k][e] - t.q.most) * c) * q_unit;
-                } else {
-                    const float top = (uint32_t)(without - 4 * g) < 4u ? most_but(x[k], without - 4 * g) : most;          // (the draft that was turned down sets no reference)
-                    if (__any_sync(0xffffffffu, top > ref)) {
-                        const float to = fmaxf(ref, warp_max(top)), by = ref == -INFINITY ? 0.f : ex2((ref - to) * c);
-                        best *= by;
-                        second *= by;
-                        bound *= by;
-                        ref = to;
+                for (int k = 0; k < U; k++) {
+                    const int g = g0 + k * VT_THREADS + lane;
+                    const float most = max_nan(max_nan(x[k][0], x[k][1]), max_nan(x[k][2], x[k][3]));
+                    bad |= !(most < INFINITY);
+                    if (GREEDY) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (x[k][e] > best) { best = x[k][e]; at = 4 * g + e; }
+                        }
+                        continue;
                     }
-                    const float from = ref == -INFINITY ? 0.f : ref;
+                    const Philox r = philox(key, (uint32_t)g, 0u);
+                    float w[4];
+                    if (RESIDUAL) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - from) * c);
-                    if ((uint32_t)(without - 4 * g) < 4u) {
+                        for (int e = 0; e < 4; e++) {
+                            y[k][e] = ex2((y[k][e] - t.q.most) * c) * q_unit;
+                            w[e] = ex2((x[k][e] - t.p.most) * c) * p_unit - y[k][e];
+                        }
+                    } else {
+                        const float top = (uint32_t)(without - 4 * g) < 4u ? most_but(x[k], without - 4 * g) : most;          // (the draft that was turned down sets no reference)
+                        if (__any_sync(0xffffffffu, top > ref)) {
+                            const float to = fmaxf(ref, warp_max(top)), by = ref == -INFINITY ? 0.f : ex2((ref - to) * c);
+                            best *= by;
+                            others *= by;
+                            bound *= by;
+                            ref = to;
+                        }
+                        const float from = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) if (4 * g + e == without) w[e] = 0.f;
-                    }
-                }
-                bool any = false;
+                        for (int e = 0; e < 4; e++) w[e] = ex2((x[k][e] - from) * c);
+                        if ((uint32_t)(without - 4 * g) < 4u) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) any |= w[e] > bound * (float)r.w[e];
-                if (__any_sync(0xffffffffu, any)) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (!(w[e] > bound * (float)r.w[e])) continue;
-                        const float score = __fdividef(w[e], wait_of(r.w[e]));
-                        if (score > second) { second = score; at2 = 4 * g + e; }
-                        if (second > best) {
-                            const float was = best;
-                            const int was_at = at;
-                            best = second; at = at2;
-                            second = was; at2 = was_at;
+                            for (int e = 0; e < 4; e++) if (4 * g + e == without) w[e] = 0.f;
                         }
                     }
-                    bound = warp_max(best) * (kClose * 2.3283064365386963e-10f);
+                    bool any = false;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) any |= w[e] > bound * (float)r.w[e];
+                    if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (!(w[e] > bound * (float)r.w[e])) continue;
+                            const float arrives = __fdividef(1.f, wait_of(r.w[e])), score = w[e] * arrives;
+                            if (score > best) {
+                                others = best;
+                                best = score;
+                                at = 4 * g + e;
+                                // (p - q with both off the other way)
+                                if (RESIDUAL) least = fmaf(-2.f * doubt * arrives, fmaf(2.f, y[k][e], w[e]), score);
+                            } else others = fmaxf(others, score);
+                        }
+                        bound = warp_max(RESIDUAL ? fmaxf(least, 0.f) : best) * (kClose * 2.3283064365386963e-10f);
+                    }
                 }
             }
-        }
-        const float most = greedy ? best : best > 0.f ? lg2(best) : -INFINITY;
-        // thread, CTA and cluster have the best and the one behind it
-        const float behind = second > 0.f ? lg2(second) : -INFINITY;
-        const Best b = {most, behind, ref, at, bad};
+        };
+        if (greedy) scan(std::true_type(), std::false_type());
+        else if (less) scan(std::false_type(), std::true_type());
+        else scan(std::false_type(), std::false_type());
+        // thread, CTA and cluster have the best and what the others come to
+        const float z = greedy ? best : best > 0.f ? lg2(best) : -INFINITY;
+        const Best b = {z, !less ? z : least > 0.f ? lg2(least) : -INFINITY, others > 0.f ? lg2(others) : -INFINITY, ref, at, bad};
         auto best_of = [&](Best x) {
             x = best_of_lanes(x, c);
             if (lane == 0) w_best[warp] = x;
             if (first_time) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
             first_time = false;
             __syncthreads();
-            const Best none = {-INFINITY, -INFINITY, less || greedy ? 0.f : -INFINITY, 0x7fffffff, 0};
+            const Best none = {-INFINITY, -INFINITY, -INFINITY, less || greedy ? 0.f : -INFINITY, 0x7fffffff, 0};
             if (warp == 0) {
                 x = best_of_lanes(lane < VT_THREADS / 32 ? w_best[lane] : none, c);
                 if (lane < ranks) {
                     const uint32_t dst = cluster_addr(&c_best[rank], lane);
                     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(x.z) : "memory");
-                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(x.z2) : "memory");
-                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(x.ref) : "memory");
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 12), "r"(x.at) : "memory");
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 16), "r"(x.bad) : "memory");
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(x.least) : "memory");
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(x.others) : "memory");
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 12), "f"(x.ref) : "memory");
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 16), "r"(x.at) : "memory");
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + 20), "r"(x.bad) : "memory");
                 }
             }
             cluster_all();
             return best_of_lanes(lane < ranks ? c_best[lane] : none, c);
         };
-        // the same in 64 bits, over the whole cluster (seldom): warp by warp, then CTA by CTA
-        auto exact_best = [&](double z, int token, Best old) {
-            for (int level = 0; level < 3; level++) {
-#pragma unroll 1
-                for (int o = 16; o > 0; o >>= 1) {
-                    const double z2 = __shfl_xor_sync(0xffffffffu, z, o);
-                    const int t2 = __shfl_xor_sync(0xffffffffu, token, o);
-                    if (z2 > z || (z2 == z && t2 < token)) { z = z2; token = t2; }
-                }
-                if (level == 2) break;
-                if (level == 0) {
-                    if (lane == 0) { x_best[warp] = z; x_at[warp] = token; }
-                    __syncthreads();
-                    z = lane < VT_THREADS / 32 ? x_best[lane] : -INFINITY;
-                    token = lane < VT_THREADS / 32 ? x_at[lane] : 0x7fffffff;
-                } else {
-                    __syncthreads();                   // (everyone has read the warps')
-                    if (warp == 0 && lane < ranks) {
-                        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&x_best[VT_THREADS / 32 + rank], lane)), "d"(z) : "memory");
-                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&x_at[VT_THREADS / 32 + rank], lane)), "r"(token) : "memory");
-                    }
-                    cluster_all();
-                    z = lane < ranks ? x_best[VT_THREADS / 32 + lane] : -INFINITY;
-                    token = lane < ranks ? x_at[VT_THREADS / 32 + lane] : 0x7fffffff;
-                }
-            }
-            old.at = token;
-            return old;
-        };
         Best all = best_of(b);
-        if (!greedy && !all.bad && all.z > -INFINITY) {
-            // What 32 bits are off by at most: 1e-4 of the waits, 1e-5 of logarithms and of products with c (tokens near the best lie within 64 of it). The difference of p and q may lose more
-            // where the two are close; such tokens are seldom drawn. All CTAs know the same: they decide together.
-            constexpr float slack = 1e-3f;
-            if (all.z2 >= all.z - slack) {             // (one call in a thousand)
-                cluster_all();                         // everyone has read what comes now is written over
-                const float by = ref == all.ref ? 0.f : (ref - all.ref) * c;
-                double z = -INFINITY;
-                int token = 0x7fffffff;
-#pragma unroll 1
-                for (int k = 0; k < 2; k++) {
-                    const float m = k ? behind : most;
-                    const int j = k ? at2 : at;
-                    if (!(m > -INFINITY && m + by >= all.z - slack)) continue;
-                    double w;
-                    if (less) {
-                        const double d = far_exp(((double)widen(row[j]) - (double)t.p.most) * rate) / (double)t.p.sum - far_exp(((double)widen(less[j]) - (double)t.q.most) * rate) / (double)t.q.sum;
-                        w = d > 0.0 ? far_log(d) : -1e30;      // (what 32 bits took for a weight was their rounding)
-                    } else w = ((double)widen(row[j]) - (double)all.ref) * rate;
-                    w -= log_wait_exact(philox(key, (uint32_t)j >> 2, 0u).w[j & 3]);
-                    if (w > z || (w == z && j < token)) { z = w; token = j; }
-                }
-                all = exact_best(z, token, all);
+        // What 32 bits are off by at most: 1e-4 of the waits, 1e-5 of logarithms and of products with c (tokens near the best lie within 64 of it). All CTAs know the same: they decide together.
+        constexpr float slack = 1e-3f;
+        if (!greedy && !all.bad && all.z > -INFINITY && !(all.others < all.least - slack)) {           // (one call in a thousand)
+            all.at = weigh<T>(v, logits, stats, splits, ranks, stop, less ? 2 : without >= 0 ? 1 : 0, all.ref, all.least, &far);
+            all.z = all.at < V ? 0.f : -INFINITY;
+        }
+        // a draft was kept or turned down by less than its rows' sums are sure of (one in some ten thousand; asked here, where the loops' registers are free)
+        if (unsettled) {
+            unsettled = false;
+            const int real = settle<T>(v, logits, stats, splits, ranks, doubt_at, &far);
+            if (real != stop) {
+                stop = real;
+                cluster_all();                         // nobody reads what the next turn writes
+                continue;
             }
         }
-        // where rounding leaves nothing of p - q (or p is nothing but the draft), p itself
-        const bool again = pass == 0 && !all.bad && all.z == -INFINITY && (less || without >= 0);
-        if (!again) {
-            if (rank == 0 && threadIdx.x == 0) {
-                accepted[s] = stop;
-                next[s] = all.bad || all.z == -INFINITY ? -1 : all.at;
-            }
-            return;
+        // where nothing is left of p - q (or p is nothing but the draft), p itself
+        if (!plain && !all.bad && all.z == -INFINITY && (less || without >= 0)) {
+            plain = true;
+            cluster_all();
+            continue;
         }
-        less = nullptr;
-        without = -1;
-        cluster_all();                                 // nobody reads what the next pass writes
+        if (rank == 0 && threadIdx.x == 0) {
+            const int s = blockIdx.x / ranks;
+            accepted[s] = stop;
+            next[s] = all.bad || all.z == -INFINITY ? -1 : all.at;
+        }
+        return;
     }
 }
 

@@ -138,3 +138,69 @@ def test_every_draft_is_close(pkg, torch_dev, pool):
     b.target[:] = torch.from_numpy(np.array(rows)).float()
     assert kept == [37, 1, 33]
     assert b.call(pkg)[0].tolist() == kept
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("vocab,lead", [(3001, 0), (40001, 1), (7, 0)])
+@pytest.mark.parametrize("gap", [1e-2, 1e-4, 2e-6])
+def test_little_is_left_of_the_difference(pkg, torch_dev, gap, vocab, lead, temperature):
+    """A drafter whose chances are nearly the target's: p - q loses its digits in 32 bits, and the token drawn is still the one that 64 bits give. Drafts outside the vocabulary are always turned down."""
+    import torch
+    n = 48
+    b = Batch(torch, torch_dev, [1] * n, vocab, vocab + int(1e7 * gap), "float32", True, (temperature,), gap=gap, lead=lead)
+    b.tokens[:] = -1
+    got, want = b.call(pkg), b.want()
+    x, d = b.target.double().cpu().numpy(), b.draft.double().cpu().numpy()
+    for s in range(n):
+        p, q = drafts_oracle.chances(x[2 * s], float(b.t[0])), drafts_oracle.chances(d[s], float(b.t[0]))
+        with np.errstate(divide="ignore"):
+            z = np.log(np.maximum(p - q, 0)) - np.log(drafts_oracle.waits(int(b.key[s]), vocab))
+        top = np.sort(z)[-2:]
+        assert top[1] - top[0] > 1e-8                    # (64 bits: 2^-53 of p, of a difference of some 1e-7 p)
+        assert (got[0][s], got[1][s]) == (0, int(np.argmax(z))) == want[s][:2], (s, got[:, s], want[s])
+
+
+@pytest.mark.parametrize("form", ["float32", "bfloat16"])
+def test_nothing_is_left_of_the_difference(pkg, torch_dev, form):
+    """The target's own distribution as the drafter's, from the same logits and from shifted ones: the token is drawn from p."""
+    import torch
+    n, vocab = 40, 2003
+    b = Batch(torch, torch_dev, [1] * n, vocab, 3, form, True)
+    b.target.copy_((b.target.float() * 16).round() / 16)
+    b.draft.copy_(b.target[::2].float() + (torch.arange(n, device=torch_dev) % 3 * 0.5)[:, None])
+    assert torch.equal(b.draft.float() - b.target[::2].float(), (torch.arange(n, device=torch_dev) % 3 * 0.5)[:, None].expand(n, vocab))
+    b.tokens[:] = vocab
+    got, x = b.call(pkg), b.target.double().cpu().numpy()
+    for s in range(n):
+        z = np.log(drafts_oracle.chances(x[2 * s], 1.0)) - np.log(drafts_oracle.waits(int(b.key[s]), vocab))
+        assert (got[0][s], got[1][s]) == (0, int(np.argmax(z)))
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("vocab,at", [(4, (0, 1, 2)), (4, (0, 1, 2, 3)), (9, (4, 5, 6, 7, 8)), (5000, (0, 1, 2049, 2051)), (40000, (12, 13, 2060, 2061, 4108, 4109)), (300, tuple(range(300)))])
+def test_many_close_calls(pkg, torch_dev, vocab, at, drafter):
+    """As many tokens as come out nearly equal, however many of them one thread looks at: alone, or as what a drafter's even chances leave."""
+    import torch
+    n = 200
+    b = Batch(torch, torch_dev, [1 if drafter else 0] * n, vocab, 81, "float32", drafter)
+    rng, at = np.random.default_rng(vocab), list(at)
+    step = 2 if drafter else 1
+    for s in range(n):
+        row = np.full(vocab, -40.0)
+        row[at] = np.log(drafts_oracle.waits(int(b.key[s]), vocab))[at] + rng.normal(size=len(at)) * 2e-6
+        b.target[step * s] = torch.from_numpy(row).float()
+    if drafter:                                          # q half of p, so that p - q is p / 2 there
+        b.tokens[:] = -1
+        p = torch.softmax(b.target[::2].double(), 1)
+        b.draft.copy_(torch.cat([p[:, :-1] / 2, p[:, -1:] / 2 + 0.5], 1).log().clamp_min(-60).float())
+    got = b.call(pkg)
+    x, d = b.target.double().cpu().numpy(), b.draft.double().cpu().numpy() if drafter else None
+    for s in range(n):
+        w = drafts_oracle.chances(x[step * s], 1.0)
+        if drafter:
+            w = np.maximum(w - drafts_oracle.chances(d[s], 1.0), 0)
+        with np.errstate(divide="ignore"):
+            z = np.log(w) - np.log(drafts_oracle.waits(int(b.key[s]), vocab))
+        top = np.sort(z)[-2:]
+        if top[1] - top[0] > 1e-12:
+            assert (got[0][s], got[1][s]) == (0, int(np.argmax(z))), (s, np.sort(z)[-4:] - z.max(), z[got[1][s]] - z.max())
