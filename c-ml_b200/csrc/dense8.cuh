@@ -119,6 +119,12 @@ template <typename T> struct RowScale {
     }
 };
 
+// A result from its sum: the scales' product is rounded, then the sum with the bias as one; the same in all kernels, so that a row's results do not depend on how many rows there are
+__device__ __noinline__ float far_cap(float y, float cap) { return soft_cap(y, cap); }          // (out of the way)
+__device__ __forceinline__ float finish8(int sum, float unit, float bias, float cap) {
+    const float y = fmaf((float)sum, unit, bias);
+    return cap > 0.f ? far_cap(y, cap) : y;
+}
 __device__ __forceinline__ float glu8(int act, float gate, float up) { return unary_act_fast(act, gate) * up; }
 
 // Values 16 c .. 16 c + 15 of a row, zeros behind its end. whole: rows lie on 16-byte boundaries.

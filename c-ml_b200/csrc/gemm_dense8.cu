@@ -90,12 +90,6 @@ __device__ __forceinline__ void tile8(int i, int tiles_m, int tiles, int& tm, in
     tn = in / rows;
 }
 
-__device__ __noinline__ float far_cap(float y, float cap) { return soft_cap(y, cap); }          // (out of the way)
-__device__ __forceinline__ float finish8(int sum, float unit, float bias, float cap) {
-    const float y = fmaf((float)sum, unit, bias);
-    return cap > 0.f ? far_cap(y, cap) : y;
-}
-
 template <bool PAIR>
 __global__ void __launch_bounds__(THREADS8, 1)
 gemm_dense8_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const Gemm8 p) {

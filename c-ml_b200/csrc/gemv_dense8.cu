@@ -116,12 +116,8 @@ gemv_dense8_kernel(const int8_t* __restrict__ W, int ldw, const T* __restrict__ 
                 const int col = tile * 16 + n;
                 if (m < M && col < out.n_out)
                     static_cast<__nv_bfloat16*>(out.y)[(size_t)m * out.ldy + col] = __float2bfloat16_rn(glu8(out.act, (float)s * (sxs[m] * out.wscale[r]), (float)s2 * (sxs[m] * out.wscale[r + 16])));
-            } else if (m < M && r < out.n_out) {
-                float y = (float)s * (sxs[m] * out.wscale[r]);
-                if (out.bias) y += out.bias[r];
-                if (out.cap > 0.f) y = soft_cap(y, out.cap);
-                static_cast<float*>(out.y)[(size_t)m * out.ldy + r] = y;
-            }
+            } else if (m < M && r < out.n_out)
+                static_cast<float*>(out.y)[(size_t)m * out.ldy + r] = finish8(s, sxs[m] * out.wscale[r], out.bias ? out.bias[r] : 0.f, out.cap);
         }
         turn++;
         tile += gridDim.x;
