@@ -8,10 +8,11 @@
  * together. --prompt needs a model with a tokenizer. Without --temperature decoding is greedy. Output: one
  * line a request, in the order given: the generated ids, and the text where there is a tokenizer.
  * --drafts: requests run one after the other, N tokens at a time proposed by another model (--drafter; otherwise the same folder
- * with 8-bit weights) and verified in one step; the distribution is not cut (no --top-k, --top-p). */
+ * with 8-bit weights, bfloat16 whatever --dtype says) and verified in one step; the distribution is not cut (no --top-k, --top-p). */
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
+#include <sys/stat.h>
 
 #include "cml_lm.h"
 
@@ -93,11 +94,16 @@ int main(int argc, char** argv) {
                     "[--top-k K] [--top-p P] [--seed S] [--eos ID] [--drafts N [--drafter DIR], without --top-k and --top-p] (--tokens 1,2,3 | --prompt TEXT) ...", NULL);
     o.dtype = !strcmp(dtype, "float32") ? DTYPE_FLOAT32 : DTYPE_BFLOAT16;
     o.max_sequences = requests < 8 ? requests : 8;
+    struct stat sb;
+    if (drafts && !drafter && !stat(model, &sb) && !S_ISDIR(sb.st_mode)) return fail("a GGUF model has no 8-bit form to draft with; give --drafter", model);
     CMLLanguageModel* lm = cml_lm_load(model, &o);
     if (!lm) return fail("cannot load", model);
     if (drafts) {
         CMLLMOptions od = o;
-        if (!drafter) od.weights = CML_LM_WEIGHTS_INT8;
+        if (!drafter) {                                /* (8-bit weights go with bfloat16; logits are 32-bit in both forms) */
+            od.weights = CML_LM_WEIGHTS_INT8;
+            od.dtype = DTYPE_BFLOAT16;
+        }
         CMLLanguageModel* other = cml_lm_load(drafter ? drafter : model, &od);
         int bad = other ? 0 : fail("cannot load the drafter", drafter ? drafter : model);
         c.max_new_tokens = max_new;
