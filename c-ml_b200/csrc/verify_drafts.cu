@@ -627,7 +627,8 @@ extern "C" int cmlb200_verify_drafts(const cmlb200_drafts* d, const void* d_logi
     CMLB_REQUIRE(vocab > 0 && vocab <= MOST_VOCAB && ld >= vocab && (!d->logits || d->ld >= vocab), "%s: %d logits, strides %ld and %ld", who, vocab, ld, d->ld);
     CMLB_REQUIRE(d->tokens || d->rows == d->sequences, "%s: %d drafts without tokens", who, d->rows - d->sequences);
     CMLB_REQUIRE(d->random || d->temperature, "%s: no random numbers, and no temperatures that could do without", who);
-    CMLB_REQUIRE((((uintptr_t)d_logits | (uintptr_t)d->logits) & (dtype == CMLB200_DT_F32 ? 3 : 1)) == 0 && ((uintptr_t)d_work & 15) == 0 && ((uintptr_t)d->random & 7) == 0,
+    const uintptr_t words = (uintptr_t)d->first | (uintptr_t)d->tokens | (uintptr_t)d->temperature | (uintptr_t)d_accepted | (uintptr_t)d_next;
+    CMLB_REQUIRE((((uintptr_t)d_logits | (uintptr_t)d->logits) & (dtype == CMLB200_DT_F32 ? 3 : 1)) == 0 && ((uintptr_t)d_work & 15) == 0 && ((uintptr_t)d->random & 7) == 0 && (words & 3) == 0,
                  "%s: pointers are not aligned to their types (workspace: 16 bytes)", who);
     const Verify v = {*d, ld, vocab};
     cudaStream_t st = as_stream(stream);
