@@ -499,7 +499,7 @@ static int check_drawn(const float* temperatures, const uint64_t* random, int n,
         cold = 0;
         if (temperatures[i] > 1e30f) { LOG_ERROR("%s: temperature %g", who, (double)temperatures[i]); return -1; }
     }
-    if (!random && !cold) { LOG_ERROR("%s: no random numbers", who); return -1; }
+    if (n && !random && !cold) { LOG_ERROR("%s: no random numbers", who); return -1; }
     return 0;
 }
 
