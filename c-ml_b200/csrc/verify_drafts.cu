@@ -336,11 +336,12 @@ __device__ __noinline__ int weigh(const Verify& v, const T* logits, const Stat* 
         const float x = widen(row[j]), y = less ? widen(less[j]) : 0.f;
         const uint32_t word = philox(key, (uint32_t)j >> 2, 0u).w[j & 3];
         const float w = less ? ex2((x - t.p.most) * c) * p_unit - ex2((y - t.q.most) * c) * q_unit : ex2((x - ref) * c);
-        if (!(w > bound * (float)word) || j == without) continue;
+        if (!(w >= bound * (float)word) || j == without) continue;
         double l;
         if (less) {
-            const double p = far_exp(((double)x - (double)t.p.most) * rate) / p_sum, more = p - far_exp(((double)y - (double)t.q.most) * rate) / q_sum;
-            if (!(more > 5.8207660913467407e-11 * p)) continue;                // (2^-34: what 64 bits' sums may be off by; the same distribution from shifted logits is nothing above itself)
+            const double e = ((double)x - (double)t.p.most) * rate, p = far_exp(e) / p_sum, more = p - far_exp(((double)y - (double)t.q.most) * rate) / q_sum;
+            // (what 64 bits' exponents and sums may be off by: the same distribution from shifted logits is nothing above itself)
+            if (!(more > (1.2e-13 + 4.4e-19 * (double)V + 4.5e-16 * fabs(e)) * p)) continue;
             l = far_log(more);
         } else l = ((double)x - (double)ref) * rate;
         l -= log_wait_exact(word);
@@ -543,7 +544,9 @@ draft_token_kernel(const __grid_constant__ Verify v, const T* __restrict__ logit
         Best all = best_of(b);
         // What 32 bits are off by at most: 1e-4 of the waits, 1e-5 of logarithms and of products with c (tokens near the best lie within 64 of it). All CTAs know the same: they decide together.
         constexpr float slack = 1e-3f;
-        if (!greedy && !all.bad && all.z > -INFINITY && !(all.others < all.least - slack)) {           // (one call in a thousand)
+        // Differences below 2^-126 are nothing in 32 bits: where the best comes to less than 2^-80 (some of them over a wait of 2^-33), all tokens are weighed.
+        if (less && all.least < -80.f) all.least = -INFINITY;
+        if (!greedy && !all.bad && (less || all.z > -INFINITY) && !(all.others < all.least - slack)) {           // (one call in a thousand)
             all.at = weigh<T>(v, logits, stats, splits, ranks, stop, less ? 2 : without >= 0 ? 1 : 0, all.ref, all.least, &far);
             all.z = all.at < V ? 0.f : -INFINITY;
         }

@@ -204,3 +204,51 @@ def test_many_close_calls(pkg, torch_dev, vocab, at, drafter):
         top = np.sort(z)[-2:]
         if top[1] - top[0] > 1e-12:
             assert (got[0][s], got[1][s]) == (0, int(np.argmax(z))), (s, np.sort(z)[-4:] - z.max(), z[got[1][s]] - z.max())
+
+
+def admissible(b, s, kept):
+    """Tokens that may follow sequence s's first `kept` drafts where 64 bits are sure to 1e-12 of p: one, but for differences of nearly equal chances."""
+    f, n, t = b.first[s], b.counts[s], float(b.t[s])
+    x, wait = b.target[f + kept].double().cpu().numpy(), np.log(drafts_oracle.waits(int(b.key[s]), b.vocab))
+    if not t >= drafts_oracle.GREEDY:
+        return {int(np.argmax(x))}
+    p = drafts_oracle.chances(x, t)
+    with np.errstate(divide="ignore"):
+        plain = int(np.argmax(np.log(p) - wait))
+        if kept == n:
+            return {plain}
+        if b.draft is None:
+            j = int(b.tokens[f - s + kept])
+            w = np.where(np.arange(b.vocab) == j, 0.0, p) if 0 <= j < b.vocab else p
+            return {int(np.argmax(np.log(w) - wait)) if w.max() > 0 else plain}
+        q = drafts_oracle.chances(b.draft[f - s + kept].double().cpu().numpy(), t)
+        sure, most = np.log(np.maximum(p - q - 1e-12 * p, 0)) - wait, np.log(np.maximum(p - q + 1e-12 * p, 0)) - wait
+    fine = {int(j) for j in np.flatnonzero((most >= sure.max()) & (most > -np.inf))}
+    return fine if sure.max() > -np.inf else fine | {plain}
+
+
+@pytest.mark.parametrize("form", ["float32", "bfloat16"])
+@pytest.mark.parametrize("spread,temperature", [(0.0, 1.0), (0.01, 1.0), (30.0, 1.0), (300.0, 1.0), (2.0, 0.01), (2.0, 1e-4), (2.0, 100.0), (2.0, 1.0), (2.0, 9e-6)])
+@pytest.mark.parametrize("drafter,gap", [(True, 0.2), (True, 1e-3), (False, 0.2)])
+def test_every_sequence(pkg, torch_dev, spread, temperature, drafter, gap, form):
+    """Flat and steep distributions, drafters near and far, some drafts from outside: all sequences as 64 bits have them, close calls among them."""
+    import torch
+    b = Batch(torch, torch_dev, [3, 0, 1, 2, 1] * 40, 3001, 18, form, drafter, (temperature,), gap * max(spread, 1e-3), spread)
+    b.tokens[::7] = -1
+    got, want, several = b.call(pkg), b.want(), 0
+    for s, w in enumerate(want):
+        fine = admissible(b, s, w[0])
+        several += len(fine) > 1
+        assert got[0][s] == w[0] and got[1][s] in fine, (s, got[:, s], w, fine)
+    assert several <= 0.05 * len(want) or temperature / max(spread, 1e-3) < 0.1      # (steep: one token has all of p and of q, as far as 64 bits go)
+
+
+@pytest.mark.parametrize("offset", [4096.0, 1e6, -1e30])
+def test_every_sequence_far_from_zero(pkg, torch_dev, offset):
+    import torch
+    b = Batch(torch, torch_dev, [2, 0, 1] * 30, 2000, 72, gap=0.3)
+    b.target += offset
+    b.draft -= offset / 4
+    got, want = b.call(pkg), b.want()
+    for s, w in enumerate(want):
+        assert (got[0][s], got[1][s]) == w[:2], (s, got[:, s], w)
