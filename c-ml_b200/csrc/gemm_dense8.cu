@@ -359,7 +359,9 @@ int encode_blocks(CUtensorMap* map, const void* base, long rows, int blocks, int
 
 // Cycles that a form would take, by its waves: a stage takes its MMAs (4 NX) or its bytes (50 a cycle and SM) or its issue (600), a tile about 2,000 to start and end and 8 a token, a
 // cluster's sum 2,000 and 8 a token more. How many clusters of 4 and 8 run at once goes by how SMs lie in groups: 33 and 15 on B200. Tokens are cut into the fewest tiles that hold them, or
-// up to three more, which may fill the last wave better.
+// up to three more, which may fill the last wave better. What the two forms that are seldom chosen gain over the best of the others: single CTAs, for a few hundred columns, 27 rows of 54x67 4.1 us (4.6), 157 of
+// 332x86 4.75 (5.3), 40 of 32000x64 6.25 (6.6), 3,517 of 2618x360 16.5 (18.0), though 1,081 of 7530x50 14.3 (13.7); clusters of two 41 rows of 5161x13999 19.7 (22.4), 84 of 4405x18379 25.0 (29.8), 32 of 6250x1964
+// 7.35 (7.4), though 180 of 4265x4423 12.0 (11.8).
 Shape8 pick_shape(int M, int N, int loads) {
     const int sms = cmlb_num_sms(), fewest = (M + 255) / 256;
     auto stage = [](int nx, int rows) { return fmax(fmax(4.0 * nx, BLOCKS * (A8 + rows * BK8) / 50.0), 600.0); };

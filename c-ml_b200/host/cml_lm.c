@@ -495,7 +495,7 @@ typedef struct { const float* temperatures; const uint64_t* random; const float*
 static int check_drawn(const float* temperatures, const uint64_t* random, int n, const char* who) {
     int cold = temperatures != NULL;
     for (int i = 0; temperatures && i < n; i++) {
-        if (!(temperatures[i] >= 1e-5f)) continue;         /* (as the device reads it) */
+        if (!(temperatures[i] >= 1e-5f)) continue;         /* (as the device reads it, which would take those refused here for 1e30) */
         cold = 0;
         if (temperatures[i] > 1e30f) { LOG_ERROR("%s: temperature %g", who, (double)temperatures[i]); return -1; }
     }

@@ -88,13 +88,14 @@ int cml_lm_step_greedy(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_
 int cml_lm_step_scored(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const int* targets, int top, float* logprobs, float* entropies, int* top_ids,
                        float* top_logprobs);
 /* The same, but draws the token of every wanted row on the device, from the softmax of its logits over the row's temperature: temperatures [sum of num_want] (NULL: 1; below 1e-5: the largest
- * logit's token), random [sum of num_want] 64-bit random numbers, each used once (NULL where all temperatures are below 1e-5). picked[sum of num_want], -1 for a row that holds no
+ * logit's token; above 1e30: refused), random [sum of num_want] 64-bit random numbers, each used once (NULL where all temperatures are below 1e-5). picked[sum of num_want], -1 for a row that holds no
  * distribution. Nothing is cut off the distribution. See cmlb200_verify_drafts. */
 int cml_lm_step_sampled(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const float* temperatures, const uint64_t* random, int* picked);
 /* Drafted tokens: an entry's first token is the one its sequence goes on with, those behind it are drafts (256 tokens of all entries together; `want` is not looked at). Runs them all, keeps
  * drafts while the model's own distribution would have had them (temperatures and random: one per entry, as above; the drafts count as chosen for certain), and draws the token behind those:
  * accepted[num_entries] drafts kept, next[num_entries] (-1: no distribution). Kept tokens and `next` are distributed as tokens of the model drawn one by one. The sequence then ends behind
- * the kept drafts; `next` is not in it yet. Models that keep a state per sequence take no drafts. */
+ * the kept drafts; `next` is not in it yet. Models that keep a state per sequence take no drafts. An 8-bit cache holds 16 tokens to a scale: there the model's distribution is the one with the drafts of
+ * a group in the cache beside the tokens that stay, and where a dropped draft raised the group's scale the kept tokens stay as coarse as it made them. */
 int cml_lm_step_verified(CMLLanguageModel* lm, const CMLLMEntry* entries, int num_entries, const float* temperatures, const uint64_t* random, int* accepted, int* next);
 /* Greedy decoding that stays on the device: `steps` steps of all sequences, each step's picks the next
  * one's tokens, out_tokens [steps][num_seqs]; *elapsed_ms (optional) is the time of the loop on the device. */
@@ -107,7 +108,7 @@ CMLGenerationResult* cml_lm_generate(CMLLanguageModel* lm, const int* prompt, in
 /* Generates from a prompt with drafts of another model of the same vocabulary, on the same device: it draws `drafts` (1 .. 32) tokens one by one, of which a step of `lm` keeps what fits its own
  * distribution (cml_lm_step_verified, with the drafter's own probabilities): the result is distributed as cml_lm_step_sampled's, whatever the drafter is, and equals it where config is greedy (up to
  * rounding: a step of several tokens multiplies in other kernels than one of a single token). The same folder loaded with 8-bit weights is a drafter. config NULL: greedy, 256 tokens; its top_k and
- * top_p are not looked at. Steps that are shorter than drafts + 1 bring as many drafts as they hold. Neither model may keep a state per sequence, and both hold the prompt and max_new_tokens. stats may be NULL. */
+ * top_p are not looked at. With an 8-bit cache of `lm` this holds as far as cml_lm_step_verified says. Steps that are shorter than drafts + 1 bring as many drafts as they hold. Neither model may keep a state per sequence, and both hold the prompt and max_new_tokens. stats may be NULL. */
 typedef struct CMLLMDraftStats {
     int steps, drafted, accepted;
 } CMLLMDraftStats;
