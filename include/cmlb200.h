@@ -794,7 +794,8 @@ int cmlb200_dense8_status(int* status, int reset);
  * behind the kept ones is drawn from p where all were kept, otherwise from what p has above q (from p where that is nothing): kept tokens and the drawn one together are distributed as
  * tokens drawn from the target one by one. A sequence without drafts has a token drawn. The drawn token has the largest weight / E, E = -ln(1 - v) standard exponentials; ties go to the lower id.
  * Random numbers come out of Philox4x32-10 with the sequence's 64-bit number as key: v of token j is word j mod 4 of counter (j / 4, 0, 0, 0), u_i word i mod 4 of counter
- * (i / 4, 1, 0, 0); v = (word + 1/2) / 2^32, u = word / 2^32. A number is used for one call of one sequence. A temperature below 1e-5 (or NaN) is greedy: a draft is kept while it is the
+ * (i / 4, 1, 0, 0); v = (word + 1/2) / 2^32, u = word / 2^32. A number is used for one call of one sequence. Which drafts are kept and which token is
+ * drawn is what 64-bit arithmetic says; what p has above q by less than that can tell is nothing. A temperature below 1e-5 (or NaN) is greedy: a draft is kept while it is the
  * largest logit's token (the lowest such id), which is taken behind the kept ones; one above 1e30 counts as that. Vocabularies up to 2^28.
  * Logits of -inf are tokens that cannot come. A target's row that holds NaN or +inf, or nothing but -inf, ends the sequence: drafts from there on are not kept, and the token is -1. A
  * drafter's row of that kind counts as none. A draft outside the vocabulary is not kept. Stands for the softmax loops on the host of src/nn/llama.c:662-737 and the
