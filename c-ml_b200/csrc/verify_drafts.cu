@@ -30,7 +30,7 @@ constexpr float kClose = 0.998f;
 // that are 30 at most where they weigh anything), 2e-6 for 32 values added, 3e-6 for parts put together three times, and 2^-24 for each of a thread's 32 values or more, of which there are V / 4096 at
 // most. Closer calls are decided in 64 bits.
 __device__ __forceinline__ double doubt_of(int vocab) { return 3.0517578125e-5 + 2.9103830456733704e-11 * (double)vocab; }
-constexpr float kLazy = 16.f;                          // a sum's reference is changed where a value is 2^16 times as large
+constexpr float kLazy = 16.f;                          // a reference is changed where a value is 2^16 times as large
 constexpr int MOST_VOCAB = 1 << 28;
 // (infinite ones would make no number of the logits of tokens that cannot come; no number at all stays that, which is greedy)
 __device__ __forceinline__ float heat_of(const cmlb200_drafts& d, int s) {
@@ -438,7 +438,7 @@ draft_token_kernel(const __grid_constant__ Verify v, const T* __restrict__ logit
         const float doubt = (float)doubt_of(V), p_unit = less ? (1.f + doubt) / t.p.sum : 0.f, q_unit = less ? (1.f - doubt) / t.q.sum : 0.f;
         const bool whole = (((uintptr_t)row | (uintptr_t)less) & (4 * sizeof(T) - 1)) == 0;
         // A warp's threads share a bound: the largest weight over wait that any of them has met. A token that comes within kClose of it with v, which is never above its wait, is looked at; there are
-        // few, and only for those a wait is worked out. Where w is p alone it is relative to the largest logit that the warp has met, so that logits far from zero lose no digits (greedy: the logits
+        // few, and only for those a wait is worked out. Where w is p alone it is relative to a logit that none that the warp has met is far above, so that logits far from zero lose no digits (greedy: the logits
         // themselves). p - q may lose all of its digits: a token counts with what it is at most, the bound is what the best is at least.
         float best = greedy ? -INFINITY : 0.f, least = 0.f, others = 0.f, bound = 0.f, ref = less || greedy ? 0.f : -INFINITY;
         int at = 0x7fffffff, bad = 0;
@@ -477,7 +477,7 @@ draft_token_kernel(const __grid_constant__ Verify v, const T* __restrict__ logit
                         }
                     } else {
                         const float top = (uint32_t)(without - 4 * g) < 4u ? most_but(x[k], without - 4 * g) : most;          // (the draft that was turned down sets no reference)
-                        if (__any_sync(0xffffffffu, top > ref)) {
+                        if (__any_sync(0xffffffffu, (top - ref) * c > kLazy)) {        // (a best token outlives three such changes at most)
                             const float to = fmaxf(ref, warp_max(top)), by = ref == -INFINITY ? 0.f : ex2((ref - to) * c);
                             best *= by;
                             others *= by;

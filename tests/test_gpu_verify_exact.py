@@ -252,3 +252,20 @@ def test_every_sequence_far_from_zero(pkg, torch_dev, offset):
     got, want = b.call(pkg), b.want()
     for s, w in enumerate(want):
         assert (got[0][s], got[1][s]) == w[:2], (s, got[:, s], w)
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("form,vocab,rise", [("float32", 200003, 1.0), ("float32", 200003, 60.0), ("float32", 1 << 20, 3.0), ("float16", 300000, 40.0), ("float32", 70000, -200.0), ("float32", 70000, 20000.0)])
+def test_rows_that_rise(pkg, torch_dev, form, vocab, rise, drafter):
+    """Every group of tokens has a larger logit than those in front of it: references change as often as they may."""
+    import torch
+    counts = [1, 0, 2] * 8
+    b = Batch(torch, torch_dev, counts, vocab, 90, form, drafter, (1.0, 0.8))
+    line = torch.linspace(0, rise, vocab, device=torch_dev)
+    b.target[:] = (line + 0.01 * b.target.float()).to(b.target.dtype)
+    if drafter:
+        b.draft[:] = (line.flip(0) * 0.5 + 0.01 * b.draft.float()).to(b.draft.dtype)
+    b.tokens[1::3] = -1
+    got, want = b.call(pkg), b.want()
+    for s, w in enumerate(want):
+        assert got[0][s] == w[0] and got[1][s] in admissible(b, s, w[0]), (s, got[:, s], w)
